@@ -50,7 +50,8 @@ enum {
   B200K_I32 = 4,
   B200K_I64 = 5,
   B200K_BOOL = 6,
-  B200K_U8 = 7
+  B200K_U8 = 7,
+  B200K_E4M3 = 8 /* 8-bit float (4 exponent, 3 mantissa bits): b200k_add_rms_norm output only */
 };
 
 /* Return codes. */
@@ -63,7 +64,8 @@ enum {
   B200K_ERR_LAUNCH = 5,      /* CUDA launch or attribute error */
   B200K_ERR_TIMEOUT = 6,     /* a device-side wait ran out of time (status word) */
   B200K_ERR_PROGRAM = 7,     /* malformed epilogue program */
-  B200K_ERR_DEVICE = 8       /* no sm_100 device current */
+  B200K_ERR_DEVICE = 8,      /* no sm_100 device current */
+  B200K_ERR_INDEX = 9        /* an index read on the device is out of range (status word) */
 };
 
 /*
@@ -453,6 +455,142 @@ typedef struct {
 #define B200K_ATTN_TEST_WITHHOLD_SCORES 1
 
 int b200k_attention(const B200kAttentionArgs* args, void* stream);
+
+/*
+ * Residual addition and RMS norm in one pass (an extension: the reference
+ * leaves the reduction to ATen and fuses pointwise fragments,
+ * compiler/optimization/fusion_pointwise.py:12-30):
+ *   sum = round(x + residual)                      the next residual
+ *   y   = sum * rsqrt(mean(sum^2) + eps) * weight  fp32
+ * over the last dim of [rows, cols] views with unit column stride; sum and
+ * out are contiguous [rows, cols] and overlap no input.  dtype (f32, f16 or
+ * bf16) is that of x, residual and sum; weight ([cols], NULL: none) is f32,
+ * f16 or bf16.  flags: B200K_ROWF_ROUND_NORMED, B200K_ROWF_WEIGHT_PLUS_ONE.
+ *   out_dtype == dtype:      out = round(y)
+ *   out_dtype == B200K_E4M3: out = e4m3(y / s), round to nearest even, and the
+ *     scales s = max(max |y|, 1e-12) / 448 of each row (group 0: scale
+ *     [rows]) or of every 128 columns (group 128, cols a multiple of it:
+ *     scale [rows, cols / 128]).
+ * A row that holds an infinity or NaN gives NaN (with a NaN scale).  Eight
+ * columns a thread when cols and the row strides are multiples of 8 and the
+ * pointers 16-byte aligned; any other layout runs one column a thread.
+ */
+typedef struct {
+  int64_t rows, cols;
+  const void* x;
+  int64_t x_row_stride;
+  const void* residual;
+  int64_t residual_row_stride;
+  const void* weight;
+  int32_t dtype;
+  int32_t w_dtype;
+  int32_t out_dtype;
+  int32_t group;
+  int32_t flags;
+  float eps;
+  void* sum;
+  void* out;
+  float* scale;
+} B200kAddNormArgs;
+
+int b200k_add_rms_norm(const B200kAddNormArgs* args, void* stream);
+
+/*
+ * Rotary embedding of new queries and keys, and the append of the keys and
+ * values to a paged cache (an extension: the reference has no cache and
+ * leaves the rotation's neg / cat to ATen):
+ *   q_out[t, h]        = rot(q[t, h], positions[t])
+ *   k_cache[slots[t]]  = rot(k[t], positions[t]),  v_cache[slots[t]] = v[t]
+ *   rot(x, p)[j]           = x[j] cos[p, j] - x[j + R/2] sin[p, j]     j < R/2
+ *   rot(x, p)[j + R/2]     = x[j + R/2] cos[p, j] + x[j] sin[p, j]
+ *   rot(x, p)[j]           = x[j]                                      j >= R
+ * with R = rot_dim (even, <= head_dim, 0: no rotation), fp32 products and
+ * sums, each result rounded once.  q, k, v: [tokens, heads, head_dim] views
+ * of one 16-bit type (token and head strides, unit element stride); q_out
+ * contiguous.  Caches: [num_pages, page_size, kv_heads, head_dim] views with
+ * cache_strides (page, slot, head; unit element stride, the same for both);
+ * a slot is page * page_size + place in the page.  cos, sin: [table_rows,
+ * R/2] of f32 or the inputs' type, row stride table_stride.  positions and
+ * slots: [tokens], i32 or i64.  A token with a negative slot is rotated but
+ * not appended.  Slots that appear twice leave one or the other token's
+ * values, element by element unspecified.  A slot past the cache, or an
+ * appended token's position outside the tables, is not appended and sets
+ * *status (may be NULL) to B200K_ERR_INDEX.  At most 2^31 - 1 slots.
+ */
+typedef struct {
+  int64_t tokens, heads, kv_heads, head_dim, rot_dim;
+  int64_t num_pages, page_size;
+  const void* q;
+  int64_t q_strides[2];
+  const void* k;
+  int64_t k_strides[2];
+  const void* v;
+  int64_t v_strides[2];
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  int64_t cache_strides[3];
+  const void* cos;
+  const void* sin;
+  int64_t table_rows, table_stride;
+  const void* positions;
+  const void* slots;
+  int32_t dtype, table_dtype, positions_dtype, slots_dtype;
+  int32_t* status;
+} B200kRopeAppendArgs;
+
+int b200k_rope_append(const B200kRopeAppendArgs* args, void* stream);
+
+/*
+ * Attention of packed queries over a paged key / value cache (an extension,
+ * as b200k_attention): sequence b has the queries q_start[b] ..
+ * q_start[b + 1] - 1 of q [tokens, heads, head_dim] and the keys 0 ..
+ * kv_len[b] - 1, key j in page page_table[b, j / page_size] at place
+ * j % page_size.  Its queries are the last of its positions: query i is at
+ * position p = kv_len[b] - queries + i and sees the keys
+ * max(0, p - window + 1) .. p (window 0: from 0).
+ *   out[t, h] = sum_j softmax_j(f(scale q . k_j)) v_j,  f(s) = s, or
+ *   softcap * tanh(s / softcap) when softcap > 0
+ * with key / value head h / (heads / kv_heads).  A query without keys (p < 0)
+ * and a token behind the last sequence get zeros.  q, caches and out are of
+ * one 16-bit type; head_dim 64 or 128; cache_strides as for
+ * b200k_rope_append; strides multiples of 8 elements, pointers 16-byte
+ * aligned; out contiguous.  Nothing is read of the caches outside the keys
+ * that a sequence's queries see, so other pages and the rest of the last one
+ * may hold anything.  Scores, softmax and sums are fp32; the probabilities are
+ * rounded to the input type for the second product.  max_q_len (0: unknown)
+ * is a hint of the longest sequence's queries: it chooses kernels and grids,
+ * never results.  Index tensors are i32 on the device; entries out of range
+ * are clamped (a page out of range reads as zeros) and set *status (may be
+ * NULL) to B200K_ERR_INDEX.  workspace: device memory of
+ * b200k_paged_attention_workspace bytes, 16-byte aligned, for this call
+ * alone until it has run.
+ */
+typedef struct {
+  int64_t tokens, seqs, heads, kv_heads, head_dim;
+  int64_t num_pages, page_size, table_cols, table_stride;
+  const void* q;
+  int64_t q_strides[2];
+  const void* k_cache;
+  const void* v_cache;
+  int64_t cache_strides[3];
+  void* out;
+  const int32_t* page_table;
+  const int32_t* q_start;
+  const int32_t* kv_len;
+  int64_t max_q_len, window;
+  float scale; /* <= 0: 1 / sqrt(head_dim) */
+  float softcap;
+  int32_t dtype;
+  int32_t test_flags; /* B200K_PAGED_TEST_* hooks (0 in production) */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  int64_t timeout_ns;
+} B200kPagedAttentionArgs;
+
+int b200k_paged_attention(const B200kPagedAttentionArgs* args, void* stream);
+int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* args, int64_t* bytes);
 
 const char* b200k_status_string(int code);
 /* Library version, for the loader's sanity check. */

@@ -1,0 +1,218 @@
+"""b200::paged_attention against the formula in 64 bits (the bound is
+derived at serving_reference.attention_close).  Everything of the caches that
+no query may see holds NaN, and tables name no page that is not needed, so a
+read outside the mask shows in the output or in the status word."""
+import pytest
+import torch
+
+import serving_reference as ref
+from compiler import runtime
+from compiler.runtime import cabi
+
+pytestmark = pytest.mark.gpu
+runtime.load()
+BF, HF = torch.bfloat16, torch.float16
+
+
+def run(inputs, softcap=0.0, window=0, max_q=0, scale=0.0):
+    q = inputs[0]
+    runtime.gemm_status()
+    out = torch.ops.b200.paged_attention(*inputs, scale, softcap, window, max_q)
+    want, size = ref.paged_attention(*inputs, scale or ref.default_scale(q.shape[2]), softcap, window)
+    ref.attention_close(out, want, size, q.dtype)
+    end = int(inputs[4][-1])
+    assert out[end:].abs().sum() == 0
+    assert runtime.gemm_status() == 0
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,hkv", [(32, 8), (8, 8), (8, 1), (7, 1), (28, 4), (40, 1), (6, 2)])
+def test_single_tokens(H, hkv, D, dtype):
+    ns = [1, 2, 15, 16, 17, 100, 333, 1, 64]
+    run(ref.paged_inputs([1] * len(ns), ns, H, hkv, D, 16, dtype))
+
+
+@pytest.mark.parametrize("page", [1, 3, 16, 24, 64, 100, 128])
+def test_page_sizes(page):
+    ns = [1, page, page + 1, 200, 3 * page - 1, 77]
+    ns = [max(1, n) for n in ns]
+    run(ref.paged_inputs([1] * len(ns), ns, 8, 2, 64, page, BF))
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "pair"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_cache_layouts(layout, D):
+    run(ref.paged_inputs([1, 4, 1], [100, 50, 7], 8, 2, D, 16, BF, layout=layout))
+
+
+@pytest.mark.parametrize("softcap,window", [(30.0, 0), (5.0, 0), (0.0, 1), (0.0, 17), (0.0, 100), (50.0, 33),
+                                            (0.0, 10**6)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_caps_and_windows(softcap, window, D):
+    qs, ns = [1, 3, 1, 8, 20], [90, 200, 5, 8, 300]
+    run(ref.paged_inputs(qs, ns, 8, 2, D, 16, BF, window=window), softcap, window)
+
+
+@pytest.mark.parametrize("max_q", [0, 1, 33])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+def test_ragged_queries_and_rows_without_keys(D, dtype, max_q):
+    # no queries, no keys, fewer keys than queries, and rows behind the last sequence
+    qs = [0, 1, 3, 33, 5, 4, 0, 2]
+    ns = [10, 40, 0, 33, 200, 2, 0, 2]
+    out = run(ref.paged_inputs(qs, ns, 8, 2, D, 16, dtype, pad=5), max_q=max_q)
+    assert out[1:4].abs().sum() == 0                       # kv_len 0
+    start = sum(qs[:5])
+    assert out[start:start + 2].abs().sum() == 0           # positions before the first key
+    assert out[start + 2:start + 4].abs().sum() > 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q,n,H,hkv", [(65, 65, 8, 2), (130, 400, 4, 4), (257, 257, 8, 1), (100, 1000, 14, 2),
+                                       (300, 301, 3, 1)])
+def test_prompts(q, n, H, hkv, D):
+    run(ref.paged_inputs([q, 1, q // 3], [n, n // 2, q], H, hkv, D, 16, BF))
+
+
+@pytest.mark.parametrize("softcap,window", [(30.0, 0), (0.0, 50), (20.0, 200)])
+def test_prompts_with_caps_and_windows(softcap, window):
+    run(ref.paged_inputs([200, 1, 90], [333, 250, 90], 8, 2, 128, 16, BF, window=window), softcap, window)
+
+
+def test_one_long_sequence_is_spread_and_joined():
+    run(ref.paged_inputs([1], [9001], 8, 2, 128, 16, BF))
+    run(ref.paged_inputs([2, 1], [5000, 3], 8, 8, 64, 32, HF))
+
+
+def test_many_sequences():
+    """More sequences than a warp's lanes and than workers, short and ragged."""
+    ns = [1 + (i * 37) % 50 for i in range(1300)]
+    run(ref.paged_inputs([1] * len(ns), ns, 2, 1, 64, 16, BF))
+
+
+def test_strided_queries():
+    q, *rest = ref.paged_inputs([1, 5, 2], [30, 60, 2], 8, 2, 64, 16, BF)
+    wide = torch.zeros(q.shape[0], 12, 64, device="cuda", dtype=BF)
+    wide[:, 3:11] = q
+    run((wide[:, 3:11], *rest))
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)
+    run((turned, *rest))
+
+
+def test_large_scores_stay_finite():
+    q, kc, vc, *rest = ref.paged_inputs([1, 3], [50, 20], 4, 2, 64, 16, BF)
+    out = torch.ops.b200.paged_attention(q * 1000, kc, vc, *rest)
+    assert out.isfinite().all()
+
+
+def test_cache_offsets_past_32_bits():
+    D, hkv, page = 128, 8, 128
+    pages = 2**31 // (page * hkv * D) + 4
+    kc, vc = (torch.zeros(pages, page, hkv, D, device="cuda", dtype=BF) for _ in range(2))
+    table = torch.tensor([[pages - 1, 0, pages - 2]], dtype=torch.int32, device="cuda")
+    for pg in table[0].tolist():
+        kc[pg].normal_()
+        vc[pg].normal_()
+    n = 2 * page + 50
+    for m in (1, 150):
+        q = torch.randn(m, 8, D, device="cuda").to(BF)
+        run((q, kc, vc, table, torch.tensor([0, m], dtype=torch.int32, device="cuda"),
+             torch.tensor([n], dtype=torch.int32, device="cuda")))
+
+
+def test_bad_indexes_are_reported_and_stay_in_bounds():
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([1, 2], [40, 20], 8, 2, 64, 16, BF)
+    for change in (lambda t, s, n: t.__setitem__((0, 1), 10**6), lambda t, s, n: t.__setitem__((1, 0), -5),
+                   lambda t, s, n: n.__setitem__(0, 10**6), lambda t, s, n: n.__setitem__(1, -3),
+                   lambda t, s, n: s.__setitem__(2, 50), lambda t, s, n: s.__setitem__(1, -2)):
+        t, s, n = table.clamp_min(0), q_start.clone(), kv_len.clone()
+        change(t, s, n)
+        runtime.gemm_status()
+        torch.ops.b200.paged_attention(q, kc, vc, t, s, n)
+        assert runtime.gemm_status() == 9
+    run((q, kc, vc, table, q_start, kv_len))
+
+
+def test_empty_calls():
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([1, 2], [40, 20], 8, 2, 64, 16, BF)
+    op = torch.ops.b200.paged_attention
+    assert op(q[:0], kc, vc, table, q_start * 0, kv_len).shape == (0, 8, 64)
+    out = op(q, kc, vc, table[:0], q_start[:1], kv_len[:0])
+    assert out.shape == q.shape and out.abs().sum() == 0
+    assert op(q, kc, vc, table[:, :0], q_start, kv_len * 0).abs().sum() == 0
+
+
+def test_refusals():
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([1, 2], [40, 20], 8, 2, 64, 16, BF)
+    op = torch.ops.b200.paged_attention
+    for bad in (lambda: op(q[:, :, :32], kc[..., :32], vc[..., :32], table, q_start, kv_len),
+                lambda: op(q[:, :7], kc, vc, table, q_start, kv_len),
+                lambda: op(q.half(), kc, vc, table, q_start, kv_len),
+                lambda: op(q, kc, vc[:1], table, q_start, kv_len),
+                lambda: op(q, kc, vc, table.long(), q_start, kv_len),
+                lambda: op(q, kc, vc, table, q_start[:2], kv_len),
+                lambda: op(q, kc, vc, table[:1], q_start, kv_len),
+                lambda: op(q, kc, vc, table, q_start, kv_len.cpu()),
+                lambda: op(q, kc, vc, table, q_start, kv_len, 0.0, -1.0),
+                lambda: op(q, kc, vc, table, q_start, kv_len, 0.0, 0.0, -1),
+                lambda: op(q.float(), kc.float(), vc.float(), table, q_start, kv_len),
+                lambda: op(q.clone().requires_grad_(), kc, vc, table, q_start, kv_len)):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
+def test_two_graphs_and_two_streams():
+    """Two captured graphs replayed on two streams at once, and eager calls
+    between them, keep to their own workspaces."""
+    a = ref.paged_inputs([1] * 4, [700, 90, 2000, 5], 8, 2, 128, 16, BF, seed=1)
+    b = ref.paged_inputs([3] * 4, [70, 900, 20, 1500], 8, 2, 128, 16, BF, seed=2)
+    op = torch.ops.b200.paged_attention
+    want_a, want_b = op(*a), op(*b)
+    graphs, outs = [], []
+    for x in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(op(*x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        op(*b)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want_a) and torch.equal(outs[1], want_b)
+
+
+def test_a_replayed_graph_follows_its_index_tensors():
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([1, 1], [200, 300], 8, 2, 64, 16, BF)
+    op = torch.ops.b200.paged_attention
+    op(q, kc, vc, table, q_start, kv_len)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = op(q, kc, vc, table, q_start, kv_len)
+    for lens in ([1, 300], [200, 16], [0, 77]):
+        kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        g.replay()
+        want, size = ref.paged_attention(q, kc, vc, table, q_start, kv_len, ref.default_scale(64))
+        ref.attention_close(out, want, size, BF)
+
+
+def test_results_repeat_bit_for_bit():
+    x = ref.paged_inputs([1, 5, 1, 40], [3000, 900, 1, 600], 8, 2, 128, 16, BF)
+    first = torch.ops.b200.paged_attention(*x)
+    for _ in range(5):
+        assert torch.equal(torch.ops.b200.paged_attention(*x), first)
+
+
+def test_c_abi():
+    x = ref.paged_inputs([1, 20], [500, 20], 8, 2, 128, 16, HF)
+    out = torch.full_like(x[0], float("nan"))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cabi.paged_attention(*x, out, status=status)
+    assert status.item() == 0
+    want, size = ref.paged_attention(*x, ref.default_scale(128))
+    ref.attention_close(out, want, size, HF)

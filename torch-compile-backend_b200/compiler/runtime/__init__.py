@@ -91,20 +91,45 @@ def _register_fakes() -> None:
     def _(a, b, cos, sin, period, out_shape):
         return a.new_empty(out_shape)
 
+    @torch.library.register_fake(lib + "add_rms_norm")
+    def _(x, residual, weight, eps, flags=0):
+        return x.new_empty(x.shape), x.new_empty(x.shape)
+
+    @torch.library.register_fake(lib + "add_rms_norm_quant")
+    def _(x, residual, weight, eps, group=0, flags=0):
+        scales = (*x.shape[:-1], 1 if group == 0 else x.shape[-1] // 128)
+        return (
+            x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty(scales, dtype=torch.float32),
+            x.new_empty(x.shape),
+        )
+
+    @torch.library.register_fake(lib + "rope_append")
+    def _(q, k, v, cos, sin, positions, slots, k_cache, v_cache):
+        return q.new_empty(q.shape)
+
+    @torch.library.register_fake(lib + "paged_attention")
+    def _(q, k_cache, v_cache, page_table, q_start, kv_len, scale=0.0, softcap=0.0, window=0, max_q_len=0):
+        return q.new_empty(q.shape)
+
 
 def gemm_status(device: int = 0, reset: bool = True) -> int:
-    """The GEMM kernels' device status word (0 = ok, 6 = a wait timed out);
-    synchronises with the device."""
+    """The kernels' device status word (0 = ok, 6 = a wait timed out, 9 = an
+    index read on the device was out of range); synchronises with the
+    device."""
     load()
     return int(torch.ops.b200.gemm_status(device, reset))
 
 
 def check_status(device: int = 0) -> None:
-    """Synchronises with the device and raises RuntimeError if a GEMM launched
-    through ``torch.ops.b200.gemm_epilogue`` reported a device-side timeout
-    since the last check (the word is then cleared)."""
+    """Synchronises with the device and raises RuntimeError if a kernel
+    launched through ``torch.ops.b200.*`` reported a device-side timeout or an
+    index out of range since the last check (the word is then cleared)."""
     load()
     v = gemm_status(device, reset=True)
+    if v == 9:
+        raise RuntimeError(f"b200::rope_append or paged_attention on cuda:{device} reported status {v}: a slot, "
+                           "position, page or length is out of range")
     if v != 0:
         raise RuntimeError(f"b200::gemm_epilogue on cuda:{device} reported status {v} "
                            "(6 = a device-side wait timed out): an earlier GEMM's output is incomplete")

@@ -18,10 +18,10 @@ MAX_DIMS = 6
 MAX_INPUTS = 8
 MAX_INSTR = 64
 
-F32, F16, BF16, F64, I32, I64, BOOL, U8 = range(8)
+F32, F16, BF16, F64, I32, I64, BOOL, U8, E4M3 = range(9)
 DTYPE = {
     torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float64: F64,
-    torch.int32: I32, torch.int64: I64, torch.bool: BOOL, torch.uint8: U8,
+    torch.int32: I32, torch.int64: I64, torch.bool: BOOL, torch.uint8: U8, torch.float8_e4m3fn: E4M3,
 }
 ROW_RMSNORM, ROW_LAYERNORM, ROW_RMSNORM_SWIGLU = 0, 1, 2
 GEMM_TEST_WITHHOLD_READY = 1  # include/b200k.h: failure-detection test hook
@@ -30,7 +30,8 @@ EXPORTED = [
     "b200k_pointwise", "b200k_gemm_epilogue", "b200k_gemm_num_configs", "b200k_gemm_config_info",
     "b200k_gemm_pick_config", "b200k_rownorm", "b200k_softmax", "b200k_status_string", "b200k_version",
     "b200k_gemm_epilogue_noalloc", "b200k_gemm_noalloc_status", "b200k_rope", "b200k_pointwise_jit_stats",
-    "b200k_pointwise_jit_compile", "b200k_attention", "b200k_gemm_rope",
+    "b200k_pointwise_jit_compile", "b200k_attention", "b200k_gemm_rope", "b200k_add_rms_norm",
+    "b200k_rope_append", "b200k_paged_attention", "b200k_paged_attention_workspace",
 ]
 
 
@@ -116,6 +117,41 @@ class AttentionArgs(ctypes.Structure):
                 ("test_flags", ctypes.c_int32), ("status", ctypes.c_void_p), ("timeout_ns", ctypes.c_int64)]
 
 
+class AddNormArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("x_row_stride", ctypes.c_int64), ("residual", ctypes.c_void_p),
+                ("residual_row_stride", ctypes.c_int64), ("weight", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("w_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("flags", ctypes.c_int32), ("eps", ctypes.c_float), ("sum", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("scale", ctypes.c_void_p)]
+
+
+class RopeAppendArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("rot_dim", ctypes.c_int64), ("num_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("q", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 2),
+                ("k", ctypes.c_void_p), ("k_strides", ctypes.c_int64 * 2), ("v", ctypes.c_void_p),
+                ("v_strides", ctypes.c_int64 * 2), ("q_out", ctypes.c_void_p), ("k_cache", ctypes.c_void_p),
+                ("v_cache", ctypes.c_void_p), ("cache_strides", ctypes.c_int64 * 3), ("cos", ctypes.c_void_p),
+                ("sin", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+                ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("table_dtype", ctypes.c_int32), ("positions_dtype", ctypes.c_int32),
+                ("slots_dtype", ctypes.c_int32), ("status", ctypes.c_void_p)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("seqs", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("num_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("table_cols", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 2), ("k_cache", ctypes.c_void_p),
+                ("v_cache", ctypes.c_void_p), ("cache_strides", ctypes.c_int64 * 3), ("out", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("max_q_len", ctypes.c_int64), ("window", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("softcap", ctypes.c_float), ("dtype", ctypes.c_int32), ("test_flags", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("status", ctypes.c_void_p),
+                ("timeout_ns", ctypes.c_int64)]
+
+
 ATTN_TEST_WITHHOLD_SCORES = 1  # include/b200k.h: failure-detection test hook
 
 _lib = None
@@ -136,6 +172,11 @@ def library() -> ctypes.CDLL:
             ("b200k_softmax", [ctypes.POINTER(SoftmaxArgs), ctypes.c_void_p]),
             ("b200k_rope", [ctypes.POINTER(RopeArgs), ctypes.c_void_p]),
             ("b200k_attention", [ctypes.POINTER(AttentionArgs), ctypes.c_void_p]),
+            ("b200k_add_rms_norm", [ctypes.POINTER(AddNormArgs), ctypes.c_void_p]),
+            ("b200k_rope_append", [ctypes.POINTER(RopeAppendArgs), ctypes.c_void_p]),
+            ("b200k_paged_attention", [ctypes.POINTER(PagedAttentionArgs), ctypes.c_void_p]),
+            ("b200k_paged_attention_workspace", [ctypes.POINTER(PagedAttentionArgs),
+                                                 ctypes.POINTER(ctypes.c_int64)]),
             ("b200k_gemm_pick_config", [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]),
             ("b200k_gemm_config_info", [ctypes.c_int] + [ctypes.POINTER(ctypes.c_int)] * 4),
             ("b200k_gemm_num_configs", []),
@@ -354,3 +395,69 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tens
     a.status = status.data_ptr() if status is not None else None
     a.timeout_ns = timeout_ns
     _check("b200k_attention", library().b200k_attention(ctypes.byref(a), _stream()))
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight, eps: float, sum_out: torch.Tensor,
+                 out: torch.Tensor, scale: torch.Tensor | None = None, group: int = 0, flags: int = 0) -> None:
+    """sum_out = x + residual and out = its RMS norm over [rows, cols] views; an e4m3
+    `out` takes its scales (one a row, or one for `group` columns) in `scale`."""
+    a = AddNormArgs()
+    a.rows, a.cols = x.shape
+    a.x, a.x_row_stride = x.data_ptr(), x.stride(0)
+    a.residual, a.residual_row_stride = residual.data_ptr(), residual.stride(0)
+    if weight is not None:
+        a.weight, a.w_dtype = weight.data_ptr(), DTYPE[weight.dtype]
+    a.dtype, a.out_dtype = DTYPE[x.dtype], DTYPE[out.dtype]
+    a.group, a.flags, a.eps = group, flags, eps
+    a.sum, a.out = sum_out.data_ptr(), out.data_ptr()
+    a.scale = scale.data_ptr() if scale is not None else None
+    _check("b200k_add_rms_norm", library().b200k_add_rms_norm(ctypes.byref(a), _stream()))
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                q_out: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """q_out = q rotated; k rotated and v written into the caches' slots."""
+    a = RopeAppendArgs()
+    a.tokens, a.heads, a.head_dim = q.shape
+    a.kv_heads, a.rot_dim = k.shape[1], 2 * cos.shape[1]
+    a.num_pages, a.page_size = k_cache.shape[:2]
+    a.q, a.k, a.v, a.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr()
+    for dst, t in ((a.q_strides, q), (a.k_strides, k), (a.v_strides, v), (a.cache_strides, k_cache)):
+        for d in range(len(dst)):
+            dst[d] = t.stride(d)
+    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    a.cos, a.sin, a.table_rows, a.table_stride = cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.stride(0)
+    a.positions, a.slots = positions.data_ptr(), slots.data_ptr()
+    a.dtype, a.table_dtype = DTYPE[q.dtype], DTYPE[cos.dtype]
+    a.positions_dtype, a.slots_dtype = DTYPE[positions.dtype], DTYPE[slots.dtype]
+    a.status = status.data_ptr() if status is not None else None
+    _check("b200k_rope_append", library().b200k_rope_append(ctypes.byref(a), _stream()))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    q_start: torch.Tensor, kv_len: torch.Tensor, out: torch.Tensor, scale: float = 0.0,
+                    softcap: float = 0.0, window: int = 0, max_q_len: int = 0, status: torch.Tensor | None = None,
+                    timeout_ns: int = 0, test_flags: int = 0) -> None:
+    """Attention of packed queries [tokens, H, D] over a paged cache, into `out`."""
+    a = PagedAttentionArgs()
+    a.tokens, a.heads, a.head_dim = q.shape
+    a.seqs, a.kv_heads = kv_len.shape[0], k_cache.shape[2]
+    a.num_pages, a.page_size = k_cache.shape[:2]
+    a.table_cols, a.table_stride = page_table.shape[1], page_table.stride(0)
+    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    for d in range(2):
+        a.q_strides[d] = q.stride(d)
+    for d in range(3):
+        a.cache_strides[d] = k_cache.stride(d)
+    a.page_table, a.q_start, a.kv_len = page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr()
+    a.max_q_len, a.window, a.scale, a.softcap = max_q_len, window, scale, softcap
+    a.dtype, a.test_flags = DTYPE[q.dtype], test_flags
+    n = ctypes.c_int64()
+    _check("b200k_paged_attention_workspace",
+           library().b200k_paged_attention_workspace(ctypes.byref(a), ctypes.byref(n)))
+    ws = torch.empty(max(1, n.value), dtype=torch.uint8, device=q.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+    a.status = status.data_ptr() if status is not None else None
+    a.timeout_ns = timeout_ns
+    _check("b200k_paged_attention", library().b200k_paged_attention(ctypes.byref(a), _stream()))

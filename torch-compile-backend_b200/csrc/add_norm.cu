@@ -1,0 +1,334 @@
+// Residual addition + RMS norm in one pass over the rows (b200k_add_rms_norm,
+// include/b200k.h), with a 16-bit / fp32 output or an e4m3 output with scales:
+//
+//   h = round(x + r)                        stored: the next residual
+//   y = h * rsqrt(mean(h^2) + eps) * w      fp32
+//   out = round(y), or q = e4m3(y * 448 / a) with scale a / 448,
+//         a = max(max |y| over the scale's columns, 1e-12)
+//
+// No reference counterpart: the reference leaves the reduction to ATen and
+// fuses only pointwise fragments (compiler/optimization/fusion_pointwise.py:12-30).
+//
+// What bounds it: HBM.  A row is read once (x and r) and written once (h and
+// out); its sums live in registers between the two, so the bytes are the
+// floor's.  h is normed as it is stored, rounded to x's type: the result is
+// that of the addition followed by b200k_rownorm.  The sum of squares and y
+// are fp32; out is rounded once (twice with B200K_ROWF_ROUND_NORMED, which
+// reproduces models that round before the weight).
+#include <algorithm>
+#include <cstring>
+
+#include "common.cuh"
+#include "host_common.h"
+#include "rowreduce.cuh"
+
+namespace b200k {
+namespace {
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kMinAmax = 1e-12f;  // keeps 448 / a finite for rows of zeros
+
+struct AddNormParams {
+  int64_t rows;
+  int32_t cols;
+  int32_t group;  // columns of one scale (quantised output): cols or 128
+  const void* x;
+  const void* r;
+  const void* w;
+  void* h;
+  void* out;
+  float* scale;
+  int64_t x_stride, r_stride;
+  float eps;
+  int32_t w_dt, flags;
+};
+
+template <int DT> struct Elem;
+template <> struct Elem<B200K_F32> { using T = float; };
+template <> struct Elem<B200K_F16> { using T = __half; };
+template <> struct Elem<B200K_BF16> { using T = __nv_bfloat16; };
+
+template <int DT>
+__device__ __forceinline__ float round_to(float v) {
+  if constexpr (DT == B200K_BF16) return round_bf16(v);
+  if constexpr (DT == B200K_F16) return round_f16(v);
+  return v;
+}
+
+__device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
+  uint16_t u;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(u) : "f"(hi), "f"(lo));
+  return u;
+}
+
+// |v| as an unsigned pattern: ordered as the magnitudes are, infinity above
+// every number and NaN above infinity, so a row's NaN reaches its scale.
+__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Sum over the TPR threads of a row; each row group of a CTA has its own
+// named barrier and slots.
+template <int TPR, bool IS_MAX>
+__device__ __forceinline__ uint32_t row_reduce(uint32_t v, uint32_t* slots, int grp) {
+  if constexpr (IS_MAX) {
+    v = __reduce_max_sync(0xffffffffu, v);
+  } else {
+    v = __float_as_uint(warp_sum(__uint_as_float(v)));
+  }
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    uint32_t* s = slots + grp * W;
+    const int t = threadIdx.x % TPR;
+    if ((t & 31) == 0) s[t >> 5] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(TPR) : "memory");
+    // every thread adds the W partials in the same order
+    uint32_t a = s[0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      if constexpr (IS_MAX) a = max(a, s[k]);
+      else a = __float_as_uint(__uint_as_float(a) + __uint_as_float(s[k]));
+    }
+    v = a;
+  }
+  return v;
+}
+
+// QUANT: 0 output of x's type, 1 e4m3 with one scale a row, 2 with one for 128
+// columns.  A thread holds VPT vectors of 8 columns, vector t + i TPR, so 16
+// neighbouring lanes hold the 128 columns of a scale.
+template <int DT, int TPR, int VPT, int QUANT, int THREADS>
+__global__ void __launch_bounds__(THREADS) add_norm_kernel(const __grid_constant__ AddNormParams p) {
+  constexpr int kGroups = THREADS / TPR;
+  using T = typename Elem<DT>::T;
+  __shared__ uint32_t slots[2][THREADS / 32];
+  const int grp = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + grp;
+  if (row >= p.rows) return;  // the whole group: its barrier is its own
+  const int nvec = p.cols >> 3;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const T* r = static_cast<const T*>(p.r) + row * p.r_stride;
+  T* h = static_cast<T*>(p.h) + row * p.cols;
+  float v[VPT][8];
+  {
+    float a[VPT][8];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {  // every load of the row before the first use
+      const int c = min(t + i * TPR, nvec - 1) * 8;
+      load_vec8(x, c, DT, v[i]);
+      load_vec8(r, c, DT, a[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = round_to<DT>(v[i][j] + a[i][j]);
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = t + i * TPR;
+    if (c < nvec) {
+      store_vec8(h, c * 8, DT, v[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+    }
+  }
+  ss = __uint_as_float(row_reduce<TPR, false>(__float_as_uint(ss), slots[0], grp));
+  const float rstd = rsqrtf(ss / static_cast<float>(p.cols) + p.eps);
+  const bool round_n = p.flags & B200K_ROWF_ROUND_NORMED, plus1 = p.flags & B200K_ROWF_WEIGHT_PLUS_ONE;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = t + i * TPR;
+    float w[8];
+    if (p.w) load_vec8(p.w, min(c, nvec - 1) * 8, p.w_dt, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float n = v[i][j] * rstd;
+      if (round_n) n = round_to<DT>(n);
+      v[i][j] = p.w ? n * (plus1 ? 1.0f + w[j] : w[j]) : n;
+    }
+    if constexpr (QUANT == 0) {
+      if (c < nvec) store_vec8(static_cast<T*>(p.out) + row * p.cols, c * 8, DT, v[i]);
+    } else if constexpr (QUANT == 1) {
+      if (c < nvec)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, mag(v[i][j]));
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, mag(v[i][j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float a = __uint_as_float(max(m, __float_as_uint(kMinAmax))), inv = kE4m3Max / a;
+      if (c < nvec) {
+        if ((t & 15) == 0) p.scale[row * (p.cols >> 7) + (c >> 4)] = a / kE4m3Max;
+        uint16_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = e4m3x2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv);
+        uint2 u = make_uint2(q[0] | (static_cast<uint32_t>(q[1]) << 16), q[2] | (static_cast<uint32_t>(q[3]) << 16));
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + row * p.cols + c * 8) = u;
+      }
+    }
+  }
+  if constexpr (QUANT == 1) {
+    top = row_reduce<TPR, true>(top, slots[1], grp);
+    const float a = __uint_as_float(max(top, __float_as_uint(kMinAmax))), inv = kE4m3Max / a;
+    if (t == 0) p.scale[row] = a / kE4m3Max;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      if (c < nvec) {
+        uint16_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = e4m3x2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv);
+        uint2 u = make_uint2(q[0] | (static_cast<uint32_t>(q[1]) << 16), q[2] | (static_cast<uint32_t>(q[3]) << 16));
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + row * p.cols + c * 8) = u;
+      }
+    }
+  }
+}
+
+// Any width, stride and alignment: a CTA per row, one element a thread and
+// step, the row read again (from L2) for the output.
+template <int DT, int QUANT>
+__global__ void __launch_bounds__(512) add_norm_any_kernel(const __grid_constant__ AddNormParams p) {
+  using T = typename Elem<DT>::T;
+  __shared__ uint32_t slots[2][16];
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const T* r = static_cast<const T*>(p.r) + row * p.r_stride;
+  T* h = static_cast<T*>(p.h) + row * p.cols;
+  auto sum_at = [&](int c) { return round_to<DT>(load_scalar(x, c, DT) + load_scalar(r, c, DT)); };
+  float ss = 0.0f;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < p.cols; c += 512) {
+    const float v = sum_at(c);
+    store_scalar(h, c, DT, v);
+    ss = fmaf(v, v, ss);
+  }
+  ss = __uint_as_float(row_reduce<512, false>(__float_as_uint(ss), slots[0], 0));
+  const float rstd = rsqrtf(ss / static_cast<float>(p.cols) + p.eps);
+  const bool round_n = p.flags & B200K_ROWF_ROUND_NORMED, plus1 = p.flags & B200K_ROWF_WEIGHT_PLUS_ONE;
+  auto y_at = [&](int c) {
+    float n = sum_at(c) * rstd;
+    if (round_n) n = round_to<DT>(n);
+    if (p.w) {
+      const float w = load_scalar(p.w, c, p.w_dt);
+      n *= plus1 ? 1.0f + w : w;
+    }
+    return n;
+  };
+  if constexpr (QUANT == 0) {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < p.cols; c += 512) store_scalar(static_cast<T*>(p.out) + row * p.cols, c, DT, y_at(c));
+  } else {
+    uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.cols;
+    if constexpr (QUANT == 1) {
+      uint32_t top = 0;
+#pragma unroll 4
+      for (int c = threadIdx.x; c < p.cols; c += 512) top = max(top, mag(y_at(c)));
+      top = row_reduce<512, true>(top, slots[1], 0);
+      const float a = __uint_as_float(max(top, __float_as_uint(kMinAmax))), inv = kE4m3Max / a;
+      if (threadIdx.x == 0) p.scale[row] = a / kE4m3Max;
+#pragma unroll 4
+      for (int c = threadIdx.x; c < p.cols; c += 512) out[c] = static_cast<uint8_t>(e4m3x2(y_at(c) * inv, 0.0f) & 0xff);
+    } else {  // a warp per scale: 128 columns, 4 a lane
+      const int lane = threadIdx.x & 31;
+      for (int g = threadIdx.x >> 5; g < (p.cols >> 7); g += 16) {
+        float y[4];
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          y[k] = y_at(g * 128 + k * 32 + lane);
+          m = max(m, mag(y[k]));
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        const float a = __uint_as_float(max(m, __float_as_uint(kMinAmax))), inv = kE4m3Max / a;
+        if (lane == 0) p.scale[row * (p.cols >> 7) + g] = a / kE4m3Max;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          out[g * 128 + k * 32 + lane] = static_cast<uint8_t>(e4m3x2(y[k] * inv, 0.0f) & 0xff);
+      }
+    }
+  }
+}
+
+template <int DT, int QUANT, int TPR, int VPT, int THREADS>
+void launch_vec(const AddNormParams& p, cudaStream_t st) {
+  constexpr int kGroups = THREADS / TPR;
+  add_norm_kernel<DT, TPR, VPT, QUANT, THREADS>
+      <<<static_cast<unsigned>((p.rows + kGroups - 1) / kGroups), THREADS, 0, st>>>(p);
+}
+
+template <int DT, int QUANT>
+void launch(const AddNormParams& p, bool vec, cudaStream_t st) {
+  const int nvec = p.cols >> 3;
+  if (!vec || nvec > 4096) {
+    add_norm_any_kernel<DT, QUANT><<<static_cast<unsigned>(p.rows), 512, 0, st>>>(p);
+  } else if (nvec <= 64) {
+    launch_vec<DT, QUANT, 32, 2, 256>(p, st);
+  } else if (nvec <= 128) {
+    launch_vec<DT, QUANT, 64, 2, 256>(p, st);
+  } else if (nvec <= 256) {
+    launch_vec<DT, QUANT, 128, 2, 256>(p, st);
+  } else if (nvec <= 512) {
+    launch_vec<DT, QUANT, 256, 2, 256>(p, st);
+  } else if (nvec <= 1024) {
+    launch_vec<DT, QUANT, 512, 2, 512>(p, st);
+  } else if (nvec <= 2048) {
+    launch_vec<DT, QUANT, 512, 4, 512>(p, st);
+  } else {
+    launch_vec<DT, QUANT, 1024, 4, 1024>(p, st);
+  }
+}
+
+template <int DT>
+void launch_quant(const AddNormParams& p, int quant, bool vec, cudaStream_t st) {
+  if (quant == 0) launch<DT, 0>(p, vec, st);
+  else if (quant == 1) launch<DT, 1>(p, vec, st);
+  else launch<DT, 2>(p, vec, st);
+}
+
+}  // namespace
+}  // namespace b200k
+
+using namespace b200k;
+
+extern "C" int b200k_add_rms_norm(const B200kAddNormArgs* a, void* stream_) {
+  if (!a) return B200K_ERR_ARG;
+  if (a->rows < 0 || a->cols < 0) return B200K_ERR_SHAPE;
+  if (a->rows == 0 || a->cols == 0) return B200K_OK;
+  if (!a->x || !a->residual || !a->sum || !a->out) return B200K_ERR_ARG;
+  if (a->rows > 0x7fffffffLL || a->cols > 0x3fffffffLL) return B200K_ERR_SHAPE;
+  if (a->dtype != B200K_F32 && a->dtype != B200K_F16 && a->dtype != B200K_BF16) return B200K_ERR_UNSUPPORTED;
+  if (a->weight && a->w_dtype != B200K_F32 && a->w_dtype != B200K_F16 && a->w_dtype != B200K_BF16)
+    return B200K_ERR_UNSUPPORTED;
+  if (a->flags & ~(B200K_ROWF_ROUND_NORMED | B200K_ROWF_WEIGHT_PLUS_ONE)) return B200K_ERR_UNSUPPORTED;
+  const int quant = a->out_dtype == B200K_E4M3 ? (a->group == 0 ? 1 : 2) : 0;
+  if (quant == 0 && a->out_dtype != a->dtype) return B200K_ERR_UNSUPPORTED;
+  if (quant != 0 && !a->scale) return B200K_ERR_ARG;
+  if (quant == 2 && (a->group != 128 || a->cols % 128 != 0)) return B200K_ERR_SHAPE;
+  AddNormParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.rows = a->rows;
+  p.cols = static_cast<int32_t>(a->cols);
+  p.x = a->x;
+  p.r = a->residual;
+  p.w = a->weight;
+  p.h = a->sum;
+  p.out = a->out;
+  p.scale = a->scale;
+  p.x_stride = a->x_row_stride;
+  p.r_stride = a->residual_row_stride;
+  p.eps = a->eps;
+  p.w_dt = a->w_dtype;
+  p.flags = a->flags;
+  // 8 columns a thread: 16-byte (fp32: two) loads of whole vectors
+  const bool vec = a->cols % 8 == 0 && a->x_row_stride % 8 == 0 && a->residual_row_stride % 8 == 0 &&
+                   aligned16(a->x) && aligned16(a->residual) && aligned16(a->sum) && aligned16(a->out) &&
+                   (!a->weight || aligned16(a->weight));
+  cudaStream_t st = static_cast<cudaStream_t>(stream_);
+  if (a->dtype == B200K_BF16) launch_quant<B200K_BF16>(p, quant, vec, st);
+  else if (a->dtype == B200K_F16) launch_quant<B200K_F16>(p, quant, vec, st);
+  else launch_quant<B200K_F32>(p, quant, vec, st);
+  return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+}

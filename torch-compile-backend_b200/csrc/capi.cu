@@ -12,6 +12,7 @@ extern "C" const char* b200k_status_string(int code) {
     case B200K_ERR_TIMEOUT: return "device-side wait timed out";
     case B200K_ERR_PROGRAM: return "malformed epilogue program";
     case B200K_ERR_DEVICE: return "no usable CUDA device";
+    case B200K_ERR_INDEX: return "an index read on the device is out of range";
     default: return "unknown b200k status";
   }
 }

@@ -1,0 +1,99 @@
+// What the kernels of b200k_paged_attention share: the launch parameters, how
+// a sequence's work is read from the index tensors, and the score transform.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200k {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kKeys = 16;      // keys of one step of the row kernel (one MMA k)
+constexpr int kRows = 16;      // query rows of one unit of the row kernel (one MMA m)
+
+struct Params {
+  int32_t T, B, H, Hkv, G;     // G = H / Hkv
+  int32_t page_size, num_pages, table_cols;
+  int32_t capacity;            // table_cols * page_size, clamped to int32
+  int32_t window;              // 0: none
+  int32_t long_rows;           // sequences of more query rows (queries * G) run the tile kernel
+  int32_t combine_rows;        // tokens of a sequence that the combine grid covers side by side
+  FastDiv div_page, div_g;
+  int64_t table_stride;
+  const uint16_t* q;
+  int64_t q_t, q_h;
+  const uint16_t *k, *v;
+  int64_t c_page, c_slot, c_head;
+  uint16_t* out;               // [T, H, D] contiguous
+  const int32_t *table, *q_start, *kv_len;
+  // base-2 scores: y = x * mul, or with a cap y = cap2 - 2 cap2 / (1 + 2^(x mul)) = cap2 tanh(x scale / cap)
+  float mul, cap2;
+  float* part_o;               // [workers][2][16][D]
+  float* part_ml;              // [workers][2][16][2]: running max (base 2) and sum
+  int64_t* prefix;             // [B + 1] steps before each sequence; [B + 1]: steps a worker takes
+  int32_t workers;
+  int32_t* status;
+  int64_t timeout_ns;
+};
+
+// One sequence's queries and keys, clamped to the tensors that hold them.
+struct Seq {
+  int t0, m;     // first token, queries
+  int n;         // keys
+  int first;     // position of the first query (may be negative: queries without keys)
+  int lo;        // first key that any query sees
+};
+
+__device__ __forceinline__ Seq seq_at(const Params& p, int b) {
+  Seq s;
+  const int a0 = __ldg(p.q_start + b), a1 = __ldg(p.q_start + b + 1), n = __ldg(p.kv_len + b);
+  s.t0 = min(max(a0, 0), p.T);
+  s.m = min(max(a1, s.t0), p.T) - s.t0;
+  s.n = min(max(n, 0), p.capacity);
+  if ((s.t0 != a0 || s.t0 + s.m != a1 || s.n != n) && p.status) atomicCAS(p.status, 0, B200K_ERR_INDEX);
+  s.first = s.n - s.m;
+  s.lo = p.window > 0 ? max(0, s.first - p.window + 1) : 0;
+  return s;
+}
+
+// Offset of a key's row in the caches, or -1: not between lo and n (nothing
+// there is read: the pages may hold anything), or a page that does not exist.
+__device__ __forceinline__ int64_t key_offset(const Params& p, int b, int key, int lo, int n, int kvh) {
+  if (key < lo || key >= n) return -1;
+  const uint32_t pi = fdiv(static_cast<uint32_t>(key), p.div_page);
+  const int page = __ldg(p.table + b * p.table_stride + pi);
+  if (page < 0 || page >= p.num_pages) {
+    if (p.status) atomicCAS(p.status, 0, B200K_ERR_INDEX);
+    return -1;
+  }
+  return static_cast<int64_t>(page) * p.c_page +
+         static_cast<int64_t>(static_cast<uint32_t>(key) - pi * static_cast<uint32_t>(p.page_size)) * p.c_slot +
+         static_cast<int64_t>(kvh) * p.c_head;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool CAP>
+__device__ __forceinline__ float score(const Params& p, float x) {
+  if (!CAP) return x * p.mul;
+  return fmaf(-2.0f * p.cap2, rcp(1.0f + ex2(x * p.mul)), p.cap2);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+}  // namespace paged
+}  // namespace b200k

@@ -1,0 +1,585 @@
+// Attention over a paged key/value cache (b200k_paged_attention,
+// include/b200k.h): packed queries of ragged sequences against each
+// sequence's pages.
+//
+//   out[t, h] = sum_j softmax_j(f(scale q[t, h] . k_j)) v_j,  f(s) = s or cap tanh(s / cap),
+//   j over the keys max(0, pos - window + 1) .. pos of the token's sequence,
+//   pos = kv_len - queries + index of the token among them
+//
+// No reference counterpart (it leaves attention to ATen and has no cache).
+//
+// The row kernel (this file), for single tokens and few queries a sequence:
+// bound by HBM, it reads each visible key and value once for the G query
+// heads that share it.  Work is one long list of steps, a step being 16 keys
+// of one unit (sequence, kv head, 16 query rows = queries x G heads); every
+// warp takes an equal run of the list, so ragged lengths balance to one step
+// whatever their order, and a single long sequence spreads over the GPU.
+// A warp streams its steps' rows of K and V into its own shared-memory ring
+// with 16-byte cp.async copies (S - 1 steps ahead, across unit boundaries; no
+// block-wide barrier anywhere), multiplies with m16n8k16 MMAs (16 rows by 8
+// keys, rows beyond the unit's are zero: the tensor pipe has the time, the
+// memory does not) and keeps its running maximum, sum and output in fp32.
+// A unit inside one run is written at once; a cut one leaves its parts
+// (max, sum, unnormalised output, fp32) in the workspace, and
+// combine_kernel joins them in the order of the keys.
+#include <algorithm>
+#include <cstring>
+
+#include "host_common.h"
+#include "paged.cuh"
+
+namespace b200k {
+namespace paged {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kCtasPerSm = 2;
+constexpr uint32_t kRingBytes = 24576;  // of one warp
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A sequence as the row kernel cuts it: `units` of `tiles` steps each.
+struct Work {
+  Seq s;
+  int base;   // first key of step 0 (lo rounded down to a step)
+  int tiles;  // 0: no keys, no queries, or the tile kernel's
+  int rts;    // 16-row blocks of a kv head
+};
+__device__ __forceinline__ Work work_at(const Params& p, int b) {
+  Work w;
+  w.s = seq_at(p, b);
+  w.base = w.s.lo & ~(kKeys - 1);
+  const int64_t rows = static_cast<int64_t>(w.s.m) * p.G;
+  w.rts = static_cast<int>((rows + kRows - 1) / kRows);
+  w.tiles = (w.s.m > 0 && w.s.n > w.base && rows <= p.long_rows) ? (w.s.n - w.base + kKeys - 1) / kKeys : 0;
+  return w;
+}
+__device__ __forceinline__ int64_t steps_of(const Params& p, const Work& w) {
+  return static_cast<int64_t>(p.Hkv) * w.rts * w.tiles;
+}
+__device__ __forceinline__ int64_t warp_add(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// A position in the list of steps.
+struct Cursor {
+  Work w;
+  int b, unit, tile;
+  __device__ __forceinline__ void next(const Params& p) {
+    if (++tile < w.tiles) return;
+    tile = 0;
+    if (++unit < p.Hkv * w.rts) return;
+    unit = 0;
+    do {
+      if (++b >= p.B) return;
+      w = work_at(p, b);
+    } while (w.tiles == 0 || w.rts == 0);
+  }
+  __device__ __forceinline__ int kvh() const { return unit / w.rts; }
+  __device__ __forceinline__ int rt() const { return unit % w.rts; }
+};
+
+template <bool BF16, int D, bool CAP>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __grid_constant__ Params p) {
+  constexpr int S = kRingBytes / (kKeys * D * 4);  // ring stages: K and V rows of a step each
+  constexpr uint32_t kRowBytes = D * 2, kTile = kKeys * kRowBytes;
+  constexpr int kChunks = D / 8;          // 16-byte chunks of a row
+  constexpr int kRowsPerCp = 32 / kChunks;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int worker = blockIdx.x * kWarps + warp;
+  const uint32_t ring = smem_addr(smem) + warp * kRingBytes;
+
+  // The whole list's length and, from it, this worker's run [w0, w1).
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    int64_t mine = 0;
+    if (b0 + lane < p.B) mine = steps_of(p, work_at(p, b0 + lane));
+    if (worker == 0) {  // for combine_kernel
+      const int64_t upto = warp_scan(mine);
+      if (b0 + lane < p.B) p.prefix[b0 + lane] = total + upto - mine;
+    }
+    total += warp_add(mine);
+  }
+  const int64_t run = (total + p.workers - 1) / p.workers;
+  if (worker == 0 && lane == 0) {
+    p.prefix[p.B] = total;
+    p.prefix[p.B + 1] = run;
+  }
+  const int64_t w0 = run * worker, w1 = min(total, w0 + run);
+  if (w0 >= w1) return;
+  Cursor cur;
+  cur.b = 0;
+  int64_t seq0 = 0;  // the list's index of cur.b's first step
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    int64_t mine = 0;
+    if (b0 + lane < p.B) mine = steps_of(p, work_at(p, b0 + lane));
+    const int64_t upto = warp_scan(mine);
+    const unsigned hit = __ballot_sync(0xffffffffu, seq0 + upto > w0);
+    if (hit) {
+      const int at = __ffs(hit) - 1;
+      cur.b = b0 + at;
+      seq0 += __shfl_sync(0xffffffffu, upto - mine, at);
+      break;
+    }
+    seq0 += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  cur.w = work_at(p, cur.b);
+  cur.unit = static_cast<int>((w0 - seq0) / cur.w.tiles);
+  cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(cur.unit) * cur.w.tiles);
+
+  Cursor ld = cur;
+  int64_t ld_t = w0;
+  // offset in the caches of the key this lane looks up for the next step loaded
+  auto lookup = [&]() -> int64_t {
+    if (ld_t >= w1) return -1;
+    return key_offset(p, ld.b, ld.w.base + ld.tile * kKeys + (lane & (kKeys - 1)), ld.w.s.lo, ld.w.s.n, ld.kvh());
+  };
+  int64_t off = lookup();
+  auto issue = [&](int stage) {
+    if (ld_t < w1) {
+      const uint32_t sk = ring + stage * 2 * kTile, sv = sk + kTile;
+      const int c = lane % kChunks;
+#pragma unroll
+      for (int i = 0; i < kKeys / kRowsPerCp; ++i) {
+        const int row = i * kRowsPerCp + lane / kChunks;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row);
+        const bool real = o >= 0;
+        const int64_t e = (real ? o : 0) + c * 8;
+        const uint32_t d = row * kRowBytes + ((c ^ (row & 7)) << 4);
+        cp16(sk + d, p.k + e, real);
+        cp16(sv + d, p.v + e, real);
+      }
+      ++ld_t;
+      if (ld_t < w1) ld.next(p);
+      off = lookup();
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue(s);
+
+  const int g = lane >> 2, quad = lane & 3;
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4];
+  float m[2], l[2];
+  int pos[2], row_first = 0, row_last = 0;
+  bool fresh = true;
+  int stage = 0;
+  int64_t unit0 = seq0 + static_cast<int64_t>(cur.unit) * cur.w.tiles;  // the current unit's first step
+  for (int64_t t = w0; t < w1; ++t) {
+    issue(stage == 0 ? S - 1 : stage - 1);
+    if (fresh) {  // a new unit: its query rows as A fragments
+      fresh = false;
+      const int rows = cur.w.s.m * p.G, r0 = cur.rt() * kRows, kvh = cur.kvh();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = r0 + g + 8 * i;
+        const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
+        const uint16_t* src = p.q + static_cast<int64_t>(cur.w.s.t0 + tok) * p.q_t +
+                              static_cast<int64_t>(kvh * p.G + (r - tok * p.G)) * p.q_h + quad * 2;
+        pos[i] = cur.w.s.first + static_cast<int>(tok);
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][i] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+          qf[k][2 + i] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+        }
+      }
+      row_first = cur.w.s.first + static_cast<int>(fdiv(static_cast<uint32_t>(r0), p.div_g));
+      row_last = cur.w.s.first + static_cast<int>(fdiv(static_cast<uint32_t>(min(r0 + kRows, rows) - 1), p.div_g));
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    }
+    cp_wait<S - 1>();
+    __syncwarp();
+    const uint32_t sk = ring + stage * 2 * kTile, sv = sk + kTile;
+    float s[2][4] = {};
+    {
+      // matrices: keys 0-7 / 8-15 by halves of the lanes, d chunk by quarters
+      const int row = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t kb[4];
+        ldm4(kb, sk + row * kRowBytes + (((k * 2 + ch) ^ (row & 7)) << 4));
+        mma<BF16>(s[0], qf[k], kb[0], kb[1]);
+        mma<BF16>(s[1], qf[k], kb[2], kb[3]);
+      }
+    }
+    const int key0 = cur.w.base + cur.tile * kKeys;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = score<CAP>(p, s[n][i]);
+    if (key0 + kKeys - 1 > row_first || (p.window > 0 && key0 <= row_last - p.window)) {  // warp-uniform
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + n * 8 + quad * 2 + (i & 1), at = pos[i >> 1];
+          if (key > at || (p.window > 0 && key <= at - p.window)) s[n][i] = -INFINITY;
+        }
+    }
+    float alpha[2];
+    bool moved = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      const float was = m[i];
+      m[i] = fmaxf(was, x);
+      const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+      alpha[i] = ex2(was - ref);
+      moved |= m[i] != was;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[n][2 * i] = ex2(s[n][2 * i] - ref);
+        s[n][2 * i + 1] = ex2(s[n][2 * i + 1] - ref);
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) l[i] *= alpha[i];
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][0] *= alpha[0];
+        o[n][1] *= alpha[0];
+        o[n][2] *= alpha[1];
+        o[n][3] *= alpha[1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) l[i] += (s[0][2 * i] + s[0][2 * i + 1]) + (s[1][2 * i] + s[1][2 * i + 1]);
+    // probabilities rounded to the input type for the second product (the
+    // sum keeps fp32): half a step each, as b200k_attention
+    const uint32_t pa[4] = {pack16<BF16>(s[0][0], s[0][1]), pack16<BF16>(s[0][2], s[0][3]),
+                            pack16<BF16>(s[1][0], s[1][1]), pack16<BF16>(s[1][2], s[1][3])};
+    {
+      const int row = lane & 15, ch = lane >> 4;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t vb[4];
+        ldm4t(vb, sv + row * kRowBytes + (((n * 2 + ch) ^ (row & 7)) << 4));
+        mma<BF16>(o[2 * n], pa, vb[0], vb[1]);
+        mma<BF16>(o[2 * n + 1], pa, vb[2], vb[3]);
+      }
+    }
+    __syncwarp();  // the stage is free
+    stage = stage + 1 == S ? 0 : stage + 1;
+
+    const bool unit_ends = cur.tile + 1 == cur.w.tiles;
+    if (unit_ends || t + 1 == w1) {
+      const int rows = cur.w.s.m * p.G, r0 = cur.rt() * kRows, kvh = cur.kvh();
+      const bool whole = unit0 >= w0 && unit_ends;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const int r = r0 + g + 8 * i;
+        if (r >= rows) continue;
+        if (whole) {
+          const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
+          uint32_t* dst = reinterpret_cast<uint32_t*>(
+              p.out + (static_cast<int64_t>(cur.w.s.t0 + tok) * p.H + kvh * p.G + (r - tok * p.G)) * D + quad * 2);
+          const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) dst[n * 4] = pack16<BF16>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+        } else {
+          const int64_t slot = static_cast<int64_t>(worker) * 2 + (unit0 < w0 ? 0 : 1);
+          const int64_t at = slot * kRows + g + 8 * i;
+          if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[i], l[i]);
+          float2* dst = reinterpret_cast<float2*>(p.part_o + at * D + quad * 2);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) dst[n * 4] = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        }
+      }
+      fresh = true;
+      unit0 = t + 1;
+    }
+    if (t + 1 < w1) cur.next(p);
+  }
+  cp_wait<0>();
+}
+
+// Joins the parts of the units that were cut, and writes zeros for the rows
+// that no step covers: queries without keys and tokens behind the last
+// sequence.  A CTA per (sequence, token, kv head), 8 warps over its G rows.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
+  constexpr int V = D / 32;  // columns of a lane
+  __shared__ float sh_o[8][D];
+  __shared__ float2 sh_ml[8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int kvh = blockIdx.x % p.Hkv, y = blockIdx.x / p.Hkv % p.combine_rows;
+  const int b = blockIdx.x / p.Hkv / p.combine_rows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto out_row = [&](int64_t tok, int h) { return p.out + (tok * p.H + h) * D; };
+  {  // tokens behind the last sequence
+    const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
+    const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(end, 0));
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < words; i += gridDim.x * 256ll) dst[i] = 0u;
+  }
+  const Work w = work_at(p, b);
+  if (static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
+  const int64_t seq0 = p.prefix[b], run = p.prefix[p.B + 1];
+  const int share = p.G >= 8 ? 1 : 8 / p.G;  // warps of a row
+  for (int i = y; i < w.s.m; i += p.combine_rows) {
+    for (int g0 = 0; g0 < p.G; g0 += 8 / share) {
+      const int g = g0 + warp / share, part = warp % share;
+      const bool mine = g < p.G && warp < share * (8 / share);
+      const int r = i * p.G + g;
+      int64_t u0 = 0, first = 0, last = 0;
+      if (mine && w.tiles > 0) {
+        u0 = seq0 + (static_cast<int64_t>(kvh) * w.rts + r / kRows) * w.tiles;
+        first = u0 / run;
+        last = min(static_cast<int64_t>(p.workers) - 1, (u0 + w.tiles - 1) / run);
+      }
+      float mx = -INFINITY, sum = 0.0f, acc[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+      if (mine && last > first) {
+        // parts in key order, `share` warps in turn
+#pragma unroll 4
+        for (int64_t wk = first + part; wk <= last; wk += share) {
+          const int64_t at = (wk * 2 + (u0 < wk * run ? 0 : 1)) * kRows + r % kRows;
+          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+          float x[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) x[j] = p.part_o[at * D + j * 32 + lane];
+          const float nm = fmaxf(mx, ml.x), ref = nm == -INFINITY ? 0.0f : nm;
+          const float a = ex2(mx - ref), c = ex2(ml.x - ref);
+          mx = nm;
+          sum = sum * a + ml.y * c;
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] = acc[j] * a + x[j] * c;
+        }
+      }
+      if (share > 1) {
+        __syncthreads();
+        if (lane == 0) sh_ml[warp] = make_float2(mx, sum);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sh_o[warp][j * 32 + lane] = acc[j];
+        __syncthreads();
+        if (part == 0 && mine) {
+          for (int k = 1; k < share; ++k) {
+            const float2 ml = sh_ml[warp + k];
+            const float nm = fmaxf(mx, ml.x), ref = nm == -INFINITY ? 0.0f : nm;
+            const float a = ex2(mx - ref), c = ex2(ml.x - ref);
+            mx = nm;
+            sum = sum * a + ml.y * c;
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = acc[j] * a + sh_o[warp + k][j * 32 + lane] * c;
+          }
+        }
+      }
+      if (mine && part == 0 && (w.tiles == 0 || last > first)) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t* dst = out_row(w.s.t0 + i, kvh * p.G + g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const uint32_t u = pack16<BF16>(acc[j] * inv, 0.0f);
+          dst[j * 32 + lane] = static_cast<uint16_t>(u);
+        }
+      }
+    }
+  }
+}
+
+template <bool BF16, int D, bool CAP>
+int launch(const Params& p, int ctas, cudaStream_t st) {
+  constexpr uint32_t kSmem = kWarps * kRingBytes;
+  auto kernel = rows_kernel<BF16, D, CAP>;
+  // cheap, and per device: set on every call rather than remembered
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    return B200K_ERR_LAUNCH;
+  kernel<<<ctas, kWarps * 32, kSmem, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return B200K_ERR_LAUNCH;
+  // The combine's launch overlaps the row kernel's end (it waits for the
+  // row kernel's writes itself, before it reads or writes anything).
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.combine_rows * p.Hkv));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel<BF16, D>, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+}
+
+template <bool BF16, int D>
+int launch_cap(const Params& p, bool cap, int ctas, cudaStream_t st) {
+  return cap ? launch<BF16, D, true>(p, ctas, st) : launch<BF16, D, false>(p, ctas, st);
+}
+
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace paged
+}  // namespace b200k
+
+using namespace b200k;
+using namespace b200k::paged;
+
+namespace {
+
+int check_shape(const B200kPagedAttentionArgs* a) {
+  if (!a) return B200K_ERR_ARG;
+  if (a->tokens < 0 || a->seqs < 0 || a->heads < 0 || a->kv_heads < 0 || a->num_pages < 0 || a->page_size < 0 ||
+      a->table_cols < 0)
+    return B200K_ERR_SHAPE;
+  if (a->tokens == 0 || a->heads == 0) return B200K_OK;  // empty output
+  if (a->head_dim != 64 && a->head_dim != 128) return B200K_ERR_UNSUPPORTED;
+  if (a->kv_heads == 0 || a->heads % a->kv_heads != 0) return B200K_ERR_SHAPE;
+  if (a->tokens > 0x3fffffffLL || a->seqs > 0xffffffLL || a->heads > 65536 || a->page_size > 0x3fffffffLL ||
+      a->num_pages > 0x3fffffffLL || a->table_cols > 0x3fffffffLL || a->tokens * (a->heads / a->kv_heads) > 0x3fffffffLL)
+    return B200K_ERR_SHAPE;
+  return B200K_OK;
+}
+
+int64_t workspace_bytes(const B200kPagedAttentionArgs* a, int sms) {
+  const int64_t slots = static_cast<int64_t>(sms) * kCtasPerSm * kWarps * 2 * kRows;
+  return align256(slots * a->head_dim * 4) + align256(slots * 8) + align256((a->seqs + 2) * 8);
+}
+
+}  // namespace
+
+extern "C" int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* a, int64_t* bytes) {
+  const int rc = check_shape(a);
+  if (rc != B200K_OK) return rc;
+  if (!bytes) return B200K_ERR_ARG;
+  *bytes = 0;
+  if (a->tokens == 0 || a->heads == 0) return B200K_OK;
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200K_ERR_DEVICE;
+  *bytes = workspace_bytes(a, sms);
+  return B200K_OK;
+}
+
+extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* stream_) {
+  const int rc = check_shape(a);
+  if (rc != B200K_OK) return rc;
+  if (a->tokens == 0 || a->heads == 0) return B200K_OK;
+  if (!a->q || !a->out) return B200K_ERR_ARG;
+  if (a->dtype != B200K_BF16 && a->dtype != B200K_F16) return B200K_ERR_UNSUPPORTED;
+  if (!(a->softcap >= 0.0f) || a->window < 0 || !(a->scale == a->scale)) return B200K_ERR_ARG;
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out)) return B200K_ERR_ALIGN;
+  for (int d = 0; d < 2; ++d)
+    if (a->q_strides[d] < 0 || a->q_strides[d] % 8) return B200K_ERR_ALIGN;
+  for (int d = 0; d < 3; ++d)
+    if (a->cache_strides[d] < 0 || a->cache_strides[d] % 8) return B200K_ERR_ALIGN;
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200K_ERR_DEVICE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream_);
+  const int64_t keys = std::min<int64_t>(a->table_cols * a->page_size, 0x3fffffff);
+  if (a->seqs == 0 || keys == 0 || a->num_pages == 0) {  // no keys at all: every row is zero
+    const size_t n = static_cast<size_t>(a->tokens) * a->heads * a->head_dim * 2;
+    return cudaMemsetAsync(a->out, 0, n, st) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+  }
+  if (!a->k_cache || !a->v_cache || !a->page_table || !a->q_start || !a->kv_len) return B200K_ERR_ARG;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < workspace_bytes(a, sms)) return B200K_ERR_ARG;
+  Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.T = static_cast<int32_t>(a->tokens);
+  p.B = static_cast<int32_t>(a->seqs);
+  p.H = static_cast<int32_t>(a->heads);
+  p.Hkv = static_cast<int32_t>(a->kv_heads);
+  p.G = p.H / p.Hkv;
+  p.page_size = static_cast<int32_t>(a->page_size);
+  p.num_pages = static_cast<int32_t>(a->num_pages);
+  p.table_cols = static_cast<int32_t>(a->table_cols);
+  p.capacity = static_cast<int32_t>(keys);
+  p.window = static_cast<int32_t>(std::min<int64_t>(a->window, 0x3fffffff));
+  p.long_rows = 0x7fffffff;
+  p.div_page = make_fastdiv(static_cast<uint32_t>(p.page_size));
+  p.div_g = make_fastdiv(static_cast<uint32_t>(p.G));
+  p.table_stride = a->table_stride;
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_t = a->q_strides[0];
+  p.q_h = a->q_strides[1];
+  p.k = static_cast<const uint16_t*>(a->k_cache);
+  p.v = static_cast<const uint16_t*>(a->v_cache);
+  p.c_page = a->cache_strides[0];
+  p.c_slot = a->cache_strides[1];
+  p.c_head = a->cache_strides[2];
+  p.out = static_cast<uint16_t*>(a->out);
+  p.table = a->page_table;
+  p.q_start = a->q_start;
+  p.kv_len = a->kv_len;
+  const bool cap = a->softcap > 0.0f;
+  const float scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
+  p.mul = cap ? 2.0f * scale / a->softcap * kLog2e : scale * kLog2e;
+  p.cap2 = a->softcap * kLog2e;
+  const int ctas = sms * kCtasPerSm;
+  p.workers = ctas * kWarps;
+  const int64_t slots = static_cast<int64_t>(p.workers) * 2 * kRows;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  ws += align256(slots * a->head_dim * 4);
+  p.part_ml = reinterpret_cast<float*>(ws);
+  ws += align256(slots * 8);
+  p.prefix = reinterpret_cast<int64_t*>(ws);
+  p.status = a->status;
+  p.timeout_ns = a->timeout_ns > 0 ? a->timeout_ns : 2000000000ll;
+  // The combine covers this many tokens of a sequence side by side and the
+  // rest in a loop; its grid stays below 2^31 CTAs.
+  const int64_t hint = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
+  p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(hint, 0x3fffffff / (static_cast<int64_t>(p.B) * p.Hkv))));
+  if (static_cast<int64_t>(p.B) * p.Hkv > 0x3fffffffLL) return B200K_ERR_SHAPE;
+  if (a->dtype == B200K_BF16)
+    return a->head_dim == 64 ? launch_cap<true, 64>(p, cap, ctas, st) : launch_cap<true, 128>(p, cap, ctas, st);
+  return a->head_dim == 64 ? launch_cap<false, 64>(p, cap, ctas, st) : launch_cap<false, 128>(p, cap, ctas, st);
+}

@@ -314,6 +314,8 @@ int64_t status_check(int64_t device, bool arm) {
   }
   if (seen != 0) {
     word.zero_();
+    TORCH_CHECK(seen != B200K_ERR_INDEX, "b200::rope_append or paged_attention on cuda:", dev, " reported ",
+                b200k_status_string(static_cast<int>(seen)), " (code ", seen, ")");
     TORCH_CHECK(false, "b200::gemm_epilogue on cuda:", dev, " reported ", b200k_status_string(static_cast<int>(seen)),
                 " (code ", seen, "): an earlier GEMM's output is incomplete");
   }
@@ -539,6 +541,248 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   return out;
 }
 
+// ------------------------------------------------- paged-cache serving ops
+// These ops have no gradient: an input that asks for one is refused rather
+// than answered with a result that is cut off from it.
+void no_grad_inputs(const char* what, std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), "b200::", what, ": no gradient is defined; call it under torch.no_grad()");
+}
+
+// The device's status word, or null when it does not exist yet and cannot be
+// made because `st` is capturing.
+int32_t* status_ptr(int dev, void* st) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  const bool capturing =
+      cudaStreamIsCapturing(static_cast<cudaStream_t>(st), &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone;
+  static std::mutex mu;
+  static std::vector<int32_t*> known;
+  std::lock_guard<std::mutex> lock(mu);
+  if (static_cast<int>(known.size()) <= dev) known.resize(dev + 1, nullptr);
+  if (!known[dev] && !capturing) known[dev] = status_word(dev).data_ptr<int32_t>();
+  return known[dev];
+}
+
+void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r_in,
+                   const c10::optional<at::Tensor>& weight, double eps, int64_t flags, int64_t group, bool quant,
+                   at::Tensor& out, at::Tensor& scale, at::Tensor& sum) {
+  TORCH_CHECK(x_in.is_cuda(), "b200::", what, ": x must be a CUDA tensor");
+  TORCH_CHECK(x_in.dim() >= 1 && x_in.sizes() == r_in.sizes(), "b200::", what, ": x ", x_in.sizes(), " and residual ",
+              r_in.sizes(), " differ in shape");
+  TORCH_CHECK(r_in.device() == x_in.device() && r_in.scalar_type() == x_in.scalar_type(), "b200::", what,
+              ": x and residual differ in dtype or device");
+  no_grad_inputs(what, {&x_in, &r_in});
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const int64_t cols = x_in.size(-1);
+  // rows that do not flatten to one stride, or columns that are apart, are copied
+  auto rows_view = [&](const at::Tensor& t) {
+    bool ok = t.stride(-1) == 1 || cols == 1;
+    for (int64_t d = t.dim() - 3; d >= 0 && ok; --d)
+      ok = t.size(d) == 1 || t.stride(d) == t.stride(d + 1) * t.size(d + 1);
+    return ok ? t : t.contiguous();
+  };
+  const at::Tensor x = rows_view(x_in), r = rows_view(r_in);
+  B200kAddNormArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.cols = cols;
+  a.rows = cols == 0 ? 0 : x.numel() / cols;
+  a.x = x.data_ptr();
+  a.residual = r.data_ptr();
+  a.x_row_stride = x.dim() >= 2 ? x.stride(-2) : cols;
+  a.residual_row_stride = r.dim() >= 2 ? r.stride(-2) : cols;
+  a.dtype = to_dt(x.scalar_type());
+  at::Tensor w;
+  if (weight.has_value() && weight->defined()) {
+    TORCH_CHECK(weight->device() == x.device() && weight->dim() == 1 && weight->size(0) == cols, "b200::", what,
+                ": weight must be [", cols, "] on x's device");
+    no_grad_inputs(what, {&*weight});
+    w = weight->contiguous();
+    a.weight = w.data_ptr();
+    a.w_dtype = to_dt(w.scalar_type());
+  }
+  sum = at::empty(x.sizes(), x.options());
+  if (quant) {
+    TORCH_CHECK(group == 0 || (group == 128 && cols % 128 == 0), "b200::", what,
+                ": group must be 0 (a scale per row) or 128 with columns a multiple of it, got ", group, " for ", cols,
+                " columns");
+    std::vector<int64_t> ss(x.sizes().begin(), x.sizes().end());
+    ss.back() = group == 0 ? 1 : cols / 128;
+    out = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    scale = at::empty(ss, x.options().dtype(at::kFloat));
+    a.scale = scale.data_ptr<float>();
+    a.out_dtype = B200K_E4M3;
+    a.group = static_cast<int32_t>(group);
+  } else {
+    out = at::empty(x.sizes(), x.options());
+    a.out_dtype = a.dtype;
+  }
+  a.flags = static_cast<int32_t>(flags);
+  a.eps = static_cast<float>(eps);
+  a.sum = sum.data_ptr();
+  a.out = out.data_ptr();
+  check(b200k_add_rms_norm(&a, stream_of(x)), what);
+}
+
+std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const at::Tensor& residual,
+                                                const c10::optional<at::Tensor>& weight, double eps, int64_t flags) {
+  at::Tensor out, scale, sum;
+  add_norm_impl("add_rms_norm", x, residual, weight, eps, flags, 0, false, out, scale, sum);
+  return {out, sum};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant(const at::Tensor& x, const at::Tensor& residual,
+                                                                  const c10::optional<at::Tensor>& weight, double eps,
+                                                                  int64_t group, int64_t flags) {
+  at::Tensor out, scale, sum;
+  add_norm_impl("add_rms_norm_quant", x, residual, weight, eps, flags, group, true, out, scale, sum);
+  return {out, scale, sum};
+}
+
+void check_caches(const char* what, const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc) {
+  TORCH_CHECK(kc.dim() == 4 && kc.sizes() == vc.sizes() && kc.strides() == vc.strides(), "b200::", what,
+              ": k_cache and v_cache must be [pages, page size, kv heads, head dim] of one shape and strides, got ",
+              kc.sizes(), " and ", vc.sizes());
+  TORCH_CHECK(kc.scalar_type() == q.scalar_type() && vc.scalar_type() == q.scalar_type(), "b200::", what,
+              ": the caches must have q's dtype");
+  TORCH_CHECK(kc.device() == q.device() && vc.device() == q.device(), "b200::", what, ": the caches must be on q's device");
+  TORCH_CHECK(kc.size(3) == q.size(2) && (kc.stride(3) == 1 || kc.numel() == 0), "b200::", what,
+              ": the caches' last dim must be head_dim with unit stride");
+}
+
+at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                       const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots, at::Tensor k_cache,
+                       at::Tensor v_cache) {
+  const char* what = "rope_append";
+  TORCH_CHECK(q.is_cuda(), "b200::rope_append: q must be a CUDA tensor");
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+              "b200::rope_append: q [tokens, heads, dim], k and v [tokens, kv heads, dim], got ", q.sizes(), ", ", k.sizes(),
+              ", ", v.sizes());
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                  v.device() == q.device(), "b200::rope_append: q, k and v differ in dtype or device");
+  for (const at::Tensor* t : {&q, &k, &v})
+    TORCH_CHECK(t->stride(2) == 1 || t->numel() == 0 || t->size(2) == 1, "b200::rope_append: q, k, v need a unit last-dim stride");
+  check_caches(what, q, k_cache, v_cache);
+  TORCH_CHECK(k_cache.size(2) == k.size(1), "b200::rope_append: the caches have ", k_cache.size(2), " heads, k has ", k.size(1));
+  TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.strides() == sin.strides() &&
+                  cos.scalar_type() == sin.scalar_type() && (cos.stride(1) == 1 || cos.size(1) <= 1) &&
+                  2 * cos.size(1) <= q.size(2),
+              "b200::rope_append: cos and sin must be [rows, rotary dim / 2] alike, at most head_dim / 2 columns of unit "
+              "stride, got ", cos.sizes(), " and ", sin.sizes());
+  TORCH_CHECK(cos.scalar_type() == at::kFloat || cos.scalar_type() == q.scalar_type(),
+              "b200::rope_append: cos and sin must be float32 or q's dtype");
+  TORCH_CHECK(positions.dim() == 1 && slots.dim() == 1 && positions.size(0) == q.size(0) && slots.size(0) == q.size(0),
+              "b200::rope_append: positions and slots must be [", q.size(0), "]");
+  for (const at::Tensor* t : {&positions, &slots})
+    TORCH_CHECK((t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->is_contiguous(),
+                "b200::rope_append: positions and slots must be contiguous int32 or int64");
+  for (const at::Tensor* t : {&cos, &sin, &positions, &slots})
+    TORCH_CHECK(t->device() == q.device(), "b200::rope_append: every tensor must be on q's device");
+  no_grad_inputs(what, {&q, &k, &v, &cos, &sin, &k_cache, &v_cache});
+  // a cache that overlaps itself (expanded) has several elements in one place
+  TORCH_CHECK(k_cache.numel() == 0 || k_cache.is_non_overlapping_and_dense() || [&] {
+    for (int d = 0; d < 4; ++d) if (k_cache.size(d) > 1 && k_cache.stride(d) == 0) return false;
+    return true;
+  }(), "b200::rope_append: the caches must not be expanded");
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  B200kRopeAppendArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.tokens = q.size(0);
+  a.heads = q.size(1);
+  a.kv_heads = k.size(1);
+  a.head_dim = q.size(2);
+  a.rot_dim = 2 * cos.size(1);
+  a.num_pages = k_cache.size(0);
+  a.page_size = k_cache.size(1);
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.q_out = out.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  for (int d = 0; d < 2; ++d) {
+    a.q_strides[d] = q.stride(d);
+    a.k_strides[d] = k.stride(d);
+    a.v_strides[d] = v.stride(d);
+  }
+  for (int d = 0; d < 3; ++d) a.cache_strides[d] = k_cache.stride(d);
+  a.cos = cos.data_ptr();
+  a.sin = sin.data_ptr();
+  a.table_rows = cos.size(0);
+  a.table_stride = cos.stride(0);
+  a.positions = positions.data_ptr();
+  a.slots = slots.data_ptr();
+  a.dtype = to_dt(q.scalar_type());
+  a.table_dtype = to_dt(cos.scalar_type());
+  a.positions_dtype = to_dt(positions.scalar_type());
+  a.slots_dtype = to_dt(slots.scalar_type());
+  void* st = stream_of(q);
+  a.status = status_ptr(q.device().index(), st);
+  check(b200k_rope_append(&a, st), what);
+  for (at::Tensor* t : {&k_cache, &v_cache})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& page_table, const at::Tensor& q_start, const at::Tensor& kv_len, double scale,
+                           double softcap, int64_t window, int64_t max_q_len) {
+  const char* what = "paged_attention";
+  TORCH_CHECK(q.is_cuda(), "b200::paged_attention: q must be a CUDA tensor");
+  TORCH_CHECK(q.dim() == 3 && (q.stride(2) == 1 || q.numel() == 0), "b200::paged_attention: q must be [tokens, heads, head dim] "
+              "with unit last-dim stride, got ", q.sizes());
+  check_caches(what, q, k_cache, v_cache);
+  TORCH_CHECK(page_table.dim() == 2 && q_start.dim() == 1 && kv_len.dim() == 1 && q_start.size(0) == kv_len.size(0) + 1 &&
+                  page_table.size(0) == kv_len.size(0),
+              "b200::paged_attention: page_table [seqs, pages], q_start [seqs + 1], kv_len [seqs], got ", page_table.sizes(),
+              ", ", q_start.sizes(), ", ", kv_len.sizes());
+  for (const at::Tensor* t : {&page_table, &q_start, &kv_len})
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->device() == q.device() && (t->size(-1) <= 1 || t->stride(-1) == 1),
+                "b200::paged_attention: page_table, q_start and kv_len must be int32 on q's device with unit last-dim stride");
+  TORCH_CHECK(page_table.stride(0) >= 0, "b200::paged_attention: page_table stride");
+  TORCH_CHECK(softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::paged_attention: softcap, window and max_q_len must not "
+              "be negative");
+  no_grad_inputs(what, {&q, &k_cache, &v_cache});
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  B200kPagedAttentionArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.tokens = q.size(0);
+  a.seqs = kv_len.size(0);
+  a.heads = q.size(1);
+  a.kv_heads = k_cache.size(2);
+  a.head_dim = q.size(2);
+  a.num_pages = k_cache.size(0);
+  a.page_size = k_cache.size(1);
+  a.table_cols = page_table.size(1);
+  a.table_stride = page_table.stride(0);
+  a.q = q.data_ptr();
+  for (int d = 0; d < 2; ++d) a.q_strides[d] = q.stride(d);
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  for (int d = 0; d < 3; ++d) a.cache_strides[d] = k_cache.stride(d);
+  a.out = out.data_ptr();
+  a.page_table = page_table.data_ptr<int32_t>();
+  a.q_start = q_start.data_ptr<int32_t>();
+  a.kv_len = kv_len.data_ptr<int32_t>();
+  a.max_q_len = max_q_len;
+  a.window = window;
+  a.scale = static_cast<float>(scale);
+  a.softcap = static_cast<float>(softcap);
+  a.dtype = to_dt(q.scalar_type());
+  void* st = stream_of(q);
+  // Parts of cut units: the caching allocator's, so each call and each
+  // captured graph has its own.
+  int64_t bytes = 0;
+  check(b200k_paged_attention_workspace(&a, &bytes), what);
+  const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = bytes;
+  a.status = status_ptr(q.device().index(), st);
+  check(b200k_paged_attention(&a, st), what);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(b200, m) {
@@ -558,6 +802,16 @@ TORCH_LIBRARY(b200, m) {
   m.def("rope(Tensor x, Tensor cos, Tensor sin, int[] out_stride=[]) -> Tensor");
   m.def("gemm_rope(Tensor a, Tensor b, Tensor cos, Tensor sin, int period, int[] out_shape) -> Tensor");
   m.def("attention(Tensor q, Tensor k, Tensor v, bool causal, float scale, int[] out_stride=[]) -> Tensor");
+  m.def("add_rms_norm(Tensor x, Tensor residual, Tensor? weight, float eps, int flags=0) -> (Tensor, Tensor)");
+  m.def(
+      "add_rms_norm_quant(Tensor x, Tensor residual, Tensor? weight, float eps, int group=0, int flags=0) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def(
+      "rope_append(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor positions, Tensor slots, "
+      "Tensor(a!) k_cache, Tensor(b!) v_cache) -> Tensor");
+  m.def(
+      "paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor q_start, Tensor kv_len, "
+      "float scale=0.0, float softcap=0.0, int window=0, int max_q_len=0) -> Tensor");
   m.def("gemm_status(int device, bool reset) -> int", &gemm_status);
   m.def("status_check(int device, bool arm) -> int", &status_check);
   m.def("gemm_test_stall_next(int timeout_ns) -> ()", &gemm_test_stall_next);
@@ -574,5 +828,9 @@ TORCH_LIBRARY_IMPL(b200, CUDA, m) {
   m.impl("rope", &rope);
   m.impl("gemm_rope", &gemm_rope);
   m.impl("attention", &attention);
+  m.impl("add_rms_norm", &add_rms_norm);
+  m.impl("add_rms_norm_quant", &add_rms_norm_quant);
+  m.impl("rope_append", &rope_append);
+  m.impl("paged_attention", &paged_attention);
 }
 
