@@ -562,7 +562,8 @@ int b200k_rope_append(const B200kRopeAppendArgs* args, void* stream);
  * is a hint of the longest sequence's queries: it chooses kernels and grids,
  * never results.  Index tensors are i32 on the device; entries out of range
  * are clamped (a page out of range reads as zeros) and set *status (may be
- * NULL) to B200K_ERR_INDEX.  workspace: device memory of
+ * NULL) to B200K_ERR_INDEX; B200K_ERR_TIMEOUT is set when a device-side wait runs out
+ * (timeout_ns, 0 = 2 s).  workspace: device memory of
  * b200k_paged_attention_workspace bytes, 16-byte aligned, for this call
  * alone until it has run.
  */
@@ -588,6 +589,12 @@ typedef struct {
   int32_t* status;
   int64_t timeout_ns;
 } B200kPagedAttentionArgs;
+
+/* Test hook (test_flags bit): in calls that run the tile kernel, the first
+ * score block of its first query tile is not signalled as ready, so a wait
+ * runs out after timeout_ns; the kernel reports B200K_ERR_TIMEOUT, drains and
+ * returns (no fault).  Failure-detection tests only. */
+#define B200K_PAGED_TEST_WITHHOLD_SCORES 1
 
 int b200k_paged_attention(const B200kPagedAttentionArgs* args, void* stream);
 int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* args, int64_t* bytes);

@@ -216,3 +216,43 @@ def test_c_abi():
     assert status.item() == 0
     want, size = ref.paged_attention(*x, ref.default_scale(128))
     ref.attention_close(out, want, size, HF)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q,n,H,hkv", [(64, 64, 8, 2), (1000, 1000, 4, 1), (33, 3000, 8, 8), (513, 700, 2, 2),
+                                       (128, 128, 2, 1), (2000, 100, 2, 1)])
+def test_tile_units(q, n, H, hkv, D, dtype):
+    """Whole and cut units, blocks that end inside a tile, causal tiles of
+    different lengths, more queries than keys."""
+    run(ref.paged_inputs([q], [n], H, hkv, D, 16, dtype))
+
+
+def test_prompts_and_single_tokens_in_one_batch():
+    qs = [1, 500, 1, 3, 77, 0, 1, 260]
+    ns = [900, 600, 1, 40, 77, 12, 2000, 260]
+    run(ref.paged_inputs(qs, ns, 16, 2, 128, 16, BF, pad=9))
+    run(ref.paged_inputs(qs, ns, 16, 2, 128, 16, BF, pad=9), max_q=500)
+    run(ref.paged_inputs(qs, ns, 16, 2, 64, 16, HF), max_q=7)  # a hint that is too small
+
+
+def test_many_prompts():
+    qs = [9 + (i * 13) % 40 for i in range(300)]
+    run(ref.paged_inputs(qs, [n + (i % 7) * 30 for i, n in enumerate(qs)], 8, 1, 64, 16, BF))
+
+
+def test_stalled_wait_times_out_and_context_survives():
+    """The test hook withholds the first score block's signal: a wait runs out
+    after 50 ms, the kernel reports B200K_ERR_TIMEOUT, drains and returns,
+    and the next call is right."""
+    x = ref.paged_inputs([300], [300], 4, 4, 128, 16, BF)
+    out = torch.zeros_like(x[0])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cabi.paged_attention(*x, out, status=status, timeout_ns=50_000_000, test_flags=cabi.PAGED_TEST_WITHHOLD_SCORES)
+    torch.cuda.synchronize()
+    assert status.item() == 6
+    status.zero_()
+    cabi.paged_attention(*x, out, status=status)
+    assert status.item() == 0
+    want, size = ref.paged_attention(*x, ref.default_scale(128))
+    ref.attention_close(out, want, size, BF)

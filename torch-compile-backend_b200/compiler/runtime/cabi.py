@@ -153,6 +153,7 @@ class PagedAttentionArgs(ctypes.Structure):
 
 
 ATTN_TEST_WITHHOLD_SCORES = 1  # include/b200k.h: failure-detection test hook
+PAGED_TEST_WITHHOLD_SCORES = 1
 
 _lib = None
 

@@ -10,6 +10,8 @@ namespace paged {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 16;      // keys of one step of the row kernel (one MMA k)
 constexpr int kRows = 16;      // query rows of one unit of the row kernel (one MMA m)
+constexpr int kBlock = 128;    // keys of one step of the tile kernel
+constexpr int kUnitRows = 256; // query rows of one unit of the tile kernel (two MMA m)
 
 struct Params {
   int32_t T, B, H, Hkv, G;     // G = H / Hkv
@@ -32,6 +34,13 @@ struct Params {
   float* part_ml;              // [workers][2][16][2]: running max (base 2) and sum
   int64_t* prefix;             // [B + 1] steps before each sequence; [B + 1]: steps a worker takes
   int32_t workers;
+  // tile kernel: [0] steps of all units, [1] steps a CTA takes, [2] entries, [3 + e] steps before entry e
+  int64_t* entry_steps;
+  int2* entries;               // (sequence, 256-row block)
+  float* tile_o;               // [CTAs][2][D / 4][256][4]
+  float* tile_ml;              // [CTAs][2][256][2]
+  int32_t tile_ctas;           // 0: not launched
+  int32_t test_flags;
   int32_t* status;
   int64_t timeout_ns;
 };
@@ -55,6 +64,41 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b) {
   s.lo = p.window > 0 ? max(0, s.first - p.window + 1) : 0;
   return s;
 }
+
+// 256 query rows of a sequence, as the tile kernel works on them.
+struct Unit {
+  Seq s;
+  int b, r0, rows;   // first row, rows of the sequence
+  int lo, hi;        // keys that its rows see
+  int ub0, ub1;      // their blocks: at least one, so that rows without keys are written
+};
+// Keys that rows [r0, r1) of a sequence see: [lo, hi), hi <= 0 when none.
+__device__ __forceinline__ void rows_keys(const Params& p, const Seq& s, int r0, int r1, int& lo, int& hi) {
+  const int a = s.first + static_cast<int>(fdiv(static_cast<uint32_t>(r0), p.div_g));
+  const int z = s.first + static_cast<int>(fdiv(static_cast<uint32_t>(r1 - 1), p.div_g));
+  lo = p.window > 0 ? max(0, a - p.window + 1) : 0;
+  hi = z + 1;
+}
+__device__ __forceinline__ Unit unit_at(const Params& p, int b, int qb) {
+  Unit u;
+  u.s = seq_at(p, b);
+  u.b = b;
+  u.r0 = qb * kUnitRows;
+  u.rows = u.s.m * p.G;
+  rows_keys(p, u.s, u.r0, min(u.r0 + kUnitRows, u.rows), u.lo, u.hi);
+  u.ub0 = u.lo / kBlock;
+  u.ub1 = max(u.ub0 + 1, (u.hi + kBlock - 1) / kBlock);
+  return u;
+}
+// Keys of tile t (rows r0 + 128 t ...) of a unit; hi <= 0 for a tile without rows.
+__device__ __forceinline__ void tile_keys(const Params& p, const Unit& u, int t, int& lo, int& hi) {
+  const int a = u.r0 + t * 128;
+  lo = hi = 0;
+  if (a < u.rows) rows_keys(p, u.s, a, min(a + 128, u.rows), lo, hi);
+}
+
+// Launches the tile kernel (paged_tiles.cu) on the plan in p.entries.
+int launch_tiles(const Params& p, bool bf16, int dim, bool cap, cudaStream_t st);
 
 // Offset of a key's row in the caches, or -1: not between lo and n (nothing
 // there is read: the pages may hold anything), or a page that does not exist.

@@ -127,6 +127,68 @@ struct Cursor {
   __device__ __forceinline__ int rt() const { return unit % w.rts; }
 };
 
+// The tile kernel's list: an entry for every 256 query rows of a sequence
+// that is its own, with the steps before it.  One CTA of 128 threads.
+__device__ __noinline__ void plan_tiles(const Params& p) {
+  __shared__ int starts[kWarps * 32 + 1];   // entries before each of 128 sequences
+  __shared__ int64_t sums[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t* before = p.entry_steps + 3;
+  int64_t steps = 0;
+  int entry0 = 0;
+  auto block_scan = [&](int64_t v, int64_t& all) {  // inclusive
+    int64_t x = warp_scan(v);
+    __syncthreads();
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) x += sums[w];
+      all += sums[w];
+    }
+    return x;
+  };
+  for (int b0 = 0; b0 < p.B; b0 += kWarps * 32) {
+    int n = 0;
+    if (b0 + tid < p.B) {
+      const int64_t rows = static_cast<int64_t>(seq_at(p, b0 + tid).m) * p.G;
+      if (rows > p.long_rows) n = static_cast<int>((rows + kUnitRows - 1) / kUnitRows);
+    }
+    int64_t all;
+    const int64_t upto = block_scan(n, all);
+    starts[tid] = static_cast<int>(upto - n);
+    if (tid == 0) starts[kWarps * 32] = static_cast<int>(all);
+    __syncthreads();
+    for (int e0 = 0; e0 < all; e0 += kWarps * 32) {
+      const int e = e0 + tid;
+      int64_t mine = 0;
+      if (e < all) {
+        int lo = 0, hi = kWarps * 32;  // the last sequence with starts <= e
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (starts[mid] <= e) lo = mid;
+          else hi = mid;
+        }
+        const Unit u = unit_at(p, b0 + lo, e - starts[lo]);
+        p.entries[entry0 + e] = make_int2(b0 + lo, e - starts[lo]);
+        mine = static_cast<int64_t>(u.ub1 - u.ub0) * p.Hkv;
+      }
+      int64_t sum;
+      const int64_t x = block_scan(mine, sum);
+      if (e < all) before[entry0 + e] = steps + x - mine;
+      steps += sum;
+    }
+    entry0 += static_cast<int>(all);
+    __syncthreads();
+  }
+  if (tid == 0) {
+    p.entry_steps[0] = steps;
+    p.entry_steps[1] = (steps + p.tile_ctas - 1) / p.tile_ctas;
+    p.entry_steps[2] = entry0;
+    before[entry0] = steps;
+  }
+}
+
 template <bool BF16, int D, bool CAP>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __grid_constant__ Params p) {
   constexpr int S = kRingBytes / (kKeys * D * 4);  // ring stages: K and V rows of a step each
@@ -137,6 +199,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int worker = blockIdx.x * kWarps + warp;
   const uint32_t ring = smem_addr(smem) + warp * kRingBytes;
+  if (worker >= p.workers) {  // the last CTA, when the tile kernel runs
+    plan_tiles(p);
+    return;
+  }
 
   // The whole list's length and, from it, this worker's run [w0, w1).
   int64_t total = 0;
@@ -351,6 +417,60 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   cp_wait<0>();
 }
 
+// Joins the tile kernel's parts of one cut unit.  Boundary i (the start of
+// CTA i's run) belongs to the unit that it cuts when it is the first boundary
+// inside that unit; block y of 8 takes 32 of its 256 rows, a thread one row
+// and every eighth group of 4 columns.
+template <bool BF16, int D>
+__device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
+  const int64_t total = p.entry_steps[0], run = p.entry_steps[1];
+  const int64_t* before = p.entry_steps + 3;
+  const int64_t w = run * i;
+  if (w >= total) return;
+  int lo = 0, hi = static_cast<int>(p.entry_steps[2]);
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (before[mid] <= w) lo = mid;
+    else hi = mid;
+  }
+  const int2 bq = p.entries[lo];
+  const Unit u = unit_at(p, bq.x, bq.y);
+  const int n = u.ub1 - u.ub0;
+  const int kvh = static_cast<int>((w - before[lo]) / n);
+  const int64_t u0 = before[lo] + static_cast<int64_t>(kvh) * n;
+  if (u0 == w) return;  // a unit begins here: nothing is cut
+  const int first = static_cast<int>(u0 / run);
+  if (first != i - 1) return;
+  const int last = min(p.tile_ctas - 1, static_cast<int>((u0 + n - 1) / run));
+  const int row = y * 32 + (threadIdx.x & 31), r = u.r0 + row;
+  if (r >= u.rows) return;
+  float m = -INFINITY;
+  for (int k = first; k <= last; ++k)
+    m = fmaxf(m, reinterpret_cast<const float2*>(p.tile_ml)[(k * 2ll + (k == first ? 1 : 0)) * kUnitRows + row].x);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
+  uint16_t* dst = p.out + (static_cast<int64_t>(u.s.t0 + tok) * p.H + kvh * p.G + (r - tok * p.G)) * D;
+#pragma unroll
+  for (int c = threadIdx.x >> 5; c < D / 4; c += 8) {
+    float sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = first; k <= last; ++k) {
+      const int64_t part = k * 2ll + (k == first ? 1 : 0);
+      const float2 ml = reinterpret_cast<const float2*>(p.tile_ml)[part * kUnitRows + row];
+      const float4 o = reinterpret_cast<const float4*>(p.tile_o)[(part * (D / 4) + c) * kUnitRows + row];
+      const float f = ex2(ml.x - ref);
+      sum = fmaf(ml.y, f, sum);
+      acc.x = fmaf(o.x, f, acc.x);
+      acc.y = fmaf(o.y, f, acc.y);
+      acc.z = fmaf(o.z, f, acc.z);
+      acc.w = fmaf(o.w, f, acc.w);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(dst + c * 4) =
+        make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
+  }
+}
+
 // Joins the parts of the units that were cut, and writes zeros for the rows
 // that no step covers: queries without keys and tokens behind the last
 // sequence.  A CTA per (sequence, token, kv head), 8 warps over its G rows.
@@ -360,6 +480,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   __shared__ float sh_o[8][D];
   __shared__ float2 sh_ml[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int row_ctas = p.B * p.combine_rows * p.Hkv;
+  if (static_cast<int>(blockIdx.x) >= row_ctas) {
+    const int at = blockIdx.x - row_ctas;
+    tile_join<BF16, D>(p, 1 + at / 8, at % 8);
+    return;
+  }
   const int kvh = blockIdx.x % p.Hkv, y = blockIdx.x / p.Hkv % p.combine_rows;
   const int b = blockIdx.x / p.Hkv / p.combine_rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -368,7 +494,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
     const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
     const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
     uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(end, 0));
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < words; i += gridDim.x * 256ll) dst[i] = 0u;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < words; i += row_ctas * 256ll) dst[i] = 0u;
   }
   const Work w = work_at(p, b);
   if (static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
@@ -443,13 +569,17 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   // cheap, and per device: set on every call rather than remembered
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
     return B200K_ERR_LAUNCH;
-  kernel<<<ctas, kWarps * 32, kSmem, st>>>(p);
+  kernel<<<ctas + (p.tile_ctas > 0 ? 1 : 0), kWarps * 32, kSmem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return B200K_ERR_LAUNCH;
+  if (p.tile_ctas > 0) {
+    const int rc = launch_tiles(p, BF16, D, CAP, st);
+    if (rc != B200K_OK) return rc;
+  }
   // The combine's launch overlaps the row kernel's end (it waits for the
   // row kernel's writes itself, before it reads or writes anything).
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.combine_rows * p.Hkv));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.combine_rows * p.Hkv + std::max(0, p.tile_ctas - 1) * 8));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at;
@@ -464,8 +594,6 @@ template <bool BF16, int D>
 int launch_cap(const Params& p, bool cap, int ctas, cudaStream_t st) {
   return cap ? launch<BF16, D, true>(p, ctas, st) : launch<BF16, D, false>(p, ctas, st);
 }
-
-int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace paged
@@ -490,9 +618,44 @@ int check_shape(const B200kPagedAttentionArgs* a) {
   return B200K_OK;
 }
 
-int64_t workspace_bytes(const B200kPagedAttentionArgs* a, int sms) {
+// Sequences of more query rows than this run the tile kernel.
+constexpr int kLongRows = 32;
+
+bool may_be_long(const B200kPagedAttentionArgs* a) {
+  const int64_t q = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
+  return q * (a->heads / a->kv_heads) > kLongRows;
+}
+
+// Where each part of the workspace begins; returns its size.
+int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p) {
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    uint8_t* r = ws + at;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
   const int64_t slots = static_cast<int64_t>(sms) * kCtasPerSm * kWarps * 2 * kRows;
-  return align256(slots * a->head_dim * 4) + align256(slots * 8) + align256((a->seqs + 2) * 8);
+  uint8_t* part_o = take(slots * a->head_dim * 4);
+  uint8_t* part_ml = take(slots * 8);
+  uint8_t* prefix = take((a->seqs + 2) * 8);
+  uint8_t *steps = ws, *entries = ws, *tile_o = ws, *tile_ml = ws;
+  if (may_be_long(a)) {
+    const int64_t n = a->tokens * (a->heads / a->kv_heads) / kUnitRows + a->seqs + 1;
+    steps = take((n + 4) * 8);
+    entries = take(n * 8);
+    tile_o = take(static_cast<int64_t>(sms) * 2 * kUnitRows * a->head_dim * 4);
+    tile_ml = take(static_cast<int64_t>(sms) * 2 * kUnitRows * 8);
+  }
+  if (p) {
+    p->part_o = reinterpret_cast<float*>(part_o);
+    p->part_ml = reinterpret_cast<float*>(part_ml);
+    p->prefix = reinterpret_cast<int64_t*>(prefix);
+    p->entry_steps = reinterpret_cast<int64_t*>(steps);
+    p->entries = reinterpret_cast<int2*>(entries);
+    p->tile_o = reinterpret_cast<float*>(tile_o);
+    p->tile_ml = reinterpret_cast<float*>(tile_ml);
+  }
+  return at;
 }
 
 }  // namespace
@@ -505,7 +668,7 @@ extern "C" int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* a,
   if (a->tokens == 0 || a->heads == 0) return B200K_OK;
   const int sms = device_sm_count();
   if (sms <= 0) return B200K_ERR_DEVICE;
-  *bytes = workspace_bytes(a, sms);
+  *bytes = place(a, sms, nullptr, nullptr);
   return B200K_OK;
 }
 
@@ -530,7 +693,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
     return cudaMemsetAsync(a->out, 0, n, st) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
   }
   if (!a->k_cache || !a->v_cache || !a->page_table || !a->q_start || !a->kv_len) return B200K_ERR_ARG;
-  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < workspace_bytes(a, sms)) return B200K_ERR_ARG;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < place(a, sms, nullptr, nullptr)) return B200K_ERR_ARG;
   Params p;
   std::memset(&p, 0, sizeof(p));
   p.T = static_cast<int32_t>(a->tokens);
@@ -543,7 +706,9 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.table_cols = static_cast<int32_t>(a->table_cols);
   p.capacity = static_cast<int32_t>(keys);
   p.window = static_cast<int32_t>(std::min<int64_t>(a->window, 0x3fffffff));
-  p.long_rows = 0x7fffffff;
+  p.tile_ctas = may_be_long(a) ? sms : 0;
+  p.long_rows = p.tile_ctas > 0 ? kLongRows : 0x7fffffff;
+  p.test_flags = a->test_flags;
   p.div_page = make_fastdiv(static_cast<uint32_t>(p.page_size));
   p.div_g = make_fastdiv(static_cast<uint32_t>(p.G));
   p.table_stride = a->table_stride;
@@ -565,20 +730,16 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.cap2 = a->softcap * kLog2e;
   const int ctas = sms * kCtasPerSm;
   p.workers = ctas * kWarps;
-  const int64_t slots = static_cast<int64_t>(p.workers) * 2 * kRows;
-  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  ws += align256(slots * a->head_dim * 4);
-  p.part_ml = reinterpret_cast<float*>(ws);
-  ws += align256(slots * 8);
-  p.prefix = reinterpret_cast<int64_t*>(ws);
+  place(a, sms, static_cast<uint8_t*>(a->workspace), &p);
   p.status = a->status;
   p.timeout_ns = a->timeout_ns > 0 ? a->timeout_ns : 2000000000ll;
   // The combine covers this many tokens of a sequence side by side and the
   // rest in a loop; its grid stays below 2^31 CTAs.
-  const int64_t hint = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
-  p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(hint, 0x3fffffff / (static_cast<int64_t>(p.B) * p.Hkv))));
-  if (static_cast<int64_t>(p.B) * p.Hkv > 0x3fffffffLL) return B200K_ERR_SHAPE;
+  const int64_t per_token = static_cast<int64_t>(p.B) * p.Hkv;
+  if (per_token > 0x1fffffffLL) return B200K_ERR_SHAPE;
+  int64_t rows = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
+  if (p.tile_ctas > 0) rows = std::min<int64_t>(rows, kLongRows / p.G);
+  p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 0x1fffffff / per_token)));
   if (a->dtype == B200K_BF16)
     return a->head_dim == 64 ? launch_cap<true, 64>(p, cap, ctas, st) : launch_cap<true, 128>(p, cap, ctas, st);
   return a->head_dim == 64 ? launch_cap<false, 64>(p, cap, ctas, st) : launch_cap<false, 128>(p, cap, ctas, st);
