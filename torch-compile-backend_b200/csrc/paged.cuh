@@ -10,8 +10,11 @@ namespace paged {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 16;      // keys of one step of the row kernel (one MMA k)
 constexpr int kRows = 16;      // query rows of one unit of the row kernel (one MMA m)
-constexpr int kBlock = 128;    // keys of one step of the tile kernel
+constexpr int kBlock = 64;     // keys of one step of the tile kernel
 constexpr int kUnitRows = 256; // query rows of one unit of the tile kernel (two MMA m)
+// What a unit's start and end cost (queries in, output out, pipeline empty),
+// in steps: counted in the list that the CTAs share out.
+constexpr int kPortionCost = 4;
 
 struct Params {
   int32_t T, B, H, Hkv, G;     // G = H / Hkv
@@ -34,12 +37,14 @@ struct Params {
   float* part_ml;              // [workers][2][16][2]: running max (base 2) and sum
   int64_t* prefix;             // [B + 1] steps before each sequence; [B + 1]: steps a worker takes
   int32_t workers;
-  // tile kernel: [0] steps of all units, [1] steps a CTA takes, [2] entries, [3 + e] steps before entry e
+  // tile kernel: steps count kPortionCost a unit; [0] all, [1] a CTA's, [2] entries, [3 + e] before entry e
   int64_t* entry_steps;
   int2* entries;               // (sequence, 256-row block)
   float* tile_o;               // [CTAs][2][D / 4][256][4]
   float* tile_ml;              // [CTAs][2][256][2]
   int32_t tile_ctas;           // 0: not launched
+  int32_t box_rows;            // rows of a TMA box of keys or values, 0: copied row by row
+  int32_t q_box;               // queries by TMA
   int32_t test_flags;
   int32_t* status;
   int64_t timeout_ns;

@@ -171,7 +171,7 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
         }
         const Unit u = unit_at(p, b0 + lo, e - starts[lo]);
         p.entries[entry0 + e] = make_int2(b0 + lo, e - starts[lo]);
-        mine = static_cast<int64_t>(u.ub1 - u.ub0) * p.Hkv;
+        mine = static_cast<int64_t>(u.ub1 - u.ub0 + kPortionCost) * p.Hkv;
       }
       int64_t sum;
       const int64_t x = block_scan(mine, sum);
@@ -435,13 +435,13 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
   }
   const int2 bq = p.entries[lo];
   const Unit u = unit_at(p, bq.x, bq.y);
-  const int n = u.ub1 - u.ub0;
-  const int kvh = static_cast<int>((w - before[lo]) / n);
-  const int64_t u0 = before[lo] + static_cast<int64_t>(kvh) * n;
-  if (u0 == w) return;  // a unit begins here: nothing is cut
-  const int first = static_cast<int>(u0 / run);
+  const int n = u.ub1 - u.ub0, len = n + kPortionCost;
+  const int kvh = static_cast<int>((w - before[lo]) / len);
+  const int64_t u0 = before[lo] + static_cast<int64_t>(kvh) * len;
+  if (w - u0 <= kPortionCost) return;  // nothing is cut: CTA i begins with the unit's first step
+  const int first = static_cast<int>((u0 + kPortionCost) / run);
   if (first != i - 1) return;
-  const int last = min(p.tile_ctas - 1, static_cast<int>((u0 + n - 1) / run));
+  const int last = min(p.tile_ctas - 1, static_cast<int>((u0 + len - 1) / run));
   const int row = y * 32 + (threadIdx.x & 31), r = u.r0 + row;
   if (r >= u.rows) return;
   float m = -INFINITY;
