@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -171,6 +172,18 @@ inline int check_form(const B200kEpilogueForm& f, const B200kProgram& prog, int 
 }
 
 int device_sm_count();
+
+// True once a device: `done` is a bit mask of one kernel's devices whose
+// attributes are set (setting them twice, from two threads, is harmless).
+// Devices past 63 are never remembered.
+inline bool attributes_set(const std::atomic<uint64_t>& done) {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev < 64 && ((done.load(std::memory_order_acquire) >> dev) & 1u);
+}
+inline void attributes_done(std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+}
 
 }  // namespace b200k
 

@@ -16,6 +16,13 @@ constexpr int kUnitRows = 256; // query rows of one unit of the tile kernel (two
 // in steps: counted in the list that the CTAs share out.
 constexpr int kPortionCost = 4;
 
+// A unit of the tile kernel whose parts lie in CTAs i (slot 1) to last (slot 0).
+struct Join {
+  int32_t last;      // 0: none
+  int32_t t0, kvh;   // the sequence's first token
+  int32_t r0, rows;
+};
+
 struct Params {
   int32_t T, B, H, Hkv, G;     // G = H / Hkv
   int32_t page_size, num_pages, table_cols;
@@ -42,6 +49,7 @@ struct Params {
   int2* entries;               // (sequence, 256-row block)
   float* tile_o;               // [CTAs][2][D / 4][256][4]
   float* tile_ml;              // [CTAs][2][256][2]
+  Join* joins;                 // [CTAs] the cut unit that begins in each CTA's run
   int32_t tile_ctas;           // 0: not launched
   int32_t box_rows;            // rows of a TMA box of keys or values, 0: copied row by row
   int32_t q_box;               // queries by TMA

@@ -24,9 +24,11 @@
 // combine_kernel joins them in the order of the keys.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "host_common.h"
 #include "paged.cuh"
+#include "rowreduce.cuh"
 
 namespace b200k {
 namespace paged {
@@ -34,6 +36,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 2;
+constexpr int kMinRun = 2;  // steps of a worker: shorter runs only add parts to join
 constexpr uint32_t kRingBytes = 24576;  // of one warp
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -134,6 +137,7 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
   __shared__ int64_t sums[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t* before = p.entry_steps + 3;
+  for (int i = tid; i < p.tile_ctas; i += kWarps * 32) p.joins[i].last = 0;
   int64_t steps = 0;
   int entry0 = 0;
   auto block_scan = [&](int64_t v, int64_t& all) {  // inclusive
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     }
     total += warp_add(mine);
   }
-  const int64_t run = (total + p.workers - 1) / p.workers;
+  const int64_t run = max(static_cast<int64_t>(kMinRun), (total + p.workers - 1) / p.workers);
   if (worker == 0 && lane == 0) {
     p.prefix[p.B] = total;
     p.prefix[p.B + 1] = run;
@@ -417,58 +421,47 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   cp_wait<0>();
 }
 
-// Joins the tile kernel's parts of one cut unit.  Boundary i (the start of
-// CTA i's run) belongs to the unit that it cuts when it is the first boundary
-// inside that unit; block y of 8 takes 32 of its 256 rows, a thread one row
-// and every eighth group of 4 columns.
+// Joins the tile kernel's parts of the cut unit that begins in CTA i's run:
+// block y of 8 takes 32 of its 256 rows, a thread one row and every eighth
+// group of 4 columns.
 template <bool BF16, int D>
 __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
-  const int64_t total = p.entry_steps[0], run = p.entry_steps[1];
-  const int64_t* before = p.entry_steps + 3;
-  const int64_t w = run * i;
-  if (w >= total) return;
-  int lo = 0, hi = static_cast<int>(p.entry_steps[2]);
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (before[mid] <= w) lo = mid;
-    else hi = mid;
-  }
-  const int2 bq = p.entries[lo];
-  const Unit u = unit_at(p, bq.x, bq.y);
-  const int n = u.ub1 - u.ub0, len = n + kPortionCost;
-  const int kvh = static_cast<int>((w - before[lo]) / len);
-  const int64_t u0 = before[lo] + static_cast<int64_t>(kvh) * len;
-  if (w - u0 <= kPortionCost) return;  // nothing is cut: CTA i begins with the unit's first step
-  const int first = static_cast<int>((u0 + kPortionCost) / run);
-  if (first != i - 1) return;
-  const int last = min(p.tile_ctas - 1, static_cast<int>((u0 + len - 1) / run));
+  const Join u = p.joins[i];
   const int row = y * 32 + (threadIdx.x & 31), r = u.r0 + row;
-  if (r >= u.rows) return;
+  if (u.last == 0 || r >= u.rows) return;
+  auto part_of = [&](int k) { return k * 2ll + (k == i ? 1 : 0); };
+  const float2* ml = reinterpret_cast<const float2*>(p.tile_ml);
   float m = -INFINITY;
-  for (int k = first; k <= last; ++k)
-    m = fmaxf(m, reinterpret_cast<const float2*>(p.tile_ml)[(k * 2ll + (k == first ? 1 : 0)) * kUnitRows + row].x);
+#pragma unroll 4
+  for (int k = i; k <= u.last; ++k) m = fmaxf(m, ml[part_of(k) * kUnitRows + row].x);
   const float ref = m == -INFINITY ? 0.0f : m;
-  const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
-  uint16_t* dst = p.out + (static_cast<int64_t>(u.s.t0 + tok) * p.H + kvh * p.G + (r - tok * p.G)) * D;
+  constexpr int C = D / 32;  // column groups of a thread
+  float sum = 0.0f;
+  float4 acc[C];
 #pragma unroll
-  for (int c = threadIdx.x >> 5; c < D / 4; c += 8) {
-    float sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = first; k <= last; ++k) {
-      const int64_t part = k * 2ll + (k == first ? 1 : 0);
-      const float2 ml = reinterpret_cast<const float2*>(p.tile_ml)[part * kUnitRows + row];
-      const float4 o = reinterpret_cast<const float4*>(p.tile_o)[(part * (D / 4) + c) * kUnitRows + row];
-      const float f = ex2(ml.x - ref);
-      sum = fmaf(ml.y, f, sum);
-      acc.x = fmaf(o.x, f, acc.x);
-      acc.y = fmaf(o.y, f, acc.y);
-      acc.z = fmaf(o.z, f, acc.z);
-      acc.w = fmaf(o.w, f, acc.w);
+  for (int c = 0; c < C; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int k = i; k <= u.last; ++k) {
+    const float2 v = ml[part_of(k) * kUnitRows + row];
+    const float f = ex2(v.x - ref);
+    sum = fmaf(v.y, f, sum);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const float4 o =
+          reinterpret_cast<const float4*>(p.tile_o)[(part_of(k) * (D / 4) + c * 8 + (threadIdx.x >> 5)) * kUnitRows + row];
+      acc[c].x = fmaf(o.x, f, acc[c].x);
+      acc[c].y = fmaf(o.y, f, acc[c].y);
+      acc[c].z = fmaf(o.z, f, acc[c].z);
+      acc[c].w = fmaf(o.w, f, acc[c].w);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(dst + c * 4) =
-        make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
   }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
+  uint16_t* dst = p.out + (static_cast<int64_t>(u.t0 + tok) * p.H + u.kvh * p.G + (r - tok * p.G)) * D;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    *reinterpret_cast<uint2*>(dst + (c * 8 + (threadIdx.x >> 5)) * 4) =
+        make_uint2(pack16<BF16>(acc[c].x * inv, acc[c].y * inv), pack16<BF16>(acc[c].z * inv, acc[c].w * inv));
 }
 
 // Joins the parts of the units that were cut, and writes zeros for the rows
@@ -476,14 +469,14 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
 // sequence.  A CTA per (sequence, token, kv head), 8 warps over its G rows.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
-  constexpr int V = D / 32;  // columns of a lane
-  __shared__ float sh_o[8][D];
-  __shared__ float2 sh_ml[8];
+  constexpr int V = D / 32;  // columns of a lane, side by side
+  using Vec = typename std::conditional<D == 128, float4, float2>::type;
+  __shared__ Vec sh_o[8][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int row_ctas = p.B * p.combine_rows * p.Hkv;
   if (static_cast<int>(blockIdx.x) >= row_ctas) {
     const int at = blockIdx.x - row_ctas;
-    tile_join<BF16, D>(p, 1 + at / 8, at % 8);
+    tile_join<BF16, D>(p, at / 8, at % 8);
     return;
   }
   const int kvh = blockIdx.x % p.Hkv, y = blockIdx.x / p.Hkv % p.combine_rows;
@@ -511,52 +504,56 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
         first = u0 / run;
         last = min(static_cast<int64_t>(p.workers) - 1, (u0 + w.tiles - 1) / run);
       }
-      float mx = -INFINITY, sum = 0.0f, acc[V];
+      const bool cut = mine && last > first;
+      float sum = 0.0f, acc[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-      if (mine && last > first) {
-        // parts in key order, `share` warps in turn
-#pragma unroll 4
-        for (int64_t wk = first + part; wk <= last; wk += share) {
-          const int64_t at = (wk * 2 + (u0 < wk * run ? 0 : 1)) * kRows + r % kRows;
-          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-          float x[V];
+      if (cut) {
+        auto row_of = [&](int64_t wk) { return (wk * 2 + (u0 < wk * run ? 0 : 1)) * kRows + r % kRows; };
+        const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+        // every warp of the row finds the maximum and the sum of all parts ...
+        float mx = -INFINITY;
+        for (int64_t wk = first + lane; wk <= last; wk += 32) mx = fmaxf(mx, ml[row_of(wk)].x);
+        mx = warp_max(mx);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        for (int64_t wk = first + lane; wk <= last; wk += 32) {
+          const float2 v = ml[row_of(wk)];
+          sum = fmaf(v.y, ex2(v.x - ref), sum);
+        }
+        sum = warp_sum(sum);
+        // ... and adds every `share`-th part's output, a lane knowing one part's weight
+        for (int64_t w0 = first + part; w0 <= last; w0 += 32 * share) {
+          const int64_t wk = w0 + lane * share;
+          const float f = wk <= last ? ex2(ml[row_of(wk)].x - ref) : 0.0f;
+          const int n = static_cast<int>(min(static_cast<int64_t>(32), (last - w0) / share + 1));
+#pragma unroll 8
+          for (int k = 0; k < n; ++k) {
+            const Vec x = reinterpret_cast<const Vec*>(p.part_o + row_of(w0 + k * share) * D)[lane];
+            const float c = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
-          for (int j = 0; j < V; ++j) x[j] = p.part_o[at * D + j * 32 + lane];
-          const float nm = fmaxf(mx, ml.x), ref = nm == -INFINITY ? 0.0f : nm;
-          const float a = ex2(mx - ref), c = ex2(ml.x - ref);
-          mx = nm;
-          sum = sum * a + ml.y * c;
-#pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = acc[j] * a + x[j] * c;
+            for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], c, acc[j]);
+          }
         }
       }
       if (share > 1) {
         __syncthreads();
-        if (lane == 0) sh_ml[warp] = make_float2(mx, sum);
+        Vec x;
 #pragma unroll
-        for (int j = 0; j < V; ++j) sh_o[warp][j * 32 + lane] = acc[j];
+        for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
+        sh_o[warp][lane] = x;
         __syncthreads();
-        if (part == 0 && mine) {
+        if (part == 0 && mine)
           for (int k = 1; k < share; ++k) {
-            const float2 ml = sh_ml[warp + k];
-            const float nm = fmaxf(mx, ml.x), ref = nm == -INFINITY ? 0.0f : nm;
-            const float a = ex2(mx - ref), c = ex2(ml.x - ref);
-            mx = nm;
-            sum = sum * a + ml.y * c;
+            const Vec y = sh_o[warp + k][lane];
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] = acc[j] * a + sh_o[warp + k][j * 32 + lane] * c;
+            for (int j = 0; j < V; ++j) acc[j] += reinterpret_cast<const float*>(&y)[j];
           }
-        }
       }
-      if (mine && part == 0 && (w.tiles == 0 || last > first)) {
+      if (mine && part == 0 && (w.tiles == 0 || cut)) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t* dst = out_row(w.s.t0 + i, kvh * p.G + g);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(w.s.t0 + i, kvh * p.G + g)) + lane * (V / 2);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const uint32_t u = pack16<BF16>(acc[j] * inv, 0.0f);
-          dst[j * 32 + lane] = static_cast<uint16_t>(u);
-        }
+        for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
       }
     }
   }
@@ -566,9 +563,12 @@ template <bool BF16, int D, bool CAP>
 int launch(const Params& p, int ctas, cudaStream_t st) {
   constexpr uint32_t kSmem = kWarps * kRingBytes;
   auto kernel = rows_kernel<BF16, D, CAP>;
-  // cheap, and per device: set on every call rather than remembered
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-    return B200K_ERR_LAUNCH;
+  static std::atomic<uint64_t> done{0};
+  if (!attributes_set(done)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+      return B200K_ERR_LAUNCH;
+    attributes_done(done);
+  }
   kernel<<<ctas + (p.tile_ctas > 0 ? 1 : 0), kWarps * 32, kSmem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return B200K_ERR_LAUNCH;
   if (p.tile_ctas > 0) {
@@ -579,7 +579,7 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   // row kernel's writes itself, before it reads or writes anything).
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.combine_rows * p.Hkv + std::max(0, p.tile_ctas - 1) * 8));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.combine_rows * p.Hkv + p.tile_ctas * 8));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at;
@@ -638,13 +638,14 @@ int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p)
   uint8_t* part_o = take(slots * a->head_dim * 4);
   uint8_t* part_ml = take(slots * 8);
   uint8_t* prefix = take((a->seqs + 2) * 8);
-  uint8_t *steps = ws, *entries = ws, *tile_o = ws, *tile_ml = ws;
+  uint8_t *steps = ws, *entries = ws, *tile_o = ws, *tile_ml = ws, *joins = ws;
   if (may_be_long(a)) {
     const int64_t n = a->tokens * (a->heads / a->kv_heads) / kUnitRows + a->seqs + 1;
     steps = take((n + 4) * 8);
     entries = take(n * 8);
     tile_o = take(static_cast<int64_t>(sms) * 2 * kUnitRows * a->head_dim * 4);
     tile_ml = take(static_cast<int64_t>(sms) * 2 * kUnitRows * 8);
+    joins = take(static_cast<int64_t>(sms) * sizeof(Join));
   }
   if (p) {
     p->part_o = reinterpret_cast<float*>(part_o);
@@ -654,6 +655,7 @@ int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p)
     p->entries = reinterpret_cast<int2*>(entries);
     p->tile_o = reinterpret_cast<float*>(tile_o);
     p->tile_ml = reinterpret_cast<float*>(tile_ml);
+    p->joins = reinterpret_cast<Join*>(joins);
   }
   return at;
 }

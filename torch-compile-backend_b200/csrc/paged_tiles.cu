@@ -494,6 +494,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = 0;
     bool ok = true;
     while (ok && walk.next(p, po)) {
+      if (!po.whole && po.slot == 1 && threadIdx.x == 0) {
+        // the run's last unit goes on in the next CTAs, the steps that are left at `run` each
+        const int left = walk.u.ub1 - po.end;
+        p.joins[blockIdx.x] = Join{static_cast<int>(blockIdx.x + (left + run - 1) / run), walk.u.s.t0, po.kvh, walk.u.r0,
+                                   walk.u.rows};
+      }
       const int r = walk.u.r0 + in_unit;
       const bool real = r < walk.u.rows;
       const uint32_t tok = fdiv(static_cast<uint32_t>(min(r, walk.u.rows - 1)), p.div_g);
@@ -653,8 +659,12 @@ bool make_map(CUtensorMap* map, bool bf16, const void* ptr, const int64_t (&size
 template <bool BF16, int D, bool CAP>
 int launch(Params p, cudaStream_t st) {
   auto kernel = tiles_kernel<BF16, D, CAP>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem) != cudaSuccess)
-    return B200K_ERR_LAUNCH;
+  static std::atomic<uint64_t> done{0};
+  if (!attributes_set(done)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem) != cudaSuccess)
+      return B200K_ERR_LAUNCH;
+    attributes_done(done);
+  }
   // Boxes of the rows that lie together in a page and in a block: the largest
   // power of two, 8 to 64, that divides the page size.
   CUtensorMap tq, tk, tv;
