@@ -97,11 +97,6 @@ __device__ __forceinline__ Work work_at(const Params& p, int b) {
 __device__ __forceinline__ int64_t steps_of(const Params& p, const Work& w) {
   return static_cast<int64_t>(p.Hkv) * w.rts * w.tiles;
 }
-__device__ __forceinline__ int64_t warp_add(int64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 __device__ __forceinline__ int64_t warp_scan(int64_t v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -201,23 +196,28 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   constexpr int kRowsPerCp = 32 / kChunks;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int worker = blockIdx.x * kWarps + warp;
+  // the first CTA plans the tile kernel's work, when that runs
+  const int worker = (static_cast<int>(blockIdx.x) - (p.tile_ctas > 0 ? 1 : 0)) * kWarps + warp;
   const uint32_t ring = smem_addr(smem) + warp * kRingBytes;
-  if (worker >= p.workers) {  // the last CTA, when the tile kernel runs
+  if (worker < 0) {
     plan_tiles(p);
     return;
   }
 
+  // combine_kernel may be launched from here on: its CTAs find room as this
+  // kernel's leave, and wait for its writes themselves.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
   // The whole list's length and, from it, this worker's run [w0, w1).
-  int64_t total = 0;
+  int64_t total = 0, mine0 = 0, upto0 = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = 0;
     if (b0 + lane < p.B) mine = steps_of(p, work_at(p, b0 + lane));
-    if (worker == 0) {  // for combine_kernel
-      const int64_t upto = warp_scan(mine);
-      if (b0 + lane < p.B) p.prefix[b0 + lane] = total + upto - mine;
-    }
-    total += warp_add(mine);
+    const int64_t upto = warp_scan(mine);
+    if (worker == 0 && b0 + lane < p.B) p.prefix[b0 + lane] = total + upto - mine;  // for combine_kernel
+    total += __shfl_sync(0xffffffffu, upto, 31);
+    mine0 = mine;
+    upto0 = upto;
   }
   const int64_t run = max(static_cast<int64_t>(kMinRun), (total + p.workers - 1) / p.workers);
   if (worker == 0 && lane == 0) {
@@ -230,9 +230,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   cur.b = 0;
   int64_t seq0 = 0;  // the list's index of cur.b's first step
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    int64_t mine = 0;
-    if (b0 + lane < p.B) mine = steps_of(p, work_at(p, b0 + lane));
-    const int64_t upto = warp_scan(mine);
+    int64_t mine = mine0, upto = upto0;  // of the last 32: all there are in a small batch
+    if (p.B > 32) {
+      mine = b0 + lane < p.B ? steps_of(p, work_at(p, b0 + lane)) : 0;
+      upto = warp_scan(mine);
+    }
     const unsigned hit = __ballot_sync(0xffffffffu, seq0 + upto > w0);
     if (hit) {
       const int at = __ffs(hit) - 1;
@@ -472,10 +474,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   constexpr int V = D / 32;  // columns of a lane, side by side
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
   __shared__ Vec sh_o[8][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int row_ctas = p.B * p.combine_rows * p.Hkv;
   if (static_cast<int>(blockIdx.x) >= row_ctas) {
     const int at = blockIdx.x - row_ctas;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     tile_join<BF16, D>(p, at / 8, at % 8);
     return;
   }
@@ -483,13 +485,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   const int b = blockIdx.x / p.Hkv / p.combine_rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto out_row = [&](int64_t tok, int h) { return p.out + (tok * p.H + h) * D; };
+  // The index tensors are older than the row kernel; what follows the wait
+  // reads or writes what the kernels before it may still be at.
+  const Work w = work_at(p, b);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   {  // tokens behind the last sequence
     const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
     const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
     uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(end, 0));
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < words; i += row_ctas * 256ll) dst[i] = 0u;
   }
-  const Work w = work_at(p, b);
   if (static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
   const int64_t seq0 = p.prefix[b], run = p.prefix[p.B + 1];
   const int share = p.G >= 8 ? 1 : 8 / p.G;  // warps of a row
@@ -511,24 +516,30 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
       if (cut) {
         auto row_of = [&](int64_t wk) { return (wk * 2 + (u0 < wk * run ? 0 : 1)) * kRows + r % kRows; };
         const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-        // every warp of the row finds the maximum and the sum of all parts ...
-        float mx = -INFINITY;
-        for (int64_t wk = first + lane; wk <= last; wk += 32) mx = fmaxf(mx, ml[row_of(wk)].x);
+        // Every warp of the row finds the maximum and the sum of all parts, a
+        // lane 32 parts apart (the first 32 stay in registers) ...
+        const int64_t n_parts = last - first + 1;
+        float2 v0 = make_float2(-INFINITY, 0.0f);
+        if (lane < n_parts) v0 = ml[row_of(first + lane)];
+        float mx = v0.x;
+        for (int64_t k = lane + 32; k < n_parts; k += 32) mx = fmaxf(mx, ml[row_of(first + k)].x);
         mx = warp_max(mx);
         const float ref = mx == -INFINITY ? 0.0f : mx;
-        for (int64_t wk = first + lane; wk <= last; wk += 32) {
-          const float2 v = ml[row_of(wk)];
+        const float f0 = ex2(v0.x - ref);
+        sum = v0.y * f0;
+        for (int64_t k = lane + 32; k < n_parts; k += 32) {
+          const float2 v = ml[row_of(first + k)];
           sum = fmaf(v.y, ex2(v.x - ref), sum);
         }
         sum = warp_sum(sum);
-        // ... and adds every `share`-th part's output, a lane knowing one part's weight
-        for (int64_t w0 = first + part; w0 <= last; w0 += 32 * share) {
-          const int64_t wk = w0 + lane * share;
-          const float f = wk <= last ? ex2(ml[row_of(wk)].x - ref) : 0.0f;
-          const int n = static_cast<int>(min(static_cast<int64_t>(32), (last - w0) / share + 1));
+        // ... and adds every `share`-th part's output, 32 parts at a time
+        for (int64_t k0 = 0; k0 < n_parts; k0 += 32) {
+          float f = f0;
+          if (k0 > 0) f = k0 + lane < n_parts ? ex2(ml[row_of(first + k0 + lane)].x - ref) : 0.0f;
+          const int n = static_cast<int>(min(static_cast<int64_t>(32), n_parts - k0));
 #pragma unroll 8
-          for (int k = 0; k < n; ++k) {
-            const Vec x = reinterpret_cast<const Vec*>(p.part_o + row_of(w0 + k * share) * D)[lane];
+          for (int k = part; k < n; k += share) {
+            const Vec x = reinterpret_cast<const Vec*>(p.part_o + row_of(first + k0 + k) * D)[lane];
             const float c = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
             for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], c, acc[j]);

@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* first_entry = reinterpret_cast<int*>(tmem_slot + 2);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the plan
   const int64_t total = p.entry_steps[0], run = p.entry_steps[1];
   const int n_entries = static_cast<int>(p.entry_steps[2]);
   const int64_t* before = p.entry_steps + 3;  // list positions before each entry
@@ -684,8 +685,19 @@ int launch(Params p, cudaStream_t st) {
     const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(p.G), 1, static_cast<cuuint32_t>(128 / p.G)};
     if (make_map(&tq, BF16, p.q, sizes, strides, box)) p.q_box = 1;
   }
-  kernel<<<p.tile_ctas, kThreads, Layout<D>::kSmem, st>>>(p, tq, tk, tv);
-  return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+  // launched under the row kernel's end, as the combine kernel is
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.tile_ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Layout<D>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p, tq, tk, tv) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
 }  // namespace
