@@ -88,9 +88,11 @@ __device__ __forceinline__ Place place_of(const AppendParams& p, int64_t t) {
   return r;
 }
 
+constexpr int kThreads = 128;  // 35.2 us for 16384 tokens of 48 heads of 64, 37.3 with CTAs of 256
+
 template <bool BF16, int TAB_DT, int NH>
-__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ AppendParams p) {
-  const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
+__global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_constant__ AppendParams p) {
+  const uint32_t gid = blockIdx.x * static_cast<uint32_t>(kThreads) + threadIdx.x;
   const uint32_t tok = fdiv(gid, p.div_tok);
   if (tok >= p.tokens) return;
   const uint32_t in_tok = gid - tok * p.div_tok.d;
@@ -195,11 +197,11 @@ int launch(AppendParams& p, bool vec, int sms, cudaStream_t st) {
     const int nh = few >= static_cast<int64_t>(sms) * 2048 * 4 ? 4 : 1;
     p.threads_per_token = p.units * ((all + nh - 1) / nh);
     const int64_t n = p.tokens * p.threads_per_token;
-    if (n + 256 <= 0x7fffffffLL) {
+    if (n + kThreads <= 0x7fffffffLL) {
       p.div_tok = make_fastdiv(static_cast<uint32_t>(p.threads_per_token));
-      const unsigned grid = static_cast<unsigned>((n + 255) / 256);
-      if (nh == 4) rope_append_kernel<BF16, TAB_DT, 4><<<grid, 256, 0, st>>>(p);
-      else rope_append_kernel<BF16, TAB_DT, 1><<<grid, 256, 0, st>>>(p);
+      const unsigned grid = static_cast<unsigned>((n + kThreads - 1) / kThreads);
+      if (nh == 4) rope_append_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
+      else rope_append_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
       return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
     }
   }
