@@ -26,6 +26,7 @@ from compiler.optimization.fusion_patchify import fuse_patchify
 from compiler.optimization.fusion_pointwise import fuse_pointwise
 from compiler.optimization.fusion_rope import fuse_gemm_rope, fuse_rope
 from compiler.optimization.fusion_rowreduce import fuse_rowreduce
+from compiler.optimization.inplace_append import appended_inputs, inplace_append
 
 runtime.load()
 
@@ -49,6 +50,8 @@ GEMMS_FUSED = 0
 def _passes(gm: fx.GraphModule) -> fx.GraphModule:
     global GRAPHS_COMPILED, GEMMS_FUSED
     GRAPHS_COMPILED += 1
+    if config.EXTENSIONS:
+        gm = inplace_append(gm)  # cache appends write their caches, not copies (extension)
     if config.EXTENSIONS and config.ENABLE_PATCHIFY:
         gm = fuse_patchify(gm)  # patch-embedding convolutions -> im2col + addmm (extension)
     if config.EXTENSIONS:
@@ -130,7 +133,9 @@ def inference_compiler(gm: fx.GraphModule, example_inputs):
     gm = _passes(gm)
     fn = make_boxed_func(gm.forward)
     if config.EXTENSIONS:
-        fn = graph_replay.wrap(gm, fn, _static_inputs())
+        caches = appended_inputs(gm)
+        if caches is not None:
+            fn = graph_replay.wrap(gm, fn, _static_inputs(), caches)
     return _checked(gm, example_inputs, fn)
 
 

@@ -12,6 +12,9 @@ Semantics are those of the op-by-op function:
   * inputs: tensors that are the same storage at every call (parameters,
     module buffers) are read in place; every other tensor input is copied
     into the graph's own input buffer before each replay;
+  * caches that the graph appends to (optimization/inplace_append.py) are read
+    and written in place and guarded by their address like parameters, and
+    returned as the caller's own tensors;
   * outputs: each replay's outputs are cloned out of the graph's buffers, so
     a result stays valid after later calls;
   * the first call runs op by op (it also warms up lazily initialised
@@ -75,7 +78,7 @@ def _is_persistent(t: torch.Tensor) -> bool:
 class GraphReplay:
     """Boxed callable: ``run(args)`` with ``args`` the graph's input list."""
 
-    def __init__(self, fn, no_clone=(), static=()):
+    def __init__(self, fn, no_clone=(), static=(), written=()):
         # AOTAutograd's marker for the list-argument calling convention (an
         # instance attribute, so that functools.wraps wrappers copy it)
         self._boxed_call = True
@@ -83,7 +86,11 @@ class GraphReplay:
         self.no_clone = frozenset(no_clone)  # output indices returned as the graph's own buffers
         # input indices AOTAutograd marks static (the module's lifted parameters
         # and buffers): read in place like parameters, guarded by their address
-        self.static = frozenset(static)
+        self.static = frozenset(static) | frozenset(written)
+        # input indices that the graph writes in place; output index -> such an
+        # input that it returns
+        self.written = frozenset(written)
+        self.returned = {}
         self.calls = 0
         self.replays = 0
         self.graph = None
@@ -123,11 +130,13 @@ class GraphReplay:
         with torch.cuda.graph(graph):
             outs = self.fn(list(self.static_in))
         outs = list(outs) if isinstance(outs, (list, tuple)) else [outs]
+        self.returned = {j: i for j, o in enumerate(outs) for i in self.written if o is self.static_in[i]}
         storages = {a.untyped_storage().data_ptr() for a in self.static_in if isinstance(a, torch.Tensor)}
-        if any(isinstance(o, torch.Tensor) and o.untyped_storage().data_ptr() in storages for o in outs):
+        if any(isinstance(o, torch.Tensor) and o.untyped_storage().data_ptr() in storages and j not in self.returned
+               for j, o in enumerate(outs)):
             raise RuntimeError("an output aliases an input")
         out_bytes = sum(o.numel() * o.element_size() for i, o in enumerate(outs)
-                        if isinstance(o, torch.Tensor) and i not in self.no_clone)
+                        if isinstance(o, torch.Tensor) and i not in self.no_clone and i not in self.returned)
         if out_bytes > config.GRAPH_MAX_OUTPUT_MB * 2**20:
             raise RuntimeError("outputs too large to clone per call")
         self.graph, self.static_out = graph, outs
@@ -159,19 +168,23 @@ class GraphReplay:
         self.replays += 1
         global REPLAYS
         REPLAYS += 1
-        return [o.clone() if isinstance(o, torch.Tensor) and i not in self.no_clone else o
+        return [args[self.returned[i]] if i in self.returned
+                else o.clone() if isinstance(o, torch.Tensor) and i not in self.no_clone else o
                 for i, o in enumerate(self.static_out)]
 
 
-def output_bytes(gm: fx.GraphModule) -> int:
-    """Bytes of the graph's tensor outputs, from the traced metadata."""
+def output_bytes(gm: fx.GraphModule, written=()) -> int:
+    """Bytes of the graph's tensor outputs, from the traced metadata, without
+    the inputs it writes in place."""
     total = 0
+    inputs = [n for n in gm.graph.nodes if n.op == "placeholder"]
+    skip = {inputs[i] for i in written}
     for node in gm.graph.nodes:
         if node.op != "output":
             continue
         outs = node.args[0] if isinstance(node.args[0], (list, tuple)) else [node.args[0]]
         for o in outs:
-            v = o.meta.get("val") if isinstance(o, fx.Node) else None
+            v = o.meta.get("val") if isinstance(o, fx.Node) and o not in skip else None
             if isinstance(v, torch.Tensor):
                 total += v.numel() * v.element_size()
     return total
@@ -291,15 +304,19 @@ def split_large_outputs(gm: fx.GraphModule, static=()):
     return TailReplay(body, tail_gm, len(small), plan, tail_args)
 
 
-def wrap(gm: fx.GraphModule, boxed_fn, static=()):
+def wrap(gm: fx.GraphModule, boxed_fn, static=(), written=()):
     """The boxed function of an inference graph, replayed as a CUDA graph when
     it launches enough kernels to gain from it: whole when its outputs are
     small enough to clone per call, else split into a replayed body and a
     tail run op by op (``split_large_outputs``); otherwise `boxed_fn`.
-    `static`: input indices read in place instead of copied per replay."""
+    `static`: input indices read in place instead of copied per replay;
+    `written`: input indices that the graph writes in place (running it twice
+    must leave what running it once does)."""
     if not config.CUDA_GRAPHS or launching_nodes(gm) < config.GRAPH_MIN_LAUNCHES:
         return boxed_fn
-    if output_bytes(gm) <= config.GRAPH_MAX_OUTPUT_MB * 2**20:
-        return GraphReplay(boxed_fn, static=static)
+    if output_bytes(gm, written) <= config.GRAPH_MAX_OUTPUT_MB * 2**20:
+        return GraphReplay(boxed_fn, static=static, written=written)
+    if written:
+        return boxed_fn  # a split graph's body returns no input
     split = split_large_outputs(gm, static)
     return split if split is not None else boxed_fn
