@@ -30,6 +30,7 @@ struct Params {
   int32_t window;              // 0: none
   int32_t long_rows;           // sequences of more query rows (queries * G) run the tile kernel
   int32_t combine_rows;        // tokens of a sequence that the combine grid covers side by side
+  int32_t join_share;          // warps of the combine kernel for one row: 1 or 4
   FastDiv div_page, div_g;
   int64_t table_stride;
   const uint16_t* q;
@@ -113,19 +114,24 @@ __device__ __forceinline__ void tile_keys(const Params& p, const Unit& u, int t,
 // Launches the tile kernel (paged_tiles.cu) on the plan in p.entries.
 int launch_tiles(const Params& p, bool bf16, int dim, bool cap, cudaStream_t st);
 
-// Offset of a key's row in the caches, or -1: not between lo and n (nothing
-// there is read: the pages may hold anything), or a page that does not exist.
-__device__ __forceinline__ int64_t key_offset(const Params& p, int b, int key, int lo, int n, int kvh) {
+// Offset of a key's row in the caches, `page` being what the table holds for
+// it, or -1: not between lo and n (nothing there is read: the pages may hold
+// anything), or a page that does not exist.
+__device__ __forceinline__ int64_t page_offset(const Params& p, int page, int key, int lo, int n, int kvh) {
   if (key < lo || key >= n) return -1;
-  const uint32_t pi = fdiv(static_cast<uint32_t>(key), p.div_page);
-  const int page = __ldg(p.table + b * p.table_stride + pi);
   if (page < 0 || page >= p.num_pages) {
     if (p.status) atomicCAS(p.status, 0, B200K_ERR_INDEX);
     return -1;
   }
+  const uint32_t pi = fdiv(static_cast<uint32_t>(key), p.div_page);
   return static_cast<int64_t>(page) * p.c_page +
          static_cast<int64_t>(static_cast<uint32_t>(key) - pi * static_cast<uint32_t>(p.page_size)) * p.c_slot +
          static_cast<int64_t>(kvh) * p.c_head;
+}
+__device__ __forceinline__ int64_t key_offset(const Params& p, int b, int key, int lo, int n, int kvh) {
+  if (key < lo || key >= n) return -1;
+  const int page = __ldg(p.table + b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
+  return page_offset(p, page, key, lo, n, kvh);
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -36,7 +36,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 2;
-constexpr int kMinRun = 2;  // steps of a worker: shorter runs only add parts to join
 constexpr uint32_t kRingBytes = 24576;  // of one warp
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -107,22 +106,23 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
   return v;
 }
 
-// A position in the list of steps.
+// A position in the list of steps: within a sequence kv head by kv head, row
+// block by row block, key by key.
 struct Cursor {
   Work w;
-  int b, unit, tile;
+  int b, kvh, rt, tile;
   __device__ __forceinline__ void next(const Params& p) {
     if (++tile < w.tiles) return;
     tile = 0;
-    if (++unit < p.Hkv * w.rts) return;
-    unit = 0;
+    if (++rt < w.rts) return;
+    rt = 0;
+    if (++kvh < p.Hkv) return;
+    kvh = 0;
     do {
       if (++b >= p.B) return;
       w = work_at(p, b);
     } while (w.tiles == 0 || w.rts == 0);
   }
-  __device__ __forceinline__ int kvh() const { return unit / w.rts; }
-  __device__ __forceinline__ int rt() const { return unit % w.rts; }
 };
 
 // The tile kernel's list: an entry for every 256 query rows of a sequence
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     mine0 = mine;
     upto0 = upto;
   }
-  const int64_t run = max(static_cast<int64_t>(kMinRun), (total + p.workers - 1) / p.workers);
+  const int64_t run = max(static_cast<int64_t>(1), (total + p.workers - 1) / p.workers);
   if (worker == 0 && lane == 0) {
     p.prefix[p.B] = total;
     p.prefix[p.B + 1] = run;
@@ -245,21 +245,28 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     seq0 += __shfl_sync(0xffffffffu, upto, 31);
   }
   cur.w = work_at(p, cur.b);
-  cur.unit = static_cast<int>((w0 - seq0) / cur.w.tiles);
-  cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(cur.unit) * cur.w.tiles);
+  const int unit = static_cast<int>((w0 - seq0) / cur.w.tiles);
+  cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(unit) * cur.w.tiles);
+  cur.kvh = unit / cur.w.rts;
+  cur.rt = unit - cur.kvh * cur.w.rts;
 
   Cursor ld = cur;
   int64_t ld_t = w0;
-  // offset in the caches of the key this lane looks up for the next step loaded
-  auto lookup = [&]() -> int64_t {
-    if (ld_t >= w1) return -1;
-    return key_offset(p, ld.b, ld.w.base + ld.tile * kKeys + (lane & (kKeys - 1)), ld.w.s.lo, ld.w.s.n, ld.kvh());
+  // The page that holds this lane's key of the next step to load: fetched a
+  // step before its first use, so that no step waits for the table.
+  int page = 0;
+  auto lookup = [&] {
+    const int key = ld.w.base + ld.tile * kKeys + (lane & (kKeys - 1));
+    page = -1;
+    if (ld_t < w1 && key >= ld.w.s.lo && key < ld.w.s.n)
+      page = __ldg(p.table + ld.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
   };
-  int64_t off = lookup();
+  lookup();
   auto issue = [&](int stage) {
     if (ld_t < w1) {
       const uint32_t sk = ring + stage * 2 * kTile, sv = sk + kTile;
       const int c = lane % kChunks;
+      const int64_t off = page_offset(p, page, ld.w.base + ld.tile * kKeys + (lane & (kKeys - 1)), ld.w.s.lo, ld.w.s.n, ld.kvh);
 #pragma unroll
       for (int i = 0; i < kKeys / kRowsPerCp; ++i) {
         const int row = i * kRowsPerCp + lane / kChunks;
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
       }
       ++ld_t;
       if (ld_t < w1) ld.next(p);
-      off = lookup();
+      lookup();
     }
     cp_commit();
   };
@@ -286,18 +293,18 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   int pos[2], row_first = 0, row_last = 0;
   bool fresh = true;
   int stage = 0;
-  int64_t unit0 = seq0 + static_cast<int64_t>(cur.unit) * cur.w.tiles;  // the current unit's first step
+  int64_t unit0 = seq0 + static_cast<int64_t>(unit) * cur.w.tiles;  // the current unit's first step
   for (int64_t t = w0; t < w1; ++t) {
     issue(stage == 0 ? S - 1 : stage - 1);
     if (fresh) {  // a new unit: its query rows as A fragments
       fresh = false;
-      const int rows = cur.w.s.m * p.G, r0 = cur.rt() * kRows, kvh = cur.kvh();
+      const int rows = cur.w.s.m * p.G, r0 = cur.rt * kRows;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = r0 + g + 8 * i;
         const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
         const uint16_t* src = p.q + static_cast<int64_t>(cur.w.s.t0 + tok) * p.q_t +
-                              static_cast<int64_t>(kvh * p.G + (r - tok * p.G)) * p.q_h + quad * 2;
+                              static_cast<int64_t>(cur.kvh * p.G + (r - tok * p.G)) * p.q_h + quad * 2;
         pos[i] = cur.w.s.first + static_cast<int>(tok);
         m[i] = -INFINITY;
         l[i] = 0.0f;
@@ -307,10 +314,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
           qf[k][2 + i] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
         }
       }
-      row_first = cur.w.s.first + static_cast<int>(fdiv(static_cast<uint32_t>(r0), p.div_g));
-      row_last = cur.w.s.first + static_cast<int>(fdiv(static_cast<uint32_t>(min(r0 + kRows, rows) - 1), p.div_g));
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+      row_first = cur.w.s.first + static_cast<int>(fdiv(static_cast<uint32_t>(r0), p.div_g));
+      row_last = cur.w.s.first + static_cast<int>(fdiv(static_cast<uint32_t>(min(r0 + kRows, rows) - 1), p.div_g));
     }
     cp_wait<S - 1>();
     __syncwarp();
@@ -328,11 +335,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
       }
     }
     const int key0 = cur.w.base + cur.tile * kKeys;
+    const bool masked = key0 + kKeys - 1 > row_first || (p.window > 0 && key0 <= row_last - p.window);  // warp-uniform
+    uint32_t pa[4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = score<CAP>(p, s[n][i]);
-    if (key0 + kKeys - 1 > row_first || (p.window > 0 && key0 <= row_last - p.window)) {  // warp-uniform
+    if (masked) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -371,11 +380,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) l[i] += (s[0][2 * i] + s[0][2 * i + 1]) + (s[1][2 * i] + s[1][2 * i + 1]);
+    for (int i = 0; i < 2; ++i)
+      l[i] += (s[0][2 * i] + s[0][2 * i + 1]) + (s[1][2 * i] + s[1][2 * i + 1]);
     // probabilities rounded to the input type for the second product (the
     // sum keeps fp32): half a step each, as b200k_attention
-    const uint32_t pa[4] = {pack16<BF16>(s[0][0], s[0][1]), pack16<BF16>(s[0][2], s[0][3]),
-                            pack16<BF16>(s[1][0], s[1][1]), pack16<BF16>(s[1][2], s[1][3])};
+    pa[0] = pack16<BF16>(s[0][0], s[0][1]);
+    pa[1] = pack16<BF16>(s[0][2], s[0][3]);
+    pa[2] = pack16<BF16>(s[1][0], s[1][1]);
+    pa[3] = pack16<BF16>(s[1][2], s[1][3]);
     {
       const int row = lane & 15, ch = lane >> 4;
 #pragma unroll
@@ -391,30 +403,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
 
     const bool unit_ends = cur.tile + 1 == cur.w.tiles;
     if (unit_ends || t + 1 == w1) {
-      const int rows = cur.w.s.m * p.G, r0 = cur.rt() * kRows, kvh = cur.kvh();
+      const int rows = cur.w.s.m * p.G, r0 = cur.rt * kRows;
       const bool whole = unit0 >= w0 && unit_ends;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int r = r0 + g + 8 * i;
+        const int in = g + 8 * i, r = r0 + in;
         if (r >= rows) continue;
         if (whole) {
           const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
           uint32_t* dst = reinterpret_cast<uint32_t*>(
-              p.out + (static_cast<int64_t>(cur.w.s.t0 + tok) * p.H + kvh * p.G + (r - tok * p.G)) * D + quad * 2);
+              p.out + (static_cast<int64_t>(cur.w.s.t0 + tok) * p.H + cur.kvh * p.G + (r - tok * p.G)) * D + quad * 2);
           const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) dst[n * 4] = pack16<BF16>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
         } else {
           const int64_t slot = static_cast<int64_t>(worker) * 2 + (unit0 < w0 ? 0 : 1);
-          const int64_t at = slot * kRows + g + 8 * i;
+          const int64_t at = slot * kRows + in;
           if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[i], l[i]);
           float2* dst = reinterpret_cast<float2*>(p.part_o + at * D + quad * 2);
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) dst[n * 4] = make_float2(o[n][2 * i], o[n][2 * i + 1]);
         }
       }
+      __syncwarp();
       fresh = true;
       unit0 = t + 1;
     }
@@ -423,13 +436,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   cp_wait<0>();
 }
 
+constexpr int kJoinWarps = 4;
+
 // Joins the tile kernel's parts of the cut unit that begins in CTA i's run:
-// block y of 8 takes 32 of its 256 rows, a thread one row and every eighth
+// block y of 8 takes 32 of its 256 rows, a thread one row and every fourth
 // group of 4 columns.
 template <bool BF16, int D>
 __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
   const Join u = p.joins[i];
-  const int row = y * 32 + (threadIdx.x & 31), r = u.r0 + row;
+  const int row = y * 32 + (threadIdx.x & 31), r = u.r0 + row, warp = threadIdx.x >> 5;
   if (u.last == 0 || r >= u.rows) return;
   auto part_of = [&](int k) { return k * 2ll + (k == i ? 1 : 0); };
   const float2* ml = reinterpret_cast<const float2*>(p.tile_ml);
@@ -437,7 +452,7 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
 #pragma unroll 4
   for (int k = i; k <= u.last; ++k) m = fmaxf(m, ml[part_of(k) * kUnitRows + row].x);
   const float ref = m == -INFINITY ? 0.0f : m;
-  constexpr int C = D / 32;  // column groups of a thread
+  constexpr int C = D / 4 / kJoinWarps;  // column groups of a thread
   float sum = 0.0f;
   float4 acc[C];
 #pragma unroll
@@ -449,8 +464,7 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
     sum = fmaf(v.y, f, sum);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const float4 o =
-          reinterpret_cast<const float4*>(p.tile_o)[(part_of(k) * (D / 4) + c * 8 + (threadIdx.x >> 5)) * kUnitRows + row];
+      const float4 o = reinterpret_cast<const float4*>(p.tile_o)[(part_of(k) * (D / 4) + c * kJoinWarps + warp) * kUnitRows + row];
       acc[c].x = fmaf(o.x, f, acc[c].x);
       acc[c].y = fmaf(o.y, f, acc[c].y);
       acc[c].z = fmaf(o.z, f, acc[c].z);
@@ -462,110 +476,110 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
   uint16_t* dst = p.out + (static_cast<int64_t>(u.t0 + tok) * p.H + u.kvh * p.G + (r - tok * p.G)) * D;
 #pragma unroll
   for (int c = 0; c < C; ++c)
-    *reinterpret_cast<uint2*>(dst + (c * 8 + (threadIdx.x >> 5)) * 4) =
+    *reinterpret_cast<uint2*>(dst + (c * kJoinWarps + warp) * 4) =
         make_uint2(pack16<BF16>(acc[c].x * inv, acc[c].y * inv), pack16<BF16>(acc[c].z * inv, acc[c].w * inv));
 }
 
 // Joins the parts of the units that were cut, and writes zeros for the rows
 // that no step covers: queries without keys and tokens behind the last
-// sequence.  A CTA per (sequence, token, kv head), 8 warps over its G rows.
-template <bool BF16, int D>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
+// sequence.  A CTA per (sequence, token, head) while that leaves SMs free (a
+// single long sequence is cut into a part for every worker, and its few rows
+// are joined from a hundred parts and more), a warp each beyond.
+template <bool BF16, int D, int SHARE>
+__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_constant__ Params p) {
   constexpr int V = D / 32;  // columns of a lane, side by side
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
-  __shared__ Vec sh_o[8][32];
-  const int row_ctas = p.B * p.combine_rows * p.Hkv;
+  __shared__ Vec sh_o[kJoinWarps][32];
+  constexpr int kPerCta = kJoinWarps / SHARE;
+  const int row_ctas = (p.B * p.combine_rows * p.H + kPerCta - 1) / kPerCta;
   if (static_cast<int>(blockIdx.x) >= row_ctas) {
     const int at = blockIdx.x - row_ctas;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     tile_join<BF16, D>(p, at / 8, at % 8);
     return;
   }
-  const int kvh = blockIdx.x % p.Hkv, y = blockIdx.x / p.Hkv % p.combine_rows;
-  const int b = blockIdx.x / p.Hkv / p.combine_rows;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto out_row = [&](int64_t tok, int h) { return p.out + (tok * p.H + h) * D; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
+  const int item = blockIdx.x * kPerCta + warp / SHARE;
+  const int h = item % p.H, y = item / p.H % p.combine_rows, b = item / p.H / p.combine_rows;
+  const int kvh = static_cast<int>(fdiv(static_cast<uint32_t>(h), p.div_g));
+  auto out_row = [&](int64_t tok, int head) { return p.out + (tok * p.H + head) * D; };
   // The index tensors are older than the row kernel; what follows the wait
   // reads or writes what the kernels before it may still be at.
-  const Work w = work_at(p, b);
+  const Work w = work_at(p, min(b, p.B - 1));
+  const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {  // tokens behind the last sequence
-    const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
     const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
     uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(end, 0));
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < words; i += row_ctas * 256ll) dst[i] = 0u;
+    const int64_t step = static_cast<int64_t>(row_ctas) * (kJoinWarps * 32);
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kJoinWarps * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
   }
-  if (static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
+  if (b >= p.B || static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
   const int64_t seq0 = p.prefix[b], run = p.prefix[p.B + 1];
-  const int share = p.G >= 8 ? 1 : 8 / p.G;  // warps of a row
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   for (int i = y; i < w.s.m; i += p.combine_rows) {
-    for (int g0 = 0; g0 < p.G; g0 += 8 / share) {
-      const int g = g0 + warp / share, part = warp % share;
-      const bool mine = g < p.G && warp < share * (8 / share);
-      const int r = i * p.G + g;
-      int64_t u0 = 0, first = 0, last = 0;
-      if (mine && w.tiles > 0) {
-        u0 = seq0 + (static_cast<int64_t>(kvh) * w.rts + r / kRows) * w.tiles;
-        first = u0 / run;
-        last = min(static_cast<int64_t>(p.workers) - 1, (u0 + w.tiles - 1) / run);
-      }
-      const bool cut = mine && last > first;
-      float sum = 0.0f, acc[V];
+    const int r = i * p.G + (h - kvh * p.G);
+    int64_t u0 = 0, first = 0;
+    int parts = 0;  // 0: no step covers the row
+    if (w.tiles > 0) {
+      u0 = seq0 + (static_cast<int64_t>(kvh) * w.rts + r / kRows) * w.tiles;
+      first = u0 / run;
+      parts = static_cast<int>(min(static_cast<int64_t>(p.workers) - 1, (u0 + w.tiles - 1) / run) - first) + 1;
+      if (parts == 1) continue;  // written by the row kernel
+    }
+    auto row_of = [&](int k) { return ((first + k) * 2 + (u0 < (first + k) * run ? 0 : 1)) * kRows + r % kRows; };
+    float sum = 0.0f, acc[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-      if (cut) {
-        auto row_of = [&](int64_t wk) { return (wk * 2 + (u0 < wk * run ? 0 : 1)) * kRows + r % kRows; };
-        const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-        // Every warp of the row finds the maximum and the sum of all parts, a
-        // lane 32 parts apart (the first 32 stay in registers) ...
-        const int64_t n_parts = last - first + 1;
-        float2 v0 = make_float2(-INFINITY, 0.0f);
-        if (lane < n_parts) v0 = ml[row_of(first + lane)];
-        float mx = v0.x;
-        for (int64_t k = lane + 32; k < n_parts; k += 32) mx = fmaxf(mx, ml[row_of(first + k)].x);
-        mx = warp_max(mx);
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float f0 = ex2(v0.x - ref);
-        sum = v0.y * f0;
-        for (int64_t k = lane + 32; k < n_parts; k += 32) {
-          const float2 v = ml[row_of(first + k)];
-          sum = fmaf(v.y, ex2(v.x - ref), sum);
-        }
-        sum = warp_sum(sum);
-        // ... and adds every `share`-th part's output, 32 parts at a time
-        for (int64_t k0 = 0; k0 < n_parts; k0 += 32) {
-          float f = f0;
-          if (k0 > 0) f = k0 + lane < n_parts ? ex2(ml[row_of(first + k0 + lane)].x - ref) : 0.0f;
-          const int n = static_cast<int>(min(static_cast<int64_t>(32), n_parts - k0));
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+    if (parts > 0) {
+      // Every warp finds the maximum and the sum of all parts, a lane 32
+      // parts apart (the first 32 stay in registers) ...
+      float2 v0 = make_float2(-INFINITY, 0.0f);
+      if (lane < parts) v0 = ml[row_of(lane)];
+      float mx = v0.x;
+      for (int k = lane + 32; k < parts; k += 32) mx = fmaxf(mx, ml[row_of(k)].x);
+      mx = warp_max(mx);
+      const float ref = mx == -INFINITY ? 0.0f : mx;
+      const float f0 = ex2(v0.x - ref);
+      sum = v0.y * f0;
+      for (int k = lane + 32; k < parts; k += 32) {
+        const float2 v = ml[row_of(k)];
+        sum = fmaf(v.y, ex2(v.x - ref), sum);
+      }
+      sum = warp_sum(sum);
+      // ... and adds every SHARE-th part's output
+      for (int k0 = 0; k0 < parts; k0 += 32) {
+        float f = f0;
+        if (k0 > 0) f = k0 + lane < parts ? ex2(ml[row_of(k0 + lane)].x - ref) : 0.0f;
+        const int n = min(32, parts - k0);
 #pragma unroll 8
-          for (int k = part; k < n; k += share) {
-            const Vec x = reinterpret_cast<const Vec*>(p.part_o + row_of(first + k0 + k) * D)[lane];
-            const float c = __shfl_sync(0xffffffffu, f, k);
+        for (int k = part; k < n; k += SHARE) {
+          const Vec x = reinterpret_cast<const Vec*>(p.part_o + row_of(k0 + k) * D)[lane];
+          const float c = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], c, acc[j]);
-          }
+          for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], c, acc[j]);
         }
       }
-      if (share > 1) {
-        __syncthreads();
-        Vec x;
+    }
+    if (SHARE > 1) {  // one row a CTA: all its warps are here
+      Vec x;
 #pragma unroll
-        for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
-        sh_o[warp][lane] = x;
-        __syncthreads();
-        if (part == 0 && mine)
-          for (int k = 1; k < share; ++k) {
-            const Vec y = sh_o[warp + k][lane];
+      for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
+      __syncthreads();  // the row before has been read
+      sh_o[warp][lane] = x;
+      __syncthreads();
+    }
+    if (part == 0) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += reinterpret_cast<const float*>(&y)[j];
-          }
+      for (int k = 1; k < SHARE; ++k) {
+        const Vec o = sh_o[k][lane];
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += reinterpret_cast<const float*>(&o)[j];
       }
-      if (mine && part == 0 && (w.tiles == 0 || cut)) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(w.s.t0 + i, kvh * p.G + g)) + lane * (V / 2);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(w.s.t0 + i, h)) + lane * (V / 2);
 #pragma unroll
-        for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
-      }
+      for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
     }
   }
 }
@@ -590,15 +604,16 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   // row kernel's writes itself, before it reads or writes anything).
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.combine_rows * p.Hkv + p.tile_ctas * 8));
-  cfg.blockDim = dim3(256);
+  const int per_cta = kJoinWarps / p.join_share;
+  cfg.gridDim = dim3(static_cast<unsigned>((p.B * p.combine_rows * p.H + per_cta - 1) / per_cta + p.tile_ctas * 8));
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<BF16, D>, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, p.join_share == 1 ? combine_kernel<BF16, D, 1> : combine_kernel<BF16, D, kJoinWarps>, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
 template <bool BF16, int D>
@@ -748,11 +763,12 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.timeout_ns = a->timeout_ns > 0 ? a->timeout_ns : 2000000000ll;
   // The combine covers this many tokens of a sequence side by side and the
   // rest in a loop; its grid stays below 2^31 CTAs.
-  const int64_t per_token = static_cast<int64_t>(p.B) * p.Hkv;
+  const int64_t per_token = static_cast<int64_t>(p.B) * p.H;
   if (per_token > 0x1fffffffLL) return B200K_ERR_SHAPE;
   int64_t rows = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
   if (p.tile_ctas > 0) rows = std::min<int64_t>(rows, kLongRows / p.G);
   p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 0x1fffffff / per_token)));
+  p.join_share = per_token * p.combine_rows <= 16ll * sms ? kJoinWarps : 1;
   if (a->dtype == B200K_BF16)
     return a->head_dim == 64 ? launch_cap<true, 64>(p, cap, ctas, st) : launch_cap<true, 128>(p, cap, ctas, st);
   return a->head_dim == 64 ? launch_cap<false, 64>(p, cap, ctas, st) : launch_cap<false, 128>(p, cap, ctas, st);
