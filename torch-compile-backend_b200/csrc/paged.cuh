@@ -30,7 +30,7 @@ struct Params {
   int32_t window;              // 0: none
   int32_t long_rows;           // sequences of more query rows (queries * G) run the tile kernel
   int32_t combine_rows;        // tokens of a sequence that the combine grid covers side by side
-  int32_t join_share;          // warps of the combine kernel for one row: 1 or 4
+  int32_t join_share;          // warps of the combine kernel for one row: 1, 4 or 16
   FastDiv div_page, div_g;
   int64_t table_stride;
   const uint16_t* q;

@@ -106,6 +106,17 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
   return v;
 }
 
+// n / d for n >= 0, d > 0: 32-bit where both fit, which every real list does
+// (a 64-bit division takes about 0.25 us, on the path to the first load).
+__device__ __forceinline__ int64_t div64(int64_t n, int64_t d) {
+  if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+// Steps that a worker takes of a list of `total`.
+__device__ __forceinline__ int64_t run_of(const Params& p, int64_t total) {
+  return max(static_cast<int64_t>(1), div64(total + p.workers - 1, p.workers));
+}
+
 // A position in the list of steps: within a sequence kv head by kv head, row
 // block by row block, key by key.
 struct Cursor {
@@ -219,7 +230,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     mine0 = mine;
     upto0 = upto;
   }
-  const int64_t run = max(static_cast<int64_t>(1), (total + p.workers - 1) / p.workers);
+  const int64_t run = run_of(p, total);
   if (worker == 0 && lane == 0) {
     p.prefix[p.B] = total;
     p.prefix[p.B + 1] = run;
@@ -245,26 +256,26 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     seq0 += __shfl_sync(0xffffffffu, upto, 31);
   }
   cur.w = work_at(p, cur.b);
-  const int unit = static_cast<int>((w0 - seq0) / cur.w.tiles);
+  const int unit = static_cast<int>(div64(w0 - seq0, cur.w.tiles));
   cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(unit) * cur.w.tiles);
   cur.kvh = unit / cur.w.rts;
   cur.rt = unit - cur.kvh * cur.w.rts;
 
   Cursor ld = cur;
   int64_t ld_t = w0;
-  // The page that holds this lane's key of the next step to load: fetched a
+  // The page that holds this lane's key of a step, -1 for no key: fetched a
   // step before its first use, so that no step waits for the table.
-  int page = 0;
-  auto lookup = [&] {
-    const int key = ld.w.base + ld.tile * kKeys + (lane & (kKeys - 1));
-    page = -1;
-    if (ld_t < w1 && key >= ld.w.s.lo && key < ld.w.s.n)
-      page = __ldg(p.table + ld.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
+  auto page_of = [&](const Cursor& c) {
+    const int key = c.w.base + c.tile * kKeys + (lane & (kKeys - 1));
+    if (key < c.w.s.lo || key >= c.w.s.n) return -1;
+    return __ldg(p.table + c.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
   };
-  lookup();
-  auto issue = [&](int stage) {
+  int page = -1;  // of the next step to load
+  page = page_of(ld);
+  int ld_stage = 0;
+  auto issue = [&] {
     if (ld_t < w1) {
-      const uint32_t sk = ring + stage * 2 * kTile, sv = sk + kTile;
+      const uint32_t sk = ring + ld_stage * 2 * kTile, sv = sk + kTile;
       const int c = lane % kChunks;
       const int64_t off = page_offset(p, page, ld.w.base + ld.tile * kKeys + (lane & (kKeys - 1)), ld.w.s.lo, ld.w.s.n, ld.kvh);
 #pragma unroll
@@ -277,14 +288,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
         cp16(sk + d, p.k + e, real);
         cp16(sv + d, p.v + e, real);
       }
-      ++ld_t;
-      if (ld_t < w1) ld.next(p);
-      lookup();
+      if (++ld_t < w1) {
+        ld.next(p);
+        page = page_of(ld);
+      }
     }
     cp_commit();
+    ld_stage = ld_stage + 1 == S ? 0 : ld_stage + 1;
   };
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s) issue(s);
 
   const int g = lane >> 2, quad = lane & 3;
   uint32_t qf[D / 16][4];
@@ -294,8 +305,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   bool fresh = true;
   int stage = 0;
   int64_t unit0 = seq0 + static_cast<int64_t>(unit) * cur.w.tiles;  // the current unit's first step
-  for (int64_t t = w0; t < w1; ++t) {
-    issue(stage == 0 ? S - 1 : stage - 1);
+  // The first S - 1 rounds only load.  One copy of the loading code: unrolled
+  // ahead of the loop, its instructions alone took 2 us to arrive.
+#pragma unroll 1
+  for (int64_t t = w0 - (S - 1); t < w1; ++t) {
+    issue();
+    if (t < w0) continue;
     if (fresh) {  // a new unit: its query rows as A fragments
       fresh = false;
       const int rows = cur.w.s.m * p.G, r0 = cur.rt * kRows;
@@ -482,40 +497,52 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
 
 // Joins the parts of the units that were cut, and writes zeros for the rows
 // that no step covers: queries without keys and tokens behind the last
-// sequence.  A CTA per (sequence, token, head) while that leaves SMs free (a
-// single long sequence is cut into a part for every worker, and its few rows
-// are joined from a hundred parts and more), a warp each beyond.
-template <bool BF16, int D, int SHARE>
-__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_constant__ Params p) {
+// sequence.  SHARE warps for each (sequence, token, head): 16 where there are
+// few rows (a single long sequence is cut into a part for every worker, and its
+// rows are joined from a hundred parts and more), 4, and one where the rows
+// alone fill the GPU.
+template <bool BF16, int D, int SHARE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) combine_kernel(const __grid_constant__ Params p) {
   constexpr int V = D / 32;  // columns of a lane, side by side
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
-  __shared__ Vec sh_o[kJoinWarps][32];
-  constexpr int kPerCta = kJoinWarps / SHARE;
+  constexpr int kBatch = SHARE == 4 ? 8 : SHARE == 16 ? 2 : 4;
+  __shared__ Vec sh_o[WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
+  constexpr int kPerCta = WARPS / SHARE;
   const int row_ctas = (p.B * p.combine_rows * p.H + kPerCta - 1) / kPerCta;
   if (static_cast<int>(blockIdx.x) >= row_ctas) {
     const int at = blockIdx.x - row_ctas;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    tile_join<BF16, D>(p, at / 8, at % 8);
+    if (warp < kJoinWarps) tile_join<BF16, D>(p, at / 8, at % 8);
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
   const int item = blockIdx.x * kPerCta + warp / SHARE;
   const int h = item % p.H, y = item / p.H % p.combine_rows, b = item / p.H / p.combine_rows;
   const int kvh = static_cast<int>(fdiv(static_cast<uint32_t>(h), p.div_g));
   auto out_row = [&](int64_t tok, int head) { return p.out + (tok * p.H + head) * D; };
-  // The index tensors are older than the row kernel; what follows the wait
-  // reads or writes what the kernels before it may still be at.
+  // The index tensors are older than the row kernel: what they say is worked
+  // out before the wait for it; what follows reads or writes what the kernels
+  // before this one may still be at.
   const Work w = work_at(p, min(b, p.B - 1));
   const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
+  int64_t seq0 = 0, run = 0;
+  if (p.B <= 32) {  // the list in one scan; else what the row kernel left
+    const int64_t mine = lane < p.B ? steps_of(p, work_at(p, lane)) : 0, upto = warp_scan(mine);
+    run = run_of(p, __shfl_sync(0xffffffffu, upto, 31));
+    seq0 = __shfl_sync(0xffffffffu, upto - mine, min(b, 31));
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {  // tokens behind the last sequence
     const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
     uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(end, 0));
-    const int64_t step = static_cast<int64_t>(row_ctas) * (kJoinWarps * 32);
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kJoinWarps * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
+    const int64_t step = static_cast<int64_t>(row_ctas) * (WARPS * 32);
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(WARPS * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
   }
   if (b >= p.B || static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
-  const int64_t seq0 = p.prefix[b], run = p.prefix[p.B + 1];
+  if (p.B > 32) {
+    seq0 = p.prefix[b];
+    run = p.prefix[p.B + 1];
+  }
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   for (int i = y; i < w.s.m; i += p.combine_rows) {
     const int r = i * p.G + (h - kvh * p.G);
@@ -523,8 +550,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     int parts = 0;  // 0: no step covers the row
     if (w.tiles > 0) {
       u0 = seq0 + (static_cast<int64_t>(kvh) * w.rts + r / kRows) * w.tiles;
-      first = u0 / run;
-      parts = static_cast<int>(min(static_cast<int64_t>(p.workers) - 1, (u0 + w.tiles - 1) / run) - first) + 1;
+      first = div64(u0, run);
+      parts = static_cast<int>(min(static_cast<int64_t>(p.workers) - 1, div64(u0 + w.tiles - 1, run)) - first) + 1;
       if (parts == 1) continue;  // written by the row kernel
     }
     auto row_of = [&](int k) { return ((first + k) * 2 + (u0 < (first + k) * run ? 0 : 1)) * kRows + r % kRows; };
@@ -533,31 +560,52 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
     if (parts > 0) {
       // Every warp finds the maximum and the sum of all parts, a lane 32
-      // parts apart (the first 32 stay in registers) ...
-      float2 v0 = make_float2(-INFINITY, 0.0f);
-      if (lane < parts) v0 = ml[row_of(lane)];
-      float mx = v0.x;
-      for (int k = lane + 32; k < parts; k += 32) mx = fmaxf(mx, ml[row_of(k)].x);
+      // parts apart (the first 32 kKept parts' in registers, loaded together) ...
+      constexpr int kKept = SHARE == 1 ? 1 : 4;
+      float2 v[kKept];
+#pragma unroll
+      for (int c = 0; c < kKept; ++c) {
+        v[c] = make_float2(-INFINITY, 0.0f);
+        if (lane + 32 * c < parts) v[c] = ml[row_of(lane + 32 * c)];
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kKept; ++c) mx = fmaxf(mx, v[c].x);
+      for (int k = lane + 32 * kKept; k < parts; k += 32) mx = fmaxf(mx, ml[row_of(k)].x);
       mx = warp_max(mx);
       const float ref = mx == -INFINITY ? 0.0f : mx;
-      const float f0 = ex2(v0.x - ref);
-      sum = v0.y * f0;
-      for (int k = lane + 32; k < parts; k += 32) {
-        const float2 v = ml[row_of(k)];
-        sum = fmaf(v.y, ex2(v.x - ref), sum);
+#pragma unroll
+      for (int c = 0; c < kKept; ++c) {
+        v[c].x = ex2(v[c].x - ref);  // the part's weight
+        sum = fmaf(v[c].y, v[c].x, sum);
+      }
+      for (int k = lane + 32 * kKept; k < parts; k += 32) {
+        const float2 u = ml[row_of(k)];
+        sum = fmaf(u.y, ex2(u.x - ref), sum);
       }
       sum = warp_sum(sum);
       // ... and adds every SHARE-th part's output
       for (int k0 = 0; k0 < parts; k0 += 32) {
-        float f = f0;
-        if (k0 > 0) f = k0 + lane < parts ? ex2(ml[row_of(k0 + lane)].x - ref) : 0.0f;
-        const int n = min(32, parts - k0);
-#pragma unroll 8
-        for (int k = part; k < n; k += SHARE) {
-          const Vec x = reinterpret_cast<const Vec*>(p.part_o + row_of(k0 + k) * D)[lane];
-          const float c = __shfl_sync(0xffffffffu, f, k);
+        float f = v[0].x;
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], c, acc[j]);
+        for (int c = 1; c < kKept; ++c)
+          if (k0 == 32 * c) f = v[c].x;
+        if (k0 >= 32 * kKept) f = k0 + lane < parts ? ex2(ml[row_of(k0 + lane)].x - ref) : 0.0f;
+        const int n = min(32, parts - k0);
+        for (int k = part; k < n; k += SHARE * kBatch) {
+          Vec x[kBatch];  // loaded together, whatever their number
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            x[i] = Vec();
+            if (k + i * SHARE < n) x[i] = reinterpret_cast<const Vec*>(p.part_o + row_of(k0 + k + i * SHARE) * D)[lane];
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const float c = __shfl_sync(0xffffffffu, f, (k + i * SHARE) & 31);
+            if (k + i * SHARE >= n) break;
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x[i])[j], c, acc[j]);
+          }
         }
       }
     }
@@ -604,16 +652,19 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   // row kernel's writes itself, before it reads or writes anything).
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  const int per_cta = kJoinWarps / p.join_share;
+  const int warps = std::max(kJoinWarps, p.join_share), per_cta = warps / p.join_share;
   cfg.gridDim = dim3(static_cast<unsigned>((p.B * p.combine_rows * p.H + per_cta - 1) / per_cta + p.tile_ctas * 8));
-  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.blockDim = dim3(warps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, p.join_share == 1 ? combine_kernel<BF16, D, 1> : combine_kernel<BF16, D, kJoinWarps>, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+  auto combine = p.join_share == 1   ? combine_kernel<BF16, D, 1, kJoinWarps>
+                 : p.join_share == 4 ? combine_kernel<BF16, D, 4, kJoinWarps>
+                                     : combine_kernel<BF16, D, 16, 16>;
+  return cudaLaunchKernelEx(&cfg, combine, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
 template <bool BF16, int D>
@@ -768,7 +819,8 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   int64_t rows = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
   if (p.tile_ctas > 0) rows = std::min<int64_t>(rows, kLongRows / p.G);
   p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 0x1fffffff / per_token)));
-  p.join_share = per_token * p.combine_rows <= 16ll * sms ? kJoinWarps : 1;
+  const int64_t join_rows = per_token * p.combine_rows;
+  p.join_share = join_rows <= 2ll * sms ? 16 : join_rows <= 16ll * sms ? 4 : 1;
   if (a->dtype == B200K_BF16)
     return a->head_dim == 64 ? launch_cap<true, 64>(p, cap, ctas, st) : launch_cap<true, 128>(p, cap, ctas, st);
   return a->head_dim == 64 ? launch_cap<false, 64>(p, cap, ctas, st) : launch_cap<false, 128>(p, cap, ctas, st);
