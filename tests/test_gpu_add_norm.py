@@ -166,3 +166,15 @@ def test_c_abi_and_another_stream():
         cabi.add_rms_norm(x, r, w, 1e-5, total, out, scale, 128)
     side.synchronize()
     check_quant(out, scale, total, x, r, w, 128)
+
+
+def test_dims_of_one_element_have_no_say_in_flattening():
+    """[4, 1, 3, cols] cut from four rows of each of four blocks: the size-one
+    dim's stride looks like a row stride and is none."""
+    x, r, w = make(16, 256, torch.bfloat16)
+    a, b = x.view(4, 1, 4, 256)[:, :, :3], r.view(4, 1, 4, 256)[:, :, :3]
+    out, total = torch.ops.b200.add_rms_norm(a, b, w, 1e-5)
+    check(out.reshape(12, 256), total.reshape(12, 256), a.reshape(12, 256), b.reshape(12, 256), w, 1e-5)
+    a, b = x.view(16, 1, 256)[::2], r.view(16, 1, 256)[1::2]
+    out, total = torch.ops.b200.add_rms_norm(a, b, w, 1e-5)
+    check(out.reshape(8, 256), total.reshape(8, 256), a.reshape(8, 256), b.reshape(8, 256), w, 1e-5)

@@ -2,6 +2,10 @@
 derived at serving_reference.attention_close).  Everything of the caches that
 no query may see holds NaN, and tables name no page that is not needed, so a
 read outside the mask shows in the output or in the status word."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -256,3 +260,51 @@ def test_stalled_wait_times_out_and_context_survives():
     assert status.item() == 0
     want, size = ref.paged_attention(*x, ref.default_scale(128))
     ref.attention_close(out, want, size, BF)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_q_start_that_runs_backwards_stays_inside_the_workspace(D):
+    """Every other sequence claims all tokens: many times the 256-row blocks
+    that the workspace is sized for.  Reported, and nothing past it written."""
+    q, kc, vc, table, _, _ = ref.paged_inputs([300], [300], 4, 2, D, 16, BF)
+    seqs = 64
+    table = table.clamp_min(0).expand(seqs, -1).contiguous()
+    q_start = torch.tensor([0, 300] * (seqs // 2) + [0], dtype=torch.int32, device="cuda")
+    kv_len = torch.full((seqs,), 300, dtype=torch.int32, device="cuda")
+    out, status = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    need = cabi.paged_attention(q, kc, vc, table, q_start, kv_len, out, status=status)
+    ws = torch.full((need + (1 << 20),), 0x5a, dtype=torch.uint8, device="cuda")
+    status.zero_()
+    cabi.paged_attention(q, kc, vc, table, q_start, kv_len, out, status=status, workspace=ws)
+    assert status.item() == 9
+    assert (ws[need:] == 0x5a).all()
+
+
+def test_strides_of_dims_of_one_element_do_not_matter():
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([1], [40], 1, 1, 64, 16, BF)
+    one = lambda t: t.as_strided(t.shape, tuple(s if n > 1 else 7 for n, s in zip(t.shape, t.stride())))  # noqa: E731
+    want = torch.ops.b200.paged_attention(q, kc, vc, table, q_start, kv_len)
+    got = torch.ops.b200.paged_attention(one(q), one(kc), vc, one(table), q_start, kv_len)
+    assert torch.equal(got, want)
+
+
+def test_a_first_call_inside_a_capture():
+    """A process whose first paged_attention calls (both kernels) are being
+    captured: no status word exists yet, no attribute is set."""
+    code = """
+import sys; sys.path[:0] = [%r, %r]
+import torch, serving_reference as ref
+from compiler import runtime
+runtime.load()
+x = ref.paged_inputs([1, 300], [90, 300], 8, 2, 64, 16, torch.bfloat16)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = torch.ops.b200.paged_attention(*x)
+g.replay()
+want, size = ref.paged_attention(*x, ref.default_scale(64))
+ref.attention_close(out, want, size, torch.bfloat16)
+print("fine")
+""" % (os.path.dirname(ref.__file__), os.path.dirname(os.path.dirname(os.path.dirname(cabi.__file__))))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]

@@ -186,3 +186,9 @@ def test_c_abi():
     cabi.rope_append(*args, out, status=status)
     assert status.item() == 0
     check(before, out, args)
+
+
+def test_strides_of_dims_of_one_element_do_not_matter():
+    q, k, v, cos, sin, pos, slots, kc, vc = make(1, 1, 1, 64, 64, 16, torch.bfloat16, fused=False)
+    one = lambda t: t.as_strided(t.shape, tuple(s if n > 1 else 7 for n, s in zip(t.shape, t.stride())))  # noqa: E731
+    run((one(q), one(k), one(v), cos, sin, pos, slots, one(kc), vc))

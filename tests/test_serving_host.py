@@ -106,6 +106,7 @@ def attn_args(**kw):
     (dict(kv_heads=0), SHAPE), (dict(q=0), ARG), (dict(dtype=cabi.F32), UNSUPPORTED), (dict(softcap=-1.0), ARG),
     (dict(window=-1), ARG), (dict(q=4098), ALIGN), (dict(q_strides=[510, 64]), ALIGN),
     (dict(cache_strides=[2048, 130, 64]), ALIGN), (dict(softcap=float("nan")), ARG),
+    (dict(softcap=float("inf")), ARG), (dict(scale=float("inf")), ARG), (dict(scale=float("nan")), ARG),
 ])
 def test_paged_attention_refuses(kw, code):
     assert cabi.library().b200k_paged_attention(ctypes.byref(attn_args(**kw)), None) == code

@@ -78,9 +78,9 @@ def _passes(gm: fx.GraphModule) -> fx.GraphModule:
 
 
 class StatusChecked:
-    """Boxed callable around a compiled graph that launches GEMMs: before each
-    call it raises if an earlier GEMM on the device reported a device-side
-    timeout, and after the call it queues an asynchronous read-back of the
+    """Boxed callable around a compiled graph that launches GEMMs or the paged
+    cache's kernels: before each call it raises if an earlier one on the
+    device reported a device-side timeout or an index out of range, and after the call it queues an asynchronous read-back of the
     device's status word (``torch.ops.b200.status_check``).  Without it a
     timed-out GEMM would hand a partly written tensor to the rest of the
     graph with no error; with it the error surfaces at the next compiled
@@ -102,10 +102,17 @@ class StatusChecked:
         return out
 
 
+# Ops whose kernels report through the device's status word: waits that run
+# out, indexes out of range.
+_REPORTING = (torch.ops.b200.gemm_epilogue.default, torch.ops.b200.rope_append.default,
+              torch.ops.b200.paged_attention.default)
+
+
 def _gemm_device(gm: fx.GraphModule, example_inputs) -> int | None:
-    """CUDA device index of the graph's GEMM launches, None when it has none."""
+    """CUDA device index of the graph's GEMM launches (and other launches that
+    report through the status word), None when it has none."""
     for n in gm.graph.nodes:
-        if n.op == "call_function" and n.target == torch.ops.b200.gemm_epilogue.default:
+        if n.op == "call_function" and n.target in _REPORTING:
             val = n.args[0].meta.get("val") if isinstance(n.args[0], fx.Node) else None
             if isinstance(val, torch.Tensor) and val.is_cuda:
                 return val.device.index if val.device.index is not None else torch.cuda.current_device()

@@ -439,8 +439,10 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     q_start: torch.Tensor, kv_len: torch.Tensor, out: torch.Tensor, scale: float = 0.0,
                     softcap: float = 0.0, window: int = 0, max_q_len: int = 0, status: torch.Tensor | None = None,
-                    timeout_ns: int = 0, test_flags: int = 0) -> None:
-    """Attention of packed queries [tokens, H, D] over a paged cache, into `out`."""
+                    timeout_ns: int = 0, test_flags: int = 0, workspace: torch.Tensor | None = None) -> int:
+    """Attention of packed queries [tokens, H, D] over a paged cache, into `out`.
+    Returns the workspace bytes it needs; `workspace` (of at least those) is
+    allocated when not given."""
     a = PagedAttentionArgs()
     a.tokens, a.heads, a.head_dim = q.shape
     a.seqs, a.kv_heads = kv_len.shape[0], k_cache.shape[2]
@@ -457,8 +459,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     n = ctypes.c_int64()
     _check("b200k_paged_attention_workspace",
            library().b200k_paged_attention_workspace(ctypes.byref(a), ctypes.byref(n)))
-    ws = torch.empty(max(1, n.value), dtype=torch.uint8, device=q.device)
+    ws = workspace if workspace is not None else torch.empty(max(1, n.value), dtype=torch.uint8, device=q.device)
+    if ws.numel() < n.value:
+        raise ValueError(f"workspace of {ws.numel()} bytes, {n.value} needed")
     a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
     a.status = status.data_ptr() if status is not None else None
     a.timeout_ns = timeout_ns
     _check("b200k_paged_attention", library().b200k_paged_attention(ctypes.byref(a), _stream()))
+    return n.value

@@ -47,7 +47,8 @@ struct Params {
   int32_t workers;
   // tile kernel: steps count kPortionCost a unit; [0] all, [1] a CTA's, [2] entries, [3 + e] before entry e
   int64_t* entry_steps;
-  int2* entries;               // (sequence, 256-row block)
+  int2* entries;               // (sequence, 256-row block), at most max_entries
+  int32_t max_entries;
   float* tile_o;               // [CTAs][2][D / 4][256][4]
   float* tile_ml;              // [CTAs][2][256][2]
   Join* joins;                 // [CTAs] the cut unit that begins in each CTA's run

@@ -169,6 +169,9 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
     }
     int64_t all;
     const int64_t upto = block_scan(n, all);
+    // A q_start that runs backwards gives tokens to several sequences: the
+    // list ends where the workspace does (seq_at reports it).
+    all = min(all, static_cast<int64_t>(p.max_entries - entry0));
     starts[tid] = static_cast<int>(upto - n);
     if (tid == 0) starts[kWarps * 32] = static_cast<int>(all);
     __syncthreads();
@@ -707,6 +710,12 @@ bool may_be_long(const B200kPagedAttentionArgs* a) {
   return q * (a->heads / a->kv_heads) > kLongRows;
 }
 
+// Entries of the tile kernel's list: 256-row blocks of sequences that share the
+// tokens out among them.
+int64_t max_entries(const B200kPagedAttentionArgs* a) {
+  return a->tokens * (a->heads / a->kv_heads) / kUnitRows + a->seqs;
+}
+
 // Where each part of the workspace begins; returns its size.
 int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p) {
   int64_t at = 0;
@@ -721,7 +730,7 @@ int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p)
   uint8_t* prefix = take((a->seqs + 2) * 8);
   uint8_t *steps = ws, *entries = ws, *tile_o = ws, *tile_ml = ws, *joins = ws;
   if (may_be_long(a)) {
-    const int64_t n = a->tokens * (a->heads / a->kv_heads) / kUnitRows + a->seqs + 1;
+    const int64_t n = max_entries(a) + 1;
     steps = take((n + 4) * 8);
     entries = take(n * 8);
     tile_o = take(static_cast<int64_t>(sms) * 2 * kUnitRows * a->head_dim * 4);
@@ -761,7 +770,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   if (a->tokens == 0 || a->heads == 0) return B200K_OK;
   if (!a->q || !a->out) return B200K_ERR_ARG;
   if (a->dtype != B200K_BF16 && a->dtype != B200K_F16) return B200K_ERR_UNSUPPORTED;
-  if (!(a->softcap >= 0.0f) || a->window < 0 || !(a->scale == a->scale)) return B200K_ERR_ARG;
+  if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap) || a->window < 0 || !std::isfinite(a->scale)) return B200K_ERR_ARG;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out)) return B200K_ERR_ALIGN;
   for (int d = 0; d < 2; ++d)
     if (a->q_strides[d] < 0 || a->q_strides[d] % 8) return B200K_ERR_ALIGN;
@@ -790,6 +799,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.capacity = static_cast<int32_t>(keys);
   p.window = static_cast<int32_t>(std::min<int64_t>(a->window, 0x3fffffff));
   p.tile_ctas = may_be_long(a) ? sms : 0;
+  p.max_entries = static_cast<int32_t>(max_entries(a));
   p.long_rows = p.tile_ctas > 0 ? kLongRows : 0x7fffffff;
   p.test_flags = a->test_flags;
   p.div_page = make_fastdiv(static_cast<uint32_t>(p.page_size));
@@ -811,6 +821,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   const float scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
   p.mul = cap ? 2.0f * scale / a->softcap * kLog2e : scale * kLog2e;
   p.cap2 = a->softcap * kLog2e;
+  if (!std::isfinite(p.mul)) return B200K_ERR_ARG;  // a cap too small for its scale
   const int ctas = sms * kCtasPerSm;
   p.workers = ctas * kWarps;
   place(a, sms, static_cast<uint8_t*>(a->workspace), &p);

@@ -575,22 +575,31 @@ void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r
   no_grad_inputs(what, {&x_in, &r_in});
   c10::cuda::CUDAGuard guard(x_in.device());
   const int64_t cols = x_in.size(-1);
-  // rows that do not flatten to one stride, or columns that are apart, are copied
-  auto rows_view = [&](const at::Tensor& t) {
-    bool ok = t.stride(-1) == 1 || cols == 1;
-    for (int64_t d = t.dim() - 3; d >= 0 && ok; --d)
-      ok = t.size(d) == 1 || t.stride(d) == t.stride(d + 1) * t.size(d + 1);
-    return ok ? t : t.contiguous();
+  // Row stride of t's flattened leading dims (those of size one have no say),
+  // -1 when they do not flatten or the columns lie apart.
+  auto row_stride = [&](const at::Tensor& t) -> int64_t {
+    if (t.stride(-1) != 1 && cols > 1) return -1;
+    int64_t stride = -1, expect = 0;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+      if (t.size(d) == 1) continue;
+      if (stride < 0) stride = expect = t.stride(d);
+      else if (t.stride(d) != expect) return -1;
+      expect *= t.size(d);
+    }
+    return stride < 0 ? cols : stride;
   };
-  const at::Tensor x = rows_view(x_in), r = rows_view(r_in);
+  int64_t xs = row_stride(x_in), rs = row_stride(r_in);
+  const at::Tensor x = xs < 0 ? x_in.contiguous() : x_in, r = rs < 0 ? r_in.contiguous() : r_in;
+  if (xs < 0) xs = cols;
+  if (rs < 0) rs = cols;
   B200kAddNormArgs a;
   std::memset(&a, 0, sizeof(a));
   a.cols = cols;
   a.rows = cols == 0 ? 0 : x.numel() / cols;
   a.x = x.data_ptr();
   a.residual = r.data_ptr();
-  a.x_row_stride = x.dim() >= 2 ? x.stride(-2) : cols;
-  a.residual_row_stride = r.dim() >= 2 ? r.stride(-2) : cols;
+  a.x_row_stride = xs;
+  a.residual_row_stride = rs;
   a.dtype = to_dt(x.scalar_type());
   at::Tensor w;
   if (weight.has_value() && weight->defined()) {
@@ -638,14 +647,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant(const at::Tens
   return {out, scale, sum};
 }
 
+// A dim's stride, 0 where it has one element (or none) and no step is taken.
+int64_t step_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 void check_caches(const char* what, const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc) {
-  TORCH_CHECK(kc.dim() == 4 && kc.sizes() == vc.sizes() && kc.strides() == vc.strides(), "b200::", what,
-              ": k_cache and v_cache must be [pages, page size, kv heads, head dim] of one shape and strides, got ",
-              kc.sizes(), " and ", vc.sizes());
+  TORCH_CHECK(kc.dim() == 4 && kc.sizes() == vc.sizes(), "b200::", what,
+              ": k_cache and v_cache must be [pages, page size, kv heads, head dim] of one shape, got ", kc.sizes(), " and ",
+              vc.sizes());
+  for (int64_t d = 0; d < 4; ++d)
+    TORCH_CHECK(step_of(kc, d) == step_of(vc, d), "b200::", what, ": k_cache and v_cache must have the same strides, got ",
+                kc.strides(), " and ", vc.strides());
   TORCH_CHECK(kc.scalar_type() == q.scalar_type() && vc.scalar_type() == q.scalar_type(), "b200::", what,
               ": the caches must have q's dtype");
   TORCH_CHECK(kc.device() == q.device() && vc.device() == q.device(), "b200::", what, ": the caches must be on q's device");
-  TORCH_CHECK(kc.size(3) == q.size(2) && (kc.stride(3) == 1 || kc.numel() == 0), "b200::", what,
+  TORCH_CHECK(kc.size(3) == q.size(2) && (kc.size(3) <= 1 || kc.stride(3) == 1 || kc.numel() == 0), "b200::", what,
               ": the caches' last dim must be head_dim with unit stride");
 }
 
@@ -663,8 +678,8 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
     TORCH_CHECK(t->stride(2) == 1 || t->numel() == 0 || t->size(2) == 1, "b200::rope_append: q, k, v need a unit last-dim stride");
   check_caches(what, q, k_cache, v_cache);
   TORCH_CHECK(k_cache.size(2) == k.size(1), "b200::rope_append: the caches have ", k_cache.size(2), " heads, k has ", k.size(1));
-  TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.strides() == sin.strides() &&
-                  cos.scalar_type() == sin.scalar_type() && (cos.stride(1) == 1 || cos.size(1) <= 1) &&
+  TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && step_of(cos, 0) == step_of(sin, 0) &&
+                  cos.scalar_type() == sin.scalar_type() && (cos.size(1) <= 1 || (cos.stride(1) == 1 && sin.stride(1) == 1)) &&
                   2 * cos.size(1) <= q.size(2),
               "b200::rope_append: cos and sin must be [rows, rotary dim / 2] alike, at most head_dim / 2 columns of unit "
               "stride, got ", cos.sizes(), " and ", sin.sizes());
@@ -678,11 +693,8 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   for (const at::Tensor* t : {&cos, &sin, &positions, &slots})
     TORCH_CHECK(t->device() == q.device(), "b200::rope_append: every tensor must be on q's device");
   no_grad_inputs(what, {&q, &k, &v, &cos, &sin, &k_cache, &v_cache});
-  // a cache that overlaps itself (expanded) has several elements in one place
-  TORCH_CHECK(k_cache.numel() == 0 || k_cache.is_non_overlapping_and_dense() || [&] {
-    for (int d = 0; d < 4; ++d) if (k_cache.size(d) > 1 && k_cache.stride(d) == 0) return false;
-    return true;
-  }(), "b200::rope_append: the caches must not be expanded");
+  for (int64_t d = 0; d < 4; ++d)  // several elements in one place
+    TORCH_CHECK(k_cache.size(d) <= 1 || k_cache.stride(d) != 0, "b200::rope_append: the caches must not be expanded");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
   B200kRopeAppendArgs a;
@@ -701,15 +713,15 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   a.k_cache = k_cache.data_ptr();
   a.v_cache = v_cache.data_ptr();
   for (int d = 0; d < 2; ++d) {
-    a.q_strides[d] = q.stride(d);
-    a.k_strides[d] = k.stride(d);
-    a.v_strides[d] = v.stride(d);
+    a.q_strides[d] = step_of(q, d);
+    a.k_strides[d] = step_of(k, d);
+    a.v_strides[d] = step_of(v, d);
   }
-  for (int d = 0; d < 3; ++d) a.cache_strides[d] = k_cache.stride(d);
+  for (int d = 0; d < 3; ++d) a.cache_strides[d] = step_of(k_cache, d);
   a.cos = cos.data_ptr();
   a.sin = sin.data_ptr();
   a.table_rows = cos.size(0);
-  a.table_stride = cos.stride(0);
+  a.table_stride = step_of(cos, 0);
   a.positions = positions.data_ptr();
   a.slots = slots.data_ptr();
   a.dtype = to_dt(q.scalar_type());
@@ -739,7 +751,6 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   for (const at::Tensor* t : {&page_table, &q_start, &kv_len})
     TORCH_CHECK(t->scalar_type() == at::kInt && t->device() == q.device() && (t->size(-1) <= 1 || t->stride(-1) == 1),
                 "b200::paged_attention: page_table, q_start and kv_len must be int32 on q's device with unit last-dim stride");
-  TORCH_CHECK(page_table.stride(0) >= 0, "b200::paged_attention: page_table stride");
   TORCH_CHECK(softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::paged_attention: softcap, window and max_q_len must not "
               "be negative");
   no_grad_inputs(what, {&q, &k_cache, &v_cache});
@@ -755,12 +766,12 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   a.num_pages = k_cache.size(0);
   a.page_size = k_cache.size(1);
   a.table_cols = page_table.size(1);
-  a.table_stride = page_table.stride(0);
+  a.table_stride = step_of(page_table, 0);
   a.q = q.data_ptr();
-  for (int d = 0; d < 2; ++d) a.q_strides[d] = q.stride(d);
+  for (int d = 0; d < 2; ++d) a.q_strides[d] = step_of(q, d);
   a.k_cache = k_cache.data_ptr();
   a.v_cache = v_cache.data_ptr();
-  for (int d = 0; d < 3; ++d) a.cache_strides[d] = k_cache.stride(d);
+  for (int d = 0; d < 3; ++d) a.cache_strides[d] = step_of(k_cache, d);
   a.out = out.data_ptr();
   a.page_table = page_table.data_ptr<int32_t>();
   a.q_start = q_start.data_ptr<int32_t>();
