@@ -471,9 +471,11 @@ int b200k_attention(const B200kAttentionArgs* args, void* stream);
  *     scales s = max(max |y|, 1e-12) / 448 of each row (group 0: scale
  *     [rows]) or of every 128 columns (group 128, cols a multiple of it:
  *     scale [rows, cols / 128]).
- * A row that holds an infinity or NaN gives NaN (with a NaN scale).  Eight
- * columns a thread when cols and the row strides are multiples of 8 and the
- * pointers 16-byte aligned; any other layout runs one column a thread.
+ * A sum that is NaN makes its whole row NaN; an infinite one makes its own
+ * column NaN and, as 1 / sqrt(inf) is 0, the row's others 0 (e4m3: NaN for
+ * every column of its scale, and the scale).  Any strides and alignment; fastest when
+ * cols and the row strides are multiples of 8 and the pointers 16-byte
+ * aligned.
  */
 typedef struct {
   int64_t rows, cols;
@@ -557,7 +559,9 @@ int b200k_rope_append(const B200kRopeAppendArgs* args, void* stream);
  * b200k_rope_append; strides multiples of 8 elements, pointers 16-byte
  * aligned; out contiguous.  Nothing is read of the caches outside the keys
  * that a sequence's queries see, so other pages and the rest of the last one
- * may hold anything.  Scores, softmax and sums are fp32; the probabilities are
+ * may hold anything.  Of the keys that some query of the sequence sees, those
+ * hidden from another query have weight 0 for it: their values must be
+ * finite, or it may become NaN, as 0 * inf does.  Scores, softmax and sums are fp32; the probabilities are
  * rounded to the input type for the second product.  max_q_len (0: unknown)
  * is a hint of the longest sequence's queries: it chooses kernels and grids,
  * never results.  Index tensors are i32 on the device; entries out of range

@@ -96,6 +96,20 @@ def test_many_sequences():
     run(ref.paged_inputs([1] * len(ns), ns, 2, 1, 64, 16, BF))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("seqs,H,hkv,max_q", [(20, 32, 4, 0), (48, 16, 2, 1), (200, 16, 2, 0)])
+def test_long_sequences_among_short_ones(seqs, H, hkv, max_q, D):
+    """Rows of one part and of hundreds in one call, as the join's warps share
+    them out: a CTA's own rows and those of all its warps, up to 32 sequences
+    and more, more rows than one a warp side by side (max_q 1, 3 queries)."""
+    ns = [i % 7 for i in range(seqs)]
+    ns[3], ns[seqs // 2] = 6000, 700
+    qs = [1] * seqs
+    qs[3] = qs[4] = 3
+    ns[4] = 2  # one of the three without keys
+    run(ref.paged_inputs(qs, ns, H, hkv, D, 16, BF), max_q=max_q)
+
+
 def test_strided_queries():
     q, *rest = ref.paged_inputs([1, 5, 2], [30, 60, 2], 8, 2, 64, 16, BF)
     wide = torch.zeros(q.shape[0], 12, 64, device="cuda", dtype=BF)

@@ -13,7 +13,8 @@ constexpr int kRows = 16;      // query rows of one unit of the row kernel (one 
 constexpr int kBlock = 64;     // keys of one step of the tile kernel
 constexpr int kUnitRows = 256; // query rows of one unit of the tile kernel (two MMA m)
 // What a unit's start and end cost (queries in, output out, pipeline empty),
-// in steps: counted in the list that the CTAs share out.
+// in steps: counted in the list that the CTAs share out.  8 prompts of 2048
+// (32 heads of 64) with 0, 2, 4 and 8: 387, 300, 277 and 297 us.
 constexpr int kPortionCost = 4;
 
 // A unit of the tile kernel whose parts lie in CTAs i (slot 1) to last (slot 0).
@@ -30,7 +31,7 @@ struct Params {
   int32_t window;              // 0: none
   int32_t long_rows;           // sequences of more query rows (queries * G) run the tile kernel
   int32_t combine_rows;        // tokens of a sequence that the combine grid covers side by side
-  int32_t join_share;          // warps of the combine kernel for one row: 1, 4 or 16
+  int32_t join_mode;           // how the combine kernel's warps share the rows
   FastDiv div_page, div_g;
   int64_t table_stride;
   const uint16_t* q;

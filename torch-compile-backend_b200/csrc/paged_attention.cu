@@ -21,7 +21,9 @@
 // memory does not) and keeps its running maximum, sum and output in fp32.
 // A unit inside one run is written at once; a cut one leaves its parts
 // (max, sum, unnormalised output, fp32) in the workspace, and
-// combine_kernel joins them in the order of the keys.
+// combine_kernel joins them in an order that only the lengths decide.
+// Measured: one token of 64 sequences to 8192 keys, 32 / 8 heads of 128, 211 us
+// = 6.48 TB/s; of 3 sequences to 65536 keys 95 us = 6.05 TB/s.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -502,139 +504,217 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
         make_uint2(pack16<BF16>(acc[c].x * inv, acc[c].y * inv), pack16<BF16>(acc[c].z * inv, acc[c].w * inv));
 }
 
-// Joins the parts of the units that were cut, and writes zeros for the rows
-// that no step covers: queries without keys and tokens behind the last
-// sequence.  SHARE warps for each (sequence, token, head): 16 where there are
-// few rows (a single long sequence is cut into a part for every worker, and its
-// rows are joined from a hundred parts and more), 4, and one where the rows
-// alone fill the GPU.
-template <bool BF16, int D, int SHARE, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) combine_kernel(const __grid_constant__ Params p) {
+// The parts of a query row, one for each worker whose run holds steps of the
+// row's unit: workers first .. first + n - 1.  n = 0: no step covers the row
+// (zeros); n = 1: the row kernel has written it.
+struct RowParts {
+  int64_t unit0, run, first;
+  int n;
+  __device__ __forceinline__ int64_t at(int k, int row) const {
+    return ((first + k) * 2 + (unit0 < (first + k) * run ? 0 : 1)) * kRows + row;
+  }
+};
+
+// Joins a row's parts (`row`: of its 16), SHARE warps together: every warp
+// finds the maximum and the sum of all parts, a lane 32 parts apart (the first
+// 32 kKept parts' in registers, loaded together), and adds every SHARE-th
+// part's output, kBatch loaded together whatever their number; the warps' sums
+// meet in shared memory.
+template <bool BF16, int D, int SHARE>
+__device__ __forceinline__ void join_row(const Params& p, const RowParts& rp, int row, uint32_t* dst,
+                                         typename std::conditional<D == 128, float4, float2>::type (*sh_o)[32]) {
   constexpr int V = D / 32;  // columns of a lane, side by side
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
-  constexpr int kBatch = SHARE == 4 ? 8 : SHARE == 16 ? 2 : 4;
-  __shared__ Vec sh_o[WARPS][32];
+  constexpr int kBatch = SHARE > 1 ? 8 : 4;
+  constexpr int kKept = SHARE > 1 ? 4 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
-  constexpr int kPerCta = WARPS / SHARE;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  const int parts = rp.n;
+  float sum = 0.0f, acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+  if (parts > 0) {
+    float2 v[kKept];
+#pragma unroll
+    for (int c = 0; c < kKept; ++c) {
+      v[c] = make_float2(-INFINITY, 0.0f);
+      if (lane + 32 * c < parts) v[c] = ml[rp.at(lane + 32 * c, row)];
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kKept; ++c) mx = fmaxf(mx, v[c].x);
+    for (int k = lane + 32 * kKept; k < parts; k += 32) mx = fmaxf(mx, ml[rp.at(k, row)].x);
+    mx = warp_max(mx);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int c = 0; c < kKept; ++c) {
+      v[c].x = ex2(v[c].x - ref);  // the part's weight
+      sum = fmaf(v[c].y, v[c].x, sum);
+    }
+    for (int k = lane + 32 * kKept; k < parts; k += 32) {
+      const float2 u = ml[rp.at(k, row)];
+      sum = fmaf(u.y, ex2(u.x - ref), sum);
+    }
+    sum = warp_sum(sum);
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      float f = v[0].x;
+#pragma unroll
+      for (int c = 1; c < kKept; ++c)
+        if (k0 == 32 * c) f = v[c].x;
+      if (k0 >= 32 * kKept) f = k0 + lane < parts ? ex2(ml[rp.at(k0 + lane, row)].x - ref) : 0.0f;
+      const int n = min(32, parts - k0);
+      for (int k = part; k < n; k += SHARE * kBatch) {
+        Vec x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          x[i] = Vec();
+          if (k + i * SHARE < n) x[i] = reinterpret_cast<const Vec*>(p.part_o + rp.at(k0 + k + i * SHARE, row) * D)[lane];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const float c = __shfl_sync(0xffffffffu, f, (k + i * SHARE) & 31);
+          if (k + i * SHARE >= n) break;
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x[i])[j], c, acc[j]);
+        }
+      }
+    }
+  }
+  if (SHARE > 1) {  // all warps of the CTA are here
+    Vec x;
+#pragma unroll
+    for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
+    __syncthreads();  // the row before has been read
+    sh_o[warp][lane] = x;
+    __syncthreads();
+  }
+  if (part == 0) {
+#pragma unroll
+    for (int k = 1; k < SHARE; ++k) {
+      const Vec o = sh_o[k][lane];
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += reinterpret_cast<const float*>(&o)[j];
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < V; j += 2) dst[lane * (V / 2) + j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
+  }
+}
+
+// Joins the parts of the units that were cut, and writes zeros for the rows
+// that no step covers: queries without keys and tokens behind the last
+// sequence.  An item is a (sequence, token, head); MODE says how the four
+// warps of a CTA share them:
+//   kRowCta    one item a CTA, all warps together: few items, each of many
+//              parts (a single long sequence has one for every worker);
+//   kRowWarp   an item a warp: many items, few of them cut;
+//   kRowMixed  an item a warp, those of more than kAlone parts all warps
+//              together (long sequences among short or empty ones).  A CTA's
+//              items lie far apart, so that a long sequence's rows go to many SMs.
+// Measured: one token of 16 sequences to 4000 keys with 32 heads 36.4 us with
+// kRowCta, 38.0 with kRowWarp; 64 sequences to 8192 keys 217 with kRowCta, 211
+// with the other two; one of 16384 keys among 63 of 100 29.4, 30.2 (kRowMixed)
+// and 39.7 (kRowWarp); 7 tokens of 70 sequences 76, 51 and 47.
+enum { kRowCta, kRowMixed, kRowWarp };
+template <bool BF16, int D, int MODE>
+__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_constant__ Params p) {
+  using Vec = typename std::conditional<D == 128, float4, float2>::type;
+  constexpr int W = kJoinWarps, kPerCta = MODE == kRowCta ? 1 : W;
+  constexpr int kAlone = 16;
+  __shared__ Vec sh_o[W][32];
+  __shared__ int shared_item[W];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row_ctas = (p.B * p.combine_rows * p.H + kPerCta - 1) / kPerCta;
   if (static_cast<int>(blockIdx.x) >= row_ctas) {
     const int at = blockIdx.x - row_ctas;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp < kJoinWarps) tile_join<BF16, D>(p, at / 8, at % 8);
+    tile_join<BF16, D>(p, at / 8, at % 8);
     return;
   }
-  const int item = blockIdx.x * kPerCta + warp / SHARE;
-  const int h = item % p.H, y = item / p.H % p.combine_rows, b = item / p.H / p.combine_rows;
-  const int kvh = static_cast<int>(fdiv(static_cast<uint32_t>(h), p.div_g));
-  auto out_row = [&](int64_t tok, int head) { return p.out + (tok * p.H + head) * D; };
-  // The index tensors are older than the row kernel: what they say is worked
-  // out before the wait for it; what follows reads or writes what the kernels
-  // before this one may still be at.
-  const Work w = work_at(p, min(b, p.B - 1));
+  auto out_row = [&](int64_t tok, int head) { return reinterpret_cast<uint32_t*>(p.out + (tok * p.H + head) * D); };
+  // What the index tensors say of an item.  They are older than the row
+  // kernel; what else is read here is of the row kernel's.
+  struct Item {
+    Work w;
+    int b, y, h, kvh;
+    int64_t seq0, run;
+  };
+  auto look = [&](int item) {
+    Item it;
+    it.h = item % p.H;
+    it.y = item / p.H % p.combine_rows;
+    it.b = item / p.H / p.combine_rows;
+    it.kvh = static_cast<int>(fdiv(static_cast<uint32_t>(it.h), p.div_g));
+    it.w = work_at(p, min(it.b, p.B - 1));
+    it.seq0 = it.run = 0;
+    if (p.B <= 32) {  // the list in one scan; else what the row kernel left
+      const int64_t mine = lane < p.B ? steps_of(p, work_at(p, lane)) : 0, upto = warp_scan(mine);
+      it.run = run_of(p, __shfl_sync(0xffffffffu, upto, 31));
+      it.seq0 = __shfl_sync(0xffffffffu, upto - mine, min(it.b, 31));
+    }
+    return it;
+  };
+  auto finish_look = [&](Item& it) {
+    if (p.B > 32) {
+      it.seq0 = p.prefix[min(it.b, p.B - 1)];
+      it.run = p.prefix[p.B + 1];
+    }
+  };
+  auto parts_of = [&](const Item& it, int r) {
+    RowParts rp{0, 0, 0, 0};
+    if (it.w.tiles > 0) {
+      rp.unit0 = it.seq0 + (static_cast<int64_t>(it.kvh) * it.w.rts + r / kRows) * it.w.tiles;
+      rp.run = it.run;
+      rp.first = div64(rp.unit0, rp.run);
+      rp.n = static_cast<int>(min(static_cast<int64_t>(p.workers) - 1, div64(rp.unit0 + it.w.tiles - 1, rp.run)) - rp.first) + 1;
+    }
+    return rp;
+  };
+  // Every row of an item whose parts `take` accepts, joined by SHARE warps.
+  auto join = [&](const Item& it, auto share, auto take) {
+    for (int i = it.y; i < it.w.s.m; i += p.combine_rows) {
+      const int r = i * p.G + (it.h - it.kvh * p.G);
+      const RowParts rp = parts_of(it, r);
+      if (rp.n != 1 && take(rp.n))
+        join_row<BF16, D, decltype(share)::value>(p, rp, r % kRows, out_row(it.w.s.t0 + i, it.h), sh_o);
+    }
+  };
+  const std::integral_constant<int, 1> alone;
+  const std::integral_constant<int, W> together;
+  const int cta = static_cast<int>(blockIdx.x);
+  const int item = MODE == kRowCta ? cta : MODE == kRowMixed ? warp * row_ctas + cta : cta * W + warp;
+  Item it = look(item);
   const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
-  int64_t seq0 = 0, run = 0;
-  if (p.B <= 32) {  // the list in one scan; else what the row kernel left
-    const int64_t mine = lane < p.B ? steps_of(p, work_at(p, lane)) : 0, upto = warp_scan(mine);
-    run = run_of(p, __shfl_sync(0xffffffffu, upto, 31));
-    seq0 = __shfl_sync(0xffffffffu, upto - mine, min(b, 31));
-  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {  // tokens behind the last sequence
     const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(end, 0));
-    const int64_t step = static_cast<int64_t>(row_ctas) * (WARPS * 32);
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(WARPS * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
+    uint32_t* dst = out_row(end, 0);
+    const int64_t step = static_cast<int64_t>(row_ctas) * (W * 32);
+    for (int64_t i = cta * static_cast<int64_t>(W * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
   }
-  if (b >= p.B || static_cast<int64_t>(w.s.m) * p.G > p.long_rows) return;
-  if (p.B > 32) {
-    seq0 = p.prefix[b];
-    run = p.prefix[p.B + 1];
-  }
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-  for (int i = y; i < w.s.m; i += p.combine_rows) {
-    const int r = i * p.G + (h - kvh * p.G);
-    int64_t u0 = 0, first = 0;
-    int parts = 0;  // 0: no step covers the row
-    if (w.tiles > 0) {
-      u0 = seq0 + (static_cast<int64_t>(kvh) * w.rts + r / kRows) * w.tiles;
-      first = div64(u0, run);
-      parts = static_cast<int>(min(static_cast<int64_t>(p.workers) - 1, div64(u0 + w.tiles - 1, run)) - first) + 1;
-      if (parts == 1) continue;  // written by the row kernel
+  const bool real = it.b < p.B && static_cast<int64_t>(it.w.s.m) * p.G <= p.long_rows;  // else the tile kernel's, or none
+  if (real) finish_look(it);
+  if constexpr (MODE == kRowCta) {
+    if (real) join(it, together, [](int) { return true; });
+  } else if constexpr (MODE == kRowWarp) {
+    if (real) join(it, alone, [](int) { return true; });
+  } else {
+    bool many = false;
+    if (real) {
+      join(it, alone, [&](int n) {
+        many |= n > kAlone;
+        return n <= kAlone;
+      });
     }
-    auto row_of = [&](int k) { return ((first + k) * 2 + (u0 < (first + k) * run ? 0 : 1)) * kRows + r % kRows; };
-    float sum = 0.0f, acc[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-    if (parts > 0) {
-      // Every warp finds the maximum and the sum of all parts, a lane 32
-      // parts apart (the first 32 kKept parts' in registers, loaded together) ...
-      constexpr int kKept = SHARE == 1 ? 1 : 4;
-      float2 v[kKept];
-#pragma unroll
-      for (int c = 0; c < kKept; ++c) {
-        v[c] = make_float2(-INFINITY, 0.0f);
-        if (lane + 32 * c < parts) v[c] = ml[row_of(lane + 32 * c)];
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < kKept; ++c) mx = fmaxf(mx, v[c].x);
-      for (int k = lane + 32 * kKept; k < parts; k += 32) mx = fmaxf(mx, ml[row_of(k)].x);
-      mx = warp_max(mx);
-      const float ref = mx == -INFINITY ? 0.0f : mx;
-#pragma unroll
-      for (int c = 0; c < kKept; ++c) {
-        v[c].x = ex2(v[c].x - ref);  // the part's weight
-        sum = fmaf(v[c].y, v[c].x, sum);
-      }
-      for (int k = lane + 32 * kKept; k < parts; k += 32) {
-        const float2 u = ml[row_of(k)];
-        sum = fmaf(u.y, ex2(u.x - ref), sum);
-      }
-      sum = warp_sum(sum);
-      // ... and adds every SHARE-th part's output
-      for (int k0 = 0; k0 < parts; k0 += 32) {
-        float f = v[0].x;
-#pragma unroll
-        for (int c = 1; c < kKept; ++c)
-          if (k0 == 32 * c) f = v[c].x;
-        if (k0 >= 32 * kKept) f = k0 + lane < parts ? ex2(ml[row_of(k0 + lane)].x - ref) : 0.0f;
-        const int n = min(32, parts - k0);
-        for (int k = part; k < n; k += SHARE * kBatch) {
-          Vec x[kBatch];  // loaded together, whatever their number
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            x[i] = Vec();
-            if (k + i * SHARE < n) x[i] = reinterpret_cast<const Vec*>(p.part_o + row_of(k0 + k + i * SHARE) * D)[lane];
-          }
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const float c = __shfl_sync(0xffffffffu, f, (k + i * SHARE) & 31);
-            if (k + i * SHARE >= n) break;
-#pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x[i])[j], c, acc[j]);
-          }
-        }
-      }
-    }
-    if (SHARE > 1) {  // one row a CTA: all its warps are here
-      Vec x;
-#pragma unroll
-      for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
-      __syncthreads();  // the row before has been read
-      sh_o[warp][lane] = x;
-      __syncthreads();
-    }
-    if (part == 0) {
-#pragma unroll
-      for (int k = 1; k < SHARE; ++k) {
-        const Vec o = sh_o[k][lane];
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += reinterpret_cast<const float*>(&o)[j];
-      }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(w.s.t0 + i, h)) + lane * (V / 2);
-#pragma unroll
-      for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
+    if (!__syncthreads_or(many)) return;
+    if (lane == 0) shared_item[warp] = many ? item : -1;
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < W; ++k) {
+      if (shared_item[k] < 0) continue;
+      it = look(shared_item[k]);
+      finish_look(it);
+      join(it, together, [](int n) { return n > kAlone; });
     }
   }
 }
@@ -659,18 +739,18 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   // row kernel's writes itself, before it reads or writes anything).
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  const int warps = std::max(kJoinWarps, p.join_share), per_cta = warps / p.join_share;
+  const int per_cta = p.join_mode == kRowCta ? 1 : kJoinWarps;
   cfg.gridDim = dim3(static_cast<unsigned>((p.B * p.combine_rows * p.H + per_cta - 1) / per_cta + p.tile_ctas * 8));
-  cfg.blockDim = dim3(warps * 32);
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  auto combine = p.join_share == 1   ? combine_kernel<BF16, D, 1, kJoinWarps>
-                 : p.join_share == 4 ? combine_kernel<BF16, D, 4, kJoinWarps>
-                                     : combine_kernel<BF16, D, 16, 16>;
+  auto combine = p.join_mode == kRowCta     ? combine_kernel<BF16, D, kRowCta>
+                 : p.join_mode == kRowMixed ? combine_kernel<BF16, D, kRowMixed>
+                                            : combine_kernel<BF16, D, kRowWarp>;
   return cudaLaunchKernelEx(&cfg, combine, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
@@ -702,7 +782,10 @@ int check_shape(const B200kPagedAttentionArgs* a) {
   return B200K_OK;
 }
 
-// Sequences of more query rows than this run the tile kernel.
+// Sequences of more query rows than this run the tile kernel.  With 16 and 64
+// in place of 32: 20 rows of 32 sequences to 4000 keys 82 and 75 us (32: 75),
+// 32 rows 85 and 91 (91), 20 rows of 2 sequences to 1000 keys 28 and 12 (12), up
+// to 68 rows of 8 sequences to 1500 keys, heads of 64, 22 and 29 (27).
 constexpr int kLongRows = 32;
 
 bool may_be_long(const B200kPagedAttentionArgs* a) {
@@ -834,8 +917,8 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   int64_t rows = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
   if (p.tile_ctas > 0) rows = std::min<int64_t>(rows, kLongRows / p.G);
   p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 0x1fffffff / per_token)));
-  const int64_t join_rows = per_token * p.combine_rows;
-  p.join_share = join_rows <= 2ll * sms ? 16 : join_rows <= 16ll * sms ? 4 : 1;
+  const int64_t items = per_token * p.combine_rows;
+  p.join_mode = items <= 4ll * sms ? kRowCta : items <= 16ll * sms ? kRowMixed : kRowWarp;
   if (a->dtype == B200K_BF16)
     return a->head_dim == 64 ? launch_cap<true, 64>(p, cap, ctas, st) : launch_cap<true, 128>(p, cap, ctas, st);
   return a->head_dim == 64 ? launch_cap<false, 64>(p, cap, ctas, st) : launch_cap<false, 128>(p, cap, ctas, st);
