@@ -125,6 +125,42 @@ def test_large_scores_stay_finite():
     assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("m", [1, 200])
+@pytest.mark.parametrize("key", [0, 6, 7, 64, 71, 150, 199])
+def test_a_nan_key_reaches_every_row_that_sees_it_and_no_other(key, m, cap, D):
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([m], [200], 8, 2, D, 16, BF)
+    op = torch.ops.b200.paged_attention
+    clean = op(q, kc, vc, table, q_start, kv_len, 0.0, cap)
+    kc = kc.clone()
+    kc[table[0, key // 16], key % 16, :, 3] = float("nan")
+    out = op(q, kc, vc, table, q_start, kv_len, 0.0, cap)
+    seen = torch.arange(200 - m, 200, device="cuda") >= key
+    assert out[seen].isnan().all() and torch.equal(out[~seen], clean[~seen])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("m", [1, 200])
+@pytest.mark.parametrize("key", [0, 6, 64, 71, 199])
+def test_an_infinite_score(key, m, D):
+    """+inf - inf is NaN in the softmax; a score of -inf has no weight."""
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs([m], [200], 8, 2, D, 16, BF)
+    seen = (torch.arange(200 - m, 200, device="cuda") >= key)[:, None]
+    at = table[0, key // 16], key % 16
+    lone = torch.arange(200 - m, 200, device="cuda")[:, None] == 0  # sees this key alone when key == 0
+    kc = kc.clone()
+    kc[at][:, 3] = float("inf")
+    out = torch.ops.b200.paged_attention(q, kc, vc, table, q_start, kv_len)
+    up, down = seen & (q[..., 3] > 0), seen & (q[..., 3] < 0)
+    assert out[up].isnan().all()
+    assert out[down & ~(lone & (key == 0))].isfinite().all() and out[~seen.expand(-1, 8)].isfinite().all()
+    kc[at][:, 3] = float(2**15)  # -2^15 |q|: no weight either
+    want = torch.ops.b200.paged_attention(q, kc, vc, table, q_start, kv_len)
+    keep = down & (q[..., 3] < -0.1) & ~(lone & (key == 0))
+    torch.testing.assert_close(out[keep], want[keep], rtol=2.0**-7, atol=2.0**-7)
+
+
 def test_cache_offsets_past_32_bits():
     D, hkv, page = 128, 8, 128
     pages = 2**31 // (page * hkv * D) + 4

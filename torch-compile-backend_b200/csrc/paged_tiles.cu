@@ -137,9 +137,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// NaN if any of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 // 2^x on the FMA pipe, for a share of the probabilities: the special-function
@@ -147,11 +153,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // integer (read off the low bits of x + 1.5 * 2^23), 2^f on [-1/2, 1/2] by
 // the polynomial of least relative error (Remez exchange; 7.5e-5 in degree 3
 // for bf16 probabilities, 2.6e-6 in degree 4 for f16: below half a step of
-// the type), n added to the exponent.  x below -125 gives 2^-125, NaN stays.
+// the type), n added to the exponent.  x below -125 gives 2^-125; x is not NaN
+// unless the row's maximum is.
 template <bool BF16>
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.0f));
+  x.x = fmaxf(x.x, -125.0f);
+  x.y = fmaxf(x.y, -125.0f);
   const float big = 12582912.0f;
   const float2 t = __fadd2_rn(x, make_float2(big, big));
   const float2 n = __fadd2_rn(t, make_float2(-big, -big));
@@ -550,14 +557,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], s[c + i], s[c + 4 + i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], s[kBlock - 4 + i]);
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int i = 0; i < 4; ++i) mx[i] = max2(mx[i], s[kBlock - 4 + i]);
+        float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
         if (!CAP) top *= p.mul;
+        const float was = m;
         float alpha = 1.0f;
         bool moved = false;
-        if (top > m + kRescaleLog2 || (m == -INFINITY && top > m)) {
-          alpha = ex2(m - top);
-          m = top;
+        // A NaN score, and an infinite one (0 * top), makes the maximum NaN and
+        // with it every probability and sum of the row from here on.
+        if (!(top <= m + kRescaleLog2)) {
+          m = fmaf(0.0f, top, top);
+          alpha = ex2(was - m);
           moved = j > jb;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
