@@ -161,3 +161,19 @@ def test_replayed_decode_steps(setting):
         return state["out"]
 
     run(setting, call)
+
+
+@pytest.mark.parametrize("backend", ["aot_eager", custom_backend])
+def test_a_training_graph_is_refused(backend):
+    x, r = (torch.randn(4, DIM, device="cuda").to(BF) for _ in range(2))
+    w = torch.ones(DIM, device="cuda", requires_grad=True)
+
+    def f(x, r, w):
+        return torch.ops.b200.add_rms_norm(x * 2, r, w, 1e-5)[0] + x
+
+    torch._dynamo.reset()
+    g = torch.compile(f, backend=backend)
+    with pytest.raises(Exception, match="no gradient is defined"):
+        g(x, r, w)
+    with torch.no_grad():
+        assert torch.equal(g(x, r, w), f(x, r, w))

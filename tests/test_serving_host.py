@@ -142,3 +142,29 @@ def test_fakes_have_the_outputs_shapes():
 def test_the_append_declares_what_it_writes():
     s = str(torch.ops.b200.rope_append.default._schema)
     assert "Tensor(a!) k_cache, Tensor(b!) v_cache" in s
+
+
+@pytest.mark.parametrize("op", ["add_rms_norm", "add_rms_norm_quant", "rope_append", "paged_attention"])
+def test_inputs_that_ask_for_a_gradient_are_refused_when_traced(op):
+    """No gradient is defined: not only the kernels but a trace (on fake
+    tensors) refuses, which would otherwise compile to a backward without the
+    op's share."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f = getattr(torch.ops.b200, op)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+        cache = t(4, 16, 2, 64), t(4, 16, 2, 64)
+        ints = t(3, dtype=torch.int32)
+        args = {"add_rms_norm": (t(3, 256), t(3, 256), None, 1e-5),
+                "add_rms_norm_quant": (t(3, 256), t(3, 256), None, 1e-5, 128),
+                "rope_append": (t(3, 8, 64), t(3, 2, 64), t(3, 2, 64), t(9, 32), t(9, 32), ints, ints, *cache),
+                "paged_attention": (t(3, 8, 64), *cache, t(2, 4, dtype=torch.int32), ints, ints[:2])}[op]
+        with torch.no_grad():
+            f(*args)
+        args[0].requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient is defined"):
+            f(*args)
+        with torch.no_grad():
+            f(*args)

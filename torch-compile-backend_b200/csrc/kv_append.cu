@@ -225,8 +225,6 @@ extern "C" int b200k_rope_append(const B200kRopeAppendArgs* a, void* stream_) {
   if (a->tokens == 0 || a->head_dim == 0 || a->heads + a->kv_heads == 0) return B200K_OK;
   if (!a->positions || !a->slots || (a->heads && (!a->q || !a->q_out))) return B200K_ERR_ARG;
   if (a->kv_heads && (!a->k || !a->v)) return B200K_ERR_ARG;
-  const int64_t total = a->num_pages * a->page_size;
-  if (a->kv_heads && total && (!a->k_cache || !a->v_cache)) return B200K_ERR_ARG;
   if (a->dtype != B200K_BF16 && a->dtype != B200K_F16) return B200K_ERR_UNSUPPORTED;
   if (a->table_dtype != B200K_F32 && a->table_dtype != a->dtype) return B200K_ERR_UNSUPPORTED;
   for (int dt : {a->positions_dtype, a->slots_dtype})
@@ -234,8 +232,10 @@ extern "C" int b200k_rope_append(const B200kRopeAppendArgs* a, void* stream_) {
   if (a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % 2) return B200K_ERR_SHAPE;
   if (a->rot_dim && (!a->cos || !a->sin || a->table_rows <= 0)) return B200K_ERR_ARG;
   if (a->heads > 65536 || a->kv_heads > 65536 || a->head_dim > 65536 || a->tokens > 0x7fffffffLL ||
-      a->page_size > 0x7fffffffLL || total > 0x7fffffffLL || a->num_pages > 0x7fffffffLL)
+      a->page_size > 0x7fffffffLL || a->num_pages > 0x7fffffffLL || a->num_pages * a->page_size > 0x7fffffffLL)
     return B200K_ERR_SHAPE;
+  const int64_t total = a->num_pages * a->page_size;
+  if (a->kv_heads && total && (!a->k_cache || !a->v_cache)) return B200K_ERR_ARG;
   const int sms = device_sm_count();
   if (sms <= 0) return B200K_ERR_DEVICE;
   AppendParams p;

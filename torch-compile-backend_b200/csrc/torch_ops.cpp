@@ -542,8 +542,6 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
 }
 
 // ------------------------------------------------- paged-cache serving ops
-// These ops have no gradient: an input that asks for one is refused rather
-// than answered with a result that is cut off from it.
 void no_grad_inputs(const char* what, std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor* t : ts)
@@ -572,7 +570,6 @@ void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r
               r_in.sizes(), " differ in shape");
   TORCH_CHECK(r_in.device() == x_in.device() && r_in.scalar_type() == x_in.scalar_type(), "b200::", what,
               ": x and residual differ in dtype or device");
-  no_grad_inputs(what, {&x_in, &r_in});
   c10::cuda::CUDAGuard guard(x_in.device());
   const int64_t cols = x_in.size(-1);
   // Row stride of t's flattened leading dims (those of size one have no say),
@@ -605,7 +602,6 @@ void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r
   if (weight.has_value() && weight->defined()) {
     TORCH_CHECK(weight->device() == x.device() && weight->dim() == 1 && weight->size(0) == cols, "b200::", what,
                 ": weight must be [", cols, "] on x's device");
-    no_grad_inputs(what, {&*weight});
     w = weight->contiguous();
     a.weight = w.data_ptr();
     a.w_dtype = to_dt(w.scalar_type());
@@ -692,7 +688,6 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
                 "b200::rope_append: positions and slots must be contiguous int32 or int64");
   for (const at::Tensor* t : {&cos, &sin, &positions, &slots})
     TORCH_CHECK(t->device() == q.device(), "b200::rope_append: every tensor must be on q's device");
-  no_grad_inputs(what, {&q, &k, &v, &cos, &sin, &k_cache, &v_cache});
   for (int64_t d = 0; d < 4; ++d)  // several elements in one place
     TORCH_CHECK(k_cache.size(d) <= 1 || k_cache.stride(d) != 0, "b200::rope_append: the caches must not be expanded");
   c10::cuda::CUDAGuard guard(q.device());
@@ -753,7 +748,6 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
                 "b200::paged_attention: page_table, q_start and kv_len must be int32 on q's device with unit last-dim stride");
   TORCH_CHECK(softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::paged_attention: softcap, window and max_q_len must not "
               "be negative");
-  no_grad_inputs(what, {&q, &k_cache, &v_cache});
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
   B200kPagedAttentionArgs a;
@@ -792,6 +786,52 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   a.status = status_ptr(q.device().index(), st);
   check(b200k_paged_attention(&a, st), what);
   return out;
+}
+
+// At the autograd key the serving ops refuse inputs that ask for a gradient
+// (none is defined, and the result would be cut off from them) and go on below
+// it.  There, not in the kernels, so that a traced training graph is refused
+// too.
+template <typename Fn, typename... Args>
+auto below_autograd(const c10::TypedOperatorHandle<Fn>& op, const char* what, std::initializer_list<const at::Tensor*> grads,
+                    Args&&... args) {
+  no_grad_inputs(what, grads);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(std::forward<Args>(args)...);
+}
+template <typename Fn>
+c10::TypedOperatorHandle<Fn> find_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
+}
+const at::Tensor& or_none(const c10::optional<at::Tensor>& t) {
+  static const at::Tensor none;
+  return t.has_value() ? *t : none;
+}
+
+std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, const at::Tensor& residual,
+                                                         const c10::optional<at::Tensor>& weight, double eps, int64_t flags) {
+  static const auto op = find_op<decltype(add_rms_norm)>("b200::add_rms_norm");
+  return below_autograd(op, "add_rms_norm", {&x, &residual, &or_none(weight)}, x, residual, weight, eps, flags);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant_autograd(const at::Tensor& x, const at::Tensor& residual,
+                                                                           const c10::optional<at::Tensor>& weight, double eps,
+                                                                           int64_t group, int64_t flags) {
+  static const auto op = find_op<decltype(add_rms_norm_quant)>("b200::add_rms_norm_quant");
+  return below_autograd(op, "add_rms_norm_quant", {&x, &residual, &or_none(weight)}, x, residual, weight, eps, group, flags);
+}
+at::Tensor rope_append_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                                const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots,
+                                at::Tensor k_cache, at::Tensor v_cache) {
+  static const auto op = find_op<decltype(rope_append)>("b200::rope_append");
+  return below_autograd(op, "rope_append", {&q, &k, &v, &cos, &sin, &k_cache, &v_cache}, q, k, v, cos, sin, positions, slots,
+                        k_cache, v_cache);
+}
+at::Tensor paged_attention_autograd(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                    const at::Tensor& page_table, const at::Tensor& q_start, const at::Tensor& kv_len,
+                                    double scale, double softcap, int64_t window, int64_t max_q_len) {
+  static const auto op = find_op<decltype(paged_attention)>("b200::paged_attention");
+  return below_autograd(op, "paged_attention", {&q, &k_cache, &v_cache}, q, k_cache, v_cache, page_table, q_start, kv_len, scale,
+                        softcap, window, max_q_len);
 }
 
 }  // namespace
@@ -845,3 +885,9 @@ TORCH_LIBRARY_IMPL(b200, CUDA, m) {
   m.impl("paged_attention", &paged_attention);
 }
 
+TORCH_LIBRARY_IMPL(b200, Autograd, m) {
+  m.impl("add_rms_norm", &add_rms_norm_autograd);
+  m.impl("add_rms_norm_quant", &add_rms_norm_quant_autograd);
+  m.impl("rope_append", &rope_append_autograd);
+  m.impl("paged_attention", &paged_attention_autograd);
+}
