@@ -110,6 +110,23 @@ def test_long_sequences_among_short_ones(seqs, H, hkv, max_q, D):
     run(ref.paged_inputs(qs, ns, H, hkv, D, 16, BF), max_q=max_q)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("steps", [1, 3, 4, 5, 8, 12])
+def test_units_of_whole_warps_and_ctas(steps, D):
+    """As many equal units as CTAs, of 16-key steps: a warp's run, parts of a
+    CTA's, exactly a CTA's, and more."""
+    ctas = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    run(ref.paged_inputs([1] * ctas, [16 * steps] * ctas, 4, 1, D, 16, BF))
+    run(ref.paged_inputs([1] * (ctas // 8), [16 * steps * 8] * (ctas // 8), 4, 1, D, 16, BF))
+
+
+@pytest.mark.parametrize("H,hkv,D", [(8, 1, 128), (16, 1, 64), (32, 1, 128), (5, 1, 128)])
+def test_one_sequence_of_one_key_head(H, hkv, D):
+    """A unit of thousands of steps: a part a CTA, a bounded number of CTAs."""
+    run(ref.paged_inputs([1], [30000], H, hkv, D, 16, BF))
+    run(ref.paged_inputs([1, 1], [20011, 64], H, hkv, D, 16, BF))
+
+
 def test_strided_queries():
     q, *rest = ref.paged_inputs([1, 5, 2], [30, 60, 2], 8, 2, 64, 16, BF)
     wide = torch.zeros(q.shape[0], 12, 64, device="cuda", dtype=BF)

@@ -20,8 +20,10 @@
 // keys, rows beyond the unit's are zero: the tensor pipe has the time, the
 // memory does not) and keeps its running maximum, sum and output in fp32.
 // A unit inside one run is written at once; a cut one leaves its parts
-// (max, sum, unnormalised output, fp32) in the workspace, and
-// combine_kernel joins them in an order that only the lengths decide.
+// (max, sum, unnormalised output, fp32) in the workspace, one for a CTA whose
+// warps are all in the unit (one token over 30000 keys of one key head: 20 us,
+// with a part a warp 42), and combine_kernel joins them in an order that only
+// the lengths decide.
 // Measured: one token of 64 sequences to 8192 keys, 32 / 8 heads of 128, 211 us
 // = 6.48 TB/s; of 3 sequences to 65536 keys 95 us = 6.05 TB/s.
 #include <algorithm>
@@ -117,9 +119,15 @@ __device__ __forceinline__ int64_t div64(int64_t n, int64_t d) {
   if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
   return n / d;
 }
-// Steps that a worker takes of a list of `total`.
-__device__ __forceinline__ int64_t run_of(const Params& p, int64_t total) {
-  return max(static_cast<int64_t>(1), div64(total + p.workers - 1, p.workers));
+// Steps that a worker takes of a list of `total` whose longest unit has
+// `longest`: an equal share, but enough that a unit has at most kMaxParts CTAs.
+// One token over 30000, 8000 and 120000 keys of one key head: 14.7, 10.5 and
+// 31 us, without the bound 19.8, 13.3 and 32, with 32 in its place 20.3, 10.6
+// and 62.
+constexpr int kMaxParts = 96;
+__device__ __forceinline__ int64_t run_of(const Params& p, int64_t total, int longest) {
+  return max(div64(total + p.workers - 1, p.workers),
+             static_cast<int64_t>(max(1, (longest + kMaxParts * kWarps - 1) / (kMaxParts * kWarps))));
 }
 
 // A position in the list of steps: within a sequence kv head by kv head, row
@@ -207,6 +215,57 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
   }
 }
 
+// A warp's part in shared memory, in its ring: rows of D sums, a maximum and
+// a sum, 32 bytes apart modulo the banks.
+template <int D>
+constexpr int kJointStride = D + 8;
+template <int D>
+__device__ __forceinline__ float* joint_rows(uint8_t* smem, int warp) {
+  static_assert(kRows * kJointStride<D> * 4 <= kRingBytes, "a part fits a ring");
+  return reinterpret_cast<float*>(smem + warp * kRingBytes);
+}
+// The CTA's warps' parts of one unit as one: written to `worker`'s slot, or to
+// the output where the CTA has the whole unit.  A warp takes every kWarps-th row.
+template <bool BF16, int D, typename Out>
+__device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int warp, int lane, int rows, int worker, int slot,
+                                           bool whole, Out out_row) {
+  constexpr int V = D / 32;
+  using Vec = typename std::conditional<D == 128, float4, float2>::type;
+  for (int in = warp; in < rows; in += kWarps) {
+    float2 ml[kWarps];
+    float mx = -INFINITY, sum = 0.0f, acc[V];
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      ml[k] = *reinterpret_cast<const float2*>(joint_rows<D>(smem, k) + in * kJointStride<D> + D);
+      mx = fmaxf(mx, ml[k].x);
+    }
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      const float f = ex2(ml[k].x - ref);
+      const Vec x = reinterpret_cast<const Vec*>(joint_rows<D>(smem, k) + in * kJointStride<D>)[lane];
+      sum = fmaf(ml[k].y, f, sum);
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], f, acc[j]);
+    }
+    if (whole) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(out_row(in)) + lane * (V / 2);
+#pragma unroll
+      for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
+    } else {
+      const int64_t at = (static_cast<int64_t>(worker) * 2 + slot) * kRows + in;
+      Vec x;
+#pragma unroll
+      for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
+      reinterpret_cast<Vec*>(p.part_o + at * D)[lane] = x;
+      if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, sum);
+    }
+  }
+}
+
 template <bool BF16, int D, bool CAP>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __grid_constant__ Params p) {
   constexpr int S = kRingBytes / (kKeys * D * 4);  // ring stages: K and V rows of a step each
@@ -229,16 +288,21 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
 
   // The whole list's length and, from it, this worker's run [w0, w1).
   int64_t total = 0, mine0 = 0, upto0 = 0;
+  int longest = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = 0;
-    if (b0 + lane < p.B) mine = steps_of(p, work_at(p, b0 + lane));
+    if (b0 + lane < p.B) {
+      const Work w = work_at(p, b0 + lane);
+      mine = steps_of(p, w);
+      longest = max(longest, w.tiles);
+    }
     const int64_t upto = warp_scan(mine);
     if (worker == 0 && b0 + lane < p.B) p.prefix[b0 + lane] = total + upto - mine;  // for combine_kernel
     total += __shfl_sync(0xffffffffu, upto, 31);
     mine0 = mine;
     upto0 = upto;
   }
-  const int64_t run = run_of(p, total);
+  const int64_t run = run_of(p, total, __reduce_max_sync(0xffffffffu, longest));
   if (worker == 0 && lane == 0) {
     p.prefix[p.B] = total;
     p.prefix[p.B + 1] = run;
@@ -313,6 +377,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   bool fresh = true;
   int stage = 0;
   int64_t unit0 = seq0 + static_cast<int64_t>(unit) * cur.w.tiles;  // the current unit's first step
+  // All of this CTA's runs lie in one unit: its warps' parts become one.
+  const int64_t c0 = run * (worker & ~(kWarps - 1)), c1 = c0 + run * kWarps;
+  const bool joint = unit0 <= c0 && c1 <= unit0 + cur.w.tiles;
   // The first S - 1 rounds only load.  One copy of the loading code: unrolled
   // ahead of the loop, its instructions alone took 2 us to arrive.
 #pragma unroll 1
@@ -429,13 +496,23 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     if (unit_ends || t + 1 == w1) {
       const int rows = cur.w.s.m * p.G, r0 = cur.rt * kRows;
       const bool whole = unit0 >= w0 && unit_ends;
+      if (joint) {  // its last step: the rings are free
+        cp_wait<0>();
+        __syncwarp();
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
         const int in = g + 8 * i, r = r0 + in;
         if (r >= rows) continue;
-        if (whole) {
+        if (joint) {
+          float* dst = joint_rows<D>(smem, warp) + in * kJointStride<D>;
+          if (quad == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[i], l[i]);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(dst + n * 8 + quad * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        } else if (whole) {
           const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
           uint32_t* dst = reinterpret_cast<uint32_t*>(
               p.out + (static_cast<int64_t>(cur.w.s.t0 + tok) * p.H + cur.kvh * p.G + (r - tok * p.G)) * D + quad * 2);
@@ -450,6 +527,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) dst[n * 4] = make_float2(o[n][2 * i], o[n][2 * i + 1]);
         }
+      }
+      if (joint) {
+        __syncthreads();  // every warp of the CTA comes here once
+        join_warps<BF16, D>(p, smem, warp, lane, min(kRows, rows - r0), worker & ~(kWarps - 1), unit0 < c0 ? 0 : 1,
+                            unit0 == c0 && c1 == unit0 + cur.w.tiles, [&](int in) {
+                              const int r = r0 + in;
+                              const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
+                              return p.out + (static_cast<int64_t>(cur.w.s.t0 + tok) * p.H + cur.kvh * p.G + (r - tok * p.G)) * D;
+                            });
+        return;
       }
       __syncwarp();
       fresh = true;
@@ -504,14 +591,29 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
         make_uint2(pack16<BF16>(acc[c].x * inv, acc[c].y * inv), pack16<BF16>(acc[c].z * inv, acc[c].w * inv));
 }
 
-// The parts of a query row, one for each worker whose run holds steps of the
-// row's unit: workers first .. first + n - 1.  n = 0: no step covers the row
-// (zeros); n = 1: the row kernel has written it.
+// The parts of a query row: one for each worker whose run holds steps of the
+// row's unit, or for each CTA whose kWarps runs all lie in it (at its first
+// worker's place).  n = 0: no step covers the row (zeros); n = 1: the row
+// kernel has written it.
 struct RowParts {
-  int64_t unit0, run, first;
-  int n;
+  int64_t unit0, run;
+  int first, lead, group0, groups, n;  // workers, then groups CTAs, then workers
+  __device__ __forceinline__ void find(int64_t begin, int64_t end, int64_t steps) {
+    unit0 = begin;
+    run = steps;
+    first = static_cast<int>(div64(begin, run));
+    const int last = static_cast<int>(div64(end - 1, run));
+    const int from = first + (begin > first * run ? 1 : 0);             // runs from .. to - 1 lie in the unit
+    const int to = last + ((last + 1) * run == end ? 1 : 0);
+    group0 = (from + kWarps - 1) / kWarps;
+    groups = max(0, to / kWarps - group0);
+    lead = groups > 0 ? group0 * kWarps - first : last - first + 1;
+    n = groups > 0 ? lead + groups + (last + 1 - (group0 + groups) * kWarps) : lead;
+  }
   __device__ __forceinline__ int64_t at(int k, int row) const {
-    return ((first + k) * 2 + (unit0 < (first + k) * run ? 0 : 1)) * kRows + row;
+    const int w = k < lead ? first + k : k < lead + groups ? (group0 + k - lead) * kWarps
+                                                           : (group0 + groups) * kWarps + (k - lead - groups);
+    return (w * 2ll + (unit0 < w * run ? 0 : 1)) * kRows + row;
   }
 };
 
@@ -526,7 +628,7 @@ __device__ __forceinline__ void join_row(const Params& p, const RowParts& rp, in
   constexpr int V = D / 32;  // columns of a lane, side by side
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
   constexpr int kBatch = SHARE > 1 ? 8 : 4;
-  constexpr int kKept = SHARE > 1 ? 4 : 1;
+  constexpr int kKept = SHARE > 1 ? 8 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   const int parts = rp.n;
@@ -648,8 +750,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     it.w = work_at(p, min(it.b, p.B - 1));
     it.seq0 = it.run = 0;
     if (p.B <= 32) {  // the list in one scan; else what the row kernel left
-      const int64_t mine = lane < p.B ? steps_of(p, work_at(p, lane)) : 0, upto = warp_scan(mine);
-      it.run = run_of(p, __shfl_sync(0xffffffffu, upto, 31));
+      int64_t mine = 0;
+      int longest = 0;
+      if (lane < p.B) {
+        const Work w = work_at(p, lane);
+        mine = steps_of(p, w);
+        longest = w.tiles;
+      }
+      const int64_t upto = warp_scan(mine);
+      it.run = run_of(p, __shfl_sync(0xffffffffu, upto, 31), __reduce_max_sync(0xffffffffu, longest));
       it.seq0 = __shfl_sync(0xffffffffu, upto - mine, min(it.b, 31));
     }
     return it;
@@ -661,12 +770,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     }
   };
   auto parts_of = [&](const Item& it, int r) {
-    RowParts rp{0, 0, 0, 0};
+    RowParts rp;
+    rp.n = 0;
     if (it.w.tiles > 0) {
-      rp.unit0 = it.seq0 + (static_cast<int64_t>(it.kvh) * it.w.rts + r / kRows) * it.w.tiles;
-      rp.run = it.run;
-      rp.first = div64(rp.unit0, rp.run);
-      rp.n = static_cast<int>(min(static_cast<int64_t>(p.workers) - 1, div64(rp.unit0 + it.w.tiles - 1, rp.run)) - rp.first) + 1;
+      const int64_t begin = it.seq0 + (static_cast<int64_t>(it.kvh) * it.w.rts + r / kRows) * it.w.tiles;
+      rp.find(begin, begin + it.w.tiles, it.run);
     }
     return rp;
   };
