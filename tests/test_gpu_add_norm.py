@@ -48,6 +48,20 @@ def test_against_the_formula(rows, cols, dtype):
     check(out, total, x, r, w, 1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 2, 13])
+@pytest.mark.parametrize("cols", [1, 2, 63, 126, 127, 129, 255, 510, 511, 513, 1022, 1023, 1025, 2047, 2049, 4095, 4097,
+                                  6143, 6145, 12289])
+def test_odd_widths(cols, rows, dtype):
+    """Rows shared out among 32 to 512 threads, several in a CTA and not a
+    multiple of them, either half of a word first."""
+    x, r, w = make(rows, cols, dtype)
+    out, total = torch.ops.b200.add_rms_norm(x, r, w, 1e-5)
+    check(out, total, x, r, w, 1e-5)
+    q, scale, total = torch.ops.b200.add_rms_norm_quant(x, r, w, 1e-5)
+    check_quant(q, scale, total, x, r, w, 0)
+
+
 @pytest.mark.parametrize("flags", [1, 8, 9])
 @pytest.mark.parametrize("cols", [1024, 99])
 def test_flags(cols, flags):

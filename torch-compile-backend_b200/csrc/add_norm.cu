@@ -286,20 +286,26 @@ __global__ void __launch_bounds__(THREADS) add_norm_kernel(const __grid_constant
 }
 
 // 16-bit rows of any width whose four tensors start on the same half of a
-// 4-byte word in every row: a CTA of 512 threads per row, PPT pairs of columns
-// a thread in registers (odd widths shift the rows' alignment one by one; the
-// columns at a row's ends are moved alone).  4096 rows of 5001: 47.5 us, with
-// add_norm_any_kernel 70.
-template <int DT, int QUANT, int PPT>
-__global__ void __launch_bounds__(512) add_norm_pair_kernel(const __grid_constant__ AddNormParams p) {
+// 4-byte word in every row: TPR threads per row, PPT pairs of columns a thread
+// in registers (odd widths shift the rows' alignment one by one; the
+// columns at a row's ends are moved alone).  Bound by its 2-byte weight loads
+// and ragged stores: 4096 rows of 5001 47.5 us (25 the bytes'; with
+// add_norm_any_kernel 70), of 1001 11.5 (with 512 threads a row 19), 30000 of 99
+// 10.2 (124).  Wider rows lose to add_norm_any_kernel: 4096 of 6501 86 and 84
+// us, of 9001 131 and 118.
+template <int DT, int QUANT, int PPT, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_norm_pair_kernel(const __grid_constant__ AddNormParams p) {
   constexpr bool BF16 = DT == B200K_BF16;
   __shared__ uint32_t slots[2][32];
-  const int64_t row = blockIdx.x;
+  constexpr int kGroups = TPR < 256 ? 256 / TPR : 1;
+  const int grp = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + grp;
+  if (row >= p.rows) return;  // the whole group: its barrier is its own
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.x_stride;
   const uint16_t* r = static_cast<const uint16_t*>(p.r) + row * p.r_stride;
   uint16_t* h = static_cast<uint16_t*>(p.h) + row * p.cols;
   const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(x) >> 1) & 1);
-  auto col = [&](int i) { return 2 * (static_cast<int>(threadIdx.x) + i * 512) - odd; };
+  auto col = [&](int i) { return 2 * (t + i * TPR) - odd; };
   uint32_t v[PPT];
   {
     uint32_t a[PPT];
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(512) add_norm_pair_kernel(const __grid_constan
     const float2 f = unpack(v[i]);
     ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
   }
-  ss = __uint_as_float(row_reduce<512, false>(__float_as_uint(ss), slots[0], 0));
+  ss = __uint_as_float(row_reduce<TPR, false>(__float_as_uint(ss), slots[0], grp));
   const float rstd = rsqrtf(ss / static_cast<float>(p.cols) + p.eps);
   const bool round_n = p.flags & B200K_ROWF_ROUND_NORMED, plus1 = p.flags & B200K_ROWF_WEIGHT_PLUS_ONE;
   float2 y[PPT];
@@ -380,10 +386,10 @@ __global__ void __launch_bounds__(512) add_norm_pair_kernel(const __grid_constan
     }
   }
   if (QUANT == 1) {
-    top = row_reduce<512, true>(top, slots[1], 0);
+    top = row_reduce<TPR, true>(top, slots[1], grp);
     float inv;
     const float sc = scale_of(top, inv);
-    if (threadIdx.x == 0) p.scale[row] = sc;
+    if (t == 0) p.scale[row] = sc;
     uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.cols;
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
@@ -482,10 +488,14 @@ void launch(const AddNormParams& p, bool vec, cudaStream_t st) {
       const auto want = half(p.x, p.rows > 1 ? p.x_stride : p.cols);
       const bool same = want == half(p.r, p.rows > 1 ? p.r_stride : p.cols) && want == half(p.h, p.cols) &&
                         (QUANT == 1 || want == half(p.out, p.cols));
-      if (same && p.cols < 16 * 1024) {
-        if (p.cols < 2 * 1024) add_norm_pair_kernel<DT, QUANT, 2><<<rows, 512, 0, st>>>(p);
-        else if (p.cols < 6 * 1024) add_norm_pair_kernel<DT, QUANT, 6><<<rows, 512, 0, st>>>(p);
-        else add_norm_pair_kernel<DT, QUANT, 16><<<rows, 512, 0, st>>>(p);
+      if (same && p.cols < 6 * 1024) {
+        // 2 PPT TPR columns and more than cols
+        if (p.cols < 128) add_norm_pair_kernel<DT, QUANT, 2, 32><<<(rows + 7) / 8, 256, 0, st>>>(p);
+        else if (p.cols < 512) add_norm_pair_kernel<DT, QUANT, 8, 32><<<(rows + 7) / 8, 256, 0, st>>>(p);
+        else if (p.cols < 1024) add_norm_pair_kernel<DT, QUANT, 4, 128><<<(rows + 1) / 2, 256, 0, st>>>(p);
+        else if (p.cols < 2 * 1024) add_norm_pair_kernel<DT, QUANT, 4, 256><<<rows, 256, 0, st>>>(p);
+        else if (p.cols < 4 * 1024) add_norm_pair_kernel<DT, QUANT, 8, 256><<<rows, 256, 0, st>>>(p);
+        else add_norm_pair_kernel<DT, QUANT, 6, 512><<<rows, 512, 0, st>>>(p);
         return;
       }
     }
