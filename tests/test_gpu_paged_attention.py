@@ -127,6 +127,25 @@ def test_one_sequence_of_one_key_head(H, hkv, D):
     run(ref.paged_inputs([1, 1], [20011, 64], H, hkv, D, 16, BF))
 
 
+@pytest.mark.parametrize("D,seqs", [(128, 8), (64, 16), (128, 260)])
+@pytest.mark.parametrize("keys", [60, 4000])
+def test_two_row_blocks_a_sequence(D, seqs, keys):
+    """Sequences of 17 to 32 rows among shorter and longer ones: the row kernel
+    for few keys (a wide table, so that many are possible) and for many
+    sequences, the tile kernel for many keys."""
+    qs = [(5, 8, 1, 6)[b % 4] for b in range(seqs)]
+    ns = [keys if seqs < 100 else 90] * seqs
+    qs[1], ns[2], ns[5] = 11, 0, 3
+    q, kc, vc, table, q_start, kv_len = ref.paged_inputs(qs, ns, 32, 8, D, 16, BF, pad=3)
+    wide = torch.full((seqs, 2000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    for max_q in (0, 11):
+        run((q, kc, vc, wide, q_start, kv_len), max_q=max_q)
+    q8 = [min(m, 8) for m in qs]
+    first = run(ref.paged_inputs(q8, ns, 32, 8, D, 16, BF), max_q=8)
+    assert torch.equal(run(ref.paged_inputs(q8, ns, 32, 8, D, 16, BF), max_q=8), first)
+
+
 def test_strided_queries():
     q, *rest = ref.paged_inputs([1, 5, 2], [30, 60, 2], 8, 2, 64, 16, BF)
     wide = torch.zeros(q.shape[0], 12, 64, device="cuda", dtype=BF)

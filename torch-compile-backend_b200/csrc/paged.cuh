@@ -29,7 +29,8 @@ struct Params {
   int32_t page_size, num_pages, table_cols;
   int32_t capacity;            // table_cols * page_size, clamped to int32
   int32_t window;              // 0: none
-  int32_t long_rows;           // sequences of more query rows (queries * G) run the tile kernel
+  int32_t long_rows;           // sequences of more query rows (queries * G) run the tile kernel,
+  int64_t mid_steps;           // those of more than kRows too where they have so many steps (0: never)
   int32_t combine_rows;        // tokens of a sequence that the combine grid covers side by side
   int32_t join_mode;           // how the combine kernel's warps share the rows
   FastDiv div_page, div_g;

@@ -91,13 +91,14 @@ struct Work {
   int tiles;  // 0: no keys, no queries, or the tile kernel's
   int rts;    // 16-row blocks of a kv head
 };
-__device__ __forceinline__ Work work_at(const Params& p, int b) {
+// `limit`: query rows above which a sequence is the tile kernel's.
+__device__ __forceinline__ Work work_at(const Params& p, int b, int limit) {
   Work w;
   w.s = seq_at(p, b);
   w.base = w.s.lo & ~(kKeys - 1);
   const int64_t rows = static_cast<int64_t>(w.s.m) * p.G;
   w.rts = static_cast<int>((rows + kRows - 1) / kRows);
-  w.tiles = (w.s.m > 0 && w.s.n > w.base && rows <= p.long_rows) ? (w.s.n - w.base + kKeys - 1) / kKeys : 0;
+  w.tiles = (w.s.m > 0 && w.s.n > w.base && rows <= limit) ? (w.s.n - w.base + kKeys - 1) / kKeys : 0;
   return w;
 }
 __device__ __forceinline__ int64_t steps_of(const Params& p, const Work& w) {
@@ -111,6 +112,21 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
     if (lane >= o) v += u;
   }
   return v;
+}
+
+// The limit of this call: p.long_rows, or kRows where the sequences between
+// the two (two row blocks, so the row kernel reads their keys twice) have
+// enough keys for the tile kernel to pay.  Every warp that asks gets the same.
+__device__ __forceinline__ int limit_of(const Params& p) {
+  if (p.mid_steps == 0) return p.long_rows;
+  int64_t steps = 0;
+  for (int b = threadIdx.x & 31; b < p.B; b += 32) {
+    const Work w = work_at(p, b, p.long_rows);
+    if (w.rts > 1) steps += static_cast<int64_t>(p.Hkv) * w.tiles;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, o);
+  return steps >= p.mid_steps ? kRows : p.long_rows;
 }
 
 // n / d for n >= 0, d > 0: 32-bit where both fit, which every real list does
@@ -135,6 +151,7 @@ __device__ __forceinline__ int64_t run_of(const Params& p, int64_t total, int lo
 struct Cursor {
   Work w;
   int b, kvh, rt, tile;
+  int limit;
   __device__ __forceinline__ void next(const Params& p) {
     if (++tile < w.tiles) return;
     tile = 0;
@@ -144,7 +161,7 @@ struct Cursor {
     kvh = 0;
     do {
       if (++b >= p.B) return;
-      w = work_at(p, b);
+      w = work_at(p, b, limit);
     } while (w.tiles == 0 || w.rts == 0);
   }
 };
@@ -157,6 +174,7 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t* before = p.entry_steps + 3;
   for (int i = tid; i < p.tile_ctas; i += kWarps * 32) p.joins[i].last = 0;
+  const int limit = limit_of(p);
   int64_t steps = 0;
   int entry0 = 0;
   auto block_scan = [&](int64_t v, int64_t& all) {  // inclusive
@@ -175,7 +193,7 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
     int n = 0;
     if (b0 + tid < p.B) {
       const int64_t rows = static_cast<int64_t>(seq_at(p, b0 + tid).m) * p.G;
-      if (rows > p.long_rows) n = static_cast<int>((rows + kUnitRows - 1) / kUnitRows);
+      if (rows > limit) n = static_cast<int>((rows + kUnitRows - 1) / kUnitRows);
     }
     int64_t all;
     const int64_t upto = block_scan(n, all);
@@ -287,12 +305,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // The whole list's length and, from it, this worker's run [w0, w1).
+  const int limit = limit_of(p);
   int64_t total = 0, mine0 = 0, upto0 = 0;
   int longest = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = 0;
     if (b0 + lane < p.B) {
-      const Work w = work_at(p, b0 + lane);
+      const Work w = work_at(p, b0 + lane, limit);
       mine = steps_of(p, w);
       longest = max(longest, w.tiles);
     }
@@ -315,7 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = mine0, upto = upto0;  // of the last 32: all there are in a small batch
     if (p.B > 32) {
-      mine = b0 + lane < p.B ? steps_of(p, work_at(p, b0 + lane)) : 0;
+      mine = b0 + lane < p.B ? steps_of(p, work_at(p, b0 + lane, limit)) : 0;
       upto = warp_scan(mine);
     }
     const unsigned hit = __ballot_sync(0xffffffffu, seq0 + upto > w0);
@@ -327,7 +346,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     }
     seq0 += __shfl_sync(0xffffffffu, upto, 31);
   }
-  cur.w = work_at(p, cur.b);
+  cur.limit = limit;
+  cur.w = work_at(p, cur.b, limit);
   const int unit = static_cast<int>(div64(w0 - seq0, cur.w.tiles));
   cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(unit) * cur.w.tiles);
   cur.kvh = unit / cur.w.rts;
@@ -741,19 +761,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     int b, y, h, kvh;
     int64_t seq0, run;
   };
+  const int limit = limit_of(p);
   auto look = [&](int item) {
     Item it;
     it.h = item % p.H;
     it.y = item / p.H % p.combine_rows;
     it.b = item / p.H / p.combine_rows;
     it.kvh = static_cast<int>(fdiv(static_cast<uint32_t>(it.h), p.div_g));
-    it.w = work_at(p, min(it.b, p.B - 1));
+    it.w = work_at(p, min(it.b, p.B - 1), limit);
     it.seq0 = it.run = 0;
     if (p.B <= 32) {  // the list in one scan; else what the row kernel left
       int64_t mine = 0;
       int longest = 0;
       if (lane < p.B) {
-        const Work w = work_at(p, lane);
+        const Work w = work_at(p, lane, limit);
         mine = steps_of(p, w);
         longest = w.tiles;
       }
@@ -800,7 +821,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     const int64_t step = static_cast<int64_t>(row_ctas) * (W * 32);
     for (int64_t i = cta * static_cast<int64_t>(W * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
   }
-  const bool real = it.b < p.B && static_cast<int64_t>(it.w.s.m) * p.G <= p.long_rows;  // else the tile kernel's, or none
+  const bool real = it.b < p.B && static_cast<int64_t>(it.w.s.m) * p.G <= limit;  // else the tile kernel's, or none
   if (real) finish_look(it);
   if constexpr (MODE == kRowCta) {
     if (real) join(it, together, [](int) { return true; });
@@ -896,10 +917,27 @@ int check_shape(const B200kPagedAttentionArgs* a) {
 // to 68 rows of 8 sequences to 1500 keys, heads of 64, 22 and 29 (27).
 constexpr int kLongRows = 32;
 
-bool may_be_long(const B200kPagedAttentionArgs* a) {
+// ... and sequences of more rows than one block of the row kernel where all
+// such have this many steps of 128 values together.  Five tokens of 16
+// sequences, 32 / 8 heads of 128, to 1000 (8000 steps), 2000, 4000 and 8000
+// keys: row kernel 30, 52, 90 and 165 us, tile kernel 32, 44, 64 and 108.  Only
+// the device knows the lengths; where the page table could hold as many steps
+// the tile kernel is launched, which costs 2 to 6 us when it has no work.
+constexpr int64_t kMidSteps = 12288;
+// Sequences that the limit is worked out for: every warp goes over them.
+constexpr int kMidSeqs = 256;
+
+int64_t most_rows(const B200kPagedAttentionArgs* a) {
   const int64_t q = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
-  return q * (a->heads / a->kv_heads) > kLongRows;
+  return q * (a->heads / a->kv_heads);
 }
+int64_t mid_steps(const B200kPagedAttentionArgs* a) {
+  const int64_t steps = kMidSteps * 128 / a->head_dim;
+  const int64_t keys = std::min<int64_t>(a->table_cols * a->page_size, 0x3fffffff);
+  const bool reach = a->seqs <= kMidSeqs && a->seqs * a->kv_heads * (keys / kKeys + 1) >= steps;
+  return most_rows(a) > kRows && reach ? steps : 0;
+}
+bool may_be_long(const B200kPagedAttentionArgs* a) { return most_rows(a) > kLongRows || mid_steps(a) > 0; }
 
 // Entries of the tile kernel's list: 256-row blocks of sequences that share the
 // tokens out among them.
@@ -992,6 +1030,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.tile_ctas = may_be_long(a) ? sms : 0;
   p.max_entries = static_cast<int32_t>(max_entries(a));
   p.long_rows = p.tile_ctas > 0 ? kLongRows : 0x7fffffff;
+  p.mid_steps = mid_steps(a);
   p.test_flags = a->test_flags;
   p.div_page = make_fastdiv(static_cast<uint32_t>(p.page_size));
   p.div_g = make_fastdiv(static_cast<uint32_t>(p.G));
