@@ -16,7 +16,7 @@
 // whatever their order, and a single long sequence spreads over the GPU.
 // A warp streams its steps' rows of K and V into its own shared-memory ring
 // with 16-byte cp.async copies (S - 1 steps ahead, across unit boundaries; no
-// block-wide barrier anywhere), multiplies with m16n8k16 MMAs (16 rows by 8
+// block-wide barrier while it streams), multiplies with m16n8k16 MMAs (16 rows by 8
 // keys, rows beyond the unit's are zero: the tensor pipe has the time, the
 // memory does not) and keeps its running maximum, sum and output in fp32.
 // A unit inside one run is written at once; a cut one leaves its parts
@@ -24,8 +24,8 @@
 // warps are all in the unit (one token over 30000 keys of one key head: 20 us,
 // with a part a warp 42), and combine_kernel joins them in an order that only
 // the lengths decide.
-// Measured: one token of 64 sequences to 8192 keys, 32 / 8 heads of 128, 211 us
-// = 6.48 TB/s; of 3 sequences to 65536 keys 95 us = 6.05 TB/s.
+// Measured: one token of 64 sequences to 8192 keys, 32 / 8 heads of 128, 215 us
+// = 6.36 TB/s; of 3 sequences to 65536 keys 95 us = 6.05 TB/s.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
