@@ -554,8 +554,9 @@ int b200k_rope_append(const B200kRopeAppendArgs* args, void* stream);
  *   out[t, h] = sum_j softmax_j(f(scale q . k_j)) v_j,  f(s) = s, or
  *   softcap * tanh(s / softcap) when softcap > 0
  * with key / value head h / (heads / kv_heads).  A query without keys (p < 0)
- * or with scores of -inf alone and a token behind the last sequence get zeros;
- * a NaN or +inf among a query's scores gives it NaN.  q, caches and out are of
+ * or with scores of -inf alone and a token of no sequence (in front of
+ * q_start[0] or behind the last sequence) get zeros; a NaN or +inf among a
+ * query's scores gives it NaN.  q, caches and out are of
  * one 16-bit type; head_dim 64 or 128; cache_strides as for
  * b200k_rope_append; strides multiples of 8 elements, pointers 16-byte
  * aligned; out contiguous.  Nothing is read of the caches outside the keys

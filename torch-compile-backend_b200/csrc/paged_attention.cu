@@ -724,8 +724,8 @@ __device__ __forceinline__ void join_row(const Params& p, const RowParts& rp, in
 }
 
 // Joins the parts of the units that were cut, and writes zeros for the rows
-// that no step covers: queries without keys and tokens behind the last
-// sequence.  An item is a (sequence, token, head); MODE says how the four
+// that no step covers: queries without keys and tokens of no sequence, in front
+// of the first and behind the last.  An item is a (sequence, token, head); MODE says how the four
 // warps of a CTA share them:
 //   kRowCta    one item a CTA, all warps together: few items, each of many
 //              parts (a single long sequence has one for every worker);
@@ -813,14 +813,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
   const int cta = static_cast<int>(blockIdx.x);
   const int item = MODE == kRowCta ? cta : MODE == kRowMixed ? warp * row_ctas + cta : cta * W + warp;
   Item it = look(item);
-  const int end = min(max(__ldg(p.q_start + p.B), 0), p.T);
+  const int first = min(max(__ldg(p.q_start), 0), p.T), end = min(max(__ldg(p.q_start + p.B), 0), p.T);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  {  // tokens behind the last sequence
-    const int64_t words = static_cast<int64_t>(p.T - end) * p.H * (D / 2);
-    uint32_t* dst = out_row(end, 0);
+  auto zero = [&](int from, int to) {
+    const int64_t words = static_cast<int64_t>(to - from) * p.H * (D / 2);
+    uint32_t* dst = out_row(from, 0);
     const int64_t step = static_cast<int64_t>(row_ctas) * (W * 32);
     for (int64_t i = cta * static_cast<int64_t>(W * 32) + threadIdx.x; i < words; i += step) dst[i] = 0u;
-  }
+  };
+  zero(0, first);  // tokens in front of the first sequence, and behind the last
+  zero(end, p.T);
   const bool real = it.b < p.B && static_cast<int64_t>(it.w.s.m) * p.G <= limit;  // else the tile kernel's, or none
   if (real) finish_look(it);
   if constexpr (MODE == kRowCta) {
