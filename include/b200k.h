@@ -563,8 +563,10 @@ int b200k_rope_append(const B200kRopeAppendArgs* args, void* stream);
  * that a sequence's queries see, so other pages and the rest of the last one
  * may hold anything.  Of the keys that some query of the sequence sees, those
  * hidden from another query have weight 0 for it: their values must be
- * finite, or it may become NaN, as 0 * inf does.  Scores, softmax and sums are fp32; the probabilities are
- * rounded to the input type for the second product.  max_q_len (0: unknown)
+ * finite, or it may become NaN, as 0 * inf does.  Scores, softmax and sums are
+ * fp32; the probabilities are rounded to the input type for the second product,
+ * half a step each (f16: those below 2^-26 of a row's maximum by less than
+ * 2^-36 of it).  max_q_len (0: unknown)
  * is a hint of the longest sequence's queries: it chooses kernels and grids,
  * never results.  Index tensors are i32 on the device; entries out of range
  * are clamped (a page out of range reads as zeros) and set *status (may be

@@ -12,6 +12,22 @@ constexpr int kKeys = 16;      // keys of one step of the row kernel (one MMA k)
 constexpr int kRows = 16;      // query rows of one unit of the row kernel (one MMA m)
 constexpr int kBlock = 64;     // keys of one step of the tile kernel
 constexpr int kUnitRows = 256; // query rows of one unit of the tile kernel (two MMA m)
+// Probabilities of the second product are rounded to the input type.  f16 ones
+// below 2^-14 would lose bits and those below 2^-25 vanish, while their sum
+// keeps them (a key 17 nats above the others and of value zero: the output 40 %
+// off), so they are computed 2^kF16Reach times too large, the sum with them,
+// which the division takes out: f16 reaches 65504.  A tile's maximum may lag
+// behind by 2^kLagF16, which its probabilities have to leave free.  8 f16
+// prompts of 2048 (32 heads of 64) with a lag of 8, 4, 3 and 2: 279, 275, 278
+// and 286 us.  bf16 has fp32's exponents.
+constexpr float kF16Reach = 15.0f;
+constexpr float kLagF16 = 3.0f, kLagBf16 = 8.0f;
+template <bool BF16>
+constexpr float kRowReach = BF16 ? 0.0f : kF16Reach;
+template <bool BF16>
+constexpr float kTileLag = BF16 ? kLagBf16 : kLagF16;
+template <bool BF16>
+constexpr float kTileReach = BF16 ? 0.0f : kF16Reach - kLagF16;
 // What a unit's start and end cost (queries in, output out, pipeline empty),
 // in steps: counted in the list that the CTAs share out.  8 prompts of 2048
 // (32 heads of 64) with 0, 2, 4 and 8: 387, 300, 277 and 297 us.

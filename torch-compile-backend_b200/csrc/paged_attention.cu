@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
       const float was = m[i];
       m[i] = fmaxf(was, x);
-      const float ref = m[i] == -INFINITY ? 0.0f : m[i];
-      alpha[i] = ex2(was - ref);
+      const float top = m[i] == -INFINITY ? 0.0f : m[i], ref = top - kRowReach<BF16>;
+      alpha[i] = ex2(was - top);
       moved |= m[i] != was;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
@@ -494,8 +494,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       l[i] += (s[0][2 * i] + s[0][2 * i + 1]) + (s[1][2 * i] + s[1][2 * i + 1]);
-    // probabilities rounded to the input type for the second product (the
-    // sum keeps fp32): half a step each, as b200k_attention
+    // probabilities rounded to the input type for the second product (the sum
+    // keeps fp32): half a step each, in f16 down to 2^-29 of the row's maximum
+    // (smaller ones by less than 2^-40 of it)
     pa[0] = pack16<BF16>(s[0][0], s[0][1]);
     pa[1] = pack16<BF16>(s[0][2], s[0][3]);
     pa[2] = pack16<BF16>(s[1][0], s[1][1]);

@@ -62,7 +62,6 @@ constexpr uint32_t kHalfBlk = kBlock * 128;
 // Of so many probabilities two are computed on the FMA pipe.  8 prompts of
 // 2048 (32 heads of 64): 277 us, 291 with none, 286 with half of them.
 constexpr int kFmaEvery = 8;
-constexpr float kRescaleLog2 = 8.0f;       // a running maximum may lag by a factor of 256
 template <int D>
 struct Layout {
   static constexpr int kStages = D == 128 ? 4 : 6;         // of K and of V
@@ -565,12 +564,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool moved = false;
         // A NaN score, and an infinite one (0 * top), makes the maximum NaN and
         // with it every probability and sum of the row from here on.
-        if (!(top <= m + kRescaleLog2)) {
+        if (!(top <= m + kTileLag<BF16>)) {
           m = fmaf(0.0f, top, top);
           alpha = ex2(was - m);
           moved = j > jb;
         }
-        const float ref = m == -INFINITY ? 0.0f : m;
+        // probabilities are rounded to the input type, half a step each, in f16
+        // down to 2^-26 of the row's maximum (smaller ones by less than 2^-36 of it)
+        const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<BF16>;
         float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         const float2 sc2 = CAP ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(-ref, -ref);
         uint32_t pk[kBlock / 2];
