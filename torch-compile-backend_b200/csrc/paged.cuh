@@ -57,8 +57,9 @@ struct Params {
   int64_t c_page, c_slot, c_head;
   uint16_t* out;               // [T, H, D] contiguous
   const int32_t *table, *q_start, *kv_len;
-  // base-2 scores: y = x * mul, or with a cap y = cap2 - 2 cap2 / (1 + 2^(x mul)) = cap2 tanh(x scale / cap)
-  float mul, cap2;
+  // base-2 scores: y = x * mul; with a cap (cap_far) mul = 2 scale log2(e) / cap,
+  // lin = scale log2(e), cap2 = cap log2(e)
+  float mul, lin, cap2;
   float* part_o;               // [workers][2][16][D]
   float* part_ml;              // [workers][2][16][2]: running max (base 2) and sum
   int64_t* prefix;             // [B + 1] steps before each sequence; [B + 1]: steps a worker takes
@@ -131,7 +132,7 @@ __device__ __forceinline__ void tile_keys(const Params& p, const Unit& u, int t,
 }
 
 // Launches the tile kernel (paged_tiles.cu) on the plan in p.entries.
-int launch_tiles(const Params& p, bool bf16, int dim, bool cap, cudaStream_t st);
+int launch_tiles(const Params& p, bool bf16, int dim, int cap, cudaStream_t st);
 
 // Offset of a key's row in the caches, `page` being what the table holds for
 // it, or -1: not between lo and n (nothing there is read: the pages may hold
@@ -163,10 +164,34 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <bool CAP>
+// A capped score in base 2: cap2 tanh(u), u = x scale / cap, with t = 2 u log2(e)
+// at hand as x mul.  Where the cap is at most kPlainCap, cap2 - 2 cap2 / (1 + 2^t):
+// the approximate units' 2^-22 and 2^-23 leave 3.6e-7 of the cap, 3.6e-5.  That
+// error stays at small u, where the terms cancel, and grows with the cap (with
+// scores of 5 and a cap of 1e6 it was 0.1).  So with larger ones (kCapSeries)
+// scores below 0.35 of the cap are the series tanh(u) = u (1 + u^2 P(u^2)) on the
+// uncapped score u cap2 = x lin, P by Remez exchange on [0, 0.35^2], 4.1e-8
+// relative; above, the first form is within 6.2e-7 of the score.  The series for
+// every cap: decode of 64 sequences to 8192 keys 232 us in place of 225, chunks
+// whose scores reach the cap 693 in place of 489.
+constexpr float kPlainCap = 100.0f;
+enum { kNoCap, kCapPlain, kCapSeries };
+constexpr float kSmallCap = 0.35f * 2.0f * kLog2e;
+__device__ __forceinline__ float cap_far(const Params& p, float t) {
+  return fmaf(-2.0f * p.cap2, rcp(1.0f + ex2(t)), p.cap2);
+}
+__device__ __forceinline__ float cap_near(const Params& p, float x, float t) {
+  constexpr float k = 1.0f / (2.0f * kLog2e);  // u = k t
+  const float w = x * p.lin, z = t * t;
+  float r = fmaf(-4.9148502e-2f * (k * k * k * k * k * k), z, 1.3299825e-1f * (k * k * k * k));
+  r = fmaf(r, z, -3.3332663e-1f * (k * k));
+  return fmaf(w, z * r, w);
+}
+template <int CAP>
 __device__ __forceinline__ float score(const Params& p, float x) {
-  if (!CAP) return x * p.mul;
-  return fmaf(-2.0f * p.cap2, rcp(1.0f + ex2(x * p.mul)), p.cap2);
+  const float t = x * p.mul;
+  if (CAP == kNoCap) return t;
+  return CAP == kCapSeries && fabsf(t) < kSmallCap ? cap_near(p, x, t) : cap_far(p, t);
 }
 
 template <bool BF16>

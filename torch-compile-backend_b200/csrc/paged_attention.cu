@@ -284,7 +284,7 @@ __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int w
   }
 }
 
-template <bool BF16, int D, bool CAP>
+template <bool BF16, int D, int CAP>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __grid_constant__ Params p) {
   constexpr int S = kRingBytes / (kKeys * D * 4);  // ring stages: K and V rows of a step each
   constexpr uint32_t kRowBytes = D * 2, kTile = kKeys * kRowBytes;
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
   }
 }
 
-template <bool BF16, int D, bool CAP>
+template <bool BF16, int D, int CAP>
 int launch(const Params& p, int ctas, cudaStream_t st) {
   constexpr uint32_t kSmem = kWarps * kRingBytes;
   auto kernel = rows_kernel<BF16, D, CAP>;
@@ -887,8 +887,9 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
 }
 
 template <bool BF16, int D>
-int launch_cap(const Params& p, bool cap, int ctas, cudaStream_t st) {
-  return cap ? launch<BF16, D, true>(p, ctas, st) : launch<BF16, D, false>(p, ctas, st);
+int launch_cap(const Params& p, int cap, int ctas, cudaStream_t st) {
+  if (cap == kNoCap) return launch<BF16, D, kNoCap>(p, ctas, st);
+  return cap == kCapPlain ? launch<BF16, D, kCapPlain>(p, ctas, st) : launch<BF16, D, kCapSeries>(p, ctas, st);
 }
 
 }  // namespace
@@ -1050,11 +1051,12 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.table = a->page_table;
   p.q_start = a->q_start;
   p.kv_len = a->kv_len;
-  const bool cap = a->softcap > 0.0f;
+  const int cap = a->softcap == 0.0f ? kNoCap : a->softcap <= kPlainCap ? kCapPlain : kCapSeries;
   const float scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
-  p.mul = cap ? 2.0f * scale / a->softcap * kLog2e : scale * kLog2e;
+  p.mul = cap != kNoCap ? 2.0f * scale / a->softcap * kLog2e : scale * kLog2e;
+  p.lin = scale * kLog2e;
   p.cap2 = a->softcap * kLog2e;
-  if (!std::isfinite(p.mul)) return B200K_ERR_ARG;  // a cap too small for its scale
+  if (!std::isfinite(p.mul) || !std::isfinite(p.lin)) return B200K_ERR_ARG;  // a cap too small for its scale
   const int ctas = sms * kCtasPerSm;
   p.workers = ctas * kWarps;
   place(a, sms, static_cast<uint8_t*>(a->workspace), &p);

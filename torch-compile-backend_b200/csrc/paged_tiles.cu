@@ -237,7 +237,7 @@ struct Walk {
   }
 };
 
-template <bool BF16, int D, bool CAP>
+template <bool BF16, int D, int CAP>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
@@ -539,9 +539,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(raw[c][i]);
         }
-        if (CAP) {
+        if (CAP != kNoCap) {
 #pragma unroll
-          for (int c = 0; c < kBlock; ++c) s[c] = score<true>(p, s[c]);
+          for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, s[c]);
         }
         const int key0 = j * kBlock;
         if (key0 + kBlock - 1 > w_lo || (p.window > 0 && key0 <= w_hi - p.window)) {  // warp-uniform
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx[i] = max2(mx[i], s[kBlock - 4 + i]);
         float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
-        if (!CAP) top *= p.mul;
+        if (CAP == kNoCap) top *= p.mul;
         const float was = m;
         float alpha = 1.0f;
         bool moved = false;
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // down to 2^-26 of the row's maximum (smaller ones by less than 2^-36 of it)
         const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<BF16>;
         float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        const float2 sc2 = CAP ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(-ref, -ref);
+        const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(-ref, -ref);
         uint32_t pk[kBlock / 2];
 #pragma unroll
         for (int c = 0; c < kBlock; c += 2) {
@@ -677,7 +677,7 @@ bool make_map(CUtensorMap* map, bool bf16, const void* ptr, const int64_t (&size
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool BF16, int D, bool CAP>
+template <bool BF16, int D, int CAP>
 int launch(Params p, cudaStream_t st) {
   auto kernel = tiles_kernel<BF16, D, CAP>;
   static std::atomic<uint64_t> done{0};
@@ -720,15 +720,17 @@ int launch(Params p, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, kernel, p, tq, tk, tv) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
+template <bool BF16, int D>
+int launch_cap(const Params& p, int cap, cudaStream_t st) {
+  if (cap == kNoCap) return launch<BF16, D, kNoCap>(p, st);
+  return cap == kCapPlain ? launch<BF16, D, kCapPlain>(p, st) : launch<BF16, D, kCapSeries>(p, st);
+}
+
 }  // namespace
 
-int launch_tiles(const Params& p, bool bf16, int dim, bool cap, cudaStream_t st) {
-  if (dim == 64) {
-    if (bf16) return cap ? launch<true, 64, true>(p, st) : launch<true, 64, false>(p, st);
-    return cap ? launch<false, 64, true>(p, st) : launch<false, 64, false>(p, st);
-  }
-  if (bf16) return cap ? launch<true, 128, true>(p, st) : launch<true, 128, false>(p, st);
-  return cap ? launch<false, 128, true>(p, st) : launch<false, 128, false>(p, st);
+int launch_tiles(const Params& p, bool bf16, int dim, int cap, cudaStream_t st) {
+  if (dim == 64) return bf16 ? launch_cap<true, 64>(p, cap, st) : launch_cap<false, 64>(p, cap, st);
+  return bf16 ? launch_cap<true, 128>(p, cap, st) : launch_cap<false, 128>(p, cap, st);
 }
 
 }  // namespace paged
