@@ -1,0 +1,57 @@
+"""What the serving operators refuse, on the CPU (fake tensors and the C ABI
+before any launch)."""
+import ctypes
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from compiler import runtime
+from compiler.runtime import cabi
+from test_serving_host import ARG, attn_args
+
+runtime.load()
+
+
+def calls():
+    """Per operator: arguments, and which of them are floating tensors."""
+    def t(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="cuda")
+    cache = t(4, 16, 2, 64), t(4, 16, 2, 64)
+    ints = t(3, dtype=torch.int32)
+    return {"add_rms_norm": (t(3, 256), t(3, 256), t(256), 1e-5),
+            "add_rms_norm_quant": (t(3, 256), t(3, 256), t(256), 1e-5, 128),
+            "rope_append": (t(3, 8, 64), t(3, 2, 64), t(3, 2, 64), t(9, 32), t(9, 32), ints, ints, *cache),
+            "paged_attention": (t(3, 8, 64), *cache, t(2, 4, dtype=torch.int32), ints, ints[:2])}
+
+
+FLOATS = {"add_rms_norm": 3, "add_rms_norm_quant": 3, "rope_append": 9, "paged_attention": 3}
+CASES = [(op, i) for op, n in FLOATS.items() for i in range(n) if not (op == "rope_append" and i in (5, 6))]
+
+
+@pytest.mark.parametrize("op,at", CASES)
+def test_inputs_with_a_tangent_are_refused(op, at):
+    """No derivative is defined in forward mode either: a tangent would be
+    dropped without a word."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f = getattr(torch.ops.b200, op)
+    with FakeTensorMode(allow_non_fake_inputs=True), forward_ad.dual_level():
+        args = list(calls()[op])
+        with torch.no_grad():
+            f(*args)
+        args[at] = forward_ad.make_dual(args[at], torch.ones_like(args[at]))
+        for grad in (True, False):  # no_grad does not switch forward mode off
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no gradient is defined"):
+                f(*args)
+
+
+@pytest.mark.parametrize("op", list(FLOATS))
+def test_functional_jvp_is_refused(op):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        first, *rest = calls()[op]
+        f = lambda x: getattr(torch.ops.b200, op)(x, *rest)  # noqa: E731
+        with pytest.raises(RuntimeError, match="no gradient is defined"):
+            torch.func.jvp(f, (first,), (torch.ones_like(first),))

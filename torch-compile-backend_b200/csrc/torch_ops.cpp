@@ -542,10 +542,16 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
 }
 
 // ------------------------------------------------- paged-cache serving ops
+// Neither reverse mode (inputs that require a gradient while gradients are
+// recorded) nor forward mode (inputs with a tangent) is defined.
 void no_grad_inputs(const char* what, std::initializer_list<const at::Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : ts)
-    TORCH_CHECK(!t->defined() || !t->requires_grad(), "b200::", what, ": no gradient is defined; call it under torch.no_grad()");
+  const bool grad = at::GradMode::is_enabled(), tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const at::Tensor* t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(!grad || !t->requires_grad(), "b200::", what, ": no gradient is defined; call it under torch.no_grad()");
+    TORCH_CHECK(!tangents || !t->_fw_grad(/*level=*/0).defined(), "b200::", what,
+                ": no gradient is defined, in forward mode either; an input has a tangent");
+  }
 }
 
 // The device's status word, or null when it does not exist yet and cannot be
@@ -788,8 +794,8 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   return out;
 }
 
-// At the autograd key the serving ops refuse inputs that ask for a gradient
-// (none is defined, and the result would be cut off from them) and go on below
+// At the autograd key the serving ops refuse inputs that ask for a gradient or
+// carry a tangent (none is defined, and the result would be cut off from them) and go on below
 // it.  There, not in the kernels, so that a traced training graph is refused
 // too.
 template <typename Fn, typename... Args>
