@@ -142,11 +142,12 @@ __device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[7])));
   return __float_as_uint(m);
 }
-// Scale of the largest magnitude `top`; inv = 448 / it (a few 2^-23 off,
-// which moves only values at the border of two e4m3 numbers).
+// Scale of the largest magnitude `top`, and inv = 448 / it, rounded once: the
+// codes' product with it moves only values next to the border of two e4m3
+// numbers.  (The fast division gives 0 for divisors above 2^126.)
 __device__ __forceinline__ float scale_of(uint32_t top, float& inv) {
   const float a = __uint_as_float(max(top, __float_as_uint(kMinAmax)));
-  inv = __fdividef(kE4m3Max, a);
+  inv = __fdiv_rn(kE4m3Max, a);
   return a * (1.0f / kE4m3Max);
 }
 
