@@ -588,8 +588,8 @@ typedef struct {
   const int32_t* q_start;
   const int32_t* kv_len;
   int64_t max_q_len, window;
-  float scale; /* <= 0: 1 / sqrt(head_dim) */
-  float softcap;
+  float scale;   /* 0: 1 / sqrt(head_dim); a negative one is refused */
+  float softcap; /* 0: none; at most 1e38 */
   int32_t dtype;
   int32_t test_flags; /* B200K_PAGED_TEST_* hooks (0 in production) */
   void* workspace;

@@ -55,3 +55,22 @@ def test_functional_jvp_is_refused(op):
         f = lambda x: getattr(torch.ops.b200, op)(x, *rest)  # noqa: E731
         with pytest.raises(RuntimeError, match="no gradient is defined"):
             torch.func.jvp(f, (first,), (torch.ones_like(first),))
+
+
+@pytest.mark.parametrize("kw", [dict(scale=-1.0), dict(scale=-1e-30), dict(scale=float("-inf")), dict(softcap=3e38)])
+def test_paged_attention_refuses_scales_and_caps_it_cannot_apply(kw):
+    """A negative scale is not the default; a cap whose base-2 form overflows."""
+    assert cabi.library().b200k_paged_attention(ctypes.byref(attn_args(**kw)), None) == ARG
+
+
+@pytest.mark.gpu
+def test_a_scale_that_cannot_be_applied_is_refused_by_the_operator():
+    """Negative, not a number, or below what fp32 holds (which reads as 0, the default)."""
+    import serving_reference as ref
+
+    x = ref.paged_inputs([1, 2], [40, 20], 8, 2, 64, 16, torch.bfloat16)
+    op = torch.ops.b200.paged_attention
+    for scale, cap in ((-1.0, 0.0), (-0.1, 30.0), (float("nan"), 0.0), (1e-60, 0.0), (0.1, 1e-60), (0.1, 3e38), (0.1, 1e60)):
+        with pytest.raises(RuntimeError):
+            op(*x, scale, cap)
+    assert torch.equal(op(*x, -0.0), op(*x)) and torch.equal(op(*x, 0.125, 0.0), op(*x))

@@ -1003,7 +1003,9 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   if (a->tokens == 0 || a->heads == 0) return B200K_OK;
   if (!a->q || !a->out) return B200K_ERR_ARG;
   if (a->dtype != B200K_BF16 && a->dtype != B200K_F16) return B200K_ERR_UNSUPPORTED;
-  if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap) || a->window < 0 || !std::isfinite(a->scale)) return B200K_ERR_ARG;
+  if (!(a->softcap >= 0.0f) || !std::isfinite(2.0f * a->softcap * kLog2e) || a->window < 0 || !(a->scale >= 0.0f) ||
+      !std::isfinite(a->scale))
+    return B200K_ERR_ARG;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out)) return B200K_ERR_ALIGN;
   for (int d = 0; d < 2; ++d)
     if (a->q_strides[d] < 0 || a->q_strides[d] % 8) return B200K_ERR_ALIGN;

@@ -752,8 +752,11 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   for (const at::Tensor* t : {&page_table, &q_start, &kv_len})
     TORCH_CHECK(t->scalar_type() == at::kInt && t->device() == q.device() && (t->size(-1) <= 1 || t->stride(-1) == 1),
                 "b200::paged_attention: page_table, q_start and kv_len must be int32 on q's device with unit last-dim stride");
-  TORCH_CHECK(softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::paged_attention: softcap, window and max_q_len must not "
-              "be negative");
+  TORCH_CHECK(scale >= 0 && softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::paged_attention: scale, softcap, window and "
+              "max_q_len must not be negative");
+  // (0 is the default scale, and no cap)
+  TORCH_CHECK((scale == 0) == (static_cast<float>(scale) == 0) && (softcap == 0) == (static_cast<float>(softcap) == 0) &&
+                  softcap <= 1e38, "b200::paged_attention: scale ", scale, " or softcap ", softcap, " is out of float32's range");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
   B200kPagedAttentionArgs a;
