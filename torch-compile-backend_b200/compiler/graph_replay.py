@@ -14,7 +14,9 @@ Semantics are those of the op-by-op function:
     into the graph's own input buffer before each replay;
   * caches that the graph appends to (optimization/inplace_append.py) are read
     and written in place and guarded by their address like parameters, and
-    returned as the caller's own tensors;
+    returned as the caller's own tensors.  Unlike parameters they may go away:
+    the replay keeps none of them alive, and two calls in a row with the same
+    other caches record the graph again (MAX_RECORDS times at most);
   * outputs: each replay's outputs are cloned out of the graph's buffers, so
     a result stays valid after later calls;
   * the first call runs op by op (it also warms up lazily initialised
@@ -48,6 +50,11 @@ aten = torch.ops.aten
 
 # Replays issued by every GraphReplay of this process (a diagnostic count).
 REPLAYS = 0
+
+# Recordings of one GraphReplay, the first one and those for other caches: each
+# costs two runs and a capture, so a caller whose caches move for ever runs
+# op by op in the end.
+MAX_RECORDS = 8
 
 # Nodes that never launch a kernel (views, metadata, Python-level getitem).
 _NO_LAUNCH = {
@@ -91,6 +98,8 @@ class GraphReplay:
         # input that it returns
         self.written = frozenset(written)
         self.returned = {}
+        self.records = 0
+        self.missed = None  # cache addresses of the last call that had others than the recording's
         self.calls = 0
         self.replays = 0
         self.graph = None
@@ -115,6 +124,7 @@ class GraphReplay:
             isinstance(a, (torch.Tensor, int, float, bool, type(None))) for a in args)
 
     def _record(self, args):
+        self.records += 1
         self.persistent = [isinstance(a, torch.Tensor) and (i in self.static or _is_persistent(a))
                            for i, a in enumerate(args)]
         self.static_in = [a if (not isinstance(a, torch.Tensor) or p) else a.clone()
@@ -139,6 +149,10 @@ class GraphReplay:
                         if isinstance(o, torch.Tensor) and i not in self.no_clone and i not in self.returned)
         if out_bytes > config.GRAPH_MAX_OUTPUT_MB * 2**20:
             raise RuntimeError("outputs too large to clone per call")
+        for i in self.written:  # the caller's to free: replays know them by address
+            self.static_in[i] = None
+        for j in self.returned:
+            outs[j] = None
         self.graph, self.static_out = graph, outs
 
     def _matches(self, args) -> bool:
@@ -146,10 +160,27 @@ class GraphReplay:
             return False
         return all(p is None or a.data_ptr() == p for a, p in zip(args, self.ptrs))
 
+    def _moved(self, args) -> bool:
+        """Whether only caches are at other addresses than recorded, and at the
+        same ones as in the last call of which that was so."""
+        if not self.written or self._signature(args) != self.sig:
+            return False
+        if any(p is not None and i not in self.written and a.data_ptr() != p
+               for i, (a, p) in enumerate(zip(args, self.ptrs))):
+            return False
+        now = [args[i].data_ptr() for i in sorted(self.written)]
+        again, self.missed = now == self.missed, now
+        return again
+
     def __call__(self, args):
         self.calls += 1
         if self.disabled or not self._eligible(args):
             return self.fn(args)
+        if self.graph is not None and not self._matches(args):
+            if self.records >= MAX_RECORDS or torch.cuda.is_current_stream_capturing() or not self._moved(args):
+                return self.fn(args)
+            torch.cuda.synchronize(next(a.device for a in args if isinstance(a, torch.Tensor)))  # the last replay is done
+            self.graph = self.static_in = self.static_out = None  # its memory is the new recording's
         if self.graph is None:
             if self.calls == 1:
                 return self.fn(args)  # op by op: warms up lazily initialised libraries
@@ -157,10 +188,9 @@ class GraphReplay:
                 self._record(args)
             except Exception:  # recording is an optimisation: fall back for good
                 self.disabled = True
-                self.graph = None
+                self.graph = self.static_in = self.static_out = None
                 return self.fn(args)
-        if not self._matches(args):
-            return self.fn(args)
+        self.missed = None
         for a, s, p in zip(args, self.static_in, self.persistent):
             if isinstance(a, torch.Tensor) and not p and a.data_ptr() != s.data_ptr():
                 s.copy_(a)
