@@ -121,3 +121,109 @@ def test_caches_replaced_again_and_again_are_recorded_a_bounded_number_of_times(
         for _ in range(2):
             d.both(mine, eager)
     assert len(records) == graph_replay.MAX_RECORDS
+
+
+# ------------------------------------------------- caches that a graph only reads
+def reader(n=17):
+    """Attends `n` times over what `get` makes of its caches."""
+    def f(q, caches, table, q_start, kv_len):
+        for i in range(n):
+            kc, vc = caches[i % len(caches)]
+            q = torch.ops.b200.paged_attention(q, kc, vc, table, q_start, kv_len) + q
+        return q
+    return f
+
+
+def halves(q, both, table, q_start, kv_len):
+    """K and V of a page side by side in one tensor, taken apart in the graph."""
+    return reader()(q, [(both[:, 0], both[:, 1])], table, q_start, kv_len)
+
+
+def traced(f, *args):
+    """The graph that AOTAutograd hands to the inference compiler, on fake tensors."""
+    from torch._dynamo.backends.common import aot_autograd
+    from torch._functorch.aot_autograd import make_boxed_func
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    seen = []
+
+    def keep(gm, _):
+        seen.append(gm)
+        return make_boxed_func(gm.forward)
+
+    torch._dynamo.reset()
+    with torch.no_grad(), FakeTensorMode(allow_non_fake_inputs=True):
+        fake = torch.utils._pytree.tree_map(lambda t: torch.empty(t.shape, dtype=t.dtype, device="cuda"), args)
+        torch.compile(f, backend=aot_autograd(fw_compiler=keep, inference_compiler=keep))(*fake)
+    torch._dynamo.reset()
+    return seen[0]
+
+
+def cpu_inputs(shape):
+    i32 = dict(dtype=torch.int32)
+    return (torch.empty(3, 8, 64, dtype=torch.bfloat16), torch.empty(shape, dtype=torch.bfloat16),
+            torch.empty(2, 4, **i32), torch.empty(3, **i32), torch.empty(2, **i32))
+
+
+def attended_shapes(gm):
+    from compiler.optimization.inplace_append import attended_inputs
+
+    inputs = [n for n in gm.graph.nodes if n.op == "placeholder"]
+    return sorted(tuple(inputs[i].meta["val"].shape) for i in attended_inputs(gm))
+
+
+def test_inputs_that_are_caches_alone_are_found():
+    q, cache, *index = cpu_inputs((9, 16, 2, 64))
+    two = lambda q, k, v, *index: reader()(q, [(k, v)], *index)  # noqa: E731
+    assert attended_shapes(traced(two, q, cache, cache.clone(), *index)) == [(9, 16, 2, 64)] * 2
+    q, both, *index = cpu_inputs((9, 2, 16, 2, 64))
+    assert attended_shapes(traced(halves, q, both, *index)) == [(9, 2, 16, 2, 64)]
+
+
+def test_inputs_that_are_more_than_caches_are_not():
+    q, cache, *index = cpu_inputs((9, 16, 2, 64))
+    summed = lambda q, k, v, *index: (reader()(q, [(k, v)], *index), k.sum())  # noqa: E731
+    assert attended_shapes(traced(summed, q, cache, cache.clone(), *index)) == [(9, 16, 2, 64)]  # v
+    seen = lambda q, k, v, *index: (reader()(q, [(k, v)], *index), k[0], v[1:])  # noqa: E731
+    assert attended_shapes(traced(seen, q, cache, cache.clone(), *index)) == []
+    asked = lambda q, *index: reader()(q, [(q.view(3, 1, 8, 64), q.view(3, 1, 8, 64))], *index)  # noqa: E731
+    assert attended_shapes(traced(asked, q, *index)) == []
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["two", "halves"])
+def test_replays_read_caches_in_place(layout, records):
+    """No copy of a cache is made or kept, changes of its contents are seen, and
+    other caches are too."""
+    import serving_reference as ref
+    from compiler.backend import custom_backend
+
+    q, kc, vc, *index = ref.paged_inputs([1, 2], [40, 30], 8, 2, 64, 16, torch.bfloat16,
+                                         layout="pair" if layout == "halves" else "nhd", spare=20000)
+    if layout == "halves":
+        f, base = halves, kc._base
+        make = lambda t: (t,)  # noqa: E731
+    else:
+        f = lambda q, k, v, *index: reader()(q, [(k, v)], *index)  # noqa: E731
+        base = torch.stack([kc, vc])
+        make = lambda t: (t[0], t[1])  # noqa: E731
+    size = kc.numel() * 2
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend=custom_backend, dynamic=False)
+    keep = []
+    with torch.no_grad():
+        for i in range(10):
+            if i in (3, 8):
+                base[:5] *= 0.5  # the caches' contents
+            if i == 5:
+                keep.append(base)
+                base = base.clone()
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            start, before = torch.cuda.memory_allocated(), graph_replay.REPLAYS
+            got = compiled(q, *make(base), *index)
+            torch.cuda.synchronize()
+            assert torch.cuda.max_memory_allocated() - start < size
+            assert torch.equal(got, f(q, *make(base), *index))
+            assert graph_replay.REPLAYS - before == (0 if i in (0, 5) else 1)
+    assert len(records) == 2

@@ -26,7 +26,7 @@ from compiler.optimization.fusion_patchify import fuse_patchify
 from compiler.optimization.fusion_pointwise import fuse_pointwise
 from compiler.optimization.fusion_rope import fuse_gemm_rope, fuse_rope
 from compiler.optimization.fusion_rowreduce import fuse_rowreduce
-from compiler.optimization.inplace_append import appended_inputs, inplace_append
+from compiler.optimization.inplace_append import appended_inputs, attended_inputs, inplace_append
 
 runtime.load()
 
@@ -142,7 +142,7 @@ def inference_compiler(gm: fx.GraphModule, example_inputs):
     if config.EXTENSIONS:
         caches = appended_inputs(gm)
         if caches is not None:
-            fn = graph_replay.wrap(gm, fn, _static_inputs(), caches)
+            fn = graph_replay.wrap(gm, fn, _static_inputs(), caches, attended_inputs(gm))
     return _checked(gm, example_inputs, fn)
 
 

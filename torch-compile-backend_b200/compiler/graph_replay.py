@@ -12,9 +12,10 @@ Semantics are those of the op-by-op function:
   * inputs: tensors that are the same storage at every call (parameters,
     module buffers) are read in place; every other tensor input is copied
     into the graph's own input buffer before each replay;
-  * caches that the graph appends to (optimization/inplace_append.py) are read
-    and written in place and guarded by their address like parameters, and
-    returned as the caller's own tensors.  Unlike parameters they may go away:
+  * caches that the graph appends to, or only attends over
+    (optimization/inplace_append.py), are read and written in place and guarded
+    by their address like parameters, and returned as the caller's own tensors
+    (copied per call, a cache costs its capacity, not its keys).  Unlike parameters they may go away:
     the replay keeps none of them alive, and two calls in a row with the same
     other caches record the graph again (MAX_RECORDS times at most);
   * outputs: each replay's outputs are cloned out of the graph's buffers, so
@@ -85,7 +86,7 @@ def _is_persistent(t: torch.Tensor) -> bool:
 class GraphReplay:
     """Boxed callable: ``run(args)`` with ``args`` the graph's input list."""
 
-    def __init__(self, fn, no_clone=(), static=(), written=()):
+    def __init__(self, fn, no_clone=(), static=(), written=(), read=()):
         # AOTAutograd's marker for the list-argument calling convention (an
         # instance attribute, so that functools.wraps wrappers copy it)
         self._boxed_call = True
@@ -93,11 +94,13 @@ class GraphReplay:
         self.no_clone = frozenset(no_clone)  # output indices returned as the graph's own buffers
         # input indices AOTAutograd marks static (the module's lifted parameters
         # and buffers): read in place like parameters, guarded by their address
-        self.static = frozenset(static) | frozenset(written)
+        self.static = frozenset(static) | frozenset(written) | frozenset(read)
         # input indices that the graph writes in place; output index -> such an
         # input that it returns
         self.written = frozenset(written)
         self.returned = {}
+        # caches, written or read: in place too, but kept by address alone
+        self.caches = self.written | frozenset(read)
         self.records = 0
         self.missed = None  # cache addresses of the last call that had others than the recording's
         self.calls = 0
@@ -149,7 +152,7 @@ class GraphReplay:
                         if isinstance(o, torch.Tensor) and i not in self.no_clone and i not in self.returned)
         if out_bytes > config.GRAPH_MAX_OUTPUT_MB * 2**20:
             raise RuntimeError("outputs too large to clone per call")
-        for i in self.written:  # the caller's to free: replays know them by address
+        for i in self.caches:  # the caller's to free: replays know them by address
             self.static_in[i] = None
         for j in self.returned:
             outs[j] = None
@@ -163,12 +166,12 @@ class GraphReplay:
     def _moved(self, args) -> bool:
         """Whether only caches are at other addresses than recorded, and at the
         same ones as in the last call of which that was so."""
-        if not self.written or self._signature(args) != self.sig:
+        if not self.caches or self._signature(args) != self.sig:
             return False
-        if any(p is not None and i not in self.written and a.data_ptr() != p
+        if any(p is not None and i not in self.caches and a.data_ptr() != p
                for i, (a, p) in enumerate(zip(args, self.ptrs))):
             return False
-        now = [args[i].data_ptr() for i in sorted(self.written)]
+        now = [args[i].data_ptr() for i in sorted(self.caches)]
         again, self.missed = now == self.missed, now
         return again
 
@@ -252,7 +255,7 @@ class TailReplay:
         return out
 
 
-def split_large_outputs(gm: fx.GraphModule, static=()):
+def split_large_outputs(gm: fx.GraphModule, static=(), read=()):
     """A TailReplay of `gm` whose tail computes the outputs larger than
     ``config.GRAPH_MAX_OUTPUT_MB``, or None when the graph does not split
     cleanly (a large output that is an input, a tail value that the body also
@@ -330,23 +333,24 @@ def split_large_outputs(gm: fx.GraphModule, static=()):
     tail_args = [("arg", placeholders.index(a)) if a.op == "placeholder" else ("body", len(small) + ext_body.index(a))
                  for a in ext]
     no_clone = range(len(small), len(small) + len(ext_body))
-    body = GraphReplay(lambda a: body_gm(*a), no_clone=no_clone, static=static)
+    body = GraphReplay(lambda a: body_gm(*a), no_clone=no_clone, static=static, read=read)
     return TailReplay(body, tail_gm, len(small), plan, tail_args)
 
 
-def wrap(gm: fx.GraphModule, boxed_fn, static=(), written=()):
+def wrap(gm: fx.GraphModule, boxed_fn, static=(), written=(), read=()):
     """The boxed function of an inference graph, replayed as a CUDA graph when
     it launches enough kernels to gain from it: whole when its outputs are
     small enough to clone per call, else split into a replayed body and a
     tail run op by op (``split_large_outputs``); otherwise `boxed_fn`.
     `static`: input indices read in place instead of copied per replay;
     `written`: input indices that the graph writes in place (running it twice
-    must leave what running it once does)."""
+    must leave what running it once does); `read`: those of caches that it only
+    reads."""
     if not config.CUDA_GRAPHS or launching_nodes(gm) < config.GRAPH_MIN_LAUNCHES:
         return boxed_fn
     if output_bytes(gm, written) <= config.GRAPH_MAX_OUTPUT_MB * 2**20:
-        return GraphReplay(boxed_fn, static=static, written=written)
+        return GraphReplay(boxed_fn, static=static, written=written, read=read)
     if written:
         return boxed_fn  # a split graph's body returns no input
-    split = split_large_outputs(gm, static)
+    split = split_large_outputs(gm, static, read)
     return split if split is not None else boxed_fn

@@ -17,7 +17,7 @@ import operator
 import torch
 import torch.fx as fx
 
-from compiler import runtime
+from compiler import graph_replay, runtime
 
 runtime.load()
 
@@ -25,8 +25,10 @@ _APPEND = torch.ops.b200.rope_append.default
 _FUNCTIONAL = torch.ops.higher_order.auto_functionalized_v2
 _PLAIN = ("q", "k", "v", "cos", "sin", "positions", "slots")
 _CACHES = ("k_cache", "v_cache")
+_ATTEND = torch.ops.b200.paged_attention.default
 # Ops that take a cache and return nothing that aliases it.
-_READERS = (torch.ops.b200.paged_attention.default, _APPEND)
+_READERS = (_ATTEND, _APPEND)
+_VIEWS = graph_replay._NO_LAUNCH | {operator.getitem}
 
 
 def _caches_of(node: fx.Node):
@@ -93,3 +95,16 @@ def appended_inputs(gm: fx.GraphModule) -> tuple:
                     return None
                 found.add(inputs.index(b))
     return tuple(sorted(found))
+
+
+def attended_inputs(gm: fx.GraphModule) -> tuple:
+    """Indices of the graph inputs that are caches and nothing else: the graph
+    attends over them, or over views of them, and has no other use for them."""
+    def cache_alone(n):
+        return bool(n.users) and all(
+            u.op == "call_function" and not u.kwargs
+            and (u.target == _ATTEND and n in u.args[1:3] and n not in (u.args[0], *u.args[3:])
+                 or u.target in _VIEWS and cache_alone(u))
+            for u in n.users)
+
+    return tuple(i for i, n in enumerate(n for n in gm.graph.nodes if n.op == "placeholder") if cache_alone(n))
