@@ -8,11 +8,15 @@ back over the inputs at the end of the call -- three passes over a cache that
 may fill most of the GPU's memory, for a few appended rows.  This pass puts
 the op itself back wherever that cannot be told apart: the caches are whole
 graph inputs (or what an earlier append of the graph left of them), and
-nothing that reads the state before the append runs after it.
+nothing that reads the state before the append runs after it.  An append that
+stays functional (caches that are parts of a larger tensor: K and V as its
+halves, layers stacked) gives the same results; it is warned of, since the
+whole tensor is copied for it.
 """
 from __future__ import annotations
 
 import operator
+import warnings
 
 import torch
 import torch.fx as fx
@@ -77,6 +81,10 @@ def inplace_append(gm: fx.GraphModule) -> fx.GraphModule:
     if changed:
         gm.graph.lint()
         gm.recompile()
+    left = sum(n.op == "call_function" and n.target == _FUNCTIONAL and n.args[:1] == (_APPEND,) for n in gm.graph.nodes)
+    if left:
+        warnings.warn(f"{left} b200::rope_append of a compiled graph copy the tensors that hold their caches, whole, at "
+                      "every call: pass each cache as a tensor of its own, and attend over it behind the append")
     return gm
 
 
