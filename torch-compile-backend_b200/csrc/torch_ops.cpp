@@ -60,14 +60,28 @@ void* stream_of(const at::Tensor& t) {
 
 std::atomic<int64_t> g_test_stall_ns{0};
 
-// Per-device status word the GEMM kernel writes when a wait times out.
+// Per-device status word that kernels write when a wait times out or an index
+// is out of range.  Made at first use, which may lie inside a stream capture:
+// so not the caching allocator's (whose zeros would become a node of the graph
+// and clear the word at every replay), and zeroed on a stream of its own.
 at::Tensor& status_word(int dev) {
   static std::mutex mu;
   static std::vector<at::Tensor> words;
   std::lock_guard<std::mutex> lock(mu);
   if (static_cast<int>(words.size()) <= dev) words.resize(dev + 1);
-  if (!words[dev].defined())
-    words[dev] = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, dev));
+  if (!words[dev].defined()) {
+    c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    void* p = nullptr;
+    cudaStream_t st = nullptr;
+    TORCH_CHECK(cudaMalloc(&p, sizeof(int32_t)) == cudaSuccess, "b200: the status word's allocation failed");
+    const bool zeroed = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                        cudaMemsetAsync(p, 0, sizeof(int32_t), st) == cudaSuccess &&
+                        cudaStreamSynchronize(st) == cudaSuccess;
+    if (st) cudaStreamDestroy(st);
+    TORCH_CHECK(zeroed, "b200: the status word was not zeroed");
+    words[dev] = at::from_blob(p, {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, dev));
+  }
   return words[dev];
 }
 
@@ -554,20 +568,6 @@ void no_grad_inputs(const char* what, std::initializer_list<const at::Tensor*> t
   }
 }
 
-// The device's status word, or null when it does not exist yet and cannot be
-// made because `st` is capturing.
-int32_t* status_ptr(int dev, void* st) {
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  const bool capturing =
-      cudaStreamIsCapturing(static_cast<cudaStream_t>(st), &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone;
-  static std::mutex mu;
-  static std::vector<int32_t*> known;
-  std::lock_guard<std::mutex> lock(mu);
-  if (static_cast<int>(known.size()) <= dev) known.resize(dev + 1, nullptr);
-  if (!known[dev] && !capturing) known[dev] = status_word(dev).data_ptr<int32_t>();
-  return known[dev];
-}
-
 void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r_in,
                    const c10::optional<at::Tensor>& weight, double eps, int64_t flags, int64_t group, bool quant,
                    at::Tensor& out, at::Tensor& scale, at::Tensor& sum) {
@@ -730,7 +730,7 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   a.positions_dtype = to_dt(positions.scalar_type());
   a.slots_dtype = to_dt(slots.scalar_type());
   void* st = stream_of(q);
-  a.status = status_ptr(q.device().index(), st);
+  a.status = status_word(q.device().index()).data_ptr<int32_t>();
   check(b200k_rope_append(&a, st), what);
   for (at::Tensor* t : {&k_cache, &v_cache})
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
@@ -792,7 +792,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
   a.workspace = ws.data_ptr();
   a.workspace_bytes = bytes;
-  a.status = status_ptr(q.device().index(), st);
+  a.status = status_word(q.device().index()).data_ptr<int32_t>();
   check(b200k_paged_attention(&a, st), what);
   return out;
 }
