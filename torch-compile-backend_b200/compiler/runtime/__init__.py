@@ -131,5 +131,5 @@ def check_status(device: int = 0) -> None:
         raise RuntimeError(f"b200::rope_append or paged_attention on cuda:{device} reported status {v}: a slot, "
                            "position, page or length is out of range")
     if v != 0:
-        raise RuntimeError(f"b200::gemm_epilogue on cuda:{device} reported status {v} "
-                           "(6 = a device-side wait timed out): an earlier GEMM's output is incomplete")
+        raise RuntimeError(f"b200::gemm_epilogue, attention or paged_attention on cuda:{device} reported status {v} "
+                           "(6 = a device-side wait timed out): an earlier call's output is incomplete")

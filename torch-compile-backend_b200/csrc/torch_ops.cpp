@@ -330,8 +330,8 @@ int64_t status_check(int64_t device, bool arm) {
     word.zero_();
     TORCH_CHECK(seen != B200K_ERR_INDEX, "b200::rope_append or paged_attention on cuda:", dev, " reported ",
                 b200k_status_string(static_cast<int>(seen)), " (code ", seen, ")");
-    TORCH_CHECK(false, "b200::gemm_epilogue on cuda:", dev, " reported ", b200k_status_string(static_cast<int>(seen)),
-                " (code ", seen, "): an earlier GEMM's output is incomplete");
+    TORCH_CHECK(false, "b200::gemm_epilogue, attention or paged_attention on cuda:", dev, " reported ",
+                b200k_status_string(static_cast<int>(seen)), " (code ", seen, "): an earlier call's output is incomplete");
   }
   return 0;
 }
