@@ -510,8 +510,8 @@ int b200k_add_rms_norm(const B200kAddNormArgs* args, void* stream);
  * sums, each result rounded once.  q, k, v: [tokens, heads, head_dim] views
  * of one 16-bit type (token and head strides, unit element stride); q_out
  * contiguous.  Caches: [num_pages, page_size, kv_heads, head_dim] views with
- * cache_strides (page, slot, head; unit element stride, the same for both);
- * a slot is page * page_size + place in the page.  cos, sin: [table_rows,
+ * cache_strides (page, slot, head; unit element stride, the same for both)
+ * that share no element; a slot is page * page_size + place in the page.  cos, sin: [table_rows,
  * R/2] of f32 or the inputs' type, row stride table_stride.  positions and
  * slots: [tokens], i32 or i64.  A token with a negative slot is rotated but
  * not appended.  Slots that appear twice leave one or the other token's

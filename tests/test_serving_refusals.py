@@ -74,3 +74,17 @@ def test_a_scale_that_cannot_be_applied_is_refused_by_the_operator():
         with pytest.raises(RuntimeError):
             op(*x, scale, cap)
     assert torch.equal(op(*x, -0.0), op(*x)) and torch.equal(op(*x, 0.125, 0.0), op(*x))
+
+
+@pytest.mark.gpu
+def test_one_tensor_as_both_caches_is_refused():
+    """Keys and values would be written to the same places."""
+    from test_gpu_rope_append import make
+
+    *args, kc, vc = make(8, 4, 2, 64, 64, 16, torch.bfloat16)
+    for same in (kc, kc.view_as(kc)):
+        with pytest.raises(RuntimeError, match="same memory"):
+            torch.ops.b200.rope_append(*args, kc, same)
+    torch.ops.b200.rope_append(*args, kc, vc)
+    torch.ops.b200.rope_append(*args, kc[:0], kc[:0])  # nothing to write, slots past the cache
+    assert runtime.gemm_status() == 9

@@ -696,6 +696,8 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
     TORCH_CHECK(t->device() == q.device(), "b200::rope_append: every tensor must be on q's device");
   for (int64_t d = 0; d < 4; ++d)  // several elements in one place
     TORCH_CHECK(k_cache.size(d) <= 1 || k_cache.stride(d) != 0, "b200::rope_append: the caches must not be expanded");
+  TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(),
+              "b200::rope_append: k_cache and v_cache are the same memory");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
   B200kRopeAppendArgs a;
