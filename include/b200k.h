@@ -562,16 +562,17 @@ int b200k_rope_append(const B200kRopeAppendArgs* args, void* stream);
  * aligned; out contiguous.  Nothing is read of the caches outside the keys
  * that a sequence's queries see, so other pages and the rest of the last one
  * may hold anything.  Of the keys that some query of the sequence sees, those
- * hidden from another query have weight 0 for it: their values must be
- * finite, or it may become NaN, as 0 * inf does.  Scores, softmax and sums are
- * fp32; the probabilities are rounded to the input type for the second product,
- * half a step each (f16: those below 2^-26 of a row's maximum by less than
- * 2^-36 of it).  max_q_len (0: unknown)
- * is a hint of the longest sequence's queries: it chooses kernels and grids,
- * never results.  Index tensors are i32 on the device; entries out of range
+ * hidden from another query have weight 0 for it (at most 2^-125 of the row's
+ * largest): their values must be finite, or it may become NaN, as 0 * inf does,
+ * and below 2^100 in bf16.  Scores, softmax and sums are fp32; the
+ * probabilities are rounded to the input type for the second product, half a
+ * step each (f16: those below 2^-26 of a row's maximum by less than 2^-36 of
+ * it).  max_q_len (0: unknown) is a hint of the longest sequence's queries: it
+ * chooses kernels and grids (the order of sums with them, so the last bits), and
+ * may be too small.  Index tensors are i32 on the device; entries out of range
  * are clamped (a page out of range reads as zeros) and set *status (may be
- * NULL) to B200K_ERR_INDEX; B200K_ERR_TIMEOUT is set when a device-side wait runs out
- * (timeout_ns, 0 = 2 s).  workspace: device memory of
+ * NULL) to B200K_ERR_INDEX; B200K_ERR_TIMEOUT is set when a device-side wait
+ * runs out (timeout_ns, 0 = 2 s).  workspace: device memory of
  * b200k_paged_attention_workspace bytes, 16-byte aligned, for this call
  * alone until it has run.
  */

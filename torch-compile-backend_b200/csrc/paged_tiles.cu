@@ -26,14 +26,16 @@
 // Tensor memory is full (S 2 x 2 x 64, O 2 x 128 columns): a tile's scores
 // alternate between two buffers, P takes the columns of its S, and S of the
 // next block is computed under this block's exponentials.  With one buffer of
-// 128 keys S, softmax and P V of a tile ran one after the other: 4400 clocks
-// for 128 keys with heads of 128.
+// 128 keys, S, softmax and P V of a tile one after the other, 128 keys with heads
+// of 128 took 4400 clocks (now ~3900).
 // Measured: 8 prompts of 2048, 32 / 8 heads of 64, causal, 277 us = 497
-// TFLOP/s; 5 chunks of 1024 behind up to 6000 keys, heads of 128, 275 us = 954
-// TFLOP/s.  Heads of 64 are bound by the softmax (per block of 64 keys ~1750
-// clocks of one warp's dependent instructions; the exponential unit alone
-// ~770), heads of 128 by the tensor pipe (N = 64 costs what N = 128 does:
-// ~1540 of ~1950 clocks a block).
+// TFLOP/s; 5 chunks of 1024 behind up to 6000 keys, heads of 128, 317 us = 828
+// TFLOP/s in calls back to back, which lower the clock under the power limit
+// (268 us in a short run).  Heads of 64 are bound by the softmax (per block of
+// 64 keys ~1750 clocks of one warp's dependent instructions; the exponential
+// unit alone ~770).  With heads of 128 the tensor pipe is active 54 % of the
+// time: of a block's ~1950 clocks the two products take ~1540 if one with
+// N = 64 costs what one with N = 128 does, the rest is waits between them.
 // Every wait is bounded (gemm_kernel.cuh): a timeout sets the status word and
 // drains.
 #include "gemm_kernel.cuh"
