@@ -51,7 +51,8 @@ enum {
   B200K_I64 = 5,
   B200K_BOOL = 6,
   B200K_U8 = 7,
-  B200K_E4M3 = 8 /* 8-bit float (4 exponent, 3 mantissa bits): b200k_add_rms_norm output only */
+  B200K_E4M3 = 8 /* 8-bit float (4 exponent, 3 mantissa bits): outputs with scales, and what
+                     b200k_scaled_mm and the 8-bit caches are made of */
 };
 
 /* Return codes. */
@@ -607,6 +608,117 @@ typedef struct {
 
 int b200k_paged_attention(const B200kPagedAttentionArgs* args, void* stream);
 int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* args, int64_t* bytes);
+
+/*
+ * Activations to e4m3 with a scale for every 128 columns (an extension: the
+ * reference has no 8-bit type):
+ *   y = x, or with `swiglu` silu(x[:, c]) * x[:, cols + c],  c < cols, fp32
+ *   scale[r, g] = max(max |y[r, 128 g ..]|, 1e-12) / 448
+ *   out[r, c]   = e4m3(y[r, c] / scale[r, c / 128]), round to nearest even
+ * of a [rows, cols] view (with `swiglu` [rows, 2 cols]: the gate in front) of
+ * f32, f16 or bf16 with unit column stride; the last group of a row may be
+ * shorter.  out [rows, cols] and scale [rows, ceil(cols / 128)] are contiguous
+ * and overlap no input.  A NaN among a group's y makes its codes and scale NaN;
+ * an infinity makes the scale infinite, its own codes NaN and the others 0.
+ * Fastest with 16-bit x, cols and the row stride multiples of 8 and x 16-byte
+ * aligned.
+ */
+typedef struct {
+  int64_t rows, cols;
+  const void* x;
+  int64_t x_row_stride;
+  int32_t dtype;
+  int32_t swiglu;
+  void* out;
+  float* scale;
+} B200kQuantGroupsArgs;
+
+int b200k_quant_groups(const B200kQuantGroupsArgs* args, void* stream);
+
+/*
+ * Product of e4m3 matrices with a scale for each block of 128 (an extension,
+ * as above):
+ *   out[m, n] = sum_g a_scale[m, g] b_scale[g, n / 128] sum_k a[m, k] b[k, n],
+ *   k over 128 g .. min(128 g + 127, K - 1)
+ * a [M, K] with unit k stride and row stride a_stride_m, b [K, N] with unit k
+ * stride and column stride b_stride_n (a linear layer's weight, transposed),
+ * both 16-byte aligned with strides of multiples of 16; any M, N and K.
+ * a_scale [M, ceil(K / 128)] and b_scale [ceil(K / 128), ceil(N / 128)] are
+ * fp32 with any strides (given row first).  out [M, N] is contiguous, of f16,
+ * bf16 or f32, 16-byte aligned.  The products of a block are summed by the
+ * tensor cores, the blocks in fp32, and the result is rounded once.  The same
+ * shapes give the same bits.  NaN codes and scales reach every product that
+ * they enter.
+ * tile: 0 the library's choice, 1 256 x 256 (a CTA pair), 2 128 x 128, 3 128 x
+ * 64; split: CTAs of a cluster that share the blocks of k of a tile of kind 2
+ * or 3, 0 the library's choice, at most 8.  status, when not NULL, receives
+ * B200K_ERR_TIMEOUT if a device-side wait runs out (timeout_ns, 0 = 2 s).
+ */
+typedef struct {
+  int64_t M, N, K;
+  const void* a;
+  int64_t a_stride_m;
+  const void* b;
+  int64_t b_stride_n;
+  const float* a_scale;
+  int64_t a_scale_strides[2];
+  const float* b_scale;
+  int64_t b_scale_strides[2];
+  void* out;
+  int32_t out_dtype;
+  int32_t tile, split;
+  int32_t test_flags; /* B200K_SCALED_MM_TEST_* hooks (0 in production) */
+  int32_t* status;
+  int64_t timeout_ns;
+} B200kScaledMmArgs;
+
+/* Test hook (test_flags bit): each CTA's first block is not signalled as
+ * ready, so a wait runs out after timeout_ns; the kernel reports
+ * B200K_ERR_TIMEOUT, drains and returns (no fault).  Failure-detection tests
+ * only. */
+#define B200K_SCALED_MM_TEST_WITHHOLD_READY 1
+
+int b200k_scaled_mm(const B200kScaledMmArgs* args, void* stream);
+
+/*
+ * b200k_rope_append to caches of e4m3: each appended row (a token's values of
+ * one head, the keys rotated, in fp32) is stored as e4m3(row / s) with
+ * s = max(max |row|, 1e-12) / 448 in k_scale / v_scale, [num_pages, page_size,
+ * kv_heads] of fp32 with scale_strides (page, slot, head; the same for both).
+ * base.k_cache and base.v_cache are e4m3, cache_strides in elements; q_out is
+ * of the inputs' type.  All else is as there; NaN and infinite values as in
+ * b200k_quant_groups.
+ */
+typedef struct {
+  B200kRopeAppendArgs base;
+  float* k_scale;
+  float* v_scale;
+  int64_t scale_strides[3];
+} B200kRopeAppendQuantArgs;
+
+int b200k_rope_append_quant(const B200kRopeAppendQuantArgs* args, void* stream);
+
+/*
+ * b200k_paged_attention over caches of e4m3 as b200k_rope_append_quant writes
+ * them: key and value rows are code * scale, with k_scale and v_scale as there.
+ * base.dtype is that of q and out, f16 or bf16; cache_strides in elements, multiples of 16.
+ * Scales are positive; value scales below 1e-12 / 448 count as it.  Scores,
+ * softmax and sums are fp32 and codes enter the products as they are; queries
+ * are rounded to f16 after each row was scaled by a power of two (bf16: exact
+ * but for values below 2^-28 of the row's largest), probabilities to f16 after
+ * they were multiplied by their values' scales.  A NaN scale or code counts as
+ * a NaN score or value.  Workspace as for that entry, by
+ * b200k_paged_attention_quant_workspace.
+ */
+typedef struct {
+  B200kPagedAttentionArgs base;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t scale_strides[3];
+} B200kPagedAttentionQuantArgs;
+
+int b200k_paged_attention_quant(const B200kPagedAttentionQuantArgs* args, void* stream);
+int b200k_paged_attention_quant_workspace(const B200kPagedAttentionQuantArgs* args, int64_t* bytes);
 
 const char* b200k_status_string(int code);
 /* Library version, for the loader's sanity check. */

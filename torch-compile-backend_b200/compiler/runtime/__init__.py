@@ -112,6 +112,18 @@ def _register_fakes() -> None:
     def _(q, k_cache, v_cache, page_table, q_start, kv_len, scale=0.0, softcap=0.0, window=0, max_q_len=0):
         return q.new_empty(q.shape)
 
+    @torch.library.register_fake(lib + "quant_groups")
+    def _(x, swiglu=False):
+        cols = x.shape[-1] // 2 if swiglu else x.shape[-1]
+        return (
+            x.new_empty((*x.shape[:-1], cols), dtype=torch.float8_e4m3fn),
+            x.new_empty((*x.shape[:-1], (cols + 127) // 128), dtype=torch.float32),
+        )
+
+    @torch.library.register_fake(lib + "scaled_mm")
+    def _(a, b, a_scale, b_scale, out_dtype):
+        return a.new_empty((a.shape[0], b.shape[1]), dtype=out_dtype)
+
 
 def gemm_status(device: int = 0, reset: bool = True) -> int:
     """The kernels' device status word (0 = ok, 6 = a wait timed out, 9 = an

@@ -158,6 +158,31 @@ PAGED_TEST_WITHHOLD_SCORES = 1
 _lib = None
 
 
+class QuantGroupsArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("x_row_stride", ctypes.c_int64), ("dtype", ctypes.c_int32), ("swiglu", ctypes.c_int32),
+                ("out", ctypes.c_void_p), ("scale", ctypes.c_void_p)]
+
+
+class ScaledMmArgs(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("a", ctypes.c_void_p),
+                ("a_stride_m", ctypes.c_int64), ("b", ctypes.c_void_p), ("b_stride_n", ctypes.c_int64),
+                ("a_scale", ctypes.c_void_p), ("a_scale_strides", ctypes.c_int64 * 2),
+                ("b_scale", ctypes.c_void_p), ("b_scale_strides", ctypes.c_int64 * 2), ("out", ctypes.c_void_p),
+                ("out_dtype", ctypes.c_int32), ("tile", ctypes.c_int32), ("split", ctypes.c_int32),
+                ("test_flags", ctypes.c_int32), ("status", ctypes.c_void_p), ("timeout_ns", ctypes.c_int64)]
+
+
+class RopeAppendQuantArgs(ctypes.Structure):
+    _fields_ = [("base", RopeAppendArgs), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("scale_strides", ctypes.c_int64 * 3)]
+
+
+class PagedAttentionQuantArgs(ctypes.Structure):
+    _fields_ = [("base", PagedAttentionArgs), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("scale_strides", ctypes.c_int64 * 3)]
+
+
 def library() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -178,6 +203,8 @@ def library() -> ctypes.CDLL:
             ("b200k_paged_attention", [ctypes.POINTER(PagedAttentionArgs), ctypes.c_void_p]),
             ("b200k_paged_attention_workspace", [ctypes.POINTER(PagedAttentionArgs),
                                                  ctypes.POINTER(ctypes.c_int64)]),
+            ("b200k_quant_groups", [ctypes.POINTER(QuantGroupsArgs), ctypes.c_void_p]),
+            ("b200k_scaled_mm", [ctypes.POINTER(ScaledMmArgs), ctypes.c_void_p]),
             ("b200k_gemm_pick_config", [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]),
             ("b200k_gemm_config_info", [ctypes.c_int] + [ctypes.POINTER(ctypes.c_int)] * 4),
             ("b200k_gemm_num_configs", []),
@@ -467,3 +494,30 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a.timeout_ns = timeout_ns
     _check("b200k_paged_attention", library().b200k_paged_attention(ctypes.byref(a), _stream()))
     return n.value
+
+
+def quant_groups(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, swiglu: bool = False) -> None:
+    """x [rows, cols] (with `swiglu` [rows, 2 cols], the gate in front) as e4m3 in `out`,
+    with a scale for every 128 columns in `scale`."""
+    a = QuantGroupsArgs()
+    a.rows, a.cols = out.shape
+    a.x, a.x_row_stride, a.dtype, a.swiglu = x.data_ptr(), x.stride(0), DTYPE[x.dtype], swiglu
+    a.out, a.scale = out.data_ptr(), scale.data_ptr()
+    _check("b200k_quant_groups", library().b200k_quant_groups(ctypes.byref(a), _stream()))
+
+
+def scaled_mm(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, out: torch.Tensor,
+              tile: int = 0, split: int = 0, status: torch.Tensor | None = None, timeout_ns: int = 0,
+              test_flags: int = 0) -> None:
+    """out = a @ b for e4m3 a [M, K] and b [K, N] (unit strides along K) with a scale
+    for each row and 128 k of a, and for each 128 x 128 block of b."""
+    g = ScaledMmArgs()
+    (g.M, g.K), g.N = a.shape, b.shape[1]
+    g.a, g.a_stride_m, g.b, g.b_stride_n = a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(1)
+    g.a_scale, g.b_scale = a_scale.data_ptr(), b_scale.data_ptr()
+    for d in range(2):
+        g.a_scale_strides[d], g.b_scale_strides[d] = a_scale.stride(d), b_scale.stride(d)
+    g.out, g.out_dtype, g.tile, g.split = out.data_ptr(), DTYPE[out.dtype], tile, split
+    g.test_flags, g.timeout_ns = test_flags, timeout_ns
+    g.status = status.data_ptr() if status is not None else None
+    _check("b200k_scaled_mm", library().b200k_scaled_mm(ctypes.byref(g), _stream()))

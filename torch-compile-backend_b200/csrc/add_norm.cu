@@ -22,15 +22,13 @@
 #include <algorithm>
 #include <cstring>
 
-#include "common.cuh"
+#include "e4m3.cuh"
 #include "host_common.h"
 #include "rowreduce.cuh"
 
 namespace b200k {
 namespace {
 
-constexpr float kE4m3Max = 448.0f;
-constexpr float kMinAmax = 1e-12f;  // keeps 448 / a finite for rows of zeros
 
 struct AddNormParams {
   int64_t rows;
@@ -59,12 +57,6 @@ __device__ __forceinline__ float round_to(float v) {
   return v;
 }
 
-__device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
-  uint16_t u;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(u) : "f"(hi), "f"(lo));
-  return u;
-}
-
 template <bool BF16>
 __device__ __forceinline__ uint32_t add16x2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -79,26 +71,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-template <bool BF16>
-__device__ __forceinline__ void unpack16(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (BF16) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
-    }
-  }
-}
-
-// |v| as an unsigned pattern: ordered as the magnitudes are, infinity above
-// every number and NaN above infinity, so a row's NaN reaches its scale.
-__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 // Sum over the TPR threads of a row; each row group of a CTA has its own
 // named barrier and slots.
 template <int TPR, bool IS_MAX>
@@ -124,31 +96,6 @@ __device__ __forceinline__ uint32_t row_reduce(uint32_t v, uint32_t* slots, int 
     v = a;
   }
   return v;
-}
-
-// 8 fp32 values as e4m3, times inv.
-__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
-  uint16_t q[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = e4m3x2(v[2 * j] * inv, v[2 * j + 1] * inv);
-  return make_uint2(q[0] | (static_cast<uint32_t>(q[1]) << 16), q[2] | (static_cast<uint32_t>(q[3]) << 16));
-}
-// The largest magnitude of 8 values, NaN above all.
-__device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
-  float m = fabsf(v[0]);
-#pragma unroll
-  for (int j = 1; j < 7; j += 2)
-    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[j])), "f"(fabsf(v[j + 1])));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[7])));
-  return __float_as_uint(m);
-}
-// Scale of the largest magnitude `top`, and inv = 448 / it, rounded once: the
-// codes' product with it moves only values next to the border of two e4m3
-// numbers.  (The fast division gives 0 for divisors above 2^126.)
-__device__ __forceinline__ float scale_of(uint32_t top, float& inv) {
-  const float a = __uint_as_float(max(top, __float_as_uint(kMinAmax)));
-  inv = __fdiv_rn(kE4m3Max, a);
-  return a * (1.0f / kE4m3Max);
 }
 
 // The row's statistics and output, from its sums in registers: a thread holds

@@ -1,0 +1,171 @@
+// Activations to e4m3 with a scale for every 128 columns (b200k_quant_groups,
+// include/b200k.h), the input of the block-scaled product:
+//
+//   y = x, or silu(x[:, :cols]) * x[:, cols:] (the gate in front),
+//   scale = max(max |y|, 1e-12) / 448 of 128 columns,  out = e4m3(y / scale)
+//
+// No reference counterpart.  fp32 throughout, one rounding to e4m3; bound by
+// HBM: x is read once, one or two bytes (four with a gate) for each byte
+// written.  16 lanes hold the 128 columns of a scale, 8 each, so its maximum
+// is four shuffles; each takes kUnits groups, whose loads are issued together.
+#include <algorithm>
+#include <cstring>
+
+#include "e4m3.cuh"
+#include "host_common.h"
+
+namespace b200k {
+namespace {
+
+struct QuantParams {
+  int64_t units;       // rows * groups
+  int32_t groups;      // of a row
+  int32_t cols;
+  int32_t swiglu;
+  int32_t big;         // units past 2^31: 64-bit division
+  FastDiv div_groups;
+  const void* x;
+  int64_t x_stride;
+  uint8_t* out;
+  float* scale;
+};
+
+// silu(g) u
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+__device__ __forceinline__ void row_of(const QuantParams& p, int64_t unit, int64_t& row, int& group) {
+  row = p.big ? unit / p.groups : fdiv(static_cast<uint32_t>(unit), p.div_groups);
+  group = static_cast<int>(unit - row * p.groups);
+}
+
+constexpr int kThreads = 256;
+constexpr int kPerCta = kThreads / 16;  // groups side by side
+
+template <bool BF16, bool SWIGLU, int UNITS>
+__global__ void __launch_bounds__(kThreads) quant16_kernel(const __grid_constant__ QuantParams p) {
+  const int c0 = (threadIdx.x & 15) * 8;
+  const int64_t first = blockIdx.x * static_cast<int64_t>(kPerCta * UNITS) + threadIdx.x / 16;
+  uint4 a[UNITS], b[UNITS];
+  int64_t row[UNITS];
+  int col[UNITS];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int64_t unit = first + i * kPerCta;
+    int g = 0;
+    row[i] = 0;
+    col[i] = p.cols;
+    a[i] = b[i] = make_uint4(0, 0, 0, 0);
+    if (unit < p.units) {
+      row_of(p, unit, row[i], g);
+      col[i] = g * 128 + c0;
+    }
+    if (col[i] < p.cols) {
+      const uint16_t* x = static_cast<const uint16_t*>(p.x) + row[i] * p.x_stride + col[i];
+      a[i] = __ldg(reinterpret_cast<const uint4*>(x));
+      if (SWIGLU) b[i] = __ldg(reinterpret_cast<const uint4*>(x + p.cols));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    float y[8];
+    unpack16<BF16>(a[i], y);
+    if (SWIGLU) {
+      float u[8];
+      unpack16<BF16>(b[i], u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = gated(y[j], u[j]);
+    }
+    uint32_t top = top8(y);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float inv;
+    const float s = scale_of(top, inv);
+    if (col[i] >= p.cols) continue;
+    *reinterpret_cast<uint2*>(p.out + row[i] * p.cols + col[i]) = e4m3x8(y, inv);
+    if (c0 == 0) p.scale[row[i] * p.groups + col[i] / 128] = s;
+  }
+}
+
+// Any type, width, stride and alignment: a warp a group, four columns a lane.
+template <int DT>
+__global__ void __launch_bounds__(kThreads) quant_any_kernel(const __grid_constant__ QuantParams p) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t unit = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / 32; unit < p.units;
+       unit += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+    int64_t row;
+    int g;
+    row_of(p, unit, row, g);
+    float y[4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = g * 128 + j * 32 + lane;
+      y[j] = 0.0f;
+      if (c < p.cols) {
+        y[j] = load_scalar(p.x, row * p.x_stride + c, DT);
+        if (p.swiglu) y[j] = gated(y[j], load_scalar(p.x, row * p.x_stride + p.cols + c, DT));
+      }
+      top = max(top, mag(y[j]));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    float inv;
+    const float s = scale_of(top, inv);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = g * 128 + j * 32 + lane;
+      if (c < p.cols) p.out[row * p.cols + c] = static_cast<uint8_t>(e4m3x2(y[j] * inv, 0.0f) & 0xff);
+    }
+    if (lane == 0) p.scale[unit] = s;
+  }
+}
+
+template <bool BF16, bool SWIGLU>
+int launch16(const QuantParams& p, int sms, cudaStream_t st) {
+  const bool many = p.units >= static_cast<int64_t>(sms) * 2048;
+  const int per = kPerCta * (many ? 4 : 1);
+  const int64_t grid = (p.units + per - 1) / per;
+  if (grid > 0x7fffffffLL) return B200K_ERR_SHAPE;
+  if (many) quant16_kernel<BF16, SWIGLU, 4><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p);
+  else quant16_kernel<BF16, SWIGLU, 1><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace b200k
+
+using namespace b200k;
+
+extern "C" int b200k_quant_groups(const B200kQuantGroupsArgs* a, void* stream_) {
+  if (!a) return B200K_ERR_ARG;
+  if (a->rows < 0 || a->cols < 0 || a->cols > 0x3fffffffLL || a->x_row_stride < 0) return B200K_ERR_SHAPE;
+  if (a->dtype != B200K_F32 && a->dtype != B200K_F16 && a->dtype != B200K_BF16) return B200K_ERR_UNSUPPORTED;
+  if (a->rows == 0 || a->cols == 0) return B200K_OK;
+  if (!a->x || !a->out || !a->scale) return B200K_ERR_ARG;
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200K_ERR_DEVICE;
+  QuantParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.groups = static_cast<int32_t>((a->cols + 127) / 128);
+  if (a->rows > (int64_t(1) << 62) / a->cols) return B200K_ERR_SHAPE;
+  p.units = a->rows * p.groups;
+  p.big = p.units > 0x7fffffffLL;
+  p.cols = static_cast<int32_t>(a->cols);
+  p.swiglu = a->swiglu ? 1 : 0;
+  p.div_groups = make_fastdiv(static_cast<uint32_t>(p.groups));
+  p.x = a->x;
+  p.x_stride = a->x_row_stride;
+  p.out = static_cast<uint8_t*>(a->out);
+  p.scale = a->scale;
+  cudaStream_t st = static_cast<cudaStream_t>(stream_);
+  const bool vec = a->dtype != B200K_F32 && a->cols % 8 == 0 && aligned16(a->x) && a->x_row_stride % 8 == 0 &&
+                   reinterpret_cast<uintptr_t>(a->out) % 8 == 0;
+  if (vec) {
+    if (a->dtype == B200K_BF16) return p.swiglu ? launch16<true, true>(p, sms, st) : launch16<true, false>(p, sms, st);
+    return p.swiglu ? launch16<false, true>(p, sms, st) : launch16<false, false>(p, sms, st);
+  }
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((p.units + 7) / 8, static_cast<int64_t>(sms) * 16));
+  if (a->dtype == B200K_F32) quant_any_kernel<B200K_F32><<<grid, kThreads, 0, st>>>(p);
+  else if (a->dtype == B200K_F16) quant_any_kernel<B200K_F16><<<grid, kThreads, 0, st>>>(p);
+  else quant_any_kernel<B200K_BF16><<<grid, kThreads, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+}

@@ -568,6 +568,21 @@ void no_grad_inputs(const char* what, std::initializer_list<const at::Tensor*> t
   }
 }
 
+// Row stride of t's flattened leading dims (those of size one have no say), -1
+// when they do not flatten or the columns lie apart.
+int64_t row_stride_of(const at::Tensor& t) {
+  const int64_t cols = t.size(-1);
+  if (t.stride(-1) != 1 && cols > 1) return -1;
+  int64_t stride = -1, expect = 0;
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (stride < 0) stride = expect = t.stride(d);
+    else if (t.stride(d) != expect) return -1;
+    expect *= t.size(d);
+  }
+  return stride < 0 ? cols : stride;
+}
+
 void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r_in,
                    const c10::optional<at::Tensor>& weight, double eps, int64_t flags, int64_t group, bool quant,
                    at::Tensor& out, at::Tensor& scale, at::Tensor& sum) {
@@ -578,20 +593,7 @@ void add_norm_impl(const char* what, const at::Tensor& x_in, const at::Tensor& r
               ": x and residual differ in dtype or device");
   c10::cuda::CUDAGuard guard(x_in.device());
   const int64_t cols = x_in.size(-1);
-  // Row stride of t's flattened leading dims (those of size one have no say),
-  // -1 when they do not flatten or the columns lie apart.
-  auto row_stride = [&](const at::Tensor& t) -> int64_t {
-    if (t.stride(-1) != 1 && cols > 1) return -1;
-    int64_t stride = -1, expect = 0;
-    for (int64_t d = t.dim() - 2; d >= 0; --d) {
-      if (t.size(d) == 1) continue;
-      if (stride < 0) stride = expect = t.stride(d);
-      else if (t.stride(d) != expect) return -1;
-      expect *= t.size(d);
-    }
-    return stride < 0 ? cols : stride;
-  };
-  int64_t xs = row_stride(x_in), rs = row_stride(r_in);
+  int64_t xs = row_stride_of(x_in), rs = row_stride_of(r_in);
   const at::Tensor x = xs < 0 ? x_in.contiguous() : x_in, r = rs < 0 ? r_in.contiguous() : r_in;
   if (xs < 0) xs = cols;
   if (rs < 0) rs = cols;
@@ -647,6 +649,89 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant(const at::Tens
   at::Tensor out, scale, sum;
   add_norm_impl("add_rms_norm_quant", x, residual, weight, eps, flags, group, true, out, scale, sum);
   return {out, scale, sum};
+}
+
+// ------------------------------------------------ block-scaled e4m3 products
+std::tuple<at::Tensor, at::Tensor> quant_groups(const at::Tensor& x_in, bool swiglu) {
+  const char* what = "quant_groups";
+  TORCH_CHECK(x_in.is_cuda(), "b200::quant_groups: x must be a CUDA tensor");
+  TORCH_CHECK(x_in.dim() >= 1 && (!swiglu || x_in.size(-1) % 2 == 0), "b200::quant_groups: x must have a last dim, with swiglu "
+              "an even one (the gate's half and the other), got ", x_in.sizes());
+  TORCH_CHECK(x_in.scalar_type() == at::kFloat || x_in.scalar_type() == at::kHalf || x_in.scalar_type() == at::kBFloat16,
+              "b200::quant_groups: x must be float32, float16 or bfloat16, got ", x_in.scalar_type());
+  c10::cuda::CUDAGuard guard(x_in.device());
+  int64_t stride = row_stride_of(x_in);
+  const at::Tensor x = stride < 0 ? x_in.contiguous() : x_in;
+  if (stride < 0) stride = x.size(-1);
+  const int64_t wide = x.size(-1), cols = swiglu ? wide / 2 : wide;
+  std::vector<int64_t> os(x.sizes().begin(), x.sizes().end()), ss = os;
+  os.back() = cols;
+  ss.back() = (cols + 127) / 128;
+  at::Tensor out = at::empty(os, x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(ss, x.options().dtype(at::kFloat));
+  B200kQuantGroupsArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.rows = wide == 0 ? 0 : x.numel() / wide;
+  a.cols = cols;
+  a.x = x.data_ptr();
+  a.x_row_stride = stride;
+  a.dtype = to_dt(x.scalar_type());
+  a.swiglu = swiglu;
+  a.out = out.data_ptr();
+  a.scale = scale.data_ptr<float>();
+  check(b200k_quant_groups(&a, stream_of(x)), what);
+  return {out, scale};
+}
+
+at::Tensor scaled_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_scale, const at::Tensor& b_scale,
+                     at::ScalarType out_dtype) {
+  const char* what = "scaled_mm";
+  TORCH_CHECK(a.is_cuda(), "b200::scaled_mm: a must be a CUDA tensor");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0), "b200::scaled_mm: a [M, K] and b [K, N], got ", a.sizes(),
+              " and ", b.sizes());
+  TORCH_CHECK(a.scalar_type() == at::kFloat8_e4m3fn && b.scalar_type() == at::kFloat8_e4m3fn,
+              "b200::scaled_mm: a and b must be float8_e4m3fn");
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(1), groups = (K + 127) / 128;
+  TORCH_CHECK(a_scale.dim() == 2 && a_scale.size(0) == M && a_scale.size(1) == groups && b_scale.dim() == 2 &&
+                  b_scale.size(0) == groups && b_scale.size(1) == (N + 127) / 128,
+              "b200::scaled_mm: a_scale must be [", M, ", ", groups, "] and b_scale [", groups, ", ", (N + 127) / 128, "], got ",
+              a_scale.sizes(), " and ", b_scale.sizes());
+  TORCH_CHECK(a_scale.scalar_type() == at::kFloat && b_scale.scalar_type() == at::kFloat, "b200::scaled_mm: the scales must be float32");
+  for (const at::Tensor* t : {&b, &a_scale, &b_scale})
+    TORCH_CHECK(t->device() == a.device(), "b200::scaled_mm: every tensor must be on a's device");
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf || out_dtype == at::kFloat,
+              "b200::scaled_mm: out_dtype must be bfloat16, float16 or float32, got ", out_dtype);
+  TORCH_CHECK((K <= 1 || (a.stride(1) == 1 && b.stride(0) == 1)) || a.numel() == 0 || b.numel() == 0,
+              "b200::scaled_mm: a and b must have unit strides along K (b a transposed [N, K] weight), got ", a.strides(), " and ",
+              b.strides());
+  auto rows_ok = [&](const at::Tensor& t, int64_t d) {
+    return t.numel() == 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                              (t.size(d) <= 1 || (t.stride(d) >= K && t.stride(d) % 16 == 0)));
+  };
+  TORCH_CHECK(rows_ok(a, 0) && rows_ok(b, 1), "b200::scaled_mm: a's rows and b's columns must start on 16-byte boundaries (K or "
+              "the row stride a multiple of 16) and not overlap, got strides ", a.strides(), " and ", b.strides());
+  c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor out = at::empty({M, N}, a.options().dtype(out_dtype));
+  B200kScaledMmArgs g;
+  std::memset(&g, 0, sizeof(g));
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.a = a.data_ptr();
+  g.a_stride_m = a.stride(0);
+  g.b = b.data_ptr();
+  g.b_stride_n = b.stride(1);
+  g.a_scale = a_scale.data_ptr<float>();
+  g.b_scale = b_scale.data_ptr<float>();
+  for (int d = 0; d < 2; ++d) {
+    g.a_scale_strides[d] = a_scale.stride(d);
+    g.b_scale_strides[d] = b_scale.stride(d);
+  }
+  g.out = out.data_ptr();
+  g.out_dtype = to_dt(out_dtype);
+  void* st = stream_of(a);
+  g.status = status_word(a.device().index()).data_ptr<int32_t>();
+  check(b200k_scaled_mm(&g, st), what);
+  return out;
 }
 
 // A dim's stride, 0 where it has one element (or none) and no step is taken.
@@ -845,6 +930,16 @@ at::Tensor paged_attention_autograd(const at::Tensor& q, const at::Tensor& k_cac
                         softcap, window, max_q_len);
 }
 
+std::tuple<at::Tensor, at::Tensor> quant_groups_autograd(const at::Tensor& x, bool swiglu) {
+  static const auto op = find_op<decltype(quant_groups)>("b200::quant_groups");
+  return below_autograd(op, "quant_groups", {&x}, x, swiglu);
+}
+at::Tensor scaled_mm_autograd(const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_scale, const at::Tensor& b_scale,
+                              at::ScalarType out_dtype) {
+  static const auto op = find_op<decltype(scaled_mm)>("b200::scaled_mm");
+  return below_autograd(op, "scaled_mm", {&a, &b, &a_scale, &b_scale}, a, b, a_scale, b_scale, out_dtype);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(b200, m) {
@@ -874,6 +969,8 @@ TORCH_LIBRARY(b200, m) {
   m.def(
       "paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor q_start, Tensor kv_len, "
       "float scale=0.0, float softcap=0.0, int window=0, int max_q_len=0) -> Tensor");
+  m.def("quant_groups(Tensor x, bool swiglu=False) -> (Tensor, Tensor)");
+  m.def("scaled_mm(Tensor a, Tensor b, Tensor a_scale, Tensor b_scale, ScalarType out_dtype) -> Tensor");
   m.def("gemm_status(int device, bool reset) -> int", &gemm_status);
   m.def("status_check(int device, bool arm) -> int", &status_check);
   m.def("gemm_test_stall_next(int timeout_ns) -> ()", &gemm_test_stall_next);
@@ -894,6 +991,8 @@ TORCH_LIBRARY_IMPL(b200, CUDA, m) {
   m.impl("add_rms_norm_quant", &add_rms_norm_quant);
   m.impl("rope_append", &rope_append);
   m.impl("paged_attention", &paged_attention);
+  m.impl("quant_groups", &quant_groups);
+  m.impl("scaled_mm", &scaled_mm);
 }
 
 TORCH_LIBRARY_IMPL(b200, Autograd, m) {
@@ -901,4 +1000,6 @@ TORCH_LIBRARY_IMPL(b200, Autograd, m) {
   m.impl("add_rms_norm_quant", &add_rms_norm_quant_autograd);
   m.impl("rope_append", &rope_append_autograd);
   m.impl("paged_attention", &paged_attention_autograd);
+  m.impl("quant_groups", &quant_groups_autograd);
+  m.impl("scaled_mm", &scaled_mm_autograd);
 }
