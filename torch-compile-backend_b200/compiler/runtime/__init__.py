@@ -112,6 +112,15 @@ def _register_fakes() -> None:
     def _(q, k_cache, v_cache, page_table, q_start, kv_len, scale=0.0, softcap=0.0, window=0, max_q_len=0):
         return q.new_empty(q.shape)
 
+    @torch.library.register_fake(lib + "rope_append_quant")
+    def _(q, k, v, cos, sin, positions, slots, k_cache, v_cache, k_scale, v_scale):
+        return q.new_empty(q.shape)
+
+    @torch.library.register_fake(lib + "paged_attention_quant")
+    def _(q, k_cache, v_cache, k_scale, v_scale, page_table, q_start, kv_len, scale=0.0, softcap=0.0, window=0,
+          max_q_len=0):
+        return q.new_empty(q.shape)
+
     @torch.library.register_fake(lib + "quant_groups")
     def _(x, swiglu=False):
         cols = x.shape[-1] // 2 if swiglu else x.shape[-1]

@@ -203,6 +203,10 @@ def library() -> ctypes.CDLL:
             ("b200k_paged_attention", [ctypes.POINTER(PagedAttentionArgs), ctypes.c_void_p]),
             ("b200k_paged_attention_workspace", [ctypes.POINTER(PagedAttentionArgs),
                                                  ctypes.POINTER(ctypes.c_int64)]),
+            ("b200k_rope_append_quant", [ctypes.POINTER(RopeAppendQuantArgs), ctypes.c_void_p]),
+            ("b200k_paged_attention_quant", [ctypes.POINTER(PagedAttentionQuantArgs), ctypes.c_void_p]),
+            ("b200k_paged_attention_quant_workspace", [ctypes.POINTER(PagedAttentionQuantArgs),
+                                                       ctypes.POINTER(ctypes.c_int64)]),
             ("b200k_quant_groups", [ctypes.POINTER(QuantGroupsArgs), ctypes.c_void_p]),
             ("b200k_scaled_mm", [ctypes.POINTER(ScaledMmArgs), ctypes.c_void_p]),
             ("b200k_gemm_pick_config", [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]),
@@ -446,6 +450,24 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
                 positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 q_out: torch.Tensor, status: torch.Tensor | None = None) -> None:
     """q_out = q rotated; k rotated and v written into the caches' slots."""
+    a = _append_args(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_out, status)
+    _check("b200k_rope_append", library().b200k_rope_append(ctypes.byref(a), _stream()))
+
+
+def rope_append_quant(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                      positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, q_out: torch.Tensor,
+                      status: torch.Tensor | None = None) -> None:
+    """rope_append to e4m3 caches with a scale for each row in k_scale and v_scale."""
+    a = RopeAppendQuantArgs()
+    a.base = _append_args(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_out, status)
+    a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    for d in range(3):
+        a.scale_strides[d] = k_scale.stride(d)
+    _check("b200k_rope_append_quant", library().b200k_rope_append_quant(ctypes.byref(a), _stream()))
+
+
+def _append_args(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_out, status) -> RopeAppendArgs:
     a = RopeAppendArgs()
     a.tokens, a.heads, a.head_dim = q.shape
     a.kv_heads, a.rot_dim = k.shape[1], 2 * cos.shape[1]
@@ -460,7 +482,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     a.dtype, a.table_dtype = DTYPE[q.dtype], DTYPE[cos.dtype]
     a.positions_dtype, a.slots_dtype = DTYPE[positions.dtype], DTYPE[slots.dtype]
     a.status = status.data_ptr() if status is not None else None
-    _check("b200k_rope_append", library().b200k_rope_append(ctypes.byref(a), _stream()))
+    return a
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -470,6 +492,28 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of packed queries [tokens, H, D] over a paged cache, into `out`.
     Returns the workspace bytes it needs; `workspace` (of at least those) is
     allocated when not given."""
+    a = _attention_args(q, k_cache, v_cache, page_table, q_start, kv_len, out, scale, softcap, window, max_q_len, status,
+                        timeout_ns, test_flags)
+    return _attend("b200k_paged_attention", a, a, q.device, workspace)
+
+
+def paged_attention_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                          v_scale: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+                          out: torch.Tensor, scale: float = 0.0, softcap: float = 0.0, window: int = 0,
+                          max_q_len: int = 0, status: torch.Tensor | None = None, timeout_ns: int = 0,
+                          test_flags: int = 0, workspace: torch.Tensor | None = None) -> int:
+    """paged_attention over e4m3 caches with a scale for each row."""
+    a = PagedAttentionQuantArgs()
+    a.base = _attention_args(q, k_cache, v_cache, page_table, q_start, kv_len, out, scale, softcap, window, max_q_len,
+                             status, timeout_ns, test_flags)
+    a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    for d in range(3):
+        a.scale_strides[d] = k_scale.stride(d)
+    return _attend("b200k_paged_attention_quant", a, a.base, q.device, workspace)
+
+
+def _attention_args(q, k_cache, v_cache, page_table, q_start, kv_len, out, scale, softcap, window, max_q_len, status,
+                    timeout_ns, test_flags) -> PagedAttentionArgs:
     a = PagedAttentionArgs()
     a.tokens, a.heads, a.head_dim = q.shape
     a.seqs, a.kv_heads = kv_len.shape[0], k_cache.shape[2]
@@ -483,16 +527,20 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a.page_table, a.q_start, a.kv_len = page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr()
     a.max_q_len, a.window, a.scale, a.softcap = max_q_len, window, scale, softcap
     a.dtype, a.test_flags = DTYPE[q.dtype], test_flags
-    n = ctypes.c_int64()
-    _check("b200k_paged_attention_workspace",
-           library().b200k_paged_attention_workspace(ctypes.byref(a), ctypes.byref(n)))
-    ws = workspace if workspace is not None else torch.empty(max(1, n.value), dtype=torch.uint8, device=q.device)
-    if ws.numel() < n.value:
-        raise ValueError(f"workspace of {ws.numel()} bytes, {n.value} needed")
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
     a.status = status.data_ptr() if status is not None else None
     a.timeout_ns = timeout_ns
-    _check("b200k_paged_attention", library().b200k_paged_attention(ctypes.byref(a), _stream()))
+    return a
+
+
+def _attend(name: str, a, base: PagedAttentionArgs, device, workspace: torch.Tensor | None) -> int:
+    lib = library()
+    n = ctypes.c_int64()
+    _check(name + "_workspace", getattr(lib, name + "_workspace")(ctypes.byref(a), ctypes.byref(n)))
+    ws = workspace if workspace is not None else torch.empty(max(1, n.value), dtype=torch.uint8, device=device)
+    if ws.numel() < n.value:
+        raise ValueError(f"workspace of {ws.numel()} bytes, {n.value} needed")
+    base.workspace, base.workspace_bytes = ws.data_ptr(), n.value
+    _check(name, getattr(lib, name)(ctypes.byref(a), _stream()))
     return n.value
 
 

@@ -19,7 +19,7 @@
 #include <algorithm>
 #include <cstring>
 
-#include "common.cuh"
+#include "e4m3.cuh"
 #include "host_common.h"
 
 namespace b200k {
@@ -42,23 +42,12 @@ struct AppendParams {
   FastDiv div_page;
   int64_t total_slots;
   int32_t* status;
+  // e4m3 caches: codes in place of k_cache and v_cache (same strides), and their scales
+  uint8_t *k8, *v8;
+  float *ks, *vs;
+  int64_t s_page, s_slot, s_head;
+  int32_t q8;
 };
-
-template <bool BF16>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (BF16) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
-    }
-  }
-}
 
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
   return is64 ? __ldg(static_cast<const long long*>(p) + i) : __ldg(static_cast<const int*>(p) + i);
@@ -69,6 +58,7 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64
 // table or the cache is reported and its token not appended.
 struct Place {
   int64_t row, cache;
+  int64_t scale;  // with cache >= 0: of the e4m3 caches' scales
 };
 __device__ __forceinline__ Place place_of(const AppendParams& p, int64_t t) {
   int64_t pos = load_index(p.positions, t, p.pos64), slot = load_index(p.slots, t, p.slot64);
@@ -79,11 +69,12 @@ __device__ __forceinline__ Place place_of(const AppendParams& p, int64_t t) {
   }
   Place r;
   r.row = pos_ok ? pos : 0;
-  r.cache = -1;
+  r.cache = r.scale = -1;
   if (slot >= 0) {
     const uint32_t page = fdiv(static_cast<uint32_t>(slot), p.div_page);
     const uint32_t off = static_cast<uint32_t>(slot) - page * static_cast<uint32_t>(p.page_size);
     r.cache = static_cast<int64_t>(page) * p.c_page + static_cast<int64_t>(off) * p.c_slot;
+    r.scale = static_cast<int64_t>(page) * p.s_page + static_cast<int64_t>(off) * p.s_slot;
   }
   return r;
 }
@@ -135,8 +126,8 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_cons
     uint4 oa = a[i], ob = b[i];
     if (turns && h < p.heads + p.kv_heads) {
       float x[8], y[8], u[8], w[8];
-      unpack8<BF16>(a[i], x);
-      unpack8<BF16>(b[i], y);
+      unpack16<BF16>(a[i], x);
+      unpack16<BF16>(b[i], y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         u[j] = x[j] * cs[j] - y[j] * sn[j];
@@ -185,6 +176,116 @@ __global__ void __launch_bounds__(256) rope_append_any_kernel(const __grid_const
   }
 }
 
+// The append to e4m3 caches (b200k_rope_append_quant): a cached row's scale
+// is its largest magnitude / 448, found by the units' threads of its head (a
+// power of two of neighbouring lanes) from the fp32 values, which are rounded
+// once.  All lanes stay to the end for the shuffles.
+template <bool BF16, int TAB_DT, int NH>
+__global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_constant__ AppendParams p) {
+  const uint32_t gid = blockIdx.x * static_cast<uint32_t>(kThreads) + threadIdx.x;
+  uint32_t tok = fdiv(gid, p.div_tok);
+  const uint32_t in_tok = gid - tok * p.div_tok.d;
+  const bool real = tok < p.tokens;
+  if (!real) tok = static_cast<uint32_t>(p.tokens - 1);
+  const uint32_t hb = fdiv(in_tok, p.div_unit);
+  const int unit = static_cast<int>(in_tok - hb * p.div_unit.d);
+  const int rot_units = p.rot >> 4;
+  const bool turns = unit < rot_units;
+  const int c0 = (turns ? unit : 2 * unit) * 8, c1 = turns ? c0 + (p.rot >> 1) : c0 + 8;
+  const int head0 = static_cast<int>(hb) * NH, all = p.heads + 2 * p.kv_heads;
+  uint4 a[NH], b[NH];
+#pragma unroll
+  for (int i = 0; i < NH; ++i) {
+    const int h = min(head0 + i, all - 1);
+    const uint16_t* src;
+    if (h < p.heads) src = p.q + tok * p.q_t + h * p.q_h;
+    else if (h < p.heads + p.kv_heads) src = p.k + tok * p.k_t + (h - p.heads) * p.k_h;
+    else src = p.v + tok * p.v_t + (h - p.heads - p.kv_heads) * p.v_h;
+    a[i] = __ldg(reinterpret_cast<const uint4*>(src + c0));
+    b[i] = __ldg(reinterpret_cast<const uint4*>(src + c1));
+  }
+  const Place pl = place_of(p, tok);
+  float cs[8], sn[8];
+  if (turns) {
+    load_vec8(p.cos, pl.row * p.table_stride + c0, TAB_DT, cs);
+    load_vec8(p.sin, pl.row * p.table_stride + c0, TAB_DT, sn);
+  }
+#pragma unroll
+  for (int i = 0; i < NH; ++i) {
+    const int h = head0 + i;
+    const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
+    float u[8], w[8];
+    unpack16<BF16>(a[i], u);
+    unpack16<BF16>(b[i], w);
+    if (turns && !is_v) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = u[j], y = w[j];
+        u[j] = x * cs[j] - y * sn[j];
+        w[j] = y * cs[j] + x * sn[j];
+      }
+    }
+    uint32_t top = max(top8(u), top8(w));
+    for (int o = 1; o < p.units; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!real || h >= all) continue;
+    if (is_q) {
+      uint16_t* dst = p.q_out + (static_cast<int64_t>(tok) * p.heads + h) * p.dim;
+      // what is not turned keeps its bits
+      *reinterpret_cast<uint4*>(dst + c0) = !turns ? a[i] : BF16 ? pack_bf16x8(u) : pack_f16x8(u);
+      *reinterpret_cast<uint4*>(dst + c1) = !turns ? b[i] : BF16 ? pack_bf16x8(w) : pack_f16x8(w);
+    } else if (pl.cache >= 0) {
+      float inv;
+      const float s = scale_of(top, inv);
+      const int kvh = h - p.heads - (is_v ? p.kv_heads : 0);
+      uint8_t* dst = (is_v ? p.v8 : p.k8) + pl.cache + kvh * p.c_head;
+      *reinterpret_cast<uint2*>(dst + c0) = e4m3x8(u, inv);
+      *reinterpret_cast<uint2*>(dst + c1) = e4m3x8(w, inv);
+      if (unit == 0) (is_v ? p.vs : p.ks)[pl.scale + kvh * p.s_head] = s;
+    }
+  }
+}
+
+// Any even rotary width, head size and alignment: a warp a row, which goes over
+// it twice.
+template <bool BF16, int TAB_DT>
+__global__ void __launch_bounds__(256) rope_append8_any_kernel(const __grid_constant__ AppendParams p) {
+  const int all = p.heads + 2 * p.kv_heads, lane = threadIdx.x & 31;
+  const int64_t rows = p.tokens * all;
+  constexpr int DT = BF16 ? B200K_BF16 : B200K_F16;
+  for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
+    const int64_t tok = r / all;
+    const int h = static_cast<int>(r - tok * all);
+    const Place pl = place_of(p, tok);
+    const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
+    const int kvh = h - p.heads - (is_v ? p.kv_heads : 0);
+    const uint16_t* src = is_q ? p.q + tok * p.q_t + h * p.q_h : is_v ? p.v + tok * p.v_t + kvh * p.v_h : p.k + tok * p.k_t + kvh * p.k_h;
+    auto value = [&](int j) {
+      if (j >= p.rot || is_v) return load_scalar(src, j, DT);
+      const int half = p.rot >> 1, i = j < half ? j : j - half;
+      const float c = load_scalar(p.cos, pl.row * p.table_stride + i, TAB_DT), s = load_scalar(p.sin, pl.row * p.table_stride + i, TAB_DT);
+      const float x = load_scalar(src, i, DT), y = load_scalar(src, i + half, DT);
+      return j < half ? x * c - y * s : y * c + x * s;
+    };
+    if (is_q) {
+      uint16_t* dst = p.q_out + (tok * p.heads + h) * p.dim;
+      for (int j = lane; j < p.dim; j += 32) {
+        if (j < p.rot) store_scalar(dst, j, DT, value(j));
+        else dst[j] = src[j];
+      }
+      continue;
+    }
+    if (pl.cache < 0) continue;
+    uint32_t top = 0;
+    for (int j = lane; j < p.dim; j += 32) top = max(top, mag(value(j)));
+    top = __reduce_max_sync(0xffffffffu, top);
+    float inv;
+    const float s = scale_of(top, inv);
+    uint8_t* dst = (is_v ? p.v8 : p.k8) + pl.cache + kvh * p.c_head;
+    for (int j = lane; j < p.dim; j += 32) dst[j] = static_cast<uint8_t>(e4m3x2(value(j) * inv, 0.0f) & 0xff);
+    if (lane == 0) (is_v ? p.vs : p.ks)[pl.scale + kvh * p.s_head] = s;
+  }
+}
+
 template <bool BF16, int TAB_DT>
 int launch(AppendParams& p, bool vec, int sms, cudaStream_t st) {
   const int all = p.heads + 2 * p.kv_heads;
@@ -202,24 +303,23 @@ int launch(AppendParams& p, bool vec, int sms, cudaStream_t st) {
     if (n + kThreads <= 0x7fffffffLL) {
       p.div_tok = make_fastdiv(static_cast<uint32_t>(p.threads_per_token));
       const unsigned grid = static_cast<unsigned>((n + kThreads - 1) / kThreads);
-      if (nh == 4) rope_append_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
+      if (p.q8) {
+        if (nh == 4) rope_append8_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
+        else rope_append8_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
+      } else if (nh == 4) rope_append_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
       else rope_append_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
       return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
     }
   }
-  const int64_t n = p.tokens * all * p.dim;
+  const int64_t n = p.tokens * all * (p.q8 ? 32 : p.dim);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, static_cast<int64_t>(sms) * 8));
-  rope_append_any_kernel<BF16, TAB_DT><<<grid, 256, 0, st>>>(p);
+  if (p.q8) rope_append8_any_kernel<BF16, TAB_DT><<<grid, 256, 0, st>>>(p);
+  else rope_append_any_kernel<BF16, TAB_DT><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
-}  // namespace
-}  // namespace b200k
-
-using namespace b200k;
-
-extern "C" int b200k_rope_append(const B200kRopeAppendArgs* a, void* stream_) {
-  if (!a) return B200K_ERR_ARG;
+// `q8` (NULL: 16-bit caches): the scales.
+int append(const B200kRopeAppendArgs* a, const B200kRopeAppendQuantArgs* q8, void* stream_) {
   if (a->tokens < 0 || a->heads < 0 || a->kv_heads < 0 || a->head_dim < 0 || a->num_pages < 0 || a->page_size < 0)
     return B200K_ERR_SHAPE;
   if (a->tokens == 0 || a->head_dim == 0 || a->heads + a->kv_heads == 0) return B200K_OK;
@@ -236,6 +336,7 @@ extern "C" int b200k_rope_append(const B200kRopeAppendArgs* a, void* stream_) {
     return B200K_ERR_SHAPE;
   const int64_t total = a->num_pages * a->page_size;
   if (a->kv_heads && total && (!a->k_cache || !a->v_cache)) return B200K_ERR_ARG;
+  if (q8 && a->kv_heads && total && (!q8->k_scale || !q8->v_scale)) return B200K_ERR_ARG;
   const int sms = device_sm_count();
   if (sms <= 0) return B200K_ERR_DEVICE;
   AppendParams p;
@@ -267,15 +368,38 @@ extern "C" int b200k_rope_append(const B200kRopeAppendArgs* a, void* stream_) {
   p.div_page = make_fastdiv(static_cast<uint32_t>(std::max<int64_t>(1, a->page_size)));
   p.total_slots = total;
   p.status = a->status;
+  if (q8) {
+    p.q8 = 1;
+    p.k8 = static_cast<uint8_t*>(a->k_cache);
+    p.v8 = static_cast<uint8_t*>(a->v_cache);
+    p.ks = q8->k_scale;
+    p.vs = q8->v_scale;
+    p.s_page = q8->scale_strides[0];
+    p.s_slot = q8->scale_strides[1];
+    p.s_head = q8->scale_strides[2];
+  }
   bool vec = a->head_dim % 16 == 0 && a->rot_dim % 16 == 0 && a->table_stride % 8 == 0;
   for (const void* x : {a->q, a->k, a->v, static_cast<const void*>(a->q_out), static_cast<const void*>(a->k_cache),
                         static_cast<const void*>(a->v_cache), a->cos, a->sin})
     vec = vec && aligned16(x);
   for (int d = 0; d < 2; ++d) vec = vec && a->q_strides[d] % 8 == 0 && a->k_strides[d] % 8 == 0 && a->v_strides[d] % 8 == 0;
   for (int d = 0; d < 3; ++d) vec = vec && a->cache_strides[d] % 8 == 0;
+  if (q8) vec = vec && (a->head_dim & (a->head_dim - 1)) == 0 && a->head_dim <= 512;  // a head's threads are lanes of one warp
   cudaStream_t st = static_cast<cudaStream_t>(stream_);
   const bool f32 = a->table_dtype == B200K_F32;
   if (a->dtype == B200K_BF16)
     return f32 ? launch<true, B200K_F32>(p, vec, sms, st) : launch<true, B200K_BF16>(p, vec, sms, st);
   return f32 ? launch<false, B200K_F32>(p, vec, sms, st) : launch<false, B200K_F16>(p, vec, sms, st);
+}
+
+}  // namespace
+}  // namespace b200k
+
+using namespace b200k;
+
+extern "C" int b200k_rope_append(const B200kRopeAppendArgs* a, void* stream_) {
+  return a ? append(a, nullptr, stream_) : B200K_ERR_ARG;
+}
+extern "C" int b200k_rope_append_quant(const B200kRopeAppendQuantArgs* a, void* stream_) {
+  return a ? append(&a->base, a, stream_) : B200K_ERR_ARG;
 }

@@ -9,6 +9,7 @@ namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 16;      // keys of one step of the row kernel (one MMA k)
+constexpr int kKeys8 = 32;     // ... over e4m3 caches: as many bytes
 constexpr int kRows = 16;      // query rows of one unit of the row kernel (one MMA m)
 constexpr int kBlock = 64;     // keys of one step of the tile kernel
 constexpr int kUnitRows = 256; // query rows of one unit of the tile kernel (two MMA m)
@@ -55,6 +56,10 @@ struct Params {
   int64_t q_t, q_h;
   const uint16_t *k, *v;
   int64_t c_page, c_slot, c_head;
+  // e4m3 caches: codes in place of k and v (same strides), and their scales
+  const uint8_t *k8, *v8;
+  const float *ks, *vs;
+  int64_t s_page, s_slot, s_head;
   uint16_t* out;               // [T, H, D] contiguous
   const int32_t *table, *q_start, *kv_len;
   // base-2 scores: y = x * mul; with a cap (cap_far) mul = 2 scale log2(e) / cap,
@@ -131,8 +136,10 @@ __device__ __forceinline__ void tile_keys(const Params& p, const Unit& u, int t,
   if (a < u.rows) rows_keys(p, u.s, a, min(a + 128, u.rows), lo, hi);
 }
 
-// Launches the tile kernel (paged_tiles.cu) on the plan in p.entries.
+// Launches the tile kernel (paged_tiles.cu, over e4m3 caches paged_tiles8.cu)
+// on the plan in p.entries.
 int launch_tiles(const Params& p, bool bf16, int dim, int cap, cudaStream_t st);
+int launch_tiles8(const Params& p, bool bf16, int dim, int cap, cudaStream_t st);
 
 // Offset of a key's row in the caches, `page` being what the table holds for
 // it, or -1: not between lo and n (nothing there is read: the pages may hold
@@ -152,6 +159,72 @@ __device__ __forceinline__ int64_t key_offset(const Params& p, int b, int key, i
   if (key < lo || key >= n) return -1;
   const int page = __ldg(p.table + b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
   return page_offset(p, page, key, lo, n, kvh);
+}
+
+// ... with the offset of its scales.
+struct Place8 {
+  int64_t row, scale;
+};
+__device__ __forceinline__ Place8 place8(const Params& p, int page, int key, int lo, int n, int kvh) {
+  Place8 r{-1, -1};
+  if (key < lo || key >= n) return r;
+  if (page < 0 || page >= p.num_pages) {
+    if (p.status) atomicCAS(p.status, 0, B200K_ERR_INDEX);
+    return r;
+  }
+  const uint32_t pi = fdiv(static_cast<uint32_t>(key), p.div_page);
+  const int64_t in = static_cast<uint32_t>(key) - pi * static_cast<uint32_t>(p.page_size);
+  r.row = static_cast<int64_t>(page) * p.c_page + in * p.c_slot + static_cast<int64_t>(kvh) * p.c_head;
+  r.scale = static_cast<int64_t>(page) * p.s_page + in * p.s_slot + static_cast<int64_t>(kvh) * p.s_head;
+  return r;
+}
+
+// Attention over e4m3 caches: key and value rows are code * scale.  The scales
+// stay out of the products: a score is (q . codes) ks_j, and with
+//   y_j = f(score_j) log2(e) + log2(vs_j),  w_j = 2^(y_j - max y)
+// the output is sum_j w_j codes_j / sum_j w_j / vs_j: one exponential for both
+// sums, and no w_j above 1 however far the values' scales lie apart.  Codes are
+// exact in f16, so both products are f16 ones whatever q's type.
+// Scales of values below kMinVs (that of rows of zeros) count as it.
+constexpr float kMinVs = 1e-12f / 448.0f;
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float value_scale(float vs) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(vs), "f"(kMinVs));
+  return r;
+}
+// Two e4m3 codes (the low or high half of a word) as f16.
+__device__ __forceinline__ uint32_t codes16(uint16_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_lo(uint32_t c) { return codes16(static_cast<uint16_t>(c)); }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t c) { return codes16(static_cast<uint16_t>(c >> 16)); }
+// bf16 queries as f16: a row is divided by a power of two that puts its
+// largest magnitude (`top`, as bits) between 2^14 and 2^15, which leaves 28
+// binades at full precision below it, and its scores are multiplied by it.
+struct RowScale {
+  float div, mul;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {
+  const uint32_t e = top >> 23;  // biased exponent of the largest magnitude
+  RowScale r{1.0f, 1.0f};
+  if (e == 255 || top == 0) return r;  // a row with an infinity or NaN, of zeros
+  const uint32_t b = max(e, 15u);
+  r.div = __uint_as_float((268u - b) << 23);
+  r.mul = __uint_as_float((b - 14u) << 23);
+  return r;
+}
+// Two bf16 values times `f` as f16.
+__device__ __forceinline__ uint32_t bf16_to_f16(uint32_t w, float f) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float(w & 0xffff0000u) * f), "f"(__uint_as_float(w << 16) * f));
+  return r;
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -91,14 +91,15 @@ struct Work {
   int tiles;  // 0: no keys, no queries, or the tile kernel's
   int rts;    // 16-row blocks of a kv head
 };
-// `limit`: query rows above which a sequence is the tile kernel's.
+// `limit`: query rows above which a sequence is the tile kernel's; KEYS: of a step.
+template <int KEYS>
 __device__ __forceinline__ Work work_at(const Params& p, int b, int limit) {
   Work w;
   w.s = seq_at(p, b);
-  w.base = w.s.lo & ~(kKeys - 1);
+  w.base = w.s.lo & ~(KEYS - 1);
   const int64_t rows = static_cast<int64_t>(w.s.m) * p.G;
   w.rts = static_cast<int>((rows + kRows - 1) / kRows);
-  w.tiles = (w.s.m > 0 && w.s.n > w.base && rows <= limit) ? (w.s.n - w.base + kKeys - 1) / kKeys : 0;
+  w.tiles = (w.s.m > 0 && w.s.n > w.base && rows <= limit) ? (w.s.n - w.base + KEYS - 1) / KEYS : 0;
   return w;
 }
 __device__ __forceinline__ int64_t steps_of(const Params& p, const Work& w) {
@@ -117,11 +118,12 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
 // The limit of this call: p.long_rows, or kRows where the sequences between
 // the two (two row blocks, so the row kernel reads their keys twice) have
 // enough keys for the tile kernel to pay.  Every warp that asks gets the same.
+template <int KEYS>
 __device__ __forceinline__ int limit_of(const Params& p) {
   if (p.mid_steps == 0) return p.long_rows;
   int64_t steps = 0;
   for (int b = threadIdx.x & 31; b < p.B; b += 32) {
-    const Work w = work_at(p, b, p.long_rows);
+    const Work w = work_at<KEYS>(p, b, p.long_rows);
     if (w.rts > 1) steps += static_cast<int64_t>(p.Hkv) * w.tiles;
   }
 #pragma unroll
@@ -148,6 +150,7 @@ __device__ __forceinline__ int64_t run_of(const Params& p, int64_t total, int lo
 
 // A position in the list of steps: within a sequence kv head by kv head, row
 // block by row block, key by key.
+template <int KEYS>
 struct Cursor {
   Work w;
   int b, kvh, rt, tile;
@@ -161,20 +164,21 @@ struct Cursor {
     kvh = 0;
     do {
       if (++b >= p.B) return;
-      w = work_at(p, b, limit);
+      w = work_at<KEYS>(p, b, limit);
     } while (w.tiles == 0 || w.rts == 0);
   }
 };
 
 // The tile kernel's list: an entry for every 256 query rows of a sequence
 // that is its own, with the steps before it.  One CTA of 128 threads.
+template <int KEYS>
 __device__ __noinline__ void plan_tiles(const Params& p) {
   __shared__ int starts[kWarps * 32 + 1];   // entries before each of 128 sequences
   __shared__ int64_t sums[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t* before = p.entry_steps + 3;
   for (int i = tid; i < p.tile_ctas; i += kWarps * 32) p.joins[i].last = 0;
-  const int limit = limit_of(p);
+  const int limit = limit_of<KEYS>(p);
   int64_t steps = 0;
   int entry0 = 0;
   auto block_scan = [&](int64_t v, int64_t& all) {  // inclusive
@@ -237,14 +241,14 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
 // a sum, 32 bytes apart modulo the banks.
 template <int D>
 constexpr int kJointStride = D + 8;
-template <int D>
+template <int D, uint32_t RING>
 __device__ __forceinline__ float* joint_rows(uint8_t* smem, int warp) {
-  static_assert(kRows * kJointStride<D> * 4 <= kRingBytes, "a part fits a ring");
-  return reinterpret_cast<float*>(smem + warp * kRingBytes);
+  static_assert(kRows * kJointStride<D> * 4 <= RING, "a part fits a ring");
+  return reinterpret_cast<float*>(smem + warp * RING);
 }
 // The CTA's warps' parts of one unit as one: written to `worker`'s slot, or to
 // the output where the CTA has the whole unit.  A warp takes every kWarps-th row.
-template <bool BF16, int D, typename Out>
+template <bool BF16, int D, uint32_t RING, typename Out>
 __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int warp, int lane, int rows, int worker, int slot,
                                            bool whole, Out out_row) {
   constexpr int V = D / 32;
@@ -254,7 +258,7 @@ __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int w
     float mx = -INFINITY, sum = 0.0f, acc[V];
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
-      ml[k] = *reinterpret_cast<const float2*>(joint_rows<D>(smem, k) + in * kJointStride<D> + D);
+      ml[k] = *reinterpret_cast<const float2*>(joint_rows<D, RING>(smem, k) + in * kJointStride<D> + D);
       mx = fmaxf(mx, ml[k].x);
     }
     const float ref = mx == -INFINITY ? 0.0f : mx;
@@ -263,7 +267,7 @@ __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int w
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
       const float f = ex2(ml[k].x - ref);
-      const Vec x = reinterpret_cast<const Vec*>(joint_rows<D>(smem, k) + in * kJointStride<D>)[lane];
+      const Vec x = reinterpret_cast<const Vec*>(joint_rows<D, RING>(smem, k) + in * kJointStride<D>)[lane];
       sum = fmaf(ml[k].y, f, sum);
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], f, acc[j]);
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   const int worker = (static_cast<int>(blockIdx.x) - (p.tile_ctas > 0 ? 1 : 0)) * kWarps + warp;
   const uint32_t ring = smem_addr(smem) + warp * kRingBytes;
   if (worker < 0) {
-    plan_tiles(p);
+    plan_tiles<kKeys>(p);
     return;
   }
 
@@ -305,13 +309,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // The whole list's length and, from it, this worker's run [w0, w1).
-  const int limit = limit_of(p);
+  const int limit = limit_of<kKeys>(p);
   int64_t total = 0, mine0 = 0, upto0 = 0;
   int longest = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = 0;
     if (b0 + lane < p.B) {
-      const Work w = work_at(p, b0 + lane, limit);
+      const Work w = work_at<kKeys>(p, b0 + lane, limit);
       mine = steps_of(p, w);
       longest = max(longest, w.tiles);
     }
@@ -328,13 +332,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   }
   const int64_t w0 = run * worker, w1 = min(total, w0 + run);
   if (w0 >= w1) return;
-  Cursor cur;
+  Cursor<kKeys> cur;
   cur.b = 0;
   int64_t seq0 = 0;  // the list's index of cur.b's first step
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = mine0, upto = upto0;  // of the last 32: all there are in a small batch
     if (p.B > 32) {
-      mine = b0 + lane < p.B ? steps_of(p, work_at(p, b0 + lane, limit)) : 0;
+      mine = b0 + lane < p.B ? steps_of(p, work_at<kKeys>(p, b0 + lane, limit)) : 0;
       upto = warp_scan(mine);
     }
     const unsigned hit = __ballot_sync(0xffffffffu, seq0 + upto > w0);
@@ -347,17 +351,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     seq0 += __shfl_sync(0xffffffffu, upto, 31);
   }
   cur.limit = limit;
-  cur.w = work_at(p, cur.b, limit);
+  cur.w = work_at<kKeys>(p, cur.b, limit);
   const int unit = static_cast<int>(div64(w0 - seq0, cur.w.tiles));
   cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(unit) * cur.w.tiles);
   cur.kvh = unit / cur.w.rts;
   cur.rt = unit - cur.kvh * cur.w.rts;
 
-  Cursor ld = cur;
+  Cursor<kKeys> ld = cur;
   int64_t ld_t = w0;
   // The page that holds this lane's key of a step, -1 for no key: fetched a
   // step before its first use, so that no step waits for the table.
-  auto page_of = [&](const Cursor& c) {
+  auto page_of = [&](const Cursor<kKeys>& c) {
     const int key = c.w.base + c.tile * kKeys + (lane & (kKeys - 1));
     if (key < c.w.s.lo || key >= c.w.s.n) return -1;
     return __ldg(p.table + c.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
@@ -528,7 +532,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
         const int in = g + 8 * i, r = r0 + in;
         if (r >= rows) continue;
         if (joint) {
-          float* dst = joint_rows<D>(smem, warp) + in * kJointStride<D>;
+          float* dst = joint_rows<D, kRingBytes>(smem, warp) + in * kJointStride<D>;
           if (quad == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[i], l[i]);
 #pragma unroll
           for (int n = 0; n < D / 8; ++n)
@@ -551,7 +555,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
       }
       if (joint) {
         __syncthreads();  // every warp of the CTA comes here once
-        join_warps<BF16, D>(p, smem, warp, lane, min(kRows, rows - r0), worker & ~(kWarps - 1), unit0 < c0 ? 0 : 1,
+        join_warps<BF16, D, kRingBytes>(p, smem, warp, lane, min(kRows, rows - r0), worker & ~(kWarps - 1), unit0 < c0 ? 0 : 1,
                             unit0 == c0 && c1 == unit0 + cur.w.tiles, [&](int in) {
                               const int r = r0 + in;
                               const uint32_t tok = fdiv(static_cast<uint32_t>(r), p.div_g);
@@ -739,7 +743,7 @@ __device__ __forceinline__ void join_row(const Params& p, const RowParts& rp, in
 // with the other two; one of 16384 keys among 63 of 100 29.4, 30.2 (kRowMixed)
 // and 39.7 (kRowWarp); 7 tokens of 70 sequences 76, 51 and 47.
 enum { kRowCta, kRowMixed, kRowWarp };
-template <bool BF16, int D, int MODE>
+template <bool BF16, int D, int MODE, int KEYS>
 __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_constant__ Params p) {
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
   constexpr int W = kJoinWarps, kPerCta = MODE == kRowCta ? 1 : W;
@@ -762,20 +766,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     int b, y, h, kvh;
     int64_t seq0, run;
   };
-  const int limit = limit_of(p);
+  const int limit = limit_of<KEYS>(p);
   auto look = [&](int item) {
     Item it;
     it.h = item % p.H;
     it.y = item / p.H % p.combine_rows;
     it.b = item / p.H / p.combine_rows;
     it.kvh = static_cast<int>(fdiv(static_cast<uint32_t>(it.h), p.div_g));
-    it.w = work_at(p, min(it.b, p.B - 1), limit);
+    it.w = work_at<KEYS>(p, min(it.b, p.B - 1), limit);
     it.seq0 = it.run = 0;
     if (p.B <= 32) {  // the list in one scan; else what the row kernel left
       int64_t mine = 0;
       int longest = 0;
       if (lane < p.B) {
-        const Work w = work_at(p, lane, limit);
+        const Work w = work_at<KEYS>(p, lane, limit);
         mine = steps_of(p, w);
         longest = w.tiles;
       }
@@ -851,10 +855,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
   }
 }
 
-template <bool BF16, int D, int CAP>
+#include "paged_rows8.cuh"
+
+// Q8: over e4m3 caches.
+template <bool BF16, int D, int CAP, bool Q8>
 int launch(const Params& p, int ctas, cudaStream_t st) {
-  constexpr uint32_t kSmem = kWarps * kRingBytes;
-  auto kernel = rows_kernel<BF16, D, CAP>;
+  constexpr uint32_t kSmem = kWarps * (Q8 ? kRing8Bytes : kRingBytes);
+  constexpr int KEYS = Q8 ? kKeys8 : kKeys;
+  void (*kernel)(const Params);
+  if constexpr (Q8) kernel = rows8_kernel<BF16, D, CAP>;
+  else kernel = rows_kernel<BF16, D, CAP>;
   static std::atomic<uint64_t> done{0};
   if (!attributes_set(done)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
@@ -864,7 +874,7 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   kernel<<<ctas + (p.tile_ctas > 0 ? 1 : 0), kWarps * 32, kSmem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return B200K_ERR_LAUNCH;
   if (p.tile_ctas > 0) {
-    const int rc = launch_tiles(p, BF16, D, CAP, st);
+    const int rc = Q8 ? launch_tiles8(p, BF16, D, CAP, st) : launch_tiles(p, BF16, D, CAP, st);
     if (rc != B200K_OK) return rc;
   }
   // The combine's launch overlaps the row kernel's end (it waits for the
@@ -880,16 +890,21 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  auto combine = p.join_mode == kRowCta     ? combine_kernel<BF16, D, kRowCta>
-                 : p.join_mode == kRowMixed ? combine_kernel<BF16, D, kRowMixed>
-                                            : combine_kernel<BF16, D, kRowWarp>;
+  auto combine = p.join_mode == kRowCta     ? combine_kernel<BF16, D, kRowCta, KEYS>
+                 : p.join_mode == kRowMixed ? combine_kernel<BF16, D, kRowMixed, KEYS>
+                                            : combine_kernel<BF16, D, kRowWarp, KEYS>;
   return cudaLaunchKernelEx(&cfg, combine, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool Q8>
 int launch_cap(const Params& p, int cap, int ctas, cudaStream_t st) {
-  if (cap == kNoCap) return launch<BF16, D, kNoCap>(p, ctas, st);
-  return cap == kCapPlain ? launch<BF16, D, kCapPlain>(p, ctas, st) : launch<BF16, D, kCapSeries>(p, ctas, st);
+  if (cap == kNoCap) return launch<BF16, D, kNoCap, Q8>(p, ctas, st);
+  return cap == kCapPlain ? launch<BF16, D, kCapPlain, Q8>(p, ctas, st) : launch<BF16, D, kCapSeries, Q8>(p, ctas, st);
+}
+template <bool Q8>
+int launch_type(const Params& p, bool bf16, int dim, int cap, int ctas, cudaStream_t st) {
+  if (bf16) return dim == 64 ? launch_cap<true, 64, Q8>(p, cap, ctas, st) : launch_cap<true, 128, Q8>(p, cap, ctas, st);
+  return dim == 64 ? launch_cap<false, 64, Q8>(p, cap, ctas, st) : launch_cap<false, 128, Q8>(p, cap, ctas, st);
 }
 
 }  // namespace
@@ -935,13 +950,14 @@ int64_t most_rows(const B200kPagedAttentionArgs* a) {
   const int64_t q = a->max_q_len > 0 ? std::min<int64_t>(a->max_q_len, a->tokens) : a->tokens;
   return q * (a->heads / a->kv_heads);
 }
-int64_t mid_steps(const B200kPagedAttentionArgs* a) {
-  const int64_t steps = kMidSteps * 128 / a->head_dim;
+int64_t mid_steps(const B200kPagedAttentionArgs* a, bool q8) {
+  const int step = q8 ? kKeys8 : kKeys;
+  const int64_t steps = kMidSteps * 128 / a->head_dim * kKeys / step;
   const int64_t keys = std::min<int64_t>(a->table_cols * a->page_size, 0x3fffffff);
-  const bool reach = a->seqs <= kMidSeqs && a->seqs * a->kv_heads * (keys / kKeys + 1) >= steps;
+  const bool reach = a->seqs <= kMidSeqs && a->seqs * a->kv_heads * (keys / step + 1) >= steps;
   return most_rows(a) > kRows && reach ? steps : 0;
 }
-bool may_be_long(const B200kPagedAttentionArgs* a) { return most_rows(a) > kLongRows || mid_steps(a) > 0; }
+bool may_be_long(const B200kPagedAttentionArgs* a, bool q8) { return most_rows(a) > kLongRows || mid_steps(a, q8) > 0; }
 
 // Entries of the tile kernel's list: 256-row blocks of sequences that share the
 // tokens out among them.
@@ -950,7 +966,7 @@ int64_t max_entries(const B200kPagedAttentionArgs* a) {
 }
 
 // Where each part of the workspace begins; returns its size.
-int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p) {
+int64_t place(const B200kPagedAttentionArgs* a, bool q8, int sms, uint8_t* ws, Params* p) {
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     uint8_t* r = ws + at;
@@ -962,7 +978,7 @@ int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p)
   uint8_t* part_ml = take(slots * 8);
   uint8_t* prefix = take((a->seqs + 2) * 8);
   uint8_t *steps = ws, *entries = ws, *tile_o = ws, *tile_ml = ws, *joins = ws;
-  if (may_be_long(a)) {
+  if (may_be_long(a, q8)) {
     const int64_t n = max_entries(a) + 1;
     steps = take((n + 4) * 8);
     entries = take(n * 8);
@@ -983,9 +999,7 @@ int64_t place(const B200kPagedAttentionArgs* a, int sms, uint8_t* ws, Params* p)
   return at;
 }
 
-}  // namespace
-
-extern "C" int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* a, int64_t* bytes) {
+int workspace(const B200kPagedAttentionArgs* a, bool q8, int64_t* bytes) {
   const int rc = check_shape(a);
   if (rc != B200K_OK) return rc;
   if (!bytes) return B200K_ERR_ARG;
@@ -993,11 +1007,12 @@ extern "C" int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* a,
   if (a->tokens == 0 || a->heads == 0) return B200K_OK;
   const int sms = device_sm_count();
   if (sms <= 0) return B200K_ERR_DEVICE;
-  *bytes = place(a, sms, nullptr, nullptr);
+  *bytes = place(a, q8, sms, nullptr, nullptr);
   return B200K_OK;
 }
 
-extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* stream_) {
+// `q8` (NULL: 16-bit caches): the scales.
+int attend(const B200kPagedAttentionArgs* a, const B200kPagedAttentionQuantArgs* q8, void* stream_) {
   const int rc = check_shape(a);
   if (rc != B200K_OK) return rc;
   if (a->tokens == 0 || a->heads == 0) return B200K_OK;
@@ -1010,7 +1025,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   for (int d = 0; d < 2; ++d)
     if (a->q_strides[d] < 0 || a->q_strides[d] % 8) return B200K_ERR_ALIGN;
   for (int d = 0; d < 3; ++d)
-    if (a->cache_strides[d] < 0 || a->cache_strides[d] % 8) return B200K_ERR_ALIGN;
+    if (a->cache_strides[d] < 0 || a->cache_strides[d] % (q8 ? 16 : 8)) return B200K_ERR_ALIGN;
   const int sms = device_sm_count();
   if (sms <= 0) return B200K_ERR_DEVICE;
   cudaStream_t st = static_cast<cudaStream_t>(stream_);
@@ -1020,7 +1035,8 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
     return cudaMemsetAsync(a->out, 0, n, st) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
   }
   if (!a->k_cache || !a->v_cache || !a->page_table || !a->q_start || !a->kv_len) return B200K_ERR_ARG;
-  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < place(a, sms, nullptr, nullptr)) return B200K_ERR_ARG;
+  if (q8 && (!q8->k_scale || !q8->v_scale)) return B200K_ERR_ARG;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < place(a, q8 != nullptr, sms, nullptr, nullptr)) return B200K_ERR_ARG;
   Params p;
   std::memset(&p, 0, sizeof(p));
   p.T = static_cast<int32_t>(a->tokens);
@@ -1033,10 +1049,10 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.table_cols = static_cast<int32_t>(a->table_cols);
   p.capacity = static_cast<int32_t>(keys);
   p.window = static_cast<int32_t>(std::min<int64_t>(a->window, 0x3fffffff));
-  p.tile_ctas = may_be_long(a) ? sms : 0;
+  p.tile_ctas = may_be_long(a, q8 != nullptr) ? sms : 0;
   p.max_entries = static_cast<int32_t>(max_entries(a));
   p.long_rows = p.tile_ctas > 0 ? kLongRows : 0x7fffffff;
-  p.mid_steps = mid_steps(a);
+  p.mid_steps = mid_steps(a, q8 != nullptr);
   p.test_flags = a->test_flags;
   p.div_page = make_fastdiv(static_cast<uint32_t>(p.page_size));
   p.div_g = make_fastdiv(static_cast<uint32_t>(p.G));
@@ -1049,6 +1065,15 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.c_page = a->cache_strides[0];
   p.c_slot = a->cache_strides[1];
   p.c_head = a->cache_strides[2];
+  if (q8) {
+    p.k8 = static_cast<const uint8_t*>(a->k_cache);
+    p.v8 = static_cast<const uint8_t*>(a->v_cache);
+    p.ks = q8->k_scale;
+    p.vs = q8->v_scale;
+    p.s_page = q8->scale_strides[0];
+    p.s_slot = q8->scale_strides[1];
+    p.s_head = q8->scale_strides[2];
+  }
   p.out = static_cast<uint16_t*>(a->out);
   p.table = a->page_table;
   p.q_start = a->q_start;
@@ -1061,7 +1086,7 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   if (!std::isfinite(p.mul) || !std::isfinite(p.lin)) return B200K_ERR_ARG;  // a cap too small for its scale
   const int ctas = sms * kCtasPerSm;
   p.workers = ctas * kWarps;
-  place(a, sms, static_cast<uint8_t*>(a->workspace), &p);
+  place(a, q8 != nullptr, sms, static_cast<uint8_t*>(a->workspace), &p);
   p.status = a->status;
   p.timeout_ns = a->timeout_ns > 0 ? a->timeout_ns : 2000000000ll;
   // The combine covers this many tokens of a sequence side by side and the
@@ -1073,7 +1098,20 @@ extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* str
   p.combine_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 0x1fffffff / per_token)));
   const int64_t items = per_token * p.combine_rows;
   p.join_mode = items <= 4ll * sms ? kRowCta : items <= 16ll * sms ? kRowMixed : kRowWarp;
-  if (a->dtype == B200K_BF16)
-    return a->head_dim == 64 ? launch_cap<true, 64>(p, cap, ctas, st) : launch_cap<true, 128>(p, cap, ctas, st);
-  return a->head_dim == 64 ? launch_cap<false, 64>(p, cap, ctas, st) : launch_cap<false, 128>(p, cap, ctas, st);
+  const bool bf16 = a->dtype == B200K_BF16;
+  const int dim = static_cast<int>(a->head_dim);
+  return q8 ? launch_type<true>(p, bf16, dim, cap, ctas, st) : launch_type<false>(p, bf16, dim, cap, ctas, st);
+}
+
+}  // namespace
+
+extern "C" int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* a, int64_t* bytes) {
+  return workspace(a, false, bytes);
+}
+extern "C" int b200k_paged_attention(const B200kPagedAttentionArgs* a, void* stream_) { return attend(a, nullptr, stream_); }
+extern "C" int b200k_paged_attention_quant_workspace(const B200kPagedAttentionQuantArgs* a, int64_t* bytes) {
+  return workspace(a ? &a->base : nullptr, true, bytes);
+}
+extern "C" int b200k_paged_attention_quant(const B200kPagedAttentionQuantArgs* a, void* stream_) {
+  return a ? attend(&a->base, a, stream_) : B200K_ERR_ARG;
 }

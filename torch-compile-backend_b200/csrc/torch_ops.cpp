@@ -737,54 +737,66 @@ at::Tensor scaled_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor&
 // A dim's stride, 0 where it has one element (or none) and no step is taken.
 int64_t step_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
-void check_caches(const char* what, const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc) {
+// `type`: the caches', q's own or e4m3.
+void check_caches(const char* what, const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, at::ScalarType type) {
   TORCH_CHECK(kc.dim() == 4 && kc.sizes() == vc.sizes(), "b200::", what,
               ": k_cache and v_cache must be [pages, page size, kv heads, head dim] of one shape, got ", kc.sizes(), " and ",
               vc.sizes());
   for (int64_t d = 0; d < 4; ++d)
     TORCH_CHECK(step_of(kc, d) == step_of(vc, d), "b200::", what, ": k_cache and v_cache must have the same strides, got ",
                 kc.strides(), " and ", vc.strides());
-  TORCH_CHECK(kc.scalar_type() == q.scalar_type() && vc.scalar_type() == q.scalar_type(), "b200::", what,
-              ": the caches must have q's dtype");
+  TORCH_CHECK(kc.scalar_type() == type && vc.scalar_type() == type, "b200::", what, ": the caches must ",
+              type == q.scalar_type() ? "have q's dtype" : "be float8_e4m3fn");
   TORCH_CHECK(kc.device() == q.device() && vc.device() == q.device(), "b200::", what, ": the caches must be on q's device");
   TORCH_CHECK(kc.size(3) == q.size(2) && (kc.size(3) <= 1 || kc.stride(3) == 1 || kc.numel() == 0), "b200::", what,
               ": the caches' last dim must be head_dim with unit stride");
 }
 
-at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
-                       const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots, at::Tensor k_cache,
-                       at::Tensor v_cache) {
-  const char* what = "rope_append";
-  TORCH_CHECK(q.is_cuda(), "b200::rope_append: q must be a CUDA tensor");
+// The scales of e4m3 caches: one for each row, the same strides for both.
+void check_scales(const char* what, const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vs) {
+  TORCH_CHECK(ks.dim() == 3 && ks.sizes() == vs.sizes() && ks.sizes() == kc.sizes().slice(0, 3), "b200::", what,
+              ": k_scale and v_scale must be [pages, page size, kv heads] as the caches, got ", ks.sizes(), " and ", vs.sizes(),
+              " for ", kc.sizes());
+  for (int64_t d = 0; d < 3; ++d)
+    TORCH_CHECK(step_of(ks, d) == step_of(vs, d), "b200::", what, ": k_scale and v_scale must have the same strides, got ",
+                ks.strides(), " and ", vs.strides());
+  TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat, "b200::", what, ": the scales must be float32");
+  TORCH_CHECK(ks.device() == kc.device() && vs.device() == kc.device(), "b200::", what, ": the scales must be on q's device");
+}
+
+// What both appends check and hand over; `out` is q's rotation.
+B200kRopeAppendArgs append_args(const char* what, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                const at::Tensor& cos, const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots,
+                                const at::Tensor& k_cache, const at::Tensor& v_cache, at::ScalarType cache_type, at::Tensor& out) {
+  TORCH_CHECK(q.is_cuda(), "b200::", what, ": q must be a CUDA tensor");
   TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
-              "b200::rope_append: q [tokens, heads, dim], k and v [tokens, kv heads, dim], got ", q.sizes(), ", ", k.sizes(),
+              "b200::", what, ": q [tokens, heads, dim], k and v [tokens, kv heads, dim], got ", q.sizes(), ", ", k.sizes(),
               ", ", v.sizes());
   TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
-                  v.device() == q.device(), "b200::rope_append: q, k and v differ in dtype or device");
+                  v.device() == q.device(), "b200::", what, ": q, k and v differ in dtype or device");
   for (const at::Tensor* t : {&q, &k, &v})
-    TORCH_CHECK(t->stride(2) == 1 || t->numel() == 0 || t->size(2) == 1, "b200::rope_append: q, k, v need a unit last-dim stride");
-  check_caches(what, q, k_cache, v_cache);
-  TORCH_CHECK(k_cache.size(2) == k.size(1), "b200::rope_append: the caches have ", k_cache.size(2), " heads, k has ", k.size(1));
+    TORCH_CHECK(t->stride(2) == 1 || t->numel() == 0 || t->size(2) == 1, "b200::", what, ": q, k, v need a unit last-dim stride");
+  check_caches(what, q, k_cache, v_cache, cache_type);
+  TORCH_CHECK(k_cache.size(2) == k.size(1), "b200::", what, ": the caches have ", k_cache.size(2), " heads, k has ", k.size(1));
   TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && step_of(cos, 0) == step_of(sin, 0) &&
                   cos.scalar_type() == sin.scalar_type() && (cos.size(1) <= 1 || (cos.stride(1) == 1 && sin.stride(1) == 1)) &&
                   2 * cos.size(1) <= q.size(2),
-              "b200::rope_append: cos and sin must be [rows, rotary dim / 2] alike, at most head_dim / 2 columns of unit "
+              "b200::", what, ": cos and sin must be [rows, rotary dim / 2] alike, at most head_dim / 2 columns of unit "
               "stride, got ", cos.sizes(), " and ", sin.sizes());
   TORCH_CHECK(cos.scalar_type() == at::kFloat || cos.scalar_type() == q.scalar_type(),
-              "b200::rope_append: cos and sin must be float32 or q's dtype");
+              "b200::", what, ": cos and sin must be float32 or q's dtype");
   TORCH_CHECK(positions.dim() == 1 && slots.dim() == 1 && positions.size(0) == q.size(0) && slots.size(0) == q.size(0),
-              "b200::rope_append: positions and slots must be [", q.size(0), "]");
+              "b200::", what, ": positions and slots must be [", q.size(0), "]");
   for (const at::Tensor* t : {&positions, &slots})
     TORCH_CHECK((t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->is_contiguous(),
-                "b200::rope_append: positions and slots must be contiguous int32 or int64");
+                "b200::", what, ": positions and slots must be contiguous int32 or int64");
   for (const at::Tensor* t : {&cos, &sin, &positions, &slots})
-    TORCH_CHECK(t->device() == q.device(), "b200::rope_append: every tensor must be on q's device");
+    TORCH_CHECK(t->device() == q.device(), "b200::", what, ": every tensor must be on q's device");
   for (int64_t d = 0; d < 4; ++d)  // several elements in one place
-    TORCH_CHECK(k_cache.size(d) <= 1 || k_cache.stride(d) != 0, "b200::rope_append: the caches must not be expanded");
+    TORCH_CHECK(k_cache.size(d) <= 1 || k_cache.stride(d) != 0, "b200::", what, ": the caches must not be expanded");
   TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(),
-              "b200::rope_append: k_cache and v_cache are the same memory");
-  c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options());
+              "b200::", what, ": k_cache and v_cache are the same memory");
+  out = at::empty(q.sizes(), q.options());
   B200kRopeAppendArgs a;
   std::memset(&a, 0, sizeof(a));
   a.tokens = q.size(0);
@@ -816,36 +828,70 @@ at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   a.table_dtype = to_dt(cos.scalar_type());
   a.positions_dtype = to_dt(positions.scalar_type());
   a.slots_dtype = to_dt(slots.scalar_type());
-  void* st = stream_of(q);
   a.status = status_word(q.device().index()).data_ptr<int32_t>();
-  check(b200k_rope_append(&a, st), what);
-  for (at::Tensor* t : {&k_cache, &v_cache})
+  return a;
+}
+void written(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+at::Tensor rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                       const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots, at::Tensor k_cache,
+                       at::Tensor v_cache) {
+  const char* what = "rope_append";
+  c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
+  at::Tensor out;
+  const B200kRopeAppendArgs a = append_args(what, q, k, v, cos, sin, positions, slots, k_cache, v_cache, q.scalar_type(), out);
+  check(b200k_rope_append(&a, stream_of(q)), what);
+  written({&k_cache, &v_cache});
+  return out;
+}
+at::Tensor rope_append_quant(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                             const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots, at::Tensor k_cache,
+                             at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale) {
+  const char* what = "rope_append_quant";
+  c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
+  B200kRopeAppendQuantArgs a;
+  std::memset(&a, 0, sizeof(a));
+  at::Tensor out;
+  a.base = append_args(what, q, k, v, cos, sin, positions, slots, k_cache, v_cache, at::kFloat8_e4m3fn, out);
+  check_scales(what, k_cache, k_scale, v_scale);
+  for (int64_t d = 0; d < 3; ++d) {  // several scales in one place
+    TORCH_CHECK(k_scale.size(d) <= 1 || k_scale.stride(d) != 0, "b200::", what, ": the scales must not be expanded");
+    a.scale_strides[d] = step_of(k_scale, d);
+  }
+  TORCH_CHECK(k_scale.numel() == 0 || k_scale.data_ptr() != v_scale.data_ptr(), "b200::", what,
+              ": k_scale and v_scale are the same memory");
+  a.k_scale = k_scale.data_ptr<float>();
+  a.v_scale = v_scale.data_ptr<float>();
+  check(b200k_rope_append_quant(&a, stream_of(q)), what);
+  written({&k_cache, &v_cache, &k_scale, &v_scale});
   return out;
 }
 
-at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
-                           const at::Tensor& page_table, const at::Tensor& q_start, const at::Tensor& kv_len, double scale,
-                           double softcap, int64_t window, int64_t max_q_len) {
-  const char* what = "paged_attention";
-  TORCH_CHECK(q.is_cuda(), "b200::paged_attention: q must be a CUDA tensor");
-  TORCH_CHECK(q.dim() == 3 && (q.stride(2) == 1 || q.numel() == 0), "b200::paged_attention: q must be [tokens, heads, head dim] "
+// What both attentions check and hand over.
+B200kPagedAttentionArgs attention_args(const char* what, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                       const at::Tensor& page_table, const at::Tensor& q_start, const at::Tensor& kv_len,
+                                       double scale, double softcap, int64_t window, int64_t max_q_len, at::ScalarType cache_type,
+                                       at::Tensor& out) {
+  TORCH_CHECK(q.is_cuda(), "b200::", what, ": q must be a CUDA tensor");
+  TORCH_CHECK(q.dim() == 3 && (q.stride(2) == 1 || q.numel() == 0), "b200::", what, ": q must be [tokens, heads, head dim] "
               "with unit last-dim stride, got ", q.sizes());
-  check_caches(what, q, k_cache, v_cache);
+  check_caches(what, q, k_cache, v_cache, cache_type);
   TORCH_CHECK(page_table.dim() == 2 && q_start.dim() == 1 && kv_len.dim() == 1 && q_start.size(0) == kv_len.size(0) + 1 &&
                   page_table.size(0) == kv_len.size(0),
-              "b200::paged_attention: page_table [seqs, pages], q_start [seqs + 1], kv_len [seqs], got ", page_table.sizes(),
+              "b200::", what, ": page_table [seqs, pages], q_start [seqs + 1], kv_len [seqs], got ", page_table.sizes(),
               ", ", q_start.sizes(), ", ", kv_len.sizes());
   for (const at::Tensor* t : {&page_table, &q_start, &kv_len})
     TORCH_CHECK(t->scalar_type() == at::kInt && t->device() == q.device() && (t->size(-1) <= 1 || t->stride(-1) == 1),
-                "b200::paged_attention: page_table, q_start and kv_len must be int32 on q's device with unit last-dim stride");
-  TORCH_CHECK(scale >= 0 && softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::paged_attention: scale, softcap, window and "
+                "b200::", what, ": page_table, q_start and kv_len must be int32 on q's device with unit last-dim stride");
+  TORCH_CHECK(scale >= 0 && softcap >= 0 && window >= 0 && max_q_len >= 0, "b200::", what, ": scale, softcap, window and "
               "max_q_len must not be negative");
   // (0 is the default scale, and no cap)
   TORCH_CHECK((scale == 0) == (static_cast<float>(scale) == 0) && (softcap == 0) == (static_cast<float>(softcap) == 0) &&
-                  softcap <= 1e38, "b200::paged_attention: scale ", scale, " or softcap ", softcap, " is out of float32's range");
-  c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options());
+                  softcap <= 1e38, "b200::", what, ": scale ", scale, " or softcap ", softcap, " is out of float32's range");
+  out = at::empty(q.sizes(), q.options());
   B200kPagedAttentionArgs a;
   std::memset(&a, 0, sizeof(a));
   a.tokens = q.size(0);
@@ -871,16 +917,51 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   a.scale = static_cast<float>(scale);
   a.softcap = static_cast<float>(softcap);
   a.dtype = to_dt(q.scalar_type());
-  void* st = stream_of(q);
-  // Parts of cut units: the caching allocator's, so each call and each
-  // captured graph has its own.
-  int64_t bytes = 0;
-  check(b200k_paged_attention_workspace(&a, &bytes), what);
+  a.status = status_word(q.device().index()).data_ptr<int32_t>();
+  return a;
+}
+// Parts of cut units: the caching allocator's, so each call and each captured
+// graph has its own.
+at::Tensor attention_workspace(B200kPagedAttentionArgs& a, const at::Tensor& q, int64_t bytes) {
   const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
   a.workspace = ws.data_ptr();
   a.workspace_bytes = bytes;
-  a.status = status_word(q.device().index()).data_ptr<int32_t>();
-  check(b200k_paged_attention(&a, st), what);
+  return ws;
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& page_table, const at::Tensor& q_start, const at::Tensor& kv_len, double scale,
+                           double softcap, int64_t window, int64_t max_q_len) {
+  const char* what = "paged_attention";
+  c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
+  at::Tensor out;
+  B200kPagedAttentionArgs a = attention_args(what, q, k_cache, v_cache, page_table, q_start, kv_len, scale, softcap, window,
+                                             max_q_len, q.scalar_type(), out);
+  int64_t bytes = 0;
+  check(b200k_paged_attention_workspace(&a, &bytes), what);
+  const at::Tensor ws = attention_workspace(a, q, bytes);
+  check(b200k_paged_attention(&a, stream_of(q)), what);
+  return out;
+}
+at::Tensor paged_attention_quant(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                 const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& page_table,
+                                 const at::Tensor& q_start, const at::Tensor& kv_len, double scale, double softcap, int64_t window,
+                                 int64_t max_q_len) {
+  const char* what = "paged_attention_quant";
+  c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
+  B200kPagedAttentionQuantArgs a;
+  std::memset(&a, 0, sizeof(a));
+  at::Tensor out;
+  a.base = attention_args(what, q, k_cache, v_cache, page_table, q_start, kv_len, scale, softcap, window, max_q_len,
+                          at::kFloat8_e4m3fn, out);
+  check_scales(what, k_cache, k_scale, v_scale);
+  a.k_scale = k_scale.data_ptr<float>();
+  a.v_scale = v_scale.data_ptr<float>();
+  for (int64_t d = 0; d < 3; ++d) a.scale_strides[d] = step_of(k_scale, d);
+  int64_t bytes = 0;
+  check(b200k_paged_attention_quant_workspace(&a, &bytes), what);
+  const at::Tensor ws = attention_workspace(a.base, q, bytes);
+  check(b200k_paged_attention_quant(&a, stream_of(q)), what);
   return out;
 }
 
@@ -930,6 +1011,21 @@ at::Tensor paged_attention_autograd(const at::Tensor& q, const at::Tensor& k_cac
                         softcap, window, max_q_len);
 }
 
+at::Tensor rope_append_quant_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                                      const at::Tensor& sin, const at::Tensor& positions, const at::Tensor& slots,
+                                      at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale) {
+  static const auto op = find_op<decltype(rope_append_quant)>("b200::rope_append_quant");
+  return below_autograd(op, "rope_append_quant", {&q, &k, &v, &cos, &sin, &k_cache, &v_cache, &k_scale, &v_scale}, q, k, v, cos, sin,
+                        positions, slots, k_cache, v_cache, k_scale, v_scale);
+}
+at::Tensor paged_attention_quant_autograd(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                          const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& page_table,
+                                          const at::Tensor& q_start, const at::Tensor& kv_len, double scale, double softcap,
+                                          int64_t window, int64_t max_q_len) {
+  static const auto op = find_op<decltype(paged_attention_quant)>("b200::paged_attention_quant");
+  return below_autograd(op, "paged_attention_quant", {&q, &k_cache, &v_cache, &k_scale, &v_scale}, q, k_cache, v_cache, k_scale,
+                        v_scale, page_table, q_start, kv_len, scale, softcap, window, max_q_len);
+}
 std::tuple<at::Tensor, at::Tensor> quant_groups_autograd(const at::Tensor& x, bool swiglu) {
   static const auto op = find_op<decltype(quant_groups)>("b200::quant_groups");
   return below_autograd(op, "quant_groups", {&x}, x, swiglu);
@@ -969,6 +1065,12 @@ TORCH_LIBRARY(b200, m) {
   m.def(
       "paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor q_start, Tensor kv_len, "
       "float scale=0.0, float softcap=0.0, int window=0, int max_q_len=0) -> Tensor");
+  m.def(
+      "rope_append_quant(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor positions, Tensor slots, "
+      "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale) -> Tensor");
+  m.def(
+      "paged_attention_quant(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor page_table, "
+      "Tensor q_start, Tensor kv_len, float scale=0.0, float softcap=0.0, int window=0, int max_q_len=0) -> Tensor");
   m.def("quant_groups(Tensor x, bool swiglu=False) -> (Tensor, Tensor)");
   m.def("scaled_mm(Tensor a, Tensor b, Tensor a_scale, Tensor b_scale, ScalarType out_dtype) -> Tensor");
   m.def("gemm_status(int device, bool reset) -> int", &gemm_status);
@@ -991,6 +1093,8 @@ TORCH_LIBRARY_IMPL(b200, CUDA, m) {
   m.impl("add_rms_norm_quant", &add_rms_norm_quant);
   m.impl("rope_append", &rope_append);
   m.impl("paged_attention", &paged_attention);
+  m.impl("rope_append_quant", &rope_append_quant);
+  m.impl("paged_attention_quant", &paged_attention_quant);
   m.impl("quant_groups", &quant_groups);
   m.impl("scaled_mm", &scaled_mm);
 }
@@ -1000,6 +1104,8 @@ TORCH_LIBRARY_IMPL(b200, Autograd, m) {
   m.impl("add_rms_norm_quant", &add_rms_norm_quant_autograd);
   m.impl("rope_append", &rope_append_autograd);
   m.impl("paged_attention", &paged_attention_autograd);
+  m.impl("rope_append_quant", &rope_append_quant_autograd);
+  m.impl("paged_attention_quant", &paged_attention_quant_autograd);
   m.impl("quant_groups", &quant_groups_autograd);
   m.impl("scaled_mm", &scaled_mm_autograd);
 }
