@@ -105,7 +105,8 @@ class StatusChecked:
 # Ops whose kernels report through the device's status word: waits that run
 # out, indexes out of range.
 _REPORTING = (torch.ops.b200.gemm_epilogue.default, torch.ops.b200.rope_append.default,
-              torch.ops.b200.paged_attention.default)
+              torch.ops.b200.paged_attention.default, torch.ops.b200.rope_append_quant.default,
+              torch.ops.b200.paged_attention_quant.default, torch.ops.b200.scaled_mm.default)
 
 
 def _gemm_device(gm: fx.GraphModule, example_inputs) -> int | None:

@@ -2,7 +2,7 @@
 writes its inputs).
 
 AOTAutograd makes a graph functional, so ``b200::rope_append``, which writes
-its two caches, arrives as ``auto_functionalized_v2``: run as it stands, that
+its two caches (``rope_append_quant``: two caches and their scales), arrives as ``auto_functionalized_v2``: run as it stands, that
 node copies both caches, appends to the copies, and the copies are written
 back over the inputs at the end of the call -- three passes over a cache that
 may fill most of the GPU's memory, for a few appended rows.  This pass puts
@@ -25,25 +25,34 @@ from compiler import graph_replay, runtime
 
 runtime.load()
 
-_APPEND = torch.ops.b200.rope_append.default
 _FUNCTIONAL = torch.ops.higher_order.auto_functionalized_v2
 _PLAIN = ("q", "k", "v", "cos", "sin", "positions", "slots")
-_CACHES = ("k_cache", "v_cache")
-_ATTEND = torch.ops.b200.paged_attention.default
+# What each append writes, its arguments behind _PLAIN.
+_APPENDS = {torch.ops.b200.rope_append.default: ("k_cache", "v_cache"),
+            torch.ops.b200.rope_append_quant.default: ("k_cache", "v_cache", "k_scale", "v_scale")}
+# Arguments of each attention that are caches, behind q.
+_ATTENDS = {torch.ops.b200.paged_attention.default: 2, torch.ops.b200.paged_attention_quant.default: 4}
 # Ops that take a cache and return nothing that aliases it.
-_READERS = (_ATTEND, _APPEND)
+_READERS = (*_ATTENDS, *_APPENDS)
 _VIEWS = graph_replay._NO_LAUNCH | {operator.getitem}
 
 
+def _is_functional(node: fx.Node) -> bool:
+    return (node.op == "call_function" and node.target == _FUNCTIONAL and len(node.args) > 0
+            and node.args[0] in _APPENDS)
+
+
 def _caches_of(node: fx.Node):
-    """The two base nodes of a functional append on whole tensors, else None."""
-    if not (node.op == "call_function" and node.target == _FUNCTIONAL and node.args[:1] == (_APPEND,)):
+    """The base nodes of a functional append on whole tensors, one for each
+    tensor that it writes, else None."""
+    if not _is_functional(node):
         return None
-    kw = node.kwargs
-    if set(kw) != {*_PLAIN, "_all_bases", *(f"_{c}_base_index" for c in _CACHES)}:
+    kw, caches = node.kwargs, _APPENDS[node.args[0]]
+    if set(kw) != {*_PLAIN, "_all_bases", *(f"_{c}_base_index" for c in caches)}:
         return None  # a cache is a view of its base: left functional
-    where = [kw[f"_{c}_base_index"] for c in _CACHES]
-    if not all(isinstance(i, int) for i in where) or where[0] == where[1] or len(kw["_all_bases"]) != 2:
+    where = [kw[f"_{c}_base_index"] for c in caches]
+    if (not all(isinstance(i, int) for i in where) or len(set(where)) != len(caches)
+            or len(kw["_all_bases"]) != len(caches)):
         return None
     bases = [kw["_all_bases"][i] for i in where]
     if not all(isinstance(b, fx.Node) and b.op == "placeholder" for b in bases):
@@ -66,7 +75,7 @@ def inplace_append(gm: fx.GraphModule) -> fx.GraphModule:
         if any(u.target is not operator.getitem for u in node.users):
             continue
         with gm.graph.inserting_before(node):
-            new = gm.graph.call_function(_APPEND, tuple(node.kwargs[n] for n in _PLAIN) + tuple(bases))
+            new = gm.graph.call_function(node.args[0], tuple(node.kwargs[n] for n in _PLAIN) + tuple(bases))
         order[new] = order[node]
         # results: the op's, then the bases' new states in the order of _all_bases
         results = [new] + list(node.kwargs["_all_bases"])
@@ -81,10 +90,11 @@ def inplace_append(gm: fx.GraphModule) -> fx.GraphModule:
     if changed:
         gm.graph.lint()
         gm.recompile()
-    left = sum(n.op == "call_function" and n.target == _FUNCTIONAL and n.args[:1] == (_APPEND,) for n in gm.graph.nodes)
-    if left:
-        warnings.warn(f"{left} b200::rope_append of a compiled graph copy the tensors that hold their caches, whole, at "
-                      "every call: pass each cache as a tensor of its own, and attend over it behind the append")
+    for op in _APPENDS:
+        left = sum(_is_functional(n) and n.args[0] == op for n in gm.graph.nodes)
+        if left:
+            warnings.warn(f"{left} {op.name()} of a compiled graph copy the tensors that hold their caches, whole, at "
+                          "every call: pass each cache as a tensor of its own, and attend over it behind the append")
     return gm
 
 
@@ -97,8 +107,8 @@ def appended_inputs(gm: fx.GraphModule) -> tuple:
     order = {n: i for i, n in enumerate(gm.graph.nodes)}
     found = set()
     for node in gm.graph.nodes:
-        if node.op == "call_function" and node.target == _APPEND:
-            for b in node.args[7:9]:
+        if node.op == "call_function" and node.target in _APPENDS:
+            for b in node.args[len(_PLAIN):]:
                 if b not in inputs or any(order[u] < order[node] for u in b.users):
                     return None
                 found.add(inputs.index(b))
@@ -111,8 +121,11 @@ def attended_inputs(gm: fx.GraphModule) -> tuple:
     def cache_alone(n):
         return bool(n.users) and all(
             u.op == "call_function" and not u.kwargs
-            and (u.target == _ATTEND and n in u.args[1:3] and n not in (u.args[0], *u.args[3:])
-                 or u.target in _VIEWS and cache_alone(u))
+            and (u.target in _ATTENDS and reads(u, n) or u.target in _VIEWS and cache_alone(u))
             for u in n.users)
+
+    def reads(u, n):
+        end = 1 + _ATTENDS[u.target]
+        return n in u.args[1:end] and n not in (u.args[0], *u.args[end:])
 
     return tuple(i for i, n in enumerate(n for n in gm.graph.nodes if n.op == "placeholder") if cache_alone(n))
