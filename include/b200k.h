@@ -649,9 +649,9 @@ int b200k_quant_groups(const B200kQuantGroupsArgs* args, void* stream);
  * tensor cores, the blocks in fp32, and the result is rounded once.  The same
  * shapes give the same bits.  NaN codes and scales reach every product that
  * they enter.
- * tile: 0 the library's choice, 1 256 x 256 (a CTA pair), 2 128 x 128, 3 128 x
- * 64; split: CTAs of a cluster that share the blocks of k of a tile of kind 2
- * or 3, 0 the library's choice, at most 8.  status, when not NULL, receives
+ * tile: 0 the library's choice, 1 tiles of 256 x 256, or 16, 32, 64 or 128: of
+ * so many rows x 128 columns; split: CTAs of a cluster that share the blocks of k
+ * of such a tile, 0 the library's choice, at most 8.  status, when not NULL, receives
  * B200K_ERR_TIMEOUT if a device-side wait runs out (timeout_ns, 0 = 2 s).
  */
 typedef struct {

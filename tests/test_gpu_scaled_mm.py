@@ -50,7 +50,7 @@ def test_against_the_formula(m, k, n, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (100, 1152, 200), (300, 2000, 520), (513, 128, 264), (600, 896, 1028)])
-@pytest.mark.parametrize("tile,split", [(1, 0), (2, 1), (2, 3), (2, 8), (3, 1), (3, 2), (3, 4), (3, 7)])
+@pytest.mark.parametrize("tile,split", [(1, 0), (16, 1), (16, 8), (32, 1), (32, 3), (64, 1), (64, 2), (64, 7), (128, 1), (128, 4)])
 def test_every_tile(tile, split, m, k, n, dtype):
     a, b, sa, sb = make(m, k, n)
     out = torch.full((m + 2, n), 7.0, device="cuda", dtype=dtype)
@@ -80,7 +80,7 @@ def test_strided_operands():
     check(torch.ops.b200.scaled_mm(a, b, sa, sb, torch.bfloat16), a, b, sa, sb)
 
 
-@pytest.mark.parametrize("m,tile,split", [(5, 3, 4), (200, 2, 2), (300, 1, 0)])
+@pytest.mark.parametrize("m,tile,split", [(5, 16, 4), (200, 128, 2), (300, 1, 0), (40, 64, 1)])
 def test_nan_and_infinity(m, tile, split):
     """A NaN code and a NaN scale reach the rows and columns that they enter, and no others."""
     a, b, sa, sb = make(m, 768, 320)
@@ -142,7 +142,7 @@ def test_two_streams():
         check(out, *args)
 
 
-@pytest.mark.parametrize("tile,split,m", [(1, 0, 600), (2, 1, 200), (3, 4, 30)])
+@pytest.mark.parametrize("tile,split,m", [(1, 0, 600), (128, 1, 200), (32, 4, 30), (16, 8, 5)])
 def test_a_wait_that_runs_out_is_reported(tile, split, m):
     """The first block is never signalled: the kernel reports, drains and
     returns, and the next call is right."""

@@ -4,26 +4,30 @@
 //   out[m, n] = sum_g sa[m, g] sb[g, n / 128] sum_{k in block g} a[m, k] b[k, n]
 //
 // No reference counterpart (its GEMM is 16-bit).  The inner sum is a 128-deep
-// tcgen05 product (kind::f8f6f4, fp32 accumulators in tensor memory); the
+// tcgen05 product (kind::f8f6f4, fp32 accumulators in tensor memory).  The
 // scales differ from block to block, so it cannot run on over k: each block's
-// product goes to one of two tensor-memory buffers, and while the tensor pipe
-// fills the other one the epilogue warps read it and add it, times its scale,
-// to fp32 sums in registers.  A thread has one row and up to 128 columns of
-// one scale block, so a block costs it one scale and 64 packed FMAs.
+// product goes to one of several tensor-memory buffers, and while the tensor
+// pipe fills the next ones the epilogue warps read it and add it, times its
+// scale, to fp32 sums in registers.
 //
 // One CTA per SM:
 //   warp 0      TMA producer (128-byte swizzled tiles of 128 k);
 //   warp 1      MMA issuer;
-//   warp 2      owns tensor memory;
-//   warps 4..   epilogue: four for every 128 (or 64) columns.
-// Kinds of tile:
-//   pair    256 x 256 on a cluster of two CTAs (cta_group::2), each with its
-//           own 128 rows: large products, a third less operand traffic than
-//           128 x 256;
-//   single  128 x 128 or 128 x 64, on a cluster of `split` CTAs that share
-//           the blocks of k out among them and add their sums over distributed
-//           shared memory in the order of the ranks: few rows, where the
-//           weights' bytes are the bound and every SM has to fetch some.
+//   warps 2, 3  bring the scales of kScaleBlocks blocks at a time to shared
+//               memory, transposed (warp 2 owns tensor memory);
+//   warps 4..   epilogue.
+// Two kinds of tile:
+//   wide        256 rows of a x 256 columns of b on a pair of CTAs (cta_group::2),
+//               each with 128 of the rows.  A thread has one row and 128 columns,
+//               of one scale block, so a block costs it one scale and 64 packed
+//               FMAs.  (128 x 256 on one CTA: the operands' way from L2 to shared
+//               memory, 12 TB/s, held it at 2050 TFLOP/s.)
+//   turned      128 columns of b as the product's rows x 16 to 128 rows of a as
+//               its columns, on a cluster of `split` CTAs that share the blocks
+//               of k out among them and add their sums over distributed shared
+//               memory in the order of the ranks.  For few rows, where b's
+//               bytes are the bound: every SM fetches some of them, and the
+//               tensor-memory lanes are full whatever the number of rows.
 #include "gemm_kernel.cuh"
 
 namespace b200k {
@@ -42,17 +46,24 @@ namespace {
 using namespace gemm;
 
 constexpr int kBlk = 128;  // k of a block, one swizzle row of bytes
-// Registers of a thread of 256-wide tiles: launched with 168, 128 control
-// threads leave theirs to 256 epilogue threads (128 sums each).
-constexpr int kCtlRegs = 40, kEpiRegs = 232;
+// Registers of a thread of wide tiles: launched with 168, 128 control threads
+// leave theirs to 256 epilogue threads (128 sums each).
+constexpr int kCtlRegs = 56, kEpiRegs = 224;
+// Blocks of k whose scales are fetched together, a 32-byte sector of a row:
+// eight neighbouring lanes read it.  (A load by each epilogue thread touched
+// 32 lines and kept all eight epilogue warps 1500 clocks for four blocks.)
+constexpr int kScaleBlocks = 8;
+constexpr int kScaleRow = 132;                                        // floats: 128 rows of a block, turned banks
+constexpr uint32_t kScaleBytes = kScaleBlocks * (kScaleRow + 4) * 4;  // with two scales of b a block
+constexpr uint32_t kStgBox = 32 * 128;    // 32 rows x 128 bytes of the output
+constexpr int kStgBoxes = 2;              // of an epilogue warp: its tile in 16 bits
+constexpr int kMaxSplit = 8;
 
 struct MmParams {
   int32_t M, N;
   int32_t tiles_m, tiles_n, num_tiles, k_blocks;
-  int32_t group_m;
-  int32_t split;            // CTAs that share a tile's blocks (single)
-  int32_t a_rows;           // rows of an A box (single)
-  int32_t tma_out;          // the output's rows can be stored by TMA
+  int32_t split;            // CTAs that share a tile's blocks (turned)
+  int32_t tma_out;          // the output's rows can be stored by TMA (wide)
   const float* sa;          // [M, k_blocks]
   int64_t sa_m, sa_k;
   const float* sb;          // [k_blocks, ceil(N / 128)]
@@ -64,39 +75,94 @@ struct MmParams {
   int64_t timeout_ns;
 };
 
-template <bool PAIR, int BN>
+// BN: columns of the product in tensor memory (256: wide).
+template <int BN>
 struct Cfg8 {
-  static constexpr int kGroups = BN == 256 ? 2 : 1;        // column groups, four warps each
+  static constexpr bool kWide = BN == 256;
+  static constexpr int kGroups = BN >= 128 ? 2 : 1;        // column groups, four epilogue warps each
   static constexpr int kCols = BN / kGroups;               // of an epilogue thread
+  static constexpr int kBufs = kWide ? 2 : 4;
+  static constexpr uint32_t kTmemCols = BN * kBufs;
   static constexpr int kThreads = 128 + 128 * kGroups;
-  static constexpr uint32_t kABytes = 128 * kBlk;
-  static constexpr uint32_t kBBytes = (PAIR ? BN / 2 : BN) * kBlk;
-  static constexpr uint32_t kStage = kABytes + kBBytes;
-  static constexpr int kStages = PAIR ? 6 : BN == 128 ? 6 : 8;
+  static constexpr uint32_t kRowBytes = 128 * kBlk;        // the product's 128 rows (of this CTA)
+  static constexpr uint32_t kStage = kRowBytes + (kWide ? BN / 2 : BN) * kBlk;
+  static constexpr int kStages = BN >= 128 ? (kWide ? 4 : 6) : 8;
   static constexpr uint32_t kOffStg = kStages * kStage;
-  static constexpr uint32_t kOffBar = kOffStg + 4 * kGroups * kStgBytes;
-  static constexpr uint32_t kSmem = 1024 + kOffBar + 256;
-  static constexpr int kPartStride = BN + 4;               // floats: rows of 16-byte words fall on other banks
+  static constexpr uint32_t kOffSc = kOffStg + (kWide ? 4 * kGroups * kStgBoxes * kStgBox : 0);  // two chunks of scales
+  static constexpr uint32_t kOffBar = kOffSc + 2 * kScaleBytes;
+  static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
+  static constexpr int kPartRow = 132;  // floats: 128 sums of a split tile's column
+  static_assert(kTmemCols >= 32 && kTmemCols <= 512, "tensor memory");
   static_assert(kSmem <= 232448 && kSmem > 232448 / 2, "one CTA per SM");
-  static_assert(128 * kPartStride * 4 <= kOffStg, "the sums of a split tile fit the ring");
+  static_assert(kWide || BN * kPartRow * 4 <= kOffStg, "the sums of a split tile fit the ring");
 };
 
-__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+// The four MMAs of a block (32 k each, 32 bytes apart in the swizzled rows).
+// Called by a whole warp and issued by one elected lane: in warp-uniform code the
+// descriptors stay in uniform registers (from a lane's branch the MMAs of a block
+// and its commits took 390 clocks to issue, a block's product itself 512).
+template <bool PAIR>
+__device__ __forceinline__ void umma_block(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+#define B200K_UMMA_BLOCK(GROUP)                                                                            \
+  asm volatile(                                                                                            \
+      "{\n\t.reg .pred e, no, yes;\n\t"                                                                    \
+      "elect.sync _|e, 0xffffffff;\n\t"                                                                    \
+      "setp.ne.b32 no, 0, 0;\n\t"                                                                          \
+      "setp.eq.b32 yes, 0, 0;\n\t"                                                                         \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %1, %5, %9, no;\n\t"                         \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %2, %6, %9, yes;\n\t"                        \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %3, %7, %9, yes;\n\t"                        \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %4, %8, %9, yes;\n\t}\n" ::"r"(d_tmem),      \
+      "l"(adesc), "l"(adesc + 2), "l"(adesc + 4), "l"(adesc + 6), "l"(bdesc), "l"(bdesc + 2), "l"(bdesc + 4), \
+      "l"(bdesc + 6), "r"(idesc)                                                                           \
+      : "memory")
+  if constexpr (PAIR) B200K_UMMA_BLOCK("2");
+  else B200K_UMMA_BLOCK("1");
+#undef B200K_UMMA_BLOCK
 }
-__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                             uint32_t accumulate) {
+// Arrives on a barrier (a pair: on both CTAs') when the MMAs so far have completed.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b16 both;\n\t"
+        "mov.b16 both, 3;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}\n" ::"r"(
+            smem_u32(bar))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
+        : "memory");
+}
+// Arrival at a barrier of the pair's even CTA.
+__device__ __forceinline__ void arrive_even(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(bar, 0)) : "memory");
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Ctl& c) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, c));
+}
+// 16 or 32 columns of this thread's tensor-memory row, and the wait for them,
+// which names the registers so that no use of them is scheduled before it.
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) { tmem_wait_ld_regs(r); }
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
@@ -110,109 +176,111 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
   return r;
 }
 
+// Tile t: wide ones go kGroupM tile rows down before they move on, so that
+// CTAs side by side share operands in L2; turned ones along the rows of a.
+template <bool WIDE>
 __device__ __forceinline__ void tile_at(int t, const MmParams& p, int& tm, int& tn) {
-  const int per_group = p.group_m * p.tiles_n;
-  const int g = t / per_group, first = g * p.group_m;
-  const int rows = min(p.tiles_m - first, p.group_m), r = t - g * per_group;
-  tm = first + r % rows;
-  tn = r / rows;
+  if (WIDE) {
+    const int per_group = kGroupM * p.tiles_n;
+    const int g = t / per_group, first = g * kGroupM;
+    const int rows = min(p.tiles_m - first, kGroupM), r = t - g * per_group;
+    tm = first + r % rows;
+    tn = r / rows;
+  } else {
+    tn = t / p.tiles_m;
+    tm = t - tn * p.tiles_m;
+  }
 }
 
-// Scale products of four blocks of k for one row and column block, 0 outside.
-struct Scales {
-  float s[4];
-  __device__ __forceinline__ void load(const MmParams& p, int m, int nb, int kb, int end) {
-    const float* a = p.sa + m * p.sa_m + kb * p.sa_k;
-    const float* b = p.sb + kb * p.sb_k + nb * p.sb_n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = 0.0f;
-      if (kb + i < end && m < p.M) s[i] = __ldg(a + i * p.sa_k) * __ldg(b + i * p.sb_k);
-    }
-  }
-};
-
-template <bool PAIR, int BN>
-__global__ void __launch_bounds__(Cfg8<PAIR, BN>::kThreads, 1)
+template <int BN>
+__global__ void __launch_bounds__(Cfg8<BN>::kThreads, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const __grid_constant__ CUtensorMap tmO, const __grid_constant__ MmParams p) {
-  using C = Cfg8<PAIR, BN>;
-  constexpr int S = C::kStages, COLS = C::kCols;
-  constexpr int kTileM = PAIR ? 256 : 128;
+  using C = Cfg8<BN>;
+  constexpr bool WIDE = C::kWide;
+  constexpr int S = C::kStages, COLS = C::kCols, BUFS = C::kBufs;
+  constexpr int kTileM = WIDE ? 256 : BN, kTileN = WIDE ? BN : 128;  // rows of a and columns of b of a tile
+  constexpr int kRowsM = WIDE ? 128 : BN;                            // rows of a of a CTA
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sbase = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   uint64_t* full = reinterpret_cast<uint64_t*>(sbase + C::kOffBar);
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
-  uint64_t* tempty = tfull + 2;
-  uint64_t* drain = tempty + 2;
+  uint64_t* tempty = tfull + BUFS;
+  uint64_t* sc_full = tempty + BUFS;  // [2]
+  uint64_t* sc_empty = sc_full + 2;
+  uint64_t* drain = sc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR || p.split > 1 ? cluster_rank() : 0;
-  const int cluster = PAIR ? 2 : p.split;
-  const bool leads = !PAIR || rank == 0;  // issues the MMAs
+  const int split = WIDE ? 1 : p.split, cluster = WIDE ? 2 : split;
+  const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+  const int part = WIDE ? 0 : static_cast<int>(rank);     // of the blocks of k
+  const int rows_at = WIDE ? static_cast<int>(rank) * 128 : 0;  // of a tile's rows
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < BUFS; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], (PAIR ? 8 : 4) * C::kGroups);
+      mbar_init(&tempty[a], 4 * C::kGroups * (WIDE ? 2 : 1));  // a pair's arrive at the even CTA's
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&sc_full[a], 2);
+      mbar_init(&sc_empty[a], 4 * C::kGroups);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_map(&tmA);
     prefetch_map(&tmB);
-    prefetch_map(&tmO);
+    if (WIDE) prefetch_map(&tmO);
   }
   if (warp == 2) {
-    if (PAIR) {
-      tmem_alloc_pair(tmem_slot, 2 * BN);
+    if (WIDE) {
+      tmem_alloc_pair(tmem_slot, C::kTmemCols);
       tmem_relinquish_pair();
     } else {
-      tmem_alloc(tmem_slot, 2 * BN);
+      tmem_alloc(tmem_slot, C::kTmemCols);
       tmem_relinquish();
     }
   }
   tc_fence_before();
-  if (cluster > 1) cluster_sync();
+  if (WIDE) cluster_sync();  // the other CTA's barriers are there too
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const Ctl ctl{abort_flag, p.status, static_cast<uint64_t>(p.timeout_ns)};
   const int cid = static_cast<int>(blockIdx.x) / cluster, ncl = static_cast<int>(gridDim.x) / cluster;
   // this CTA's blocks of k
-  const int kb0 = PAIR ? 0 : static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.split);
-  const int kb1 = PAIR ? p.k_blocks : static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / p.split);
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
 
   if (warp < 4) {
-    if (C::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtlRegs));
+    if (WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtlRegs));
     if (warp == 0 && lane == 0) {
       // -------------------------------------------------------------- producer
       int s = 0;
       uint32_t ph = 0;
       int64_t issued = 0;
       bool ok = true;
-      const uint32_t tx = PAIR ? 2 * C::kStage : static_cast<uint32_t>(p.a_rows) * kBlk + C::kBBytes;
       for (int t = cid; t < p.num_tiles && ok; t += ncl) {
         int tm, tn;
-        tile_at(t, p, tm, tn);
+        tile_at<WIDE>(t, p, tm, tn);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = wait_bar(&empty[s], ph ^ 1u, ctl))) break;
-          uint8_t* sa = sbase + s * C::kStage;
-          if (PAIR) {
-            const uint32_t fb = cluster_addr(&full[s], 0);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);
-            tma_load_2d_pair(sa, &tmA, fb, kb * kBlk, tm * kTileM + static_cast<int>(rank) * 128);
-            tma_load_2d_pair(sa + C::kABytes, &tmB, fb, kb * kBlk, tn * BN + static_cast<int>(rank) * (BN / 2));
+          uint8_t* rows = sbase + s * C::kStage;
+          if (WIDE) {  // both CTAs' bytes are counted on the even one's barrier
+            const uint32_t bar = cluster_addr(&full[s], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::kStage);
+            tma_load_2d_pair(rows, &tmA, bar, kb * kBlk, tm * kTileM + rows_at);
+            tma_load_2d_pair(rows + C::kRowBytes, &tmB, bar, kb * kBlk, tn * kTileN + static_cast<int>(rank) * (BN / 2));
           } else {
-            mbar_arrive_expect_tx(&full[s], tx);
-            tma_load_2d(sa, &tmA, &full[s], kb * kBlk, tm * kTileM);
-            tma_load_2d(sa + C::kABytes, &tmB, &full[s], kb * kBlk, tn * BN);
+            mbar_arrive_expect_tx(&full[s], C::kStage);
+            tma_load_2d(rows + C::kRowBytes, &tmA, &full[s], kb * kBlk, tm * kTileM);
+            tma_load_2d(rows, &tmB, &full[s], kb * kBlk, tn * kTileN);
           }
           ++issued;
           if (++s == S) {
@@ -221,229 +289,273 @@ __global__ void __launch_bounds__(Cfg8<PAIR, BN>::kThreads, 1)
           }
         }
       }
-      // every stage that was filled has been read: no load is in flight, and
-      // no commit of the leading CTA targets this CTA's barriers any more
+      // No load is in flight, and no commit of the even CTA's on its way to the
+      // odd one's barriers, when the MMAs have read every stage; after a timeout
+      // the loads that no MMA waited for are waited for here.
       for (int x = 0; x < S; ++x)
-        if (issued > x) wait_bar_drain(&empty[x], x < s ? ph : (ph ^ 1u), 100000000ull);
-      if (!ok && !PAIR) {  // after a timeout: the loads that no MMA waited for
+        if (issued > x) wait_bar_drain(&empty[x], x < s ? ph : (ph ^ 1u), ok ? 100000000ull : 1000000ull);
+      if (!ok && rank == 0) {
         for (int64_t k = issued > S ? issued - S : 0; k < issued; ++k)
           wait_bar_drain(&full[k % S], static_cast<uint32_t>((k / S) & 1), 100000000ull);
       }
-    } else if (warp == 1 && lane == 0 && leads) {
+    } else if (warp == 1 && (!WIDE || rank == 0)) {
       // ------------------------------------------------------------ MMA issuer
       // fp32 accumulators, both operands e4m3 (format 0) and K-major
-      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) | ((WIDE ? 256u : 128u) >> 4 << 24);
+      const uint64_t da0 = sw128_desc(smem_u32(sbase), 16, 1024);
+      const uint64_t db0 = sw128_desc(smem_u32(sbase + C::kRowBytes), 16, 1024);
       int s = 0, buf = 0;
       uint32_t ph = 0, bph = 0;
-      bool ok = true, first = true;
+      bool ok = true, signal = !(p.test_flags & B200K_SCALED_MM_TEST_WITHHOLD_READY);
       for (int t = cid; t < p.num_tiles && ok; t += ncl) {
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = wait_bar(&full[s], ph, ctl) && wait_bar(&tempty[buf], bph ^ 1u, ctl))) break;
+          if (!(ok = warp_wait(&full[s], ph, ctl) && warp_wait(&tempty[buf], bph ^ 1u, ctl))) break;
           tc_fence_after();
-          const uint64_t da = sw128_desc(smem_u32(sbase + s * C::kStage), 16, 1024);
-          const uint64_t db = sw128_desc(smem_u32(sbase + s * C::kStage + C::kABytes), 16, 1024);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (PAIR) umma_f8_pair(tmem_base + buf * BN, da + 2 * k, db + 2 * k, idesc, k != 0);
-            else umma_f8(tmem_base + buf * BN, da + 2 * k, db + 2 * k, idesc, k != 0);
-          }
-          const bool signal = !(first && (p.test_flags & B200K_SCALED_MM_TEST_WITHHOLD_READY));
-          first = false;
-          if (PAIR) {
-            umma_commit_pair(smem_u32(&empty[s]));
-            umma_commit_pair(cluster_addr(&empty[s], 1));
-            if (signal) {
-              umma_commit_pair(smem_u32(&tfull[buf]));
-              umma_commit_pair(cluster_addr(&tfull[buf], 1));
-            }
-          } else {
-            umma_commit(&empty[s]);
-            if (signal) umma_commit(&tfull[buf]);
-          }
+          const uint32_t stage = (s * C::kStage) >> 4;
+          umma_block<WIDE>(tmem_base + buf * BN, da0 + stage, db0 + stage, idesc);
+          commit<WIDE>(&empty[s]);
+          if (signal) commit<WIDE>(&tfull[buf]);
+          signal = true;
           if (++s == S) {
             s = 0;
             ph ^= 1u;
           }
-          buf ^= 1;
-          if (buf == 0) bph ^= 1u;
+          if (++buf == BUFS) {
+            buf = 0;
+            bph ^= 1u;
+          }
         }
       }
-      // every MMA of this thread completes before tensor memory is freed
-      if (PAIR) umma_commit_pair(smem_u32(drain));
-      else umma_commit(drain);
+      // every MMA of this warp completes before tensor memory is freed
+      commit<WIDE>(drain);
       wait_bar_drain(drain, 0, 100000000ull);
+    } else if (warp >= 2) {
+      // ---------------------------------------------------------------- scales
+      // of this CTA's rows of a; turned: multiplied by b's, of which a tile has one
+      constexpr int kEach = kRowsM * kScaleBlocks / 64, kAtOnce = kEach < 8 ? kEach : 8;
+      const int sub = (warp - 2) * 32 + lane, kbl = sub % kScaleBlocks, r0 = sub / kScaleBlocks;
+      int c = 0;
+      bool ok = true;
+      for (int t = cid; t < p.num_tiles && ok; t += ncl) {
+        int tm, tn;
+        tile_at<WIDE>(t, p, tm, tn);
+        for (int kb = kb0; kb < kb1; kb += kScaleBlocks, ++c) {
+          float b = 0.0f;
+          const bool in = kb + kbl < kb1;
+          const float* pa = p.sa + (kb + kbl) * p.sa_k;
+          const int n = tn * kTileN + (WIDE ? (r0 & 1) * 128 : 0);
+          if (in && n < p.N) b = __ldg(p.sb + (kb + kbl) * p.sb_k + n / kBlk * p.sb_n);
+          float* to = reinterpret_cast<float*>(sbase + C::kOffSc + (c & 1) * kScaleBytes) + kbl * (kScaleRow + 4);
+          if (!(ok = warp_wait(&sc_empty[c & 1], ((c >> 1) & 1) ^ 1, ctl))) break;
+#pragma unroll 1
+          for (int i0 = 0; i0 < kEach; i0 += kAtOnce) {
+            float a[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+              const int m = tm * kTileM + rows_at + r0 + (i0 + i) * (64 / kScaleBlocks);
+              a[i] = in && m < p.M ? __ldg(pa + m * p.sa_m) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) to[r0 + (i0 + i) * (64 / kScaleBlocks)] = WIDE ? a[i] : a[i] * b;
+          }
+          if (WIDE && r0 < 2) to[kScaleRow + r0] = b;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[c & 1]);
+        }
+      }
     }
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue
-    if (C::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+    if (WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     const int quarter = warp & 3, cg = (warp - 4) >> 2;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cg * COLS;
-    uint8_t* stg = sbase + C::kOffStg + (warp - 4) * kStgBytes;
-    const int rank_rows = PAIR ? static_cast<int>(rank) * 128 : 0;
     const bool bf16 = p.out_dt == B200K_BF16;
-    int buf = 0;
+    int buf = 0, c = 0;  // c: chunks of scales
     uint32_t bph = 0;
     bool ok = true;
     for (int t = cid; t < p.num_tiles && ok; t += ncl) {
       int tm, tn;
-      tile_at(t, p, tm, tn);
-      const int row0 = tm * kTileM + rank_rows + quarter * 32, m = row0 + lane;
-      const int n0 = tn * BN + cg * COLS;
-      const int nb = min(n0, p.N - 1) / kBlk;
+      tile_at<WIDE>(t, p, tm, tn);
+      // wide: this thread's row and first column; turned: its column and first row
+      const int row0 = tm * kTileM + rows_at + (WIDE ? quarter * 32 : cg * COLS), n0 = tn * kTileN + (WIDE ? cg * COLS : quarter * 32);
       const bool any = row0 < p.M && n0 < p.N;  // warp-uniform
       float2 acc[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-      Scales next;
-      next.load(p, m, nb, kb0, kb1);
-      for (int kb = kb0; ok && kb < kb1; kb += 4) {
-        const Scales now = next;
-        next.load(p, m, nb, kb + 4, kb1);
+      // Block by block, kLd columns a load; a buffer is released when its last
+      // load has landed.
+      constexpr int kLd = COLS < 32 ? 16 : 32, J = COLS / kLd;
+      for (int kb = kb0, in = 0; kb < kb1; ++kb) {
+        const float* sc = reinterpret_cast<const float*>(sbase + C::kOffSc + (c & 1) * kScaleBytes) + in * (kScaleRow + 4);
+        ok = (in != 0 || warp_wait(&sc_full[c & 1], (c >> 1) & 1, ctl)) && warp_wait(&tfull[buf], bph, ctl);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t raw[2][kLd];
+        tmem_get(t_row + buf * BN, raw[0]);
+        const float scale = WIDE ? sc[quarter * 32 + lane] * sc[kScaleRow + cg] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kb + i >= kb1) break;
-          ok = __all_sync(0xffffffffu, wait_bar(&tfull[buf], bph, ctl));
-          if (!ok) break;
-          tc_fence_after();
-          if (any) {
-            const float2 sc = make_float2(now.s[i], now.s[i]);
-            uint32_t raw[2][32];
-            tmem_ld32(t_row + buf * BN, raw[0]);
-#pragma unroll
-            for (int c = 0; c < COLS / 32; ++c) {
-              tmem_wait_ld_regs(raw[c & 1]);
-              if (c + 1 < COLS / 32) tmem_ld32(t_row + buf * BN + (c + 1) * 32, raw[(c + 1) & 1]);
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                acc[c * 16 + j] = __ffma2_rn(make_float2(__uint_as_float(raw[c & 1][2 * j]), __uint_as_float(raw[c & 1][2 * j + 1])),
-                                             sc, acc[c * 16 + j]);
+        for (int j = 0; j < J; ++j) {
+          tmem_wait(raw[j & 1]);
+          if (j + 1 < J) {
+            tmem_get(t_row + buf * BN + (j + 1) * kLd, raw[(j + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (WIDE && rank != 0) arrive_even(&tempty[buf]);
+              else mbar_arrive(&tempty[buf]);
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (PAIR && rank != 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
-            else mbar_arrive(&tempty[buf]);
+#pragma unroll
+          for (int k = 0; k < kLd / 2; ++k) {
+            const float2 v = make_float2(__uint_as_float(raw[j & 1][2 * k]), __uint_as_float(raw[j & 1][2 * k + 1]));
+            const float2 f = WIDE ? make_float2(scale, scale) : *reinterpret_cast<const float2*>(sc + cg * COLS + j * kLd + 2 * k);
+            acc[j * (kLd / 2) + k] = __ffma2_rn(v, f, acc[j * (kLd / 2) + k]);
           }
-          buf ^= 1;
-          if (buf == 0) bph ^= 1u;
+        }
+        if (++in == kScaleBlocks || kb + 1 == kb1) {  // done with the chunk of scales
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[c & 1]);
+          ++c;
+          in = 0;
+        }
+        if (++buf == BUFS) {
+          buf = 0;
+          bph ^= 1u;
         }
       }
-      if (!PAIR && p.split > 1) {
-        // every load has landed and been read: the ring holds the sums
-        float* part = reinterpret_cast<float*>(sbase) + (quarter * 32 + lane) * C::kPartStride;
+      if (!WIDE && split > 1) {
+        // every load has landed and been read: the ring holds the sums, [BN][128]
+        float* part = reinterpret_cast<float*>(sbase) + cg * COLS * C::kPartRow + quarter * 32 + lane;
         if (ok && any) {
 #pragma unroll
-          for (int i = 0; i < COLS / 4; ++i)
-            reinterpret_cast<float4*>(part)[i] = make_float4(acc[2 * i].x, acc[2 * i].y, acc[2 * i + 1].x, acc[2 * i + 1].y);
+          for (int i = 0; i < COLS / 2; ++i) {
+            part[2 * i * C::kPartRow] = acc[i].x;
+            part[(2 * i + 1) * C::kPartRow] = acc[i].y;
+          }
         }
         break;  // one tile a cluster; joined below
       }
       if (!ok || !any) continue;
-      if (p.tma_out) {
-        // staged as rows of 128 bytes, 128-byte swizzle, and stored by TMA
-        const bool f32 = p.out_dt == B200K_F32;
+      if constexpr (!WIDE) {
+        // a warp's lanes are neighbouring columns of the output
+        const int n = n0 + lane;
 #pragma unroll
-        for (int h = 0; h < COLS / 32; ++h) {
-          if (n0 + h * 32 >= p.N) break;
-          const int half = f32 ? 0 : h & 1;
-          if (half == 0) {
-            if (lane == 0) bulk_wait_read_all();  // the store before has read the rows
-            __syncwarp();
-          }
-          if (f32) {
-#pragma unroll
-            for (int g = 0; g < 8; ++g)
-              *reinterpret_cast<float4*>(stg + lane * 128 + ((g ^ (lane & 7)) << 4)) =
-                  make_float4(acc[h * 16 + 2 * g].x, acc[h * 16 + 2 * g].y, acc[h * 16 + 2 * g + 1].x, acc[h * 16 + 2 * g + 1].y);
-          } else {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float2* v = acc + h * 16 + 4 * g;
-              *reinterpret_cast<uint4*>(stg + lane * 128 + (((half * 4 + g) ^ (lane & 7)) << 4)) =
-                  make_uint4(pack16(v[0].x, v[0].y, bf16), pack16(v[1].x, v[1].y, bf16), pack16(v[2].x, v[2].y, bf16),
-                             pack16(v[3].x, v[3].y, bf16));
-            }
-          }
-          if (f32 || half == 1 || n0 + (h + 1) * 32 >= p.N) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&tmO, stg, n0 + (f32 ? h : h & ~1) * 32, row0);
-              bulk_commit();
-            }
-          }
-        }
+        for (int i = 0; i < COLS; ++i)
+          if (row0 + i < p.M && n < p.N)
+            store_scalar(p.out, static_cast<int64_t>(row0 + i) * p.N + n, p.out_dt, i & 1 ? acc[i / 2].y : acc[i / 2].x);
       } else {
-        // rows that TMA cannot store: 32 columns at a time through shared
-        // memory (33 floats a row), a warp's lanes on neighbouring columns
-        float* tile = reinterpret_cast<float*>(stg);
+        uint8_t* stg = sbase + C::kOffStg + (warp - 4) * kStgBoxes * kStgBox;
+        if (p.tma_out) {
+          // staged as boxes of 32 rows x 128 bytes (128-byte swizzle), stored by
+          // TMA under the next tile; fp32 takes two rounds
+          const bool f32 = p.out_dt == B200K_F32;
+          const int step = f32 ? 32 : 64;  // columns of a box
 #pragma unroll
-        for (int h = 0; h < COLS / 16; ++h) {
-          if (n0 + h * 16 >= p.N) break;
-          __syncwarp();
+          for (int h = 0; h < COLS / 32; ++h) {  // 32 columns: a box of fp32, half of one of 16 bits
+            if (h == 0 || (f32 && h == 2)) {
+              if (lane == 0) bulk_wait_read_all();  // the stores before have read the boxes
+              __syncwarp();
+            }
+            const float2* v = acc + h * 16;
+            uint8_t* row = stg + (f32 ? h & 1 : h >> 1) * kStgBox + lane * 128;
+            if (f32) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            tile[lane * 17 + 2 * j] = acc[h * 8 + j].x;
-            tile[lane * 17 + 2 * j + 1] = acc[h * 8 + j].y;
+              for (int g = 0; g < 8; ++g)
+                *reinterpret_cast<float4*>(row + ((g ^ (lane & 7)) << 4)) = make_float4(v[2 * g].x, v[2 * g].y, v[2 * g + 1].x, v[2 * g + 1].y);
+            } else {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint4*>(row + ((((h & 1) * 4 + g) ^ (lane & 7)) << 4)) =
+                    make_uint4(pack16(v[4 * g].x, v[4 * g].y, bf16), pack16(v[4 * g + 1].x, v[4 * g + 1].y, bf16),
+                               pack16(v[4 * g + 2].x, v[4 * g + 2].y, bf16), pack16(v[4 * g + 3].x, v[4 * g + 3].y, bf16));
+            }
+            if (f32 ? h & 1 : h == COLS / 32 - 1) {
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                const int first = f32 ? n0 + (h - 1) * 32 : n0;
+                if (first < p.N) tma_store_2d(&tmO, stg, first, row0);
+                if (first + step < p.N) tma_store_2d(&tmO, stg + kStgBox, first + step, row0);
+                bulk_commit();
+              }
+            }
+          }
+        } else {
+          // rows that TMA cannot store: eight columns at a time through shared
+          // memory, a warp's lanes on neighbouring columns
+          float* tile = reinterpret_cast<float*>(stg);
+#pragma unroll
+          for (int h = 0; h < COLS / 8; ++h) {
+            if (n0 + h * 8 >= p.N) break;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              tile[lane * 9 + 2 * j] = acc[h * 4 + j].x;
+              tile[lane * 9 + 2 * j + 1] = acc[h * 4 + j].y;
+            }
+            __syncwarp();
+            const int n = n0 + h * 8 + (lane & 7);
+            for (int r = lane >> 3; r < 32 && row0 + r < p.M; r += 4)
+              if (n < p.N) store_scalar(p.out, static_cast<int64_t>(row0 + r) * p.N + n, p.out_dt, tile[r * 9 + (lane & 7)]);
           }
           __syncwarp();
-          const int n = n0 + h * 16 + (lane & 15);
-          for (int r = lane >> 4; r < 32 && row0 + r < p.M; r += 2)
-            if (n < p.N) store_scalar(p.out, static_cast<int64_t>(row0 + r) * p.N + n, p.out_dt, tile[r * 17 + (lane & 15)]);
         }
-        __syncwarp();
       }
     }
-    if (p.tma_out) {
+    if (WIDE && p.tma_out) {
       if (lane == 0) bulk_wait_all();
       __syncwarp();
     }
   }
 
-  if (!PAIR && p.split > 1) {
+  if (!WIDE && split > 1) {
     // Every CTA of the cluster adds up a share of the rows, in the ranks' order.
     cluster_sync();
     int tm, tn;
-    tile_at(cid, p, tm, tn);
-    const int rows = min(128, p.M - tm * 128), cols = min(BN, p.N - tn * BN);
-    constexpr int kPer = BN / 4;  // threads of a row
+    tile_at<WIDE>(cid, p, tm, tn);
+    const int rows = min(kTileM, p.M - tm * kTileM), cols = min(kTileN, p.N - tn * kTileN);
     const bool bf16 = p.out_dt == B200K_BF16, vec = p.N % 4 == 0;
-    const int c = (threadIdx.x % kPer) * 4;
-    if (!*abort_flag && c < cols) {
-      for (int r = static_cast<int>(rank) + p.split * static_cast<int>(threadIdx.x / kPer); r < rows;
-           r += p.split * (C::kThreads / kPer)) {
-        const float* mine = reinterpret_cast<const float*>(sbase) + r * C::kPartStride + c;
-        float4 sum = ld_cluster4(cluster_addr(mine, 0));
-        for (int k = 1; k < p.split; ++k) {
-          const float4 v = ld_cluster4(cluster_addr(mine, k));
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
-        }
-        const int64_t at = static_cast<int64_t>(tm * 128 + r) * p.N + tn * BN + c;
+    const int n = lane * 4;
+    if (!*abort_flag && n < cols) {
+      for (int r = static_cast<int>(rank) + split * warp; r < rows; r += split * (C::kThreads / 32)) {
+        const float* mine = reinterpret_cast<const float*>(sbase) + r * C::kPartRow + n;
+        float4 v[kMaxSplit];
+#pragma unroll
+        for (int k = 0; k < kMaxSplit; ++k)
+          if (k < split) v[k] = ld_cluster4(cluster_addr(mine, k));
+        float4 sum = v[0];
+#pragma unroll
+        for (int k = 1; k < kMaxSplit; ++k)
+          if (k < split) {
+            sum.x += v[k].x;
+            sum.y += v[k].y;
+            sum.z += v[k].z;
+            sum.w += v[k].w;
+          }
+        const int64_t at = static_cast<int64_t>(tm * kTileM + r) * p.N + tn * kTileN + n;
         if (vec && p.out_dt == B200K_F32) {
           *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = sum;
         } else if (vec) {
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack16(sum.x, sum.y, bf16), pack16(sum.z, sum.w, bf16));
         } else {
-          const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+          const float x[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (c + j < cols) store_scalar(p.out, at + j, p.out_dt, v[j]);
+            if (n + j < cols) store_scalar(p.out, at + j, p.out_dt, x[j]);
         }
       }
     }
+    cluster_sync();  // no CTA leaves while another may read its shared memory
   }
   tc_fence_before();
   __syncthreads();
-  if (cluster > 1) cluster_sync();  // no CTA leaves while another may signal or read its shared memory
+  if (WIDE) cluster_sync();  // no CTA leaves while the other may still signal its barriers
   if (warp == 2) {
     tc_fence_after();
-    if (PAIR) tmem_dealloc_pair(tmem_base, 2 * BN);
-    else tmem_dealloc(tmem_base, 2 * BN);
+    if (WIDE) tmem_dealloc_pair(tmem_base, C::kTmemCols);
+    else tmem_dealloc(tmem_base, C::kTmemCols);
   }
 }
 
@@ -460,10 +572,10 @@ bool make_map2(CUtensorMap* map, CUtensorMapDataType dt, const void* ptr, uint64
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool PAIR, int BN>
+template <int BN>
 int launch(MmParams p, const B200kScaledMmArgs* a, int sms, cudaStream_t st) {
-  using C = Cfg8<PAIR, BN>;
-  auto kernel = mm_kernel<PAIR, BN>;
+  using C = Cfg8<BN>;
+  auto kernel = mm_kernel<BN>;
   static std::atomic<uint64_t> done{0};
   if (!attributes_set(done)) {
     cudaFuncAttributes fa;
@@ -471,29 +583,27 @@ int launch(MmParams p, const B200kScaledMmArgs* a, int sms, cudaStream_t st) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
       return B200K_ERR_LAUNCH;
     // the epilogue's registers come out of what the launch has: with fewer, setmaxnreg would wait
-    if (C::kGroups == 2 && fa.numRegs * C::kThreads < kCtlRegs * 128 + kEpiRegs * 256) return B200K_ERR_LAUNCH;
+    if (C::kWide && fa.numRegs * C::kThreads < kCtlRegs * 128 + kEpiRegs * 256) return B200K_ERR_LAUNCH;
     attributes_done(done);
   }
   CUtensorMap ta, tb, to;
-  const uint64_t K = static_cast<uint64_t>(a->K);
-  p.a_rows = PAIR ? 128 : static_cast<int32_t>(std::min<int64_t>(128, (a->M + 7) / 8 * 8));
+  const uint64_t K = static_cast<uint64_t>(a->K), one_row = (K + 15) / 16 * 16;  // the stride of a single row is never stepped
+  constexpr int kTileM = C::kWide ? 256 : BN, kTileN = C::kWide ? BN : 128;
   const int ob = a->out_dtype == B200K_F32 ? 4 : 2;
-  if (!make_map2(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->a, K, a->M, a->M == 1 ? (K + 15) / 16 * 16 : a->a_stride_m, kBlk, p.a_rows) ||
-      !make_map2(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->b, K, a->N, a->N == 1 ? (K + 15) / 16 * 16 : a->b_stride_n, kBlk,
-                 PAIR ? BN / 2 : BN))
+  if (!make_map2(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->a, K, a->M, a->M == 1 ? one_row : a->a_stride_m, kBlk, C::kWide ? 128 : BN) ||
+      !make_map2(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->b, K, a->N, a->N == 1 ? one_row : a->b_stride_n, kBlk, 128))
     return B200K_ERR_LAUNCH;
   std::memset(&to, 0, sizeof(to));
-  p.tma_out = a->N * ob % 16 == 0 && p.split == 1;
-  if (p.tma_out && !make_map2(&to, tma_dtype(a->out_dtype), a->out, a->N, a->M, a->N * ob, 128 / ob, 32)) return B200K_ERR_LAUNCH;
-  const int tile_m = PAIR ? 256 : 128;
-  const int64_t tm = (a->M + tile_m - 1) / tile_m, tn = (a->N + BN - 1) / BN;
-  const int cluster = PAIR ? 2 : p.split;
-  if (tm * tn * cluster > 0x7fffffffLL) return B200K_ERR_SHAPE;
+  p.tma_out = C::kWide && a->N * ob % 16 == 0;
+  if (p.tma_out && !make_map2(&to, tma_dtype(a->out_dtype), a->out, a->N, a->M, a->N * ob, 128 / ob, 32))
+    return B200K_ERR_LAUNCH;
+  const int64_t tm = (a->M + kTileM - 1) / kTileM, tn = (a->N + kTileN - 1) / kTileN;
+  if (tm * tn > 0x7fffffffLL / kMaxSplit) return B200K_ERR_SHAPE;
   p.tiles_m = static_cast<int32_t>(tm);
   p.tiles_n = static_cast<int32_t>(tn);
   p.num_tiles = static_cast<int32_t>(tm * tn);
-  p.group_m = PAIR ? kGroupMPair : kGroupM;
-  const int64_t clusters = !PAIR && p.split > 1 ? tm * tn : std::min<int64_t>(tm * tn, sms / cluster);
+  const int cluster = C::kWide ? 2 : p.split;
+  const int64_t clusters = !C::kWide && p.split > 1 ? tm * tn : std::min<int64_t>(tm * tn, sms / cluster);
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
@@ -519,7 +629,9 @@ extern "C" int b200k_scaled_mm(const B200kScaledMmArgs* a, void* stream_) {
   if (!a) return B200K_ERR_ARG;
   if (a->M < 0 || a->N < 0 || a->K < 0 || a->M > 0x3fffffff || a->N > 0x3fffffff || a->K > 0x3fffffff) return B200K_ERR_SHAPE;
   if (a->out_dtype != B200K_BF16 && a->out_dtype != B200K_F16 && a->out_dtype != B200K_F32) return B200K_ERR_UNSUPPORTED;
-  if (a->tile < 0 || a->tile > 3 || a->split < 0 || a->split > 8) return B200K_ERR_ARG;
+  if ((a->tile != 0 && a->tile != 1 && a->tile != 16 && a->tile != 32 && a->tile != 64 && a->tile != 128) || a->split < 0 ||
+      a->split > mm8::kMaxSplit)
+    return B200K_ERR_ARG;
   if (a->M == 0 || a->N == 0) return B200K_OK;
   if (!a->out) return B200K_ERR_ARG;
   if (!aligned16(a->out)) return B200K_ERR_ALIGN;
@@ -550,14 +662,21 @@ extern "C" int b200k_scaled_mm(const B200kScaledMmArgs* a, void* stream_) {
   p.test_flags = a->test_flags;
   p.status = a->status;
   p.timeout_ns = a->timeout_ns > 0 ? a->timeout_ns : 2000000000ll;
+  // tile: 0 the choice below, 1 wide, else the turned tiles' rows of a
+  int tile = a->tile;
   p.split = 1;
-  const int64_t tiles = (a->M + 255) / 256 * ((a->N + 255) / 256);
-  if (a->tile == 1 || (a->tile == 0 && a->M > 128 && tiles * 2 >= sms)) return mm8::launch<true, 256>(p, a, sms, st);
-  const bool narrow = a->tile == 3 || (a->tile == 0 && a->M <= 128);
-  const int64_t single = (a->M + 127) / 128 * ((a->N + (narrow ? 63 : 127)) / (narrow ? 64 : 128));
-  int split = 1;
-  while (split < 8 && single * split * 2 <= sms && p.k_blocks >= split * 4) split *= 2;
-  if (a->split > 0) split = a->split;
-  p.split = split;
-  return narrow ? mm8::launch<false, 64>(p, a, sms, st) : mm8::launch<false, 128>(p, a, sms, st);
+  if (tile == 0) {
+    const int64_t wide = (a->M + 255) / 256 * ((a->N + 255) / 256) * 2;
+    tile = a->M > 128 && wide * 2 > sms ? 1 : a->M <= 16 ? 16 : a->M <= 32 ? 32 : a->M <= 64 ? 64 : 128;
+  }
+  if (tile == 1) return mm8::launch<256>(p, a, sms, st);
+  const int64_t tiles = (a->M + tile - 1) / tile * ((a->N + 127) / 128);
+  while (p.split < mm8::kMaxSplit && tiles * p.split * 2 <= sms && p.k_blocks >= p.split * 4) p.split *= 2;
+  if (a->split > 0) p.split = a->split;
+  switch (tile) {
+    case 16: return mm8::launch<16>(p, a, sms, st);
+    case 32: return mm8::launch<32>(p, a, sms, st);
+    case 64: return mm8::launch<64>(p, a, sms, st);
+    default: return mm8::launch<128>(p, a, sms, st);
+  }
 }
