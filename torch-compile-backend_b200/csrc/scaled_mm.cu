@@ -10,11 +10,13 @@
 // pipe fills the next ones the epilogue warps read it and add it, times its
 // scale, to fp32 sums in registers.
 //
-// One CTA per SM:
+// Warps of a CTA:
 //   warp 0      TMA producer (128-byte swizzled tiles of 128 k);
-//   warp 1      MMA issuer;
-//   warps 2, 3  bring the scales of kScaleBlocks blocks at a time to shared
-//               memory, transposed (warp 2 owns tensor memory);
+//   warps 1, 3  MMA issuers, of every other block: the waits and the issue of a
+//               block take one warp 600 clocks, more than a block of few rows
+//               takes to arrive;
+//   warp 2      brings the scales of kScaleBlocks blocks at a time to shared
+//               memory, transposed (and owns tensor memory);
 //   warps 4..   epilogue.
 // Two kinds of tile:
 //   wide        256 rows of a x 256 columns of b on a pair of CTAs (cta_group::2),
@@ -49,9 +51,9 @@ constexpr int kBlk = 128;  // k of a block, one swizzle row of bytes
 // Registers of a thread of wide tiles: launched with 168, 128 control threads
 // leave theirs to 256 epilogue threads (128 sums each).
 constexpr int kCtlRegs = 56, kEpiRegs = 224;
-// Blocks of k whose scales are fetched together, a 32-byte sector of a row:
-// eight neighbouring lanes read it.  (A load by each epilogue thread touched
-// 32 lines and kept all eight epilogue warps 1500 clocks for four blocks.)
+// Blocks of k whose scales are fetched together, a 32-byte sector of a row.  (A
+// load by each epilogue thread touched 32 lines for each block and kept all eight
+// epilogue warps 1500 clocks for four blocks.)
 constexpr int kScaleBlocks = 8;
 constexpr int kScaleRow = 132;                                        // floats: 128 rows of a block, turned banks
 constexpr uint32_t kScaleBytes = kScaleBlocks * (kScaleRow + 4) * 4;  // with two scales of b a block
@@ -66,6 +68,7 @@ struct MmParams {
   int32_t tma_out;          // the output's rows can be stored by TMA (wide)
   const float* sa;          // [M, k_blocks]
   int64_t sa_m, sa_k;
+  int32_t sa_vec;           // four neighbouring blocks' scales lie 16-byte aligned
   const float* sb;          // [k_blocks, ceil(N / 128)]
   int64_t sb_k, sb_n;
   void* out;                // [M, N] contiguous
@@ -86,14 +89,18 @@ struct Cfg8 {
   static constexpr int kThreads = 128 + 128 * kGroups;
   static constexpr uint32_t kRowBytes = 128 * kBlk;        // the product's 128 rows (of this CTA)
   static constexpr uint32_t kStage = kRowBytes + (kWide ? BN / 2 : BN) * kBlk;
-  static constexpr int kStages = BN >= 128 ? (kWide ? 4 : 6) : 8;
+  // Few rows: two CTAs an SM, so that one's waits, start and end lie under the
+  // other's (64 rows of [4096, 14336] with one: 20.7 us).
+  static constexpr int kCtas = BN <= 64 ? 2 : 1;
+  static constexpr int kStages = BN >= 128 ? (kWide ? 4 : 6) : 4;
   static constexpr uint32_t kOffStg = kStages * kStage;
   static constexpr uint32_t kOffSc = kOffStg + (kWide ? 4 * kGroups * kStgBoxes * kStgBox : 0);  // two chunks of scales
   static constexpr uint32_t kOffBar = kOffSc + 2 * kScaleBytes;
   static constexpr uint32_t kSmem = 1024 + kOffBar + 512;
   static constexpr int kPartRow = 132;  // floats: 128 sums of a split tile's column
   static_assert(kTmemCols >= 32 && kTmemCols <= 512, "tensor memory");
-  static_assert(kSmem <= 232448 && kSmem > 232448 / 2, "one CTA per SM");
+  static_assert(kSmem <= (kCtas == 1 ? 232448u : 115712u) && kCtas * kTmemCols <= 512, "fits the SM");
+  static_assert(kCtas > 1 || kSmem > 232448 / 2, "one CTA per SM");
   static_assert(kWide || BN * kPartRow * 4 <= kOffStg, "the sums of a split tile fit the ring");
 };
 
@@ -142,7 +149,17 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 __device__ __forceinline__ void arrive_even(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(bar, 0)) : "memory");
 }
+// A phase that has completed costs a test (the wait alone took 30 clocks more).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Ctl& c) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, done)) return true;
   return __all_sync(0xffffffffu, wait_bar(bar, parity, c));
 }
 // 16 or 32 columns of this thread's tensor-memory row, and the wait for them,
@@ -193,7 +210,7 @@ __device__ __forceinline__ void tile_at(int t, const MmParams& p, int& tm, int& 
 }
 
 template <int BN>
-__global__ void __launch_bounds__(Cfg8<BN>::kThreads, 1)
+__global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
     mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const __grid_constant__ CUtensorMap tmO, const __grid_constant__ MmParams p) {
   using C = Cfg8<BN>;
@@ -209,8 +226,8 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, 1)
   uint64_t* tempty = tfull + BUFS;
   uint64_t* sc_full = tempty + BUFS;  // [2]
   uint64_t* sc_empty = sc_full + 2;
-  uint64_t* drain = sc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* drain = sc_empty + 2;     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -228,10 +245,10 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, 1)
       mbar_init(&tempty[a], 4 * C::kGroups * (WIDE ? 2 : 1));  // a pair's arrive at the even CTA's
     }
     for (int a = 0; a < 2; ++a) {
-      mbar_init(&sc_full[a], 2);
+      mbar_init(&sc_full[a], 1);
+      mbar_init(&drain[a], 1);
       mbar_init(&sc_empty[a], 4 * C::kGroups);
     }
-    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_map(&tmA);
@@ -298,67 +315,87 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, 1)
         for (int64_t k = issued > S ? issued - S : 0; k < issued; ++k)
           wait_bar_drain(&full[k % S], static_cast<uint32_t>((k / S) & 1), 100000000ull);
       }
-    } else if (warp == 1 && (!WIDE || rank == 0)) {
-      // ------------------------------------------------------------ MMA issuer
+    } else if ((warp & 1) && (!WIDE || rank == 0)) {
+      // ----------------------------------------------------------- MMA issuers
       // fp32 accumulators, both operands e4m3 (format 0) and K-major
       const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) | ((WIDE ? 256u : 128u) >> 4 << 24);
       const uint64_t da0 = sw128_desc(smem_u32(sbase), 16, 1024);
       const uint64_t db0 = sw128_desc(smem_u32(sbase + C::kRowBytes), 16, 1024);
-      int s = 0, buf = 0;
-      uint32_t ph = 0, bph = 0;
+      const int which = warp >> 1;
       bool ok = true, signal = !(p.test_flags & B200K_SCALED_MM_TEST_WITHHOLD_READY);
-      for (int t = cid; t < p.num_tiles && ok; t += ncl) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = warp_wait(&full[s], ph, ctl) && warp_wait(&tempty[buf], bph ^ 1u, ctl))) break;
-          tc_fence_after();
-          const uint32_t stage = (s * C::kStage) >> 4;
-          umma_block<WIDE>(tmem_base + buf * BN, da0 + stage, db0 + stage, idesc);
-          commit<WIDE>(&empty[s]);
-          if (signal) commit<WIDE>(&tfull[buf]);
-          signal = true;
-          if (++s == S) {
-            s = 0;
-            ph ^= 1u;
-          }
-          if (++buf == BUFS) {
-            buf = 0;
-            bph ^= 1u;
-          }
+      const int64_t blocks = static_cast<int64_t>(cid < p.num_tiles ? (p.num_tiles - cid + ncl - 1) / ncl : 0) * (kb1 - kb0);
+      static_assert(S % 2 == 0 && BUFS % 2 == 0, "an issuer's blocks have stages and buffers of their own");
+      int s = which, buf = which;
+      uint32_t ph = 0, bph = 0;
+      for (int64_t i = which; i < blocks; i += 2) {
+        if (!(ok = warp_wait(&full[s], ph, ctl) && warp_wait(&tempty[buf], bph ^ 1u, ctl))) break;
+        tc_fence_after();
+        const uint32_t stage = (s * C::kStage) >> 4;
+        umma_block<WIDE>(tmem_base + buf * BN, da0 + stage, db0 + stage, idesc);
+        if (signal) commit<WIDE>(&tfull[buf]);
+        commit<WIDE>(&empty[s]);
+        signal = true;
+        if ((s += 2) >= S) {
+          s = which;
+          ph ^= 1u;
+        }
+        if ((buf += 2) >= BUFS) {
+          buf = which;
+          bph ^= 1u;
         }
       }
       // every MMA of this warp completes before tensor memory is freed
-      commit<WIDE>(drain);
-      wait_bar_drain(drain, 0, 100000000ull);
-    } else if (warp >= 2) {
+      commit<WIDE>(&drain[which]);
+      wait_bar_drain(&drain[which], 0, 100000000ull);
+    } else if (warp == 2) {
       // ---------------------------------------------------------------- scales
-      // of this CTA's rows of a; turned: multiplied by b's, of which a tile has one
-      constexpr int kEach = kRowsM * kScaleBlocks / 64, kAtOnce = kEach < 8 ? kEach : 8;
-      const int sub = (warp - 2) * 32 + lane, kbl = sub % kScaleBlocks, r0 = sub / kScaleBlocks;
+      // of this CTA's rows of a; turned: multiplied by b's, of which a tile has
+      // one.  Two lanes take a row's eight blocks, four each.
+      constexpr int kEach = kRowsM / 16, kAtOnce = WIDE ? 2 : kEach;
+      const int kb4 = (lane & 1) * 4, r0 = lane >> 1;
+      const bool vec = p.sa_vec && kb0 % 4 == 0;
       int c = 0;
       bool ok = true;
       for (int t = cid; t < p.num_tiles && ok; t += ncl) {
         int tm, tn;
         tile_at<WIDE>(t, p, tm, tn);
         for (int kb = kb0; kb < kb1; kb += kScaleBlocks, ++c) {
-          float b = 0.0f;
-          const bool in = kb + kbl < kb1;
-          const float* pa = p.sa + (kb + kbl) * p.sa_k;
-          const int n = tn * kTileN + (WIDE ? (r0 & 1) * 128 : 0);
-          if (in && n < p.N) b = __ldg(p.sb + (kb + kbl) * p.sb_k + n / kBlk * p.sb_n);
-          float* to = reinterpret_cast<float*>(sbase + C::kOffSc + (c & 1) * kScaleBytes) + kbl * (kScaleRow + 4);
-          if (!(ok = warp_wait(&sc_empty[c & 1], ((c >> 1) & 1) ^ 1, ctl))) break;
+          const int k0 = kb + kb4, left = kb1 - k0;  // this lane's blocks
+          const int n = tn * kTileN + (WIDE ? (lane >> 1 & 1) * 128 : 0);
+          float b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = j < left && n < p.N ? __ldg(p.sb + (k0 + j) * p.sb_k + n / kBlk * p.sb_n) : 0.0f;
+          float* to = reinterpret_cast<float*>(sbase + C::kOffSc + (c & 1) * kScaleBytes) + kb4 * (kScaleRow + 4);
+          if (WIDE && !(ok = warp_wait(&sc_empty[c & 1], ((c >> 1) & 1) ^ 1, ctl))) break;
 #pragma unroll 1
           for (int i0 = 0; i0 < kEach; i0 += kAtOnce) {
-            float a[kAtOnce];
+            float a[kAtOnce][4];
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
-              const int m = tm * kTileM + rows_at + r0 + (i0 + i) * (64 / kScaleBlocks);
-              a[i] = in && m < p.M ? __ldg(pa + m * p.sa_m) : 0.0f;
-            }
+              const int m = tm * kTileM + rows_at + r0 + (i0 + i) * 16;
+              const float* pa = p.sa + m * p.sa_m + k0 * p.sa_k;
+              if (vec && left > 0 && k0 + 4 <= p.k_blocks && m < p.M) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(pa));
+                a[i][0] = v.x;
+                a[i][1] = v.y;
+                a[i][2] = v.z;
+                a[i][3] = v.w;
+              } else {
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) to[r0 + (i0 + i) * (64 / kScaleBlocks)] = WIDE ? a[i] : a[i] * b;
+                for (int j = 0; j < 4; ++j) a[i][j] = j < left && m < p.M ? __ldg(pa + j * p.sa_k) : 0.0f;
+              }
+            }
+            if (!WIDE && i0 == 0 && !(ok = warp_wait(&sc_empty[c & 1], ((c >> 1) & 1) ^ 1, ctl))) break;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) to[j * (kScaleRow + 4) + r0 + (i0 + i) * 16] = WIDE ? a[i][j] : a[i][j] * b[j];
           }
-          if (WIDE && r0 < 2) to[kScaleRow + r0] = b;
+          if (!ok) break;
+          if (WIDE && lane < 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j * (kScaleRow + 4) + kScaleRow + (lane >> 1)] = b[j];
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[c & 1]);
         }
@@ -603,7 +640,7 @@ int launch(MmParams p, const B200kScaledMmArgs* a, int sms, cudaStream_t st) {
   p.tiles_n = static_cast<int32_t>(tn);
   p.num_tiles = static_cast<int32_t>(tm * tn);
   const int cluster = C::kWide ? 2 : p.split;
-  const int64_t clusters = !C::kWide && p.split > 1 ? tm * tn : std::min<int64_t>(tm * tn, sms / cluster);
+  const int64_t clusters = !C::kWide && p.split > 1 ? tm * tn : std::min<int64_t>(tm * tn, sms * C::kCtas / cluster);
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
@@ -654,6 +691,7 @@ extern "C" int b200k_scaled_mm(const B200kScaledMmArgs* a, void* stream_) {
   p.sa = a->a_scale;
   p.sa_m = a->a_scale_strides[0];
   p.sa_k = a->a_scale_strides[1];
+  p.sa_vec = p.sa_k == 1 && p.sa_m % 4 == 0 && aligned16(p.sa);
   p.sb = a->b_scale;
   p.sb_k = a->b_scale_strides[0];
   p.sb_n = a->b_scale_strides[1];
@@ -662,7 +700,10 @@ extern "C" int b200k_scaled_mm(const B200kScaledMmArgs* a, void* stream_) {
   p.test_flags = a->test_flags;
   p.status = a->status;
   p.timeout_ns = a->timeout_ns > 0 ? a->timeout_ns : 2000000000ll;
-  // tile: 0 the choice below, 1 wide, else the turned tiles' rows of a
+  // tile: 0 the choice below, 1 wide, else the turned tiles' rows of a.  Wide
+  // tiles pay once they fill half of the GPU: rows x [4096, 4096] as wide and as
+  // turned tiles of 128: 512 (32 pairs) 21.9 and 20.1 us, 1024 (64 pairs) 22.9 and
+  // 35.2; 512 x [8192, 8192] 37.7 and 55.5.
   int tile = a->tile;
   p.split = 1;
   if (tile == 0) {
@@ -670,8 +711,22 @@ extern "C" int b200k_scaled_mm(const B200kScaledMmArgs* a, void* stream_) {
     tile = a->M > 128 && wide * 2 > sms ? 1 : a->M <= 16 ? 16 : a->M <= 32 ? 32 : a->M <= 64 ? 64 : 128;
   }
   if (tile == 1) return mm8::launch<256>(p, a, sms, st);
-  const int64_t tiles = (a->M + tile - 1) / tile * ((a->N + 127) / 128);
-  while (p.split < mm8::kMaxSplit && tiles * p.split * 2 <= sms && p.k_blocks >= p.split * 4) p.split *= 2;
+  // The split with the least rounds x (blocks of a CTA + what its start and,
+  // when split, its join cost, in blocks).  64 rows of [4096, 14336] (112 tiles)
+  // with 1, 2 and 4: 22, 18 and 25 us; a row of [8192, 2048] (16 tiles) with 4 and
+  // 8: 9.7 and 8.0.  Clusters of 8 CTAs that have an SM each do not all find room
+  // at once: 128 rows of [8192, 2048] with 4 and 8: 12.5 and 20.6 us.
+  const int64_t tiles = (a->M + tile - 1) / tile * ((a->N + 127) / 128), slots = static_cast<int64_t>(sms) * (tile <= 64 ? 2 : 1);
+  int64_t best = INT64_MAX;
+  for (int split = 1; split <= std::min<int32_t>(tile <= 64 ? mm8::kMaxSplit : 4, p.k_blocks); ++split) {
+    const int64_t rounds = split == 1 ? 1 : (tiles * split + slots - 1) / slots;
+    const int64_t each = split == 1 ? (tiles + slots - 1) / slots * p.k_blocks : (p.k_blocks + split - 1) / split;
+    const int64_t cost = rounds * (each + 6 + (split > 1 ? 2 : 0));
+    if (cost < best) {
+      best = cost;
+      p.split = split;
+    }
+  }
   if (a->split > 0) p.split = a->split;
   switch (tile) {
     case 16: return mm8::launch<16>(p, a, sms, st);
