@@ -89,16 +89,17 @@ struct Work {
   Seq s;
   int base;   // first key of step 0 (lo rounded down to a step)
   int tiles;  // 0: no keys, no queries, or the tile kernel's
-  int rts;    // 16-row blocks of a kv head
+  int rts;    // row blocks of a kv head
 };
-// `limit`: query rows above which a sequence is the tile kernel's; KEYS: of a step.
-template <int KEYS>
+// `limit`: query rows above which a sequence is the tile kernel's; KEYS: of a step,
+// ROWS: query rows of a unit.
+template <int KEYS, int ROWS>
 __device__ __forceinline__ Work work_at(const Params& p, int b, int limit) {
   Work w;
   w.s = seq_at(p, b);
   w.base = w.s.lo & ~(KEYS - 1);
   const int64_t rows = static_cast<int64_t>(w.s.m) * p.G;
-  w.rts = static_cast<int>((rows + kRows - 1) / kRows);
+  w.rts = static_cast<int>((rows + ROWS - 1) / ROWS);
   w.tiles = (w.s.m > 0 && w.s.n > w.base && rows <= limit) ? (w.s.n - w.base + KEYS - 1) / KEYS : 0;
   return w;
 }
@@ -118,12 +119,12 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
 // The limit of this call: p.long_rows, or kRows where the sequences between
 // the two (two row blocks, so the row kernel reads their keys twice) have
 // enough keys for the tile kernel to pay.  Every warp that asks gets the same.
-template <int KEYS>
+template <int KEYS, int ROWS>
 __device__ __forceinline__ int limit_of(const Params& p) {
   if (p.mid_steps == 0) return p.long_rows;
   int64_t steps = 0;
   for (int b = threadIdx.x & 31; b < p.B; b += 32) {
-    const Work w = work_at<KEYS>(p, b, p.long_rows);
+    const Work w = work_at<KEYS, ROWS>(p, b, p.long_rows);
     if (w.rts > 1) steps += static_cast<int64_t>(p.Hkv) * w.tiles;
   }
 #pragma unroll
@@ -150,7 +151,7 @@ __device__ __forceinline__ int64_t run_of(const Params& p, int64_t total, int lo
 
 // A position in the list of steps: within a sequence kv head by kv head, row
 // block by row block, key by key.
-template <int KEYS>
+template <int KEYS, int ROWS>
 struct Cursor {
   Work w;
   int b, kvh, rt, tile;
@@ -164,21 +165,21 @@ struct Cursor {
     kvh = 0;
     do {
       if (++b >= p.B) return;
-      w = work_at<KEYS>(p, b, limit);
+      w = work_at<KEYS, ROWS>(p, b, limit);
     } while (w.tiles == 0 || w.rts == 0);
   }
 };
 
 // The tile kernel's list: an entry for every 256 query rows of a sequence
 // that is its own, with the steps before it.  One CTA of 128 threads.
-template <int KEYS>
+template <int KEYS, int ROWS>
 __device__ __noinline__ void plan_tiles(const Params& p) {
   __shared__ int starts[kWarps * 32 + 1];   // entries before each of 128 sequences
   __shared__ int64_t sums[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t* before = p.entry_steps + 3;
   for (int i = tid; i < p.tile_ctas; i += kWarps * 32) p.joins[i].last = 0;
-  const int limit = limit_of<KEYS>(p);
+  const int limit = limit_of<KEYS, ROWS>(p);
   int64_t steps = 0;
   int entry0 = 0;
   auto block_scan = [&](int64_t v, int64_t& all) {  // inclusive
@@ -241,14 +242,14 @@ __device__ __noinline__ void plan_tiles(const Params& p) {
 // a sum, 32 bytes apart modulo the banks.
 template <int D>
 constexpr int kJointStride = D + 8;
-template <int D, uint32_t RING>
+template <int D, uint32_t RING, int ROWS = kRows>
 __device__ __forceinline__ float* joint_rows(uint8_t* smem, int warp) {
-  static_assert(kRows * kJointStride<D> * 4 <= RING, "a part fits a ring");
+  static_assert(ROWS * kJointStride<D> * 4 <= RING, "a part fits a ring");
   return reinterpret_cast<float*>(smem + warp * RING);
 }
 // The CTA's warps' parts of one unit as one: written to `worker`'s slot, or to
 // the output where the CTA has the whole unit.  A warp takes every kWarps-th row.
-template <bool BF16, int D, uint32_t RING, typename Out>
+template <bool BF16, int D, uint32_t RING, int ROWS = kRows, typename Out>
 __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int warp, int lane, int rows, int worker, int slot,
                                            bool whole, Out out_row) {
   constexpr int V = D / 32;
@@ -258,7 +259,7 @@ __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int w
     float mx = -INFINITY, sum = 0.0f, acc[V];
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
-      ml[k] = *reinterpret_cast<const float2*>(joint_rows<D, RING>(smem, k) + in * kJointStride<D> + D);
+      ml[k] = *reinterpret_cast<const float2*>(joint_rows<D, RING, ROWS>(smem, k) + in * kJointStride<D> + D);
       mx = fmaxf(mx, ml[k].x);
     }
     const float ref = mx == -INFINITY ? 0.0f : mx;
@@ -267,7 +268,7 @@ __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int w
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
       const float f = ex2(ml[k].x - ref);
-      const Vec x = reinterpret_cast<const Vec*>(joint_rows<D, RING>(smem, k) + in * kJointStride<D>)[lane];
+      const Vec x = reinterpret_cast<const Vec*>(joint_rows<D, RING, ROWS>(smem, k) + in * kJointStride<D>)[lane];
       sum = fmaf(ml[k].y, f, sum);
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[j] = fmaf(reinterpret_cast<const float*>(&x)[j], f, acc[j]);
@@ -278,7 +279,7 @@ __device__ __forceinline__ void join_warps(const Params& p, uint8_t* smem, int w
 #pragma unroll
       for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(acc[j] * inv, acc[j + 1] * inv);
     } else {
-      const int64_t at = (static_cast<int64_t>(worker) * 2 + slot) * kRows + in;
+      const int64_t at = (static_cast<int64_t>(worker) * 2 + slot) * ROWS + in;
       Vec x;
 #pragma unroll
       for (int j = 0; j < V; ++j) reinterpret_cast<float*>(&x)[j] = acc[j];
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   const int worker = (static_cast<int>(blockIdx.x) - (p.tile_ctas > 0 ? 1 : 0)) * kWarps + warp;
   const uint32_t ring = smem_addr(smem) + warp * kRingBytes;
   if (worker < 0) {
-    plan_tiles<kKeys>(p);
+    plan_tiles<kKeys, kRows>(p);
     return;
   }
 
@@ -309,13 +310,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // The whole list's length and, from it, this worker's run [w0, w1).
-  const int limit = limit_of<kKeys>(p);
+  const int limit = limit_of<kKeys, kRows>(p);
   int64_t total = 0, mine0 = 0, upto0 = 0;
   int longest = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = 0;
     if (b0 + lane < p.B) {
-      const Work w = work_at<kKeys>(p, b0 + lane, limit);
+      const Work w = work_at<kKeys, kRows>(p, b0 + lane, limit);
       mine = steps_of(p, w);
       longest = max(longest, w.tiles);
     }
@@ -332,13 +333,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
   }
   const int64_t w0 = run * worker, w1 = min(total, w0 + run);
   if (w0 >= w1) return;
-  Cursor<kKeys> cur;
+  Cursor<kKeys, kRows> cur;
   cur.b = 0;
   int64_t seq0 = 0;  // the list's index of cur.b's first step
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     int64_t mine = mine0, upto = upto0;  // of the last 32: all there are in a small batch
     if (p.B > 32) {
-      mine = b0 + lane < p.B ? steps_of(p, work_at<kKeys>(p, b0 + lane, limit)) : 0;
+      mine = b0 + lane < p.B ? steps_of(p, work_at<kKeys, kRows>(p, b0 + lane, limit)) : 0;
       upto = warp_scan(mine);
     }
     const unsigned hit = __ballot_sync(0xffffffffu, seq0 + upto > w0);
@@ -351,17 +352,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) rows_kernel(const __g
     seq0 += __shfl_sync(0xffffffffu, upto, 31);
   }
   cur.limit = limit;
-  cur.w = work_at<kKeys>(p, cur.b, limit);
+  cur.w = work_at<kKeys, kRows>(p, cur.b, limit);
   const int unit = static_cast<int>(div64(w0 - seq0, cur.w.tiles));
   cur.tile = static_cast<int>((w0 - seq0) - static_cast<int64_t>(unit) * cur.w.tiles);
   cur.kvh = unit / cur.w.rts;
   cur.rt = unit - cur.kvh * cur.w.rts;
 
-  Cursor<kKeys> ld = cur;
+  Cursor<kKeys, kRows> ld = cur;
   int64_t ld_t = w0;
   // The page that holds this lane's key of a step, -1 for no key: fetched a
   // step before its first use, so that no step waits for the table.
-  auto page_of = [&](const Cursor<kKeys>& c) {
+  auto page_of = [&](const Cursor<kKeys, kRows>& c) {
     const int key = c.w.base + c.tile * kKeys + (lane & (kKeys - 1));
     if (key < c.w.s.lo || key >= c.w.s.n) return -1;
     return __ldg(p.table + c.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
@@ -620,6 +621,7 @@ __device__ __forceinline__ void tile_join(const Params& p, int i, int y) {
 // row's unit, or for each CTA whose kWarps runs all lie in it (at its first
 // worker's place).  n = 0: no step covers the row (zeros); n = 1: the row
 // kernel has written it.
+template <int ROWS>
 struct RowParts {
   int64_t unit0, run;
   int first, lead, group0, groups, n;  // workers, then groups CTAs, then workers
@@ -638,7 +640,7 @@ struct RowParts {
   __device__ __forceinline__ int64_t at(int k, int row) const {
     const int w = k < lead ? first + k : k < lead + groups ? (group0 + k - lead) * kWarps
                                                            : (group0 + groups) * kWarps + (k - lead - groups);
-    return (w * 2ll + (unit0 < w * run ? 0 : 1)) * kRows + row;
+    return (w * 2ll + (unit0 < w * run ? 0 : 1)) * ROWS + row;
   }
 };
 
@@ -647,8 +649,8 @@ struct RowParts {
 // 32 kKept parts' in registers, loaded together), and adds every SHARE-th
 // part's output, kBatch loaded together whatever their number; the warps' sums
 // meet in shared memory.
-template <bool BF16, int D, int SHARE>
-__device__ __forceinline__ void join_row(const Params& p, const RowParts& rp, int row, uint32_t* dst,
+template <bool BF16, int D, int SHARE, int ROWS>
+__device__ __forceinline__ void join_row(const Params& p, const RowParts<ROWS>& rp, int row, uint32_t* dst,
                                          typename std::conditional<D == 128, float4, float2>::type (*sh_o)[32]) {
   constexpr int V = D / 32;  // columns of a lane, side by side
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
@@ -743,7 +745,7 @@ __device__ __forceinline__ void join_row(const Params& p, const RowParts& rp, in
 // with the other two; one of 16384 keys among 63 of 100 29.4, 30.2 (kRowMixed)
 // and 39.7 (kRowWarp); 7 tokens of 70 sequences 76, 51 and 47.
 enum { kRowCta, kRowMixed, kRowWarp };
-template <bool BF16, int D, int MODE, int KEYS>
+template <bool BF16, int D, int MODE, int KEYS, int ROWS>
 __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_constant__ Params p) {
   using Vec = typename std::conditional<D == 128, float4, float2>::type;
   constexpr int W = kJoinWarps, kPerCta = MODE == kRowCta ? 1 : W;
@@ -766,20 +768,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     int b, y, h, kvh;
     int64_t seq0, run;
   };
-  const int limit = limit_of<KEYS>(p);
+  const int limit = limit_of<KEYS, ROWS>(p);
   auto look = [&](int item) {
     Item it;
     it.h = item % p.H;
     it.y = item / p.H % p.combine_rows;
     it.b = item / p.H / p.combine_rows;
     it.kvh = static_cast<int>(fdiv(static_cast<uint32_t>(it.h), p.div_g));
-    it.w = work_at<KEYS>(p, min(it.b, p.B - 1), limit);
+    it.w = work_at<KEYS, ROWS>(p, min(it.b, p.B - 1), limit);
     it.seq0 = it.run = 0;
     if (p.B <= 32) {  // the list in one scan; else what the row kernel left
       int64_t mine = 0;
       int longest = 0;
       if (lane < p.B) {
-        const Work w = work_at<KEYS>(p, lane, limit);
+        const Work w = work_at<KEYS, ROWS>(p, lane, limit);
         mine = steps_of(p, w);
         longest = w.tiles;
       }
@@ -796,10 +798,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
     }
   };
   auto parts_of = [&](const Item& it, int r) {
-    RowParts rp;
+    RowParts<ROWS> rp;
     rp.n = 0;
     if (it.w.tiles > 0) {
-      const int64_t begin = it.seq0 + (static_cast<int64_t>(it.kvh) * it.w.rts + r / kRows) * it.w.tiles;
+      const int64_t begin = it.seq0 + (static_cast<int64_t>(it.kvh) * it.w.rts + r / ROWS) * it.w.tiles;
       rp.find(begin, begin + it.w.tiles, it.run);
     }
     return rp;
@@ -808,9 +810,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
   auto join = [&](const Item& it, auto share, auto take) {
     for (int i = it.y; i < it.w.s.m; i += p.combine_rows) {
       const int r = i * p.G + (it.h - it.kvh * p.G);
-      const RowParts rp = parts_of(it, r);
+      const RowParts<ROWS> rp = parts_of(it, r);
       if (rp.n != 1 && take(rp.n))
-        join_row<BF16, D, decltype(share)::value>(p, rp, r % kRows, out_row(it.w.s.t0 + i, it.h), sh_o);
+        join_row<BF16, D, decltype(share)::value, ROWS>(p, rp, r % ROWS, out_row(it.w.s.t0 + i, it.h), sh_o);
     }
   };
   const std::integral_constant<int, 1> alone;
@@ -857,13 +859,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const __grid_c
 
 #include "paged_rows8.cuh"
 
-// Q8: over e4m3 caches.
-template <bool BF16, int D, int CAP, bool Q8>
+// Q8: over e4m3 caches, in units of ROWS query rows.
+template <bool BF16, int D, int CAP, bool Q8, int ROWS>
 int launch(const Params& p, int ctas, cudaStream_t st) {
-  constexpr uint32_t kSmem = kWarps * (Q8 ? kRing8Bytes : kRingBytes);
+  constexpr uint32_t kSmem = kWarps * (Q8 ? kRing8Bytes<ROWS> : kRingBytes);
   constexpr int KEYS = Q8 ? kKeys8 : kKeys;
   void (*kernel)(const Params);
-  if constexpr (Q8) kernel = rows8_kernel<BF16, D, CAP>;
+  if constexpr (Q8) kernel = rows8_kernel<BF16, D, CAP, ROWS>;
   else kernel = rows_kernel<BF16, D, CAP>;
   static std::atomic<uint64_t> done{0};
   if (!attributes_set(done)) {
@@ -890,21 +892,21 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  auto combine = p.join_mode == kRowCta     ? combine_kernel<BF16, D, kRowCta, KEYS>
-                 : p.join_mode == kRowMixed ? combine_kernel<BF16, D, kRowMixed, KEYS>
-                                            : combine_kernel<BF16, D, kRowWarp, KEYS>;
+  auto combine = p.join_mode == kRowCta     ? combine_kernel<BF16, D, kRowCta, KEYS, ROWS>
+                 : p.join_mode == kRowMixed ? combine_kernel<BF16, D, kRowMixed, KEYS, ROWS>
+                                            : combine_kernel<BF16, D, kRowWarp, KEYS, ROWS>;
   return cudaLaunchKernelEx(&cfg, combine, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
-template <bool BF16, int D, bool Q8>
+template <bool BF16, int D, bool Q8, int ROWS>
 int launch_cap(const Params& p, int cap, int ctas, cudaStream_t st) {
-  if (cap == kNoCap) return launch<BF16, D, kNoCap, Q8>(p, ctas, st);
-  return cap == kCapPlain ? launch<BF16, D, kCapPlain, Q8>(p, ctas, st) : launch<BF16, D, kCapSeries, Q8>(p, ctas, st);
+  if (cap == kNoCap) return launch<BF16, D, kNoCap, Q8, ROWS>(p, ctas, st);
+  return cap == kCapPlain ? launch<BF16, D, kCapPlain, Q8, ROWS>(p, ctas, st) : launch<BF16, D, kCapSeries, Q8, ROWS>(p, ctas, st);
 }
-template <bool Q8>
+template <bool Q8, int ROWS>
 int launch_type(const Params& p, bool bf16, int dim, int cap, int ctas, cudaStream_t st) {
-  if (bf16) return dim == 64 ? launch_cap<true, 64, Q8>(p, cap, ctas, st) : launch_cap<true, 128, Q8>(p, cap, ctas, st);
-  return dim == 64 ? launch_cap<false, 64, Q8>(p, cap, ctas, st) : launch_cap<false, 128, Q8>(p, cap, ctas, st);
+  if (bf16) return dim == 64 ? launch_cap<true, 64, Q8, ROWS>(p, cap, ctas, st) : launch_cap<true, 128, Q8, ROWS>(p, cap, ctas, st);
+  return dim == 64 ? launch_cap<false, 64, Q8, ROWS>(p, cap, ctas, st) : launch_cap<false, 128, Q8, ROWS>(p, cap, ctas, st);
 }
 
 }  // namespace
@@ -973,6 +975,7 @@ int64_t place(const B200kPagedAttentionArgs* a, bool q8, int sms, uint8_t* ws, P
     at += (bytes + 255) / 256 * 256;
     return r;
   };
+  static_assert(kCtas8<128, 8> * 8 <= kCtasPerSm * kRows, "parts of units of 8 rows");
   const int64_t slots = static_cast<int64_t>(sms) * kCtasPerSm * kWarps * 2 * kRows;
   uint8_t* part_o = take(slots * a->head_dim * 4);
   uint8_t* part_ml = take(slots * 8);
@@ -1073,6 +1076,8 @@ int attend(const B200kPagedAttentionArgs* a, const B200kPagedAttentionQuantArgs*
     p.s_page = q8->scale_strides[0];
     p.s_slot = q8->scale_strides[1];
     p.s_head = q8->scale_strides[2];
+    const int64_t last = (a->num_pages - 1) * p.c_page + (a->page_size - 1) * p.c_slot + (a->kv_heads - 1) * p.c_head;
+    p.far_rows = (last >> 4) >= 0xffffffffLL;
   }
   p.out = static_cast<uint16_t*>(a->out);
   p.table = a->page_table;
@@ -1084,7 +1089,10 @@ int attend(const B200kPagedAttentionArgs* a, const B200kPagedAttentionQuantArgs*
   p.lin = scale * kLog2e;
   p.cap2 = a->softcap * kLog2e;
   if (!std::isfinite(p.mul) || !std::isfinite(p.lin)) return B200K_ERR_ARG;  // a cap too small for its scale
-  const int ctas = sms * kCtasPerSm;
+  // Over e4m3 caches, when no sequence is said to have more than 8 query rows,
+  // units of so many.
+  const bool few = q8 && most_rows(a) <= 8;
+  const int ctas = sms * (few ? kCtas8<128, 8> : kCtasPerSm);
   p.workers = ctas * kWarps;
   place(a, q8 != nullptr, sms, static_cast<uint8_t*>(a->workspace), &p);
   p.status = a->status;
@@ -1100,7 +1108,8 @@ int attend(const B200kPagedAttentionArgs* a, const B200kPagedAttentionQuantArgs*
   p.join_mode = items <= 4ll * sms ? kRowCta : items <= 16ll * sms ? kRowMixed : kRowWarp;
   const bool bf16 = a->dtype == B200K_BF16;
   const int dim = static_cast<int>(a->head_dim);
-  return q8 ? launch_type<true>(p, bf16, dim, cap, ctas, st) : launch_type<false>(p, bf16, dim, cap, ctas, st);
+  if (!q8) return launch_type<false, kRows>(p, bf16, dim, cap, ctas, st);
+  return few ? launch_type<true, 8>(p, bf16, dim, cap, ctas, st) : launch_type<true, kRows>(p, bf16, dim, cap, ctas, st);
 }
 
 }  // namespace
