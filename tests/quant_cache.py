@@ -39,3 +39,26 @@ def attend(x, scale, softcap=0.0, window=0):
     """(out, sum_j p_j |v_j|) in 64 bits."""
     q, k8, v8, ks, vs, *rest = x
     return ref.paged_attention(q, values(k8, ks), values(v8, vs), *rest, scale, softcap, window)
+
+
+def rounded(x, dtype):
+    """paged_inputs' caches with every key and value rounded to `dtype`, as sequences of many query
+    rows take them: codes times scales as the values, scales of one."""
+    q, k8, v8, ks, vs, *rest = x
+    k, v = values(k8, ks).to(dtype), values(v8, vs).to(dtype)
+    return (q, k, v, *rest)
+
+
+def attention_close(got, x, scale, softcap=0.0, window=0):
+    """serving_reference.attention_close for each sequence, on what the codes and scales stand for or
+    on that rounded to q's type, whichever the sequence's kernel takes."""
+    q, starts = x[0], x[6].tolist()
+    want, size = attend(x, scale, softcap, window)
+    near, near_size = ref.paged_attention(*rounded(x, q.dtype), scale, softcap, window)
+    for a, b in zip([0, *starts], [*starts, len(q)]):
+        if a == b:
+            continue
+        try:
+            ref.attention_close(got[a:b], want[a:b], size[a:b], q.dtype)
+        except AssertionError:
+            ref.attention_close(got[a:b], near[a:b], near_size[a:b], q.dtype)

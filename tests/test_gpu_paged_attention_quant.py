@@ -1,7 +1,9 @@
 """b200::paged_attention_quant against the formula in 64 bits on what the
-caches' codes and scales stand for (the bound is derived at
-serving_reference.attention_close; the weights here are always rounded to f16,
-whose half step is below bf16's).  Everything of the caches and scales that no
+caches' codes and scales stand for: in sequences of few query rows that itself,
+in those of many each value rounded to q's type (quant_cache.attention_close
+takes a sequence by either).  The bound is derived at
+serving_reference.attention_close; for few rows the weights are rounded to f16,
+whose half step is below bf16's.  Everything of the caches and scales that no
 query may see holds NaN, and tables name no page that is not needed."""
 import pytest
 import torch
@@ -22,8 +24,7 @@ def run(inputs, softcap=0.0, window=0, max_q=0, scale=0.0):
     q = inputs[0]
     runtime.gemm_status()
     out = op(*inputs, scale, softcap, window, max_q)
-    want, size = qc.attend(inputs, scale or ref.default_scale(q.shape[2]), softcap, window)
-    ref.attention_close(out, want, size, q.dtype)
+    qc.attention_close(out, inputs, scale or ref.default_scale(q.shape[2]), softcap, window)
     end = int(inputs[6][-1])
     assert out[end:].abs().sum() == 0
     assert runtime.gemm_status() == 0
@@ -36,6 +37,32 @@ def run(inputs, softcap=0.0, window=0, max_q=0, scale=0.0):
 def test_single_tokens(H, hkv, D, dtype):
     ns = [1, 2, 15, 16, 17, 31, 32, 33, 100, 333, 1, 64]
     run(qc.paged_inputs([1] * len(ns), ns, H, hkv, D, 16, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,hkv,q", [(32, 8, 1), (8, 8, 1), (8, 1, 1), (7, 1, 1), (28, 4, 1), (8, 8, 5), (16, 8, 4), (16, 16, 8)])
+def test_units_of_eight_rows(H, hkv, q, D, dtype):
+    """Calls whose longest sequence is said to have at most 8 query rows; and a hint that is too small."""
+    ns = [1, 31, 32, 33, 64, 700, 5, 2000, 0, 130]
+    qs = [min(q, max(1, n)) for n in ns]
+    run(qc.paged_inputs(qs, ns, H, hkv, D, 16, dtype, pad=2), max_q=q)
+    qs[3], qs[5] = 20, 40
+    run(qc.paged_inputs(qs, ns, H, hkv, D, 16, dtype, spread=4), max_q=q)
+    run(qc.paged_inputs(qs, ns, H, hkv, D, 24, dtype, window=50), softcap=20.0, window=50, max_q=q)
+
+
+@pytest.mark.parametrize("max_q", [0, 1])
+@pytest.mark.parametrize("what", ["k", "v_scale"])
+def test_a_nan_in_units_of_eight_rows(what, max_q):
+    q, k8, v8, ks, vs, table, q_start, kv_len = qc.paged_inputs([1, 1], [200, 90], 8, 2, 128, 16, BF)
+    clean = op(q, k8, v8, ks, vs, table, q_start, kv_len, 0.0, 0.0, 0, max_q)
+    if what == "k":
+        k8.view(torch.uint8)[table[0, 3].long(), 5, 1, 7] = 0x7F
+    else:
+        vs[table[0, 3].long(), 5, 1] = float("nan")
+    out = op(q, k8, v8, ks, vs, table, q_start, kv_len, 0.0, 0.0, 0, max_q)
+    assert out[0, 4:].isnan().all() and torch.equal(out[0, :4], clean[0, :4]) and torch.equal(out[1], clean[1])
 
 
 @pytest.mark.parametrize("m", [1, 100])
@@ -116,10 +143,10 @@ def test_far_magnitudes_of_bf16_queries(m, scale):
     run((q, *rest), scale=0.125 / scale)
 
 
-@pytest.mark.parametrize("m", [1, 70])
-def test_key_scales_of_any_size(m):
-    """Keys of 1e30 and of 1e-30: the scales are put into the fp32 scores."""
-    q, k8, v8, ks, vs, *rest = qc.paged_inputs([m], [150], 4, 2, 128, 16, HF)
+@pytest.mark.parametrize("m,dtype", [(1, HF), (1, BF), (70, BF)])  # (many rows: keys in q's type)
+def test_key_scales_of_any_size(m, dtype):
+    """Keys of 1e30 and of 1e-30."""
+    q, k8, v8, ks, vs, *rest = qc.paged_inputs([m], [150], 4, 2, 128, 16, dtype)
     run((q, k8, v8, ks * 2.0**100, vs, *rest), scale=2.0**-100 * 0.1)
     run((q, k8, v8, ks * 2.0**-100, vs, *rest), scale=2.0**100 * 0.1)
 
@@ -263,8 +290,7 @@ def test_cache_offsets_past_32_bits():
         start = torch.tensor([0, m], dtype=torch.int32, device="cuda")
         out = op(q, k8, v8, ks, vs, table, start, n)
         near = torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda")
-        want, size = qc.attend((q, *small, near, start, n), ref.default_scale(D))
-        ref.attention_close(out, want, size, BF)
+        qc.attention_close(out, (q, *small, near, start, n), ref.default_scale(D))
 
 
 def test_bad_indexes_are_reported_and_stay_in_bounds():
@@ -336,8 +362,7 @@ def test_a_replayed_graph_follows_its_index_tensors():
     for lens in ([1, 300], [200, 16], [0, 77]):
         x[7].copy_(torch.tensor(lens, dtype=torch.int32))
         g.replay()
-        want, size = qc.attend(x, ref.default_scale(64))
-        ref.attention_close(out, want, size, BF)
+        qc.attention_close(out, x, ref.default_scale(64))
 
 
 def test_results_repeat_bit_for_bit():
@@ -353,8 +378,7 @@ def test_c_abi():
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     cabi.paged_attention_quant(*x, out, status=status)
     assert status.item() == 0
-    want, size = qc.attend(x, ref.default_scale(128))
-    ref.attention_close(out, want, size, HF)
+    qc.attention_close(out, x, ref.default_scale(128))
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -369,8 +393,7 @@ def test_stalled_wait_times_out_and_context_survives(D, dtype):
     status.zero_()
     cabi.paged_attention_quant(*x, out, status=status)
     assert status.item() == 0
-    want, size = qc.attend(x, ref.default_scale(D))
-    ref.attention_close(out, want, size, dtype)
+    qc.attention_close(out, x, ref.default_scale(D))
 
 
 @pytest.mark.parametrize("D", [64, 128])

@@ -132,8 +132,7 @@ def test_every_stage_against_its_formula(setting):
         for codes, scale, row in ((kept[0], kept[2], ref.rotate(k, cos[pos.long()], sin[pos.long()])[0]), (kept[1], kept[3], v.double())):
             z = row / scale.double()[..., None]
             assert ((codes.double() - z).abs() <= quant.code_step(z) + 448 * 2.0**-20).all()
-        want, size = qc.attend((s["q"], *caches, table, q_start, kv_len), ref.default_scale(D))
-        ref.attention_close(s["a"], want, size, BF)
+        qc.attention_close(s["a"], (s["q"], *caches, table, q_start, kv_len), ref.default_scale(D))
         quant_close(s["a8"], s["as_"], s["a"].flatten(1).double(), 2.0**-21)
         mm_close(s["o"], layer.o, s["a8"], s["as_"])
         total, y = ref.add_rms_norm(s["o"], total, layer.norm2, 1e-5)

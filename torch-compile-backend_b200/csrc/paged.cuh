@@ -60,7 +60,8 @@ struct Params {
   const uint8_t *k8, *v8;
   const float *ks, *vs;
   int64_t s_page, s_slot, s_head;
-  int32_t far_rows;            // row offsets past 2^32 times 16 bytes
+  uint32_t c16_page, c16_slot, c16_head;  // their strides in 16 bytes
+  int32_t far_rows;            // offsets past 2^32 in those, or in scales
   uint16_t* out;               // [T, H, D] contiguous
   const int32_t *table, *q_start, *kv_len;
   // base-2 scores: y = x * mul; with a cap (cap_far) mul = 2 scale log2(e) / cap,

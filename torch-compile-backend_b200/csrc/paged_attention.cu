@@ -30,6 +30,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "e4m3.cuh"
 #include "host_common.h"
 #include "paged.cuh"
 #include "rowreduce.cuh"
@@ -1038,7 +1039,11 @@ int attend(const B200kPagedAttentionArgs* a, const B200kPagedAttentionQuantArgs*
     return cudaMemsetAsync(a->out, 0, n, st) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
   }
   if (!a->k_cache || !a->v_cache || !a->page_table || !a->q_start || !a->kv_len) return B200K_ERR_ARG;
-  if (q8 && (!q8->k_scale || !q8->v_scale)) return B200K_ERR_ARG;
+  if (q8) {
+    if (!q8->k_scale || !q8->v_scale) return B200K_ERR_ARG;
+    for (int d = 0; d < 3; ++d)
+      if (q8->scale_strides[d] < 0) return B200K_ERR_SHAPE;
+  }
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < place(a, q8 != nullptr, sms, nullptr, nullptr)) return B200K_ERR_ARG;
   Params p;
   std::memset(&p, 0, sizeof(p));
@@ -1076,8 +1081,13 @@ int attend(const B200kPagedAttentionArgs* a, const B200kPagedAttentionQuantArgs*
     p.s_page = q8->scale_strides[0];
     p.s_slot = q8->scale_strides[1];
     p.s_head = q8->scale_strides[2];
-    const int64_t last = (a->num_pages - 1) * p.c_page + (a->page_size - 1) * p.c_slot + (a->kv_heads - 1) * p.c_head;
-    p.far_rows = (last >> 4) >= 0xffffffffLL;
+    p.c16_page = static_cast<uint32_t>(p.c_page / 16);
+    p.c16_slot = static_cast<uint32_t>(p.c_slot / 16);
+    p.c16_head = static_cast<uint32_t>(p.c_head / 16);
+    auto last = [&](int64_t page, int64_t slot, int64_t head) {
+      return static_cast<double>(a->num_pages) * page + static_cast<double>(a->page_size) * slot + static_cast<double>(a->kv_heads) * head;
+    };
+    p.far_rows = last(p.c_page, p.c_slot, p.c_head) / 16 > 4.2e9 || last(p.s_page, p.s_slot, p.s_head) > 4.2e9;
   }
   p.out = static_cast<uint16_t*>(a->out);
   p.table = a->page_table;

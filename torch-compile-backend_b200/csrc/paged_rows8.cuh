@@ -145,27 +145,44 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas8<D, ROWS>) rows8_kernel(con
     if (ld_t < w1) {
       const uint32_t sk = ring + ld_stage * kStage, sv = sk + kTile, sc = sv + kTile;
       const int c = lane % kChunks;
-      const Place8 at = place8(p, page, ld.w.base + ld.tile * kKeys8 + lane, ld.w.s.lo, ld.w.s.n, ld.kvh);
-      // rows start on 16 bytes: an offset in those goes through one shuffle
-      const uint32_t at16 = at.row >= 0 ? static_cast<uint32_t>(at.row >> 4) : ~0u;
-      const unsigned none = p.far_rows ? __ballot_sync(0xffffffffu, at.row < 0) : 0;
-#pragma unroll
-      for (int i = 0; i < kKeys8 / kRowsPerCp; ++i) {
-        const int row = i * kRowsPerCp + lane / kChunks;
-        uint32_t o16 = __shfl_sync(0xffffffffu, at16, row);
-        bool real = o16 != ~0u;
-        int64_t e = static_cast<int64_t>(real ? o16 : 0u) * 16 + c * 16;
-        if (p.far_rows) {  // past 2^32 of them
-          const uint32_t hi = __shfl_sync(0xffffffffu, static_cast<uint32_t>(at.row >> 36), row);
-          real = !((none >> row) & 1u);
-          e = real ? (static_cast<int64_t>(hi) << 36) + static_cast<int64_t>(o16) * 16 + c * 16 : 0;
+      const int key = ld.w.base + ld.tile * kKeys8 + lane;
+      if (!p.far_rows) {
+        // Offsets in rows' 16 bytes and in scales, 32 bits each: one shuffle and
+        // one multiply-add an address.
+        uint32_t row16 = ~0u, scale = 0;
+        if (page >= 0 && page < p.num_pages) {  // -1: no key
+          const uint32_t in = static_cast<uint32_t>(key) - fdiv(static_cast<uint32_t>(key), p.div_page) * static_cast<uint32_t>(p.page_size);
+          row16 = static_cast<uint32_t>(page) * p.c16_page + in * p.c16_slot + static_cast<uint32_t>(ld.kvh) * p.c16_head;
+          scale = static_cast<uint32_t>(page) * static_cast<uint32_t>(p.s_page) + in * static_cast<uint32_t>(p.s_slot) +
+                  static_cast<uint32_t>(ld.kvh) * static_cast<uint32_t>(p.s_head);
+        } else if (key >= ld.w.s.lo && key < ld.w.s.n && p.status) {
+          atomicCAS(p.status, 0, B200K_ERR_INDEX);
         }
-        cp16(sk + k8_at<D>(row, c), p.k8 + e, real);
-        cp16(sv + v8_at<D>(row, c), p.v8 + e, real);
+        const uint8_t *kc = p.k8 + c * 16, *vc = p.v8 + c * 16;
+#pragma unroll
+        for (int i = 0; i < kKeys8 / kRowsPerCp; ++i) {
+          const int row = i * kRowsPerCp + lane / kChunks;
+          const uint32_t o = __shfl_sync(0xffffffffu, row16, row);
+          const uint64_t e = static_cast<uint64_t>(o == ~0u ? 0u : o) * 16;
+          cp16(sk + k8_at<D>(row, c), kc + e, o != ~0u);
+          cp16(sv + v8_at<D>(row, c), vc + e, o != ~0u);
+        }
+        cp4(sc + lane * 4, p.ks + scale, row16 != ~0u);
+        cp4(sc + 128 + lane * 4, p.vs + scale, row16 != ~0u);
+      } else {
+        const Place8 at = place8(p, page, key, ld.w.s.lo, ld.w.s.n, ld.kvh);
+#pragma unroll 1
+        for (int i = 0; i < kKeys8 / kRowsPerCp; ++i) {
+          const int row = i * kRowsPerCp + lane / kChunks;
+          const int64_t o = __shfl_sync(0xffffffffu, at.row, row);
+          const int64_t e = (o >= 0 ? o : 0) + c * 16;
+          cp16(sk + k8_at<D>(row, c), p.k8 + e, o >= 0);
+          cp16(sv + v8_at<D>(row, c), p.v8 + e, o >= 0);
+        }
+        const bool real = at.scale >= 0;
+        cp4(sc + lane * 4, p.ks + (real ? at.scale : 0), real);
+        cp4(sc + 128 + lane * 4, p.vs + (real ? at.scale : 0), real);
       }
-      const bool real = at.scale >= 0;
-      cp4(sc + lane * 4, p.ks + (real ? at.scale : 0), real);
-      cp4(sc + 128 + lane * 4, p.vs + (real ? at.scale : 0), real);
       if (++ld_t < w1) {
         ld.next(p);
         page = page_of(ld);

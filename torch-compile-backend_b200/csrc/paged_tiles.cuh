@@ -190,6 +190,252 @@ struct Walk {
   }
 };
 
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTmemO = 256;
+// Tensor-memory columns: scores of block g of tile t at 128 t + 64 (g & 1),
+// its probabilities in the first 32 of them, O_t at 256 + D t.
+
+// What the roles of a CTA share: barriers, and 16-bit tiles in shared memory.
+struct Shared {
+  uint64_t *q_full, *q_empty;
+  uint64_t *k_full, *k_empty, *v_full, *v_empty;  // [stages]
+  uint64_t *s_full, *p_full, *o_done;             // [4] by tile and buffer
+  uint64_t *o_free;                               // [2] by tile
+  uint64_t *drain;                                // [4] by issuer
+  uint8_t *sQ, *sK, *sV;
+  const volatile int* copied;                     // [2 stages] of K, of V: the stage's block came by cp.async
+};
+
+// The MMA issuers: warps 8, 9 of S_t = Q_t K^T of tile t = 0, 1, warps 10, 11 of
+// O_t += P_t V.  S: stages; Q8: converted blocks, whose writers fence themselves.
+template <bool BF16, int D, int S, bool Q8>
+__device__ __forceinline__ void issue_products(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
+                                               int warp, int lane) {
+  constexpr uint32_t kTile = kHalfTile * (D / 64), kBlk = kHalfBlk * (D / 64);
+  Portion po;
+  const int t = warp & 1;
+  const bool scores = warp < 10;
+  const uint32_t fmt = BF16 ? 1u : 0u;
+  // fp32 accumulators; B of Q K^T K-major, of P V N-major
+  const uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kBlock >> 3) << 17) | ((128u >> 4) << 24);
+  const uint32_t idesc_pv =
+      (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
+  const uint32_t tS = tmem_base + t * 128, tO = tmem_base + kTmemO + t * D;
+  const uint64_t dq = gemm::sw128_desc(smem_u32(b.sQ) + t * kTile, 16, 1024);
+  const uint64_t dk = gemm::sw128_desc(smem_u32(b.sK), 16, 1024);
+  const uint64_t dv = gemm::sw128_desc(smem_u32(b.sV), kHalfBlk, 1024);
+  uint64_t* full = scores ? b.k_full : b.v_full;
+  uint64_t* empty = scores ? b.k_empty : b.v_empty;
+  const volatile int* by_copy = scores ? b.copied : b.copied + S;
+  int c = 0;      // key blocks passed, over all portions
+  int g = 0;      // of them this tile's
+  int done = 0;   // portions in which this tile had steps
+  bool ok = true;
+  for (int li = 0; ok && walk.next(p, po); ++li) {
+    if (scores) {
+      ok = warp_wait(b.q_full, li & 1, ctl);
+      if (p.q_box == 0) gemm::fence_async_smem();
+    }
+    for (int j = po.beg; ok && j < po.end; ++j, ++c) {
+      const int st = c % S;
+      if (!(ok = warp_wait(&full[st], (c / S) & 1, ctl))) break;
+      if (j < po.t_beg[t] || j >= po.t_end[t]) {
+        // not a block of this tile (the arrival follows the landing, so it
+        // belongs to this phase)
+        if (lane == 0) gemm::mbar_arrive(&empty[st]);
+        __syncwarp();
+        continue;
+      }
+      if (!Q8 && by_copy[st]) gemm::fence_async_smem();  // cp.async's writes, before the MMA's reads
+      const int buf = g & 1;
+      if (scores) {
+        // P V of the block two before has read P from this buffer
+        if (g > 1 && !(ok = warp_wait(&b.o_done[t * 2 + buf], ((g >> 1) - 1) & 1, ctl))) break;
+        gemm::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_ss(tS + buf * 64, dq + (((k >> 2) * kHalfTile + (k & 3) * 32) >> 4),
+                  dk + ((st * kBlk + (k >> 2) * kHalfBlk + (k & 3) * 32) >> 4), idesc_s, k != 0);
+        if (!(t == 0 && g == 0 && (p.test_flags & B200K_PAGED_TEST_WITHHOLD_SCORES))) commit(&b.s_full[t * 2 + buf]);
+        commit(&b.k_empty[st]);
+        if (j + 1 == po.t_end[t]) commit(b.q_empty);
+      } else {
+        const bool first = j == po.t_beg[t];
+        // the epilogue of the portion before has read O
+        if (first && done > 0 && !(ok = warp_wait(&b.o_free[t], (done - 1) & 1, ctl))) break;
+        if (!(ok = warp_wait(&b.p_full[t * 2 + buf], (g >> 1) & 1, ctl))) break;
+        gemm::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kBlock / 16; ++k)
+          umma_ts(tO, tS + buf * 64 + k * 8, dv + ((st * kBlk + k * 2048) >> 4), idesc_pv, (!first || k != 0) ? 1u : 0u);
+        commit(&b.o_done[t * 2 + buf]);
+        commit(&b.v_empty[st]);
+      }
+      ++g;
+    }
+    if (!ok) break;
+    if (po.t_end[t] > po.t_beg[t]) ++done;
+    else if (scores && lane == 0) gemm::mbar_arrive(b.q_empty);
+    __syncwarp();
+  }
+  // every MMA of this warp completes before tensor memory is freed
+  commit(&b.drain[warp - 8]);
+  gemm::wait_bar_drain(&b.drain[warp - 8], 0, 100000000ull);
+  __syncwarp();
+}
+
+// The softmax warps 0-7, one thread a query row.
+template <bool BF16, int D, int CAP>
+__device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
+                                             int64_t run, int warp, int lane) {
+  Portion po;
+  const int t = warp >> 2, quarter = warp & 3;
+  const int in_unit = t * 128 + quarter * 32 + lane;
+  const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t tS = t_lane + t * 128, tO = t_lane + kTmemO + t * D;
+  int g = 0;
+  bool ok = true;
+  while (ok && walk.next(p, po)) {
+    if (!po.whole && po.slot == 1 && threadIdx.x == 0) {
+      // the run's last unit goes on in the next CTAs, the steps that are left at `run` each
+      const int left = walk.u.ub1 - po.end;
+      p.joins[blockIdx.x] = Join{static_cast<int>(blockIdx.x + (left + run - 1) / run), walk.u.s.t0, po.kvh, walk.u.r0,
+                                 walk.u.rows};
+    }
+    const int r = walk.u.r0 + in_unit;
+    const bool real = r < walk.u.rows;
+    const uint32_t tok = fdiv(static_cast<uint32_t>(min(r, walk.u.rows - 1)), p.div_g);
+    const int pos = walk.u.s.first + static_cast<int>(tok);
+    // positions of the warp's first and last row
+    const int w_lo = __shfl_sync(0xffffffffu, pos, 0), w_hi = __shfl_sync(0xffffffffu, pos, 31);
+    float m = -INFINITY, l = 0.0f;
+    const int jb = po.t_beg[t], je = po.t_end[t];
+    for (int j = jb; j < je; ++j, ++g) {
+      const uint32_t buf = g & 1;
+      if (!(ok = warp_wait(&b.s_full[t * 2 + buf], (g >> 1) & 1, ctl))) break;
+      gemm::tc_fence_after();
+      float s[kBlock];
+      {
+        uint32_t raw[kBlock / 32][32];
+#pragma unroll
+        for (int c = 0; c < kBlock / 32; ++c) gemm::tmem_ld32(tS + buf * 64 + c * 32, raw[c]);
+        gemm::tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kBlock / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(raw[c][i]);
+      }
+      if (CAP != kNoCap) {
+#pragma unroll
+        for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, s[c]);
+      }
+      const int key0 = j * kBlock;
+      if (key0 + kBlock - 1 > w_lo || (p.window > 0 && key0 <= w_hi - p.window)) {  // warp-uniform
+        const int hi = pos - key0, lo = p.window > 0 ? hi - p.window : -1;
+#pragma unroll
+        for (int c = 0; c < kBlock; ++c)
+          if (c > hi || c <= lo) s[c] = -INFINITY;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c + 8 <= kBlock; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], s[c + i], s[c + 4 + i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = max2(mx[i], s[kBlock - 4 + i]);
+      float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
+      if (CAP == kNoCap) top *= p.mul;
+      const float was = m;
+      float alpha = 1.0f;
+      bool moved = false;
+      // A NaN score, and an infinite one (0 * top), makes the maximum NaN and
+      // with it every probability and sum of the row from here on.
+      if (!(top <= m + kTileLag<BF16>)) {
+        m = fmaf(0.0f, top, top);
+        alpha = ex2(was - m);
+        moved = j > jb;
+      }
+      // probabilities are rounded to the input type, half a step each, in f16
+      // down to 2^-26 of the row's maximum (smaller ones by less than 2^-36 of it)
+      const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<BF16>;
+      float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(-ref, -ref);
+      uint32_t pk[kBlock / 2];
+#pragma unroll
+      for (int c = 0; c < kBlock; c += 2) {
+        const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
+        const float2 e = c % kFmaEvery == kFmaEvery - 2 ? ex2_fma<BF16>(x) : make_float2(ex2(x.x), ex2(x.y));
+        sum2[c / 2 % 2] = __fadd2_rn(sum2[c / 2 % 2], e);
+        pk[c / 2] = pack16<BF16>(e.x, e.y);
+      }
+      l = fmaf(l, alpha, (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
+      if (__any_sync(0xffffffffu, moved)) {
+        // P V of the block before has written O
+        if (!(ok = warp_wait(&b.o_done[t * 2 + (buf ^ 1)], ((g - 1) >> 1) & 1, ctl))) break;
+        gemm::tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          gemm::tmem_ld32(tO + c * 32, o);
+          gemm::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(tO + c * 32, o);
+        }
+      }
+      tmem_st32(tS + buf * 64, pk);
+      tmem_wait_st();
+      gemm::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) gemm::mbar_arrive(&b.p_full[t * 2 + buf]);
+    }
+    if (!ok) break;
+    const bool had = je > jb;
+    if (had && !(ok = warp_wait(&b.o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, ctl))) break;
+    gemm::tc_fence_after();
+    // a row without keys has m = -inf (and l the sum of its 2^-125)
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    const int64_t part = static_cast<int64_t>(blockIdx.x) * 2 + po.slot;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t o[32];
+      if (had) {
+        gemm::tmem_ld32(tO + c * 32, o);
+        gemm::tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+      if (real && po.whole) {
+        uint16_t* dst = p.out + (static_cast<int64_t>(walk.u.s.t0 + tok) * p.H + po.kvh * p.G + (r - tok * p.G)) * D + c * 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint4 u;
+          u.x = pack16<BF16>(__uint_as_float(o[i * 8 + 0]) * inv, __uint_as_float(o[i * 8 + 1]) * inv);
+          u.y = pack16<BF16>(__uint_as_float(o[i * 8 + 2]) * inv, __uint_as_float(o[i * 8 + 3]) * inv);
+          u.z = pack16<BF16>(__uint_as_float(o[i * 8 + 4]) * inv, __uint_as_float(o[i * 8 + 5]) * inv);
+          u.w = pack16<BF16>(__uint_as_float(o[i * 8 + 6]) * inv, __uint_as_float(o[i * 8 + 7]) * inv);
+          reinterpret_cast<uint4*>(dst)[i] = u;
+        }
+      } else if (real) {
+        // [4 columns][256 rows]: a warp's rows side by side
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          reinterpret_cast<uint4*>(p.tile_o)[(part * (D / 4) + c * 8 + i) * kUnitRows + in_unit] =
+              make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+      }
+      __syncwarp();  // the next load is warp-collective
+    }
+    if (had) {
+      gemm::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) gemm::mbar_arrive(&b.o_free[t]);
+    }
+    if (!po.whole && real)
+      reinterpret_cast<float2*>(p.tile_ml)[part * kUnitRows + in_unit] = make_float2(m, l);
+  }
+}
+
 // Boxes of a 4-d view, inner dim first; sizes and strides in elements of `bytes`.
 bool make_map(CUtensorMap* map, CUtensorMapDataType type, int bytes, CUtensorMapSwizzle swizzle, const void* ptr, const int64_t (&sizes)[4], const int64_t (&strides)[3],
               const cuuint32_t (&box)[4]) {
