@@ -225,8 +225,11 @@ __global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_con
         w[j] = y * cs[j] + x * sn[j];
       }
     }
-    uint32_t top = max(top8(u), top8(w));
-    for (int o = 1; o < p.units; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    uint32_t top = 0;
+    if (__any_sync(0xffffffffu, !is_q)) {
+      top = max(top8(u), top8(w));
+      for (int o = 1; o < p.units; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
     if (!real || h >= all) continue;
     if (is_q) {
       uint16_t* dst = p.q_out + (static_cast<int64_t>(tok) * p.heads + h) * p.dim;
@@ -296,15 +299,17 @@ int launch(AppendParams& p, bool vec, int sms, cudaStream_t st) {
     // threads; one below, where a launch is bound by the latency of its loads.
     // Of 48 heads of 128 with four and with one: 8192 tokens 33.7 and 37.7 us,
     // 1000 5.9 and 6.6, 500 3.5 and 3.7, 250 3.2 and 2.8, 100 2.8 and 2.3.
+    // e4m3 rows take more registers, so two: 16384 tokens of 48 heads of 64 with
+    // four, two and one 49.7, 43.5 and 49.1 us.
     const int64_t few = p.tokens * all * p.units;
-    const int nh = few >= static_cast<int64_t>(sms) * 1024 ? 4 : 1;
+    const int nh = few >= static_cast<int64_t>(sms) * 1024 ? (p.q8 ? 2 : 4) : 1;
     p.threads_per_token = p.units * ((all + nh - 1) / nh);
     const int64_t n = p.tokens * p.threads_per_token;
     if (n + kThreads <= 0x7fffffffLL) {
       p.div_tok = make_fastdiv(static_cast<uint32_t>(p.threads_per_token));
       const unsigned grid = static_cast<unsigned>((n + kThreads - 1) / kThreads);
       if (p.q8) {
-        if (nh == 4) rope_append8_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
+        if (nh == 2) rope_append8_kernel<BF16, TAB_DT, 2><<<grid, kThreads, 0, st>>>(p);
         else rope_append8_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
       } else if (nh == 4) rope_append_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
       else rope_append_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
