@@ -140,13 +140,13 @@ extern "C" int b200k_quant_groups(const B200kQuantGroupsArgs* a, void* stream_) 
   if (a->rows < 0 || a->cols < 0 || a->cols > 0x3fffffffLL || a->x_row_stride < 0) return B200K_ERR_SHAPE;
   if (a->dtype != B200K_F32 && a->dtype != B200K_F16 && a->dtype != B200K_BF16) return B200K_ERR_UNSUPPORTED;
   if (a->rows == 0 || a->cols == 0) return B200K_OK;
+  if (a->rows > (int64_t(1) << 62) / a->cols) return B200K_ERR_SHAPE;
   if (!a->x || !a->out || !a->scale) return B200K_ERR_ARG;
   const int sms = device_sm_count();
   if (sms <= 0) return B200K_ERR_DEVICE;
   QuantParams p;
   std::memset(&p, 0, sizeof(p));
   p.groups = static_cast<int32_t>((a->cols + 127) / 128);
-  if (a->rows > (int64_t(1) << 62) / a->cols) return B200K_ERR_SHAPE;
   p.units = a->rows * p.groups;
   p.big = p.units > 0x7fffffffLL;
   p.cols = static_cast<int32_t>(a->cols);
