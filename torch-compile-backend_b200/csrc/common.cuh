@@ -237,4 +237,11 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
   return t;
 }
 
+// The writes of the kernels before this one in the stream are there (launch_early);
+// kernels behind it may be launched from now on and wait for its writes in turn.
+__device__ __forceinline__ void wait_for_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 }  // namespace b200k

@@ -185,6 +185,25 @@ inline void attributes_done(std::atomic<uint64_t>& done) {
   if (cudaGetDevice(&dev) == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
 }
 
+// Launches a kernel that may start under the end of the one before it in the
+// stream and waits for its writes itself (griddepcontrol.wait, ahead of its first
+// access to global memory).  In a chain of short kernels that is about 1 us each.
+template <typename... P, typename... A>
+inline int launch_early(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+}
+
 }  // namespace b200k
 
 #define make_fastdiv(d) ::b200k::make_fastdiv_t<::b200k::FastDiv>(d)

@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(256) rope_append_any_kernel(const __grid_const
 // once.  All lanes stay to the end for the shuffles.
 template <bool BF16, int TAB_DT, int NH>
 __global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_constant__ AppendParams p) {
+  wait_for_earlier();
   const uint32_t gid = blockIdx.x * static_cast<uint32_t>(kThreads) + threadIdx.x;
   uint32_t tok = fdiv(gid, p.div_tok);
   const uint32_t in_tok = gid - tok * p.div_tok.d;
@@ -252,6 +253,7 @@ __global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_con
 // it twice.
 template <bool BF16, int TAB_DT>
 __global__ void __launch_bounds__(256) rope_append8_any_kernel(const __grid_constant__ AppendParams p) {
+  wait_for_earlier();
   const int all = p.heads + 2 * p.kv_heads, lane = threadIdx.x & 31;
   const int64_t rows = p.tokens * all;
   constexpr int DT = BF16 ? B200K_BF16 : B200K_F16;
@@ -309,8 +311,7 @@ int launch(AppendParams& p, bool vec, int sms, cudaStream_t st) {
       p.div_tok = make_fastdiv(static_cast<uint32_t>(p.threads_per_token));
       const unsigned grid = static_cast<unsigned>((n + kThreads - 1) / kThreads);
       if (p.q8) {
-        if (nh == 2) rope_append8_kernel<BF16, TAB_DT, 2><<<grid, kThreads, 0, st>>>(p);
-        else rope_append8_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
+        return launch_early(nh == 2 ? rope_append8_kernel<BF16, TAB_DT, 2> : rope_append8_kernel<BF16, TAB_DT, 1>, grid, kThreads, 0, st, p);
       } else if (nh == 4) rope_append_kernel<BF16, TAB_DT, 4><<<grid, kThreads, 0, st>>>(p);
       else rope_append_kernel<BF16, TAB_DT, 1><<<grid, kThreads, 0, st>>>(p);
       return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
@@ -318,8 +319,8 @@ int launch(AppendParams& p, bool vec, int sms, cudaStream_t st) {
   }
   const int64_t n = p.tokens * all * (p.q8 ? 32 : p.dim);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, static_cast<int64_t>(sms) * 8));
-  if (p.q8) rope_append8_any_kernel<BF16, TAB_DT><<<grid, 256, 0, st>>>(p);
-  else rope_append_any_kernel<BF16, TAB_DT><<<grid, 256, 0, st>>>(p);
+  if (p.q8) return launch_early(rope_append8_any_kernel<BF16, TAB_DT>, grid, 256, 0, st, p);
+  rope_append_any_kernel<BF16, TAB_DT><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 

@@ -874,8 +874,13 @@ int launch(const Params& p, int ctas, cudaStream_t st) {
       return B200K_ERR_LAUNCH;
     attributes_done(done);
   }
-  kernel<<<ctas + (p.tile_ctas > 0 ? 1 : 0), kWarps * 32, kSmem, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return B200K_ERR_LAUNCH;
+  const unsigned grid = static_cast<unsigned>(ctas + (p.tile_ctas > 0 ? 1 : 0));
+  if (Q8) {
+    if (const int rc = launch_early(kernel, grid, kWarps * 32, kSmem, st, p); rc != B200K_OK) return rc;
+  } else {
+    kernel<<<grid, kWarps * 32, kSmem, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return B200K_ERR_LAUNCH;
+  }
   if (p.tile_ctas > 0) {
     const int rc = Q8 ? launch_tiles8(p, BF16, D, CAP, st) : launch_tiles(p, BF16, D, CAP, st);
     if (rc != B200K_OK) return rc;

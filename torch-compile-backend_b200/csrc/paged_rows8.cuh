@@ -66,6 +66,7 @@ template <int D, int ROWS>
 constexpr int kCtas8 = ROWS == 8 ? 3 : 2;
 template <bool BF16, int D, int CAP, int ROWS>
 __global__ void __launch_bounds__(kWarps * 32, kCtas8<D, ROWS>) rows8_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early, ahead of its launch_dependents for the later ones' sake
   constexpr uint32_t kTile = kKeys8 * D, kStage = 2 * kTile + 512;  // codes of K and V, ks, vs, log2 vs, 1 / vs
   constexpr int S = kRing8Bytes<ROWS> / kStage;
   constexpr int NT = ROWS / 8;            // query rows, eight at a time

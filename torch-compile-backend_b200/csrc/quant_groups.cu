@@ -43,6 +43,7 @@ constexpr int kPerCta = kThreads / 16;  // groups side by side
 
 template <bool BF16, bool SWIGLU, int UNITS>
 __global__ void __launch_bounds__(kThreads) quant16_kernel(const __grid_constant__ QuantParams p) {
+  wait_for_earlier();
   const int c0 = (threadIdx.x & 15) * 8;
   const int64_t first = blockIdx.x * static_cast<int64_t>(kPerCta * UNITS) + threadIdx.x / 16;
   uint4 a[UNITS], b[UNITS];
@@ -89,6 +90,7 @@ __global__ void __launch_bounds__(kThreads) quant16_kernel(const __grid_constant
 // Any type, width, stride and alignment: a warp a group, four columns a lane.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) quant_any_kernel(const __grid_constant__ QuantParams p) {
+  wait_for_earlier();
   const int lane = threadIdx.x & 31;
   for (int64_t unit = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / 32; unit < p.units;
        unit += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
@@ -125,9 +127,8 @@ int launch16(const QuantParams& p, int sms, cudaStream_t st) {
   const int per = kPerCta * (many ? 4 : 1);
   const int64_t grid = (p.units + per - 1) / per;
   if (grid > 0x7fffffffLL) return B200K_ERR_SHAPE;
-  if (many) quant16_kernel<BF16, SWIGLU, 4><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p);
-  else quant16_kernel<BF16, SWIGLU, 1><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+  return launch_early(many ? quant16_kernel<BF16, SWIGLU, 4> : quant16_kernel<BF16, SWIGLU, 1>, static_cast<unsigned>(grid), kThreads,
+                      0, st, p);
 }
 
 }  // namespace
@@ -164,8 +165,7 @@ extern "C" int b200k_quant_groups(const B200kQuantGroupsArgs* a, void* stream_) 
     return p.swiglu ? launch16<false, true>(p, sms, st) : launch16<false, false>(p, sms, st);
   }
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((p.units + 7) / 8, static_cast<int64_t>(sms) * 16));
-  if (a->dtype == B200K_F32) quant_any_kernel<B200K_F32><<<grid, kThreads, 0, st>>>(p);
-  else if (a->dtype == B200K_F16) quant_any_kernel<B200K_F16><<<grid, kThreads, 0, st>>>(p);
-  else quant_any_kernel<B200K_BF16><<<grid, kThreads, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
+  auto kernel = a->dtype == B200K_F32 ? quant_any_kernel<B200K_F32> : a->dtype == B200K_F16 ? quant_any_kernel<B200K_F16>
+                                                                                            : quant_any_kernel<B200K_BF16>;
+  return launch_early(kernel, grid, kThreads, 0, st, p);
 }

@@ -265,6 +265,10 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
     }
   }
   tc_fence_before();
+  // Launched under the end of the kernel before, whose writes are waited for
+  // here; what follows in the stream may be launched from now on and does so too.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (WIDE) cluster_sync();  // the other CTA's barriers are there too
   else __syncthreads();
   tc_fence_after();
@@ -647,12 +651,14 @@ int launch(MmParams p, const B200kScaledMmArgs* a, int sms, cudaStream_t st) {
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = static_cast<unsigned>(cluster);
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, to, p) == cudaSuccess ? B200K_OK : B200K_ERR_LAUNCH;
 }
 
