@@ -293,6 +293,34 @@ def test_cache_offsets_past_32_bits():
         qc.attention_close(out, (q, *small, near, start, n), ref.default_scale(D))
 
 
+@pytest.mark.parametrize("m", [1, 40])
+def test_cache_offsets_past_64_gib(m):
+    """Rows further apart than 2^32 times 16 bytes (the row kernel's other way to
+    them), of a tensor of 75 GB of which three pages are touched; appended, then read."""
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GiB")
+    D, hkv, page, far = 64, 2, 16, 37_500_000_000 // 4096 * 4096
+    big = torch.empty(2 * far + (1 << 16), device="cuda", dtype=torch.uint8)
+    sizes, strides = (3, page, hkv, D), (far, hkv * D, D, 1)
+    k8, v8 = (big.as_strided(sizes, strides, o).view(quant.E4M3) for o in (0, 1 << 15))
+    ks, vs = (torch.empty(3, page, hkv, device="cuda") for _ in range(2))
+    n = 40
+    g = torch.Generator("cuda").manual_seed(3)
+    q, k, v = (torch.randn(n, h, D, device="cuda", generator=g).to(BF) for h in (8, hkv, hkv))
+    one, none = torch.ones(1, 0, device="cuda"), torch.zeros(n, device="cuda", dtype=torch.int32)
+    slots = torch.arange(n, device="cuda") + page * torch.tensor([2, 0, -2], device="cuda").repeat_interleave(page)[:n]
+    torch.ops.b200.rope_append_quant(q, k, v, one, one, none, slots, k8, v8, ks, vs)
+    i32 = dict(device="cuda", dtype=torch.int32)
+    table, start, lens = torch.tensor([[2, 1, 0]], **i32), torch.tensor([0, m], **i32), torch.tensor([n], **i32)
+    out = op(q[:m], k8, v8, ks, vs, table, start, lens)
+    near = [torch.stack([c.view(torch.uint8)[i].clone() for i in range(3)]).view(quant.E4M3) for c in (k8, v8)]
+    qc.attention_close(out, (q[:m], *near, ks, vs, table, start, lens), ref.default_scale(D))
+    assert ((near[1].double() * vs.double()[..., None])[2, :page] - v[:page].double()).abs().max() < 0.2
+    assert runtime.gemm_status() == 0
+    del big, k8, v8
+    torch.cuda.empty_cache()
+
+
 def test_bad_indexes_are_reported_and_stay_in_bounds():
     *head, table, q_start, kv_len = qc.paged_inputs([1, 2], [40, 20], 8, 2, 64, 16, BF)
     for change in (lambda t, s, n: t.__setitem__((0, 1), 10**6), lambda t, s, n: t.__setitem__((1, 0), -5),
