@@ -30,6 +30,8 @@
 //               memory in the order of the ranks.  For few rows, where b's
 //               bytes are the bound: every SM fetches some of them, and the
 //               tensor-memory lanes are full whatever the number of rows.
+#include <type_traits>
+
 #include "gemm_kernel.cuh"
 
 namespace b200k {
@@ -524,22 +526,57 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
             }
           }
         } else {
-          // rows that TMA cannot store: eight columns at a time through shared
-          // memory, a warp's lanes on neighbouring columns
-          float* tile = reinterpret_cast<float*>(stg);
+          // Rows that TMA cannot store (N no multiple of 16 bytes): 256 bytes of 32
+          // rows through shared memory (chunks of 16 turned by the row), then a warp
+          // a row, eight bytes a lane, in pieces as large as N's alignment.
+          const bool f32 = p.out_dt == B200K_F32;
+          const int per = f32 ? 2 : 4;                             // columns of eight bytes
+          const int fit = p.N % per == 0 ? 8 : f32 || p.N % 2 ? (f32 ? 4 : 2) : 4;
+          // (the sums stay in registers: each of the three fills has its own constants)
+          auto fill = [&](auto wide_type, auto first) {
 #pragma unroll
-          for (int h = 0; h < COLS / 8; ++h) {
-            if (n0 + h * 8 >= p.N) break;
+            for (int g = 0; g < 16; ++g) {
+              uint4 u;
+              if constexpr (decltype(wide_type)::value) {
+                const float2 x = acc[decltype(first)::value + 2 * g], y = acc[decltype(first)::value + 2 * g + 1];
+                u = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
+              } else {
+                u = make_uint4(pack16(acc[4 * g].x, acc[4 * g].y, bf16), pack16(acc[4 * g + 1].x, acc[4 * g + 1].y, bf16),
+                               pack16(acc[4 * g + 2].x, acc[4 * g + 2].y, bf16), pack16(acc[4 * g + 3].x, acc[4 * g + 3].y, bf16));
+              }
+              *reinterpret_cast<uint4*>(stg + lane * 256 + ((g ^ (lane & 15)) << 4)) = u;
+            }
+          };
+          auto empty_out = [&](int h) {
             __syncwarp();
+            const int n = n0 + h * 64 + lane * per;
+            for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+              const uint2 u = *reinterpret_cast<const uint2*>(stg + r * 256 + (((lane >> 1) ^ (r & 15)) << 4) + (lane & 1) * 8);
+              uint8_t* dst = static_cast<uint8_t*>(p.out) + (static_cast<int64_t>(row0 + r) * p.N + n) * (f32 ? 4 : 2);
+              if (fit == 8) {
+                if (n < p.N) *reinterpret_cast<uint2*>(dst) = u;
+              } else if (fit == 4) {
+                if (n < p.N) *reinterpret_cast<uint32_t*>(dst) = u.x;
+                if (n + per / 2 < p.N) *reinterpret_cast<uint32_t*>(dst + 4) = u.y;
+              } else {
+                const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              tile[lane * 9 + 2 * j] = acc[h * 4 + j].x;
-              tile[lane * 9 + 2 * j + 1] = acc[h * 4 + j].y;
+                for (int k = 0; k < 4; ++k)
+                  if (n + k < p.N) reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(w[k >> 1] >> (k & 1) * 16);
+              }
             }
             __syncwarp();
-            const int n = n0 + h * 8 + (lane & 7);
-            for (int r = lane >> 3; r < 32 && row0 + r < p.M; r += 4)
-              if (n < p.N) store_scalar(p.out, static_cast<int64_t>(row0 + r) * p.N + n, p.out_dt, tile[r * 9 + (lane & 7)]);
+          };
+          const std::integral_constant<int, 0> front;
+          const std::integral_constant<int, 32> back;
+          if (f32) {
+            fill(std::true_type(), front);
+            empty_out(0);
+            fill(std::true_type(), back);
+            empty_out(1);
+          } else {
+            fill(std::false_type(), front);
+            empty_out(0);
           }
           __syncwarp();
         }
