@@ -1,9 +1,7 @@
 """b200::paged_attention_quant against the formula in 64 bits on what the
-caches' codes and scales stand for: in sequences of few query rows that itself,
-in those of many each value rounded to q's type (quant_cache.attention_close
-takes a sequence by either).  The bound is derived at
-serving_reference.attention_close; for few rows the weights are rounded to f16,
-whose half step is below bf16's.  Everything of the caches and scales that no
+caches' codes and scales stand for (quant_cache.attention_close; the bound is
+derived at serving_reference.attention_close: weights are rounded to f16 here,
+whose half step is below bf16's).  Everything of the caches and scales that no
 query may see holds NaN, and tables name no page that is not needed."""
 import pytest
 import torch
@@ -133,6 +131,21 @@ def test_a_key_far_above_the_others(D, nats, sink, m, dtype):
     run((q, k8, v8, ks, vs, table, q_start, kv_len))
 
 
+@pytest.mark.parametrize("e", [-30, 30, 60])
+@pytest.mark.parametrize("m", [1, 70])
+def test_value_scales_of_any_size(m, e):
+    """Values of 2^e, and pages of other sizes beside ordinary ones."""
+    q, k8, v8, ks, vs, *rest = qc.paged_inputs([m, m], [150, 300], 4, 2, 128, 16, BF)
+    x = (q, k8, v8, ks, vs * 2.0**e, *rest)
+    out = op(*x)
+    want, size = qc.attend(x, ref.default_scale(128))
+    ref.attention_close((out.double() * 2.0**-e), want * 2.0**-e, size * 2.0**-e, BF)
+    vs = vs.clone()
+    vs[rest[0][1, 5].long()] *= 2.0**20   # a page far above the others
+    vs[rest[0][1, 9].long()] *= 2.0**-20
+    run((q, k8, v8, ks, vs, *rest))
+
+
 @pytest.mark.parametrize("scale", [2.0**-100, 2.0**-20, 2.0**20, 2.0**100])
 @pytest.mark.parametrize("m", [1, 70])
 def test_far_magnitudes_of_bf16_queries(m, scale):
@@ -143,7 +156,8 @@ def test_far_magnitudes_of_bf16_queries(m, scale):
     run((q, *rest), scale=0.125 / scale)
 
 
-@pytest.mark.parametrize("m,dtype", [(1, HF), (1, BF), (70, BF)])  # (many rows: keys in q's type)
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("m", [1, 70])
 def test_key_scales_of_any_size(m, dtype):
     """Keys of 1e30 and of 1e-30."""
     q, k8, v8, ks, vs, *rest = qc.paged_inputs([m], [150], 4, 2, 128, 16, dtype)

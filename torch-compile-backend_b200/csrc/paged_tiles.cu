@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     walk.in = static_cast<int>(in - static_cast<int64_t>(walk.kvh) * len);
   }
   const Ctl ctl{abort_flag, p.status, static_cast<uint64_t>(p.timeout_ns)};
-  const Shared b{q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_free, drain, sQ, sK, sV, copied};
+  const Shared b{q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_free, drain, sQ, sK, sV, copied,
+                 nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   Portion po;
 
   if (warp >= 8 && warp < 12) {
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
   } else {
-    softmax_rows<BF16, D, CAP>(p, walk, ctl, b, tmem_base, run, warp, lane);
+    softmax_rows<BF16, D, CAP, false>(p, walk, ctl, b, tmem_base, run, warp, lane);
   }
 
   gemm::tc_fence_before();

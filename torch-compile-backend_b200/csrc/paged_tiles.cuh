@@ -204,10 +204,17 @@ struct Shared {
   uint64_t *drain;                                // [4] by issuer
   uint8_t *sQ, *sK, *sV;
   const volatile int* copied;                     // [2 stages] of K, of V: the stage's block came by cp.async
+  // over e4m3 caches (paged_tiles8.cu)
+  uint64_t *sc_full, *sc_empty;                   // [kScaleSlots] by block
+  uint64_t *rs_full, *rs_empty;                   // [2] by portion: bf16 queries made f16
+  const float* sc;                                // [kScaleSlots][kScaleFloats]: 64 keys' scales, E, 2^-E
+  const float* rs;                                // [2][256] the query rows' powers of two
 };
+constexpr int kScaleSlots = 4, kScaleFloats = kBlock + 4;
 
 // The MMA issuers: warps 8, 9 of S_t = Q_t K^T of tile t = 0, 1, warps 10, 11 of
-// O_t += P_t V.  S: stages; Q8: converted blocks, whose writers fence themselves.
+// O_t += P_t V.  S: stages; Q8: blocks made f16 by
+// warps that fence their writes themselves.
 template <bool BF16, int D, int S, bool Q8>
 __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
                                                int warp, int lane) {
@@ -215,7 +222,7 @@ __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, cons
   Portion po;
   const int t = warp & 1;
   const bool scores = warp < 10;
-  const uint32_t fmt = BF16 ? 1u : 0u;
+  const uint32_t fmt = BF16 && !Q8 ? 1u : 0u;
   // fp32 accumulators; B of Q K^T K-major, of P V N-major
   const uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kBlock >> 3) << 17) | ((128u >> 4) << 24);
   const uint32_t idesc_pv =
@@ -233,8 +240,8 @@ __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, cons
   bool ok = true;
   for (int li = 0; ok && walk.next(p, po); ++li) {
     if (scores) {
-      ok = warp_wait(b.q_full, li & 1, ctl);
-      if (p.q_box == 0) gemm::fence_async_smem();
+      ok = Q8 && BF16 ? warp_wait(&b.rs_full[li & 1], (li >> 1) & 1, ctl) : warp_wait(b.q_full, li & 1, ctl);
+      if (p.q_box == 0 && !(Q8 && BF16)) gemm::fence_async_smem();
     }
     for (int j = po.beg; ok && j < po.end; ++j, ++c) {
       const int st = c % S;
@@ -284,16 +291,20 @@ __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, cons
   __syncwarp();
 }
 
-// The softmax warps 0-7, one thread a query row.
-template <bool BF16, int D, int CAP>
+// The softmax warps 0-7, one thread a query row.  Q8: scores are of codes, so each
+// is multiplied by its key's scale; values have been divided by a power of two a
+// block, 2^E, so the weights of a block are 2^(score + E - max (score + E)), and
+// their sum's share is multiplied by 2^-E.
+template <bool BF16, int D, int CAP, bool Q8>
 __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
                                              int64_t run, int warp, int lane) {
+  constexpr bool P16 = BF16 && !Q8;  // weights of the second product in bf16
   Portion po;
   const int t = warp >> 2, quarter = warp & 3;
   const int in_unit = t * 128 + quarter * 32 + lane;
   const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t tS = t_lane + t * 128, tO = t_lane + kTmemO + t * D;
-  int g = 0;
+  int g = 0, c = 0, li = 0;  // c, li: blocks and portions passed
   bool ok = true;
   while (ok && walk.next(p, po)) {
     if (!po.whole && po.slot == 1 && threadIdx.x == 0) {
@@ -308,9 +319,29 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
     const int pos = walk.u.s.first + static_cast<int>(tok);
     // positions of the warp's first and last row
     const int w_lo = __shfl_sync(0xffffffffu, pos, 0), w_hi = __shfl_sync(0xffffffffu, pos, 31);
+    float row_mul = 1.0f;
+    if (Q8 && BF16) {
+      if (!(ok = warp_wait(&b.rs_full[li & 1], (li >> 1) & 1, ctl))) break;
+      if (real) row_mul = b.rs[(li & 1) * kUnitRows + in_unit];
+      __syncwarp();
+      if (lane == 0) gemm::mbar_arrive(&b.rs_empty[li & 1]);
+      ++li;
+    }
+    if (CAP == kNoCap) row_mul *= p.mul;
     float m = -INFINITY, l = 0.0f;
     const int jb = po.t_beg[t], je = po.t_end[t];
-    for (int j = jb; j < je; ++j, ++g) {
+    for (int j = Q8 ? po.beg : jb; j < (Q8 ? po.end : je); ++j) {
+      const int slot = c % kScaleSlots;
+      if (Q8) {
+        if (!(ok = warp_wait(&b.sc_full[slot], (c / kScaleSlots) & 1, ctl))) break;
+        ++c;
+        if (j < jb || j >= je) {  // not a block of this tile
+          if (lane == 0) gemm::mbar_arrive(&b.sc_empty[slot]);
+          __syncwarp();
+          continue;
+        }
+      }
+      const float* scales = b.sc + slot * kScaleFloats;
       const uint32_t buf = g & 1;
       if (!(ok = warp_wait(&b.s_full[t * 2 + buf], (g >> 1) & 1, ctl))) break;
       gemm::tc_fence_after();
@@ -325,9 +356,27 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
 #pragma unroll
           for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(raw[c][i]);
       }
+      float shift = 0.0f, unshift = 1.0f;  // E, 2^-E
+      if (Q8) {
+#pragma unroll
+        for (int c = 0; c < kBlock; c += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(scales + c);
+          const float2 x = __fmul2_rn(make_float2(s[c], s[c + 1]), make_float2(k.x, k.y));
+          const float2 y = __fmul2_rn(make_float2(s[c + 2], s[c + 3]), make_float2(k.z, k.w));
+          s[c] = x.x;
+          s[c + 1] = x.y;
+          s[c + 2] = y.x;
+          s[c + 3] = y.y;
+        }
+        const float2 e = *reinterpret_cast<const float2*>(scales + kBlock);
+        shift = e.x;
+        unshift = e.y;
+        __syncwarp();
+        if (lane == 0) gemm::mbar_arrive(&b.sc_empty[slot]);
+      }
       if (CAP != kNoCap) {
 #pragma unroll
-        for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, s[c]);
+        for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, Q8 && BF16 ? s[c] * row_mul : s[c]);
       }
       const int key0 = j * kBlock;
       if (key0 + kBlock - 1 > w_lo || (p.window > 0 && key0 <= w_hi - p.window)) {  // warp-uniform
@@ -344,31 +393,34 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx[i] = max2(mx[i], s[kBlock - 4 + i]);
       float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
-      if (CAP == kNoCap) top *= p.mul;
+      if (CAP == kNoCap) top *= row_mul;
+      if (Q8) top += shift;
       const float was = m;
       float alpha = 1.0f;
       bool moved = false;
       // A NaN score, and an infinite one (0 * top), makes the maximum NaN and
       // with it every probability and sum of the row from here on.
-      if (!(top <= m + kTileLag<BF16>)) {
+      if (!(top <= m + kTileLag<P16>)) {
         m = fmaf(0.0f, top, top);
         alpha = ex2(was - m);
         moved = j > jb;
       }
       // probabilities are rounded to the input type, half a step each, in f16
       // down to 2^-26 of the row's maximum (smaller ones by less than 2^-36 of it)
-      const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<BF16>;
+      const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<P16>;
       float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-      const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(-ref, -ref);
+      const float off = Q8 ? shift - ref : -ref;
+      const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(row_mul, row_mul), nm2 = make_float2(off, off);
       uint32_t pk[kBlock / 2];
 #pragma unroll
       for (int c = 0; c < kBlock; c += 2) {
         const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
-        const float2 e = c % kFmaEvery == kFmaEvery - 2 ? ex2_fma<BF16>(x) : make_float2(ex2(x.x), ex2(x.y));
+        const float2 e = c % kFmaEvery == kFmaEvery - 2 ? ex2_fma<P16>(x) : make_float2(ex2(x.x), ex2(x.y));
         sum2[c / 2 % 2] = __fadd2_rn(sum2[c / 2 % 2], e);
-        pk[c / 2] = pack16<BF16>(e.x, e.y);
+        pk[c / 2] = pack16<P16>(e.x, e.y);
       }
-      l = fmaf(l, alpha, (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
+      const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+      l = fmaf(l, alpha, Q8 ? sum * unshift : sum);
       if (__any_sync(0xffffffffu, moved)) {
         // P V of the block before has written O
         if (!(ok = warp_wait(&b.o_done[t * 2 + (buf ^ 1)], ((g - 1) >> 1) & 1, ctl))) break;
@@ -388,6 +440,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
       gemm::tc_fence_before();
       __syncwarp();
       if (lane == 0) gemm::mbar_arrive(&b.p_full[t * 2 + buf]);
+      ++g;
     }
     if (!ok) break;
     const bool had = je > jb;

@@ -2,12 +2,16 @@
 // rows over e4m3 caches.  The plan, the portions, the products, the softmax and
 // the parts are the 16-bit tile kernel's (paged_tiles.cuh); here
 //   warps 12, 13 load codes (TMA boxes or 16-byte cp.async copies) and scales,
-//   warps 16, 17 and 18, 19 turn a block's key and value codes into the 16-bit
-//                tiles that the products take: code * scale in fp32, rounded once.
-// The scales are taken in where a value is made and not, as in the row kernel,
-// where it is used: in the scores and sums they cost the softmax, which bounds
-// the kernel, 1000 of 2900 clocks a block of 64 keys.  The registers are shared
-// out by setmaxnreg: five warpgroups are launched with 96 a thread.
+//   warps 16-19  make a block's codes f16 in shared memory, 16 and 17 the keys'
+//                as they are, 18 and 19 the values' times scale / 2^E, rounded
+//                once, 2^E a power of two that no scale of the block is above (so
+//                any magnitude fits f16); and, for bf16, a portion's queries, each
+//                row divided by a power of two (row_scale).
+// Both products are f16 ones.  The keys' scales stay out of them: rounded into
+// the keys they would move every score (in bf16 the output by 0.4 %).  With the
+// values' scales too in the softmax, which bounds the kernel, a block of 64 keys
+// took 2900 clocks.  The registers are shared out by setmaxnreg: five warpgroups
+// are launched with 96 a thread.
 #include "paged_tiles.cuh"
 
 namespace b200k {
@@ -19,10 +23,10 @@ constexpr int kLaunchRegs = 96, kSoftmaxRegs = 144, kIssueRegs = 56, kConvertReg
 static_assert(2 * kSoftmaxRegs + 2 * kIssueRegs + kConvertRegs <= 5 * kLaunchRegs, "what the launch has");
 template <int D>
 struct Layout8 {
-  static constexpr int kStages = D == 128 ? 3 : 4;         // of 16-bit keys and of values
+  static constexpr int kStages = D == 128 ? 3 : 4;         // of f16 keys and of values
   static constexpr int kRaw = D == 128 ? 3 : 4;            // of codes
   static constexpr uint32_t kTile = kHalfTile * (D / 64);  // a query tile
-  static constexpr uint32_t kBlk = kHalfBlk * (D / 64);    // a 16-bit block
+  static constexpr uint32_t kBlk = kHalfBlk * (D / 64);    // an f16 block
   static constexpr uint32_t kCodes = kBlock * D;           // a block of codes
   static constexpr uint32_t kOffK = 2 * kTile;
   static constexpr uint32_t kOffV = kOffK + kStages * kBlk;
@@ -30,7 +34,9 @@ struct Layout8 {
   static constexpr uint32_t kOffRawV = kOffRawK + kRaw * kCodes;
   static constexpr uint32_t kOffRawKs = kOffRawV + kRaw * kCodes;      // [kRaw][64] scales
   static constexpr uint32_t kOffRawVs = kOffRawKs + kRaw * kBlock * 4;
-  static constexpr uint32_t kOffBar = kOffRawVs + kRaw * kBlock * 4;
+  static constexpr uint32_t kOffSc = kOffRawVs + kRaw * kBlock * 4;          // Shared::sc
+  static constexpr uint32_t kOffRs = kOffSc + kScaleSlots * kScaleFloats * 4;  // Shared::rs
+  static constexpr uint32_t kOffBar = kOffRs + 2 * kUnitRows * 4;
   static constexpr uint32_t kSmem = 1024 + kOffBar + 1024;
   static_assert(kSmem <= 232448 && kSmem > 116 * 1024, "one CTA per SM");
 };
@@ -60,7 +66,13 @@ __global__ void __launch_bounds__(kThreads8, 1)
   uint64_t* o_done = p_full + 4;     // [4]
   uint64_t* o_free = o_done + 4;     // [2] by tile
   uint64_t* drain = o_free + 2;      // [4] by issuer
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 4);
+  uint64_t* sc_full = drain + 4;     // [kScaleSlots]
+  uint64_t* sc_empty = sc_full + kScaleSlots;
+  uint64_t* rs_full = sc_empty + kScaleSlots;  // [2]
+  uint64_t* rs_empty = rs_full + 2;
+  float* sc = reinterpret_cast<float*>(sbase + L::kOffSc);
+  float* rs = reinterpret_cast<float*>(sbase + L::kOffRs);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rs_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* first_entry = reinterpret_cast<int*>(tmem_slot + 2);
 
@@ -105,6 +117,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
         gemm::mbar_init(&drain[t * 2 + i], 1);
       }
       gemm::mbar_init(&o_free[t], 4);
+      gemm::mbar_init(&rs_full[t], 4);
+      gemm::mbar_init(&rs_empty[t], 8);
+    }
+    for (int i = 0; i < kScaleSlots; ++i) {
+      gemm::mbar_init(&sc_full[i], 2);
+      gemm::mbar_init(&sc_empty[i], 8);
     }
     *abort_flag = 0;
     gemm::fence_mbar_init();
@@ -130,7 +148,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
     walk.in = static_cast<int>(in - static_cast<int64_t>(walk.kvh) * len);
   }
   const Ctl ctl{abort_flag, p.status, static_cast<uint64_t>(p.timeout_ns)};
-  const Shared b{q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_free, drain, sQ, sK, sV, nullptr};
+  const Shared b{q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_free, drain, sQ, sK, sV, nullptr,
+                 sc_full, sc_empty, rs_full, rs_empty, sc, rs};
 
   if (warp >= 8 && warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -148,28 +167,77 @@ __global__ void __launch_bounds__(kThreads8, 1)
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
     constexpr int kChunks = D / 16;  // 16-byte chunks of a row of codes
+    const bool signs = (warp & 1) == 0;  // this warp leaves the block's scales
     Portion po;
     int c = 0;
     bool ok = true;
-    while (ok && walk.next(p, po)) {
+    for (int li = 0; ok && walk.next(p, po); ++li) {
+      if (BF16) {
+        // the portion's queries in place, a row of each tile a thread
+        if (!(ok = warp_wait(q_full, li & 1, ctl) && warp_wait(&rs_empty[li & 1], ((li >> 1) & 1) ^ 1, ctl))) break;
+        const int row = (warp - 16) * 32 + lane;
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          if (walk.u.r0 + t * 128 >= walk.u.rows) break;
+          uint8_t* q = sQ + t * L::kTile + row * 128;
+          uint32_t top = 0;
+#pragma unroll
+          for (int k = 0; k < D / 8; ++k) {
+            const uint4 x = *reinterpret_cast<const uint4*>(q + (k >> 3) * kHalfTile + (((k & 7) ^ (row & 7)) << 4));
+#pragma unroll
+            for (uint32_t w : {x.x, x.y, x.z, x.w}) top = max(top, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+          }
+          const RowScale s = row_scale(top);
+#pragma unroll
+          for (int k = 0; k < D / 8; ++k) {
+            uint4* at = reinterpret_cast<uint4*>(q + (k >> 3) * kHalfTile + (((k & 7) ^ (row & 7)) << 4));
+            const uint4 x = *at;
+            *at = make_uint4(bf16_to_f16(x.x, s.div), bf16_to_f16(x.y, s.div), bf16_to_f16(x.z, s.div), bf16_to_f16(x.w, s.div));
+          }
+          rs[(li & 1) * kUnitRows + t * 128 + row] = s.mul;
+        }
+        gemm::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) gemm::mbar_arrive(&rs_full[li & 1]);
+      }
       for (int j = po.beg; j < po.end; ++j, ++c) {
-        const int rst = c % R, st = c % S;
+        const int rst = c % R, st = c % S, slot = c % kScaleSlots;
         if (!(ok = warp_wait(&r_full[rst], (c / R) & 1, ctl) && warp_wait(&empty[st], ((c / S) & 1) ^ 1, ctl))) break;
         const uint4* src = reinterpret_cast<const uint4*>(raw + rst * L::kCodes);
         uint8_t* dst = dst0 + st * L::kBlk;
+        const float s0 = raw_sc[rst * kBlock + lane], s1 = raw_sc[rst * kBlock + 32 + lane];
+        // 2^E from the exponent of the largest scale (a NaN or infinite one
+        // makes its own row NaN), and 2^-E
+        float up = 1.0f, down = 1.0f;
+        if (is_v) {
+          auto bits = [](float x) { return x < 3e38f ? __float_as_uint(fmaxf(x, kMinVs)) : __float_as_uint(kMinVs); };
+          const uint32_t e = min((__reduce_max_sync(0xffffffffu, max(bits(s0), bits(s1))) >> 23) + 1, 253u);
+          up = __uint_as_float(e << 23);
+          down = __uint_as_float((254u - e) << 23);
+        }
+        if (signs) {
+          if (!(ok = warp_wait(&sc_empty[slot], ((c / kScaleSlots) & 1) ^ 1, ctl))) break;
+          float* to = sc + slot * kScaleFloats;
+          if (!is_v) {
+            to[lane] = s0;
+            to[32 + lane] = s1;
+          } else if (lane == 0) {
+            to[kBlock] = static_cast<float>(static_cast<int>(__float_as_uint(up) >> 23) - 127);
+            to[kBlock + 1] = down;
+          }
+        }
 #pragma unroll 2
         for (int i = 0; i < kBlock * kChunks / 64; ++i) {
           const int idx = i * 64 + first, row = idx / kChunks, ch = idx % kChunks;
           const uint4 x = src[idx];
-          const float scale = raw_sc[rst * kBlock + row];
-          uint32_t y[8];
-          int k = 0;
+          uint32_t y[8] = {codes_lo(x.x), codes_hi(x.x), codes_lo(x.y), codes_hi(x.y), codes_lo(x.z), codes_hi(x.z), codes_lo(x.w), codes_hi(x.w)};
+          if (is_v) {
+            const float f = raw_sc[rst * kBlock + row] * down;
 #pragma unroll
-          for (uint32_t w : {x.x, x.y, x.z, x.w}) {
-            const uint32_t lo = codes_lo(w), hi = codes_hi(w);
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), z = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            y[k++] = pack16<BF16>(a.x * scale, a.y * scale);
-            y[k++] = pack16<BF16>(z.x * scale, z.y * scale);
+            for (int k = 0; k < 8; ++k) {
+              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&y[k]));
+              y[k] = pack16<false>(a.x * f, a.y * f);
+            }
           }
           // two 16-byte chunks; the upper half's lanes write theirs the other way
           // round, so that eight lanes cover all banks
@@ -184,6 +252,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
         if (lane == 0) {
           gemm::mbar_arrive(&full[st]);
           gemm::mbar_arrive(&r_empty[rst]);
+          if (signs) gemm::mbar_arrive(&sc_full[slot]);
         }
       }
     }
@@ -299,7 +368,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_rows<BF16, D, CAP>(p, walk, ctl, b, tmem_base, run, warp, lane);
+    softmax_rows<BF16, D, CAP, true>(p, walk, ctl, b, tmem_base, run, warp, lane);
   }
 
   gemm::tc_fence_before();
