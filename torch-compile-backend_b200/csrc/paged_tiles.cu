@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const Ctl ctl{abort_flag, p.status, static_cast<uint64_t>(p.timeout_ns)};
   const Shared b{q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_free, drain, sQ, sK, sV, copied,
-                 nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+                 nullptr, nullptr, nullptr};
   Portion po;
 
   if (warp >= 8 && warp < 12) {

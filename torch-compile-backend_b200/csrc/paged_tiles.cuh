@@ -135,6 +135,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const 
   return __all_sync(0xffffffffu, ok);
 }
 
+// The same for a phase that has nearly always completed: tested first.
+__device__ __forceinline__ bool warp_test_wait(uint64_t* bar, uint32_t parity, const Ctl& c) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, done) || warp_wait(bar, parity, c);
+}
+
 // A CTA's consecutive steps of one unit (Walk::u until the next one).
 struct Portion {
   int kvh;
@@ -206,15 +219,13 @@ struct Shared {
   const volatile int* copied;                     // [2 stages] of K, of V: the stage's block came by cp.async
   // over e4m3 caches (paged_tiles8.cu)
   uint64_t *sc_full, *sc_empty;                   // [kScaleSlots] by block
-  uint64_t *rs_full, *rs_empty;                   // [2] by portion: bf16 queries made f16
   const float* sc;                                // [kScaleSlots][kScaleFloats]: 64 keys' scales, E, 2^-E
-  const float* rs;                                // [2][256] the query rows' powers of two
 };
-constexpr int kScaleSlots = 4, kScaleFloats = kBlock + 4;
+constexpr int kScaleSlots = 8, kScaleFloats = kBlock + 4;
 
 // The MMA issuers: warps 8, 9 of S_t = Q_t K^T of tile t = 0, 1, warps 10, 11 of
-// O_t += P_t V.  S: stages; Q8: blocks made f16 by
-// warps that fence their writes themselves.
+// O_t += P_t V.  S: stages; Q8: blocks made 16-bit
+// by warps that fence their writes themselves, keys in q's type, values in f16.
 template <bool BF16, int D, int S, bool Q8>
 __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
                                                int warp, int lane) {
@@ -222,11 +233,11 @@ __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, cons
   Portion po;
   const int t = warp & 1;
   const bool scores = warp < 10;
-  const uint32_t fmt = BF16 && !Q8 ? 1u : 0u;
+  const uint32_t fmt = BF16 ? 1u : 0u, fmt_pv = BF16 && !Q8 ? 1u : 0u;
   // fp32 accumulators; B of Q K^T K-major, of P V N-major
   const uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kBlock >> 3) << 17) | ((128u >> 4) << 24);
   const uint32_t idesc_pv =
-      (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
+      (1u << 4) | (fmt_pv << 7) | (fmt_pv << 10) | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);
   const uint32_t tS = tmem_base + t * 128, tO = tmem_base + kTmemO + t * D;
   const uint64_t dq = gemm::sw128_desc(smem_u32(b.sQ) + t * kTile, 16, 1024);
   const uint64_t dk = gemm::sw128_desc(smem_u32(b.sK), 16, 1024);
@@ -240,8 +251,8 @@ __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, cons
   bool ok = true;
   for (int li = 0; ok && walk.next(p, po); ++li) {
     if (scores) {
-      ok = Q8 && BF16 ? warp_wait(&b.rs_full[li & 1], (li >> 1) & 1, ctl) : warp_wait(b.q_full, li & 1, ctl);
-      if (p.q_box == 0 && !(Q8 && BF16)) gemm::fence_async_smem();
+      ok = warp_wait(b.q_full, li & 1, ctl);
+      if (p.q_box == 0) gemm::fence_async_smem();
     }
     for (int j = po.beg; ok && j < po.end; ++j, ++c) {
       const int st = c % S;
@@ -304,7 +315,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
   const int in_unit = t * 128 + quarter * 32 + lane;
   const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t tS = t_lane + t * 128, tO = t_lane + kTmemO + t * D;
-  int g = 0, c = 0, li = 0;  // c, li: blocks and portions passed
+  int g = 0, c = 0;  // c: blocks passed
   bool ok = true;
   while (ok && walk.next(p, po)) {
     if (!po.whole && po.slot == 1 && threadIdx.x == 0) {
@@ -319,21 +330,12 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
     const int pos = walk.u.s.first + static_cast<int>(tok);
     // positions of the warp's first and last row
     const int w_lo = __shfl_sync(0xffffffffu, pos, 0), w_hi = __shfl_sync(0xffffffffu, pos, 31);
-    float row_mul = 1.0f;
-    if (Q8 && BF16) {
-      if (!(ok = warp_wait(&b.rs_full[li & 1], (li >> 1) & 1, ctl))) break;
-      if (real) row_mul = b.rs[(li & 1) * kUnitRows + in_unit];
-      __syncwarp();
-      if (lane == 0) gemm::mbar_arrive(&b.rs_empty[li & 1]);
-      ++li;
-    }
-    if (CAP == kNoCap) row_mul *= p.mul;
     float m = -INFINITY, l = 0.0f;
     const int jb = po.t_beg[t], je = po.t_end[t];
     for (int j = Q8 ? po.beg : jb; j < (Q8 ? po.end : je); ++j) {
       const int slot = c % kScaleSlots;
       if (Q8) {
-        if (!(ok = warp_wait(&b.sc_full[slot], (c / kScaleSlots) & 1, ctl))) break;
+        if (!(ok = warp_test_wait(&b.sc_full[slot], (c / kScaleSlots) & 1, ctl))) break;
         ++c;
         if (j < jb || j >= je) {  // not a block of this tile
           if (lane == 0) gemm::mbar_arrive(&b.sc_empty[slot]);
@@ -376,7 +378,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
       }
       if (CAP != kNoCap) {
 #pragma unroll
-        for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, Q8 && BF16 ? s[c] * row_mul : s[c]);
+        for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, s[c]);
       }
       const int key0 = j * kBlock;
       if (key0 + kBlock - 1 > w_lo || (p.window > 0 && key0 <= w_hi - p.window)) {  // warp-uniform
@@ -393,7 +395,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx[i] = max2(mx[i], s[kBlock - 4 + i]);
       float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
-      if (CAP == kNoCap) top *= row_mul;
+      if (CAP == kNoCap) top *= p.mul;
       if (Q8) top += shift;
       const float was = m;
       float alpha = 1.0f;
@@ -410,7 +412,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
       const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<P16>;
       float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
       const float off = Q8 ? shift - ref : -ref;
-      const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(row_mul, row_mul), nm2 = make_float2(off, off);
+      const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(off, off);
       uint32_t pk[kBlock / 2];
 #pragma unroll
       for (int c = 0; c < kBlock; c += 2) {

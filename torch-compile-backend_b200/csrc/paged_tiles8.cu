@@ -2,16 +2,17 @@
 // rows over e4m3 caches.  The plan, the portions, the products, the softmax and
 // the parts are the 16-bit tile kernel's (paged_tiles.cuh); here
 //   warps 12, 13 load codes (TMA boxes or 16-byte cp.async copies) and scales,
-//   warps 16-19  make a block's codes f16 in shared memory, 16 and 17 the keys'
-//                as they are, 18 and 19 the values' times scale / 2^E, rounded
-//                once, 2^E a power of two that no scale of the block is above (so
-//                any magnitude fits f16); and, for bf16, a portion's queries, each
-//                row divided by a power of two (row_scale).
-// Both products are f16 ones.  The keys' scales stay out of them: rounded into
-// the keys they would move every score (in bf16 the output by 0.4 %).  With the
-// values' scales too in the softmax, which bounds the kernel, a block of 64 keys
-// took 2900 clocks.  The registers are shared out by setmaxnreg: five warpgroups
-// are launched with 96 a thread.
+//   warps 16, 17 make a block's key codes 16-bit in shared memory, of q's type and
+//                as they are (both types hold every code);
+//   warps 18, 19 its values f16, code * scale / 2^E rounded once, 2^E a power of
+//                two that no scale of the block is above, so that any magnitude
+//                fits.
+// Q K^T runs in q's type, P V in f16.  The keys' scales stay out of the products:
+// rounded into bf16 keys they would move every score, the output by 0.4 %.  The
+// softmax, which bounds the kernel, multiplies the scores by them; with the
+// values' scales there too, and queries made f16 first, chunks of prompts took
+// 517 us.  The registers are shared out by setmaxnreg: five warpgroups are
+// launched with 96 a thread.
 #include "paged_tiles.cuh"
 
 namespace b200k {
@@ -23,10 +24,10 @@ constexpr int kLaunchRegs = 96, kSoftmaxRegs = 144, kIssueRegs = 56, kConvertReg
 static_assert(2 * kSoftmaxRegs + 2 * kIssueRegs + kConvertRegs <= 5 * kLaunchRegs, "what the launch has");
 template <int D>
 struct Layout8 {
-  static constexpr int kStages = D == 128 ? 3 : 4;         // of f16 keys and of values
+  static constexpr int kStages = D == 128 ? 3 : 4;         // of 16-bit keys and of values
   static constexpr int kRaw = D == 128 ? 3 : 4;            // of codes
   static constexpr uint32_t kTile = kHalfTile * (D / 64);  // a query tile
-  static constexpr uint32_t kBlk = kHalfBlk * (D / 64);    // an f16 block
+  static constexpr uint32_t kBlk = kHalfBlk * (D / 64);    // a 16-bit block
   static constexpr uint32_t kCodes = kBlock * D;           // a block of codes
   static constexpr uint32_t kOffK = 2 * kTile;
   static constexpr uint32_t kOffV = kOffK + kStages * kBlk;
@@ -35,8 +36,7 @@ struct Layout8 {
   static constexpr uint32_t kOffRawKs = kOffRawV + kRaw * kCodes;      // [kRaw][64] scales
   static constexpr uint32_t kOffRawVs = kOffRawKs + kRaw * kBlock * 4;
   static constexpr uint32_t kOffSc = kOffRawVs + kRaw * kBlock * 4;          // Shared::sc
-  static constexpr uint32_t kOffRs = kOffSc + kScaleSlots * kScaleFloats * 4;  // Shared::rs
-  static constexpr uint32_t kOffBar = kOffRs + 2 * kUnitRows * 4;
+  static constexpr uint32_t kOffBar = kOffSc + kScaleSlots * kScaleFloats * 4;
   static constexpr uint32_t kSmem = 1024 + kOffBar + 1024;
   static_assert(kSmem <= 232448 && kSmem > 116 * 1024, "one CTA per SM");
 };
@@ -68,11 +68,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
   uint64_t* drain = o_free + 2;      // [4] by issuer
   uint64_t* sc_full = drain + 4;     // [kScaleSlots]
   uint64_t* sc_empty = sc_full + kScaleSlots;
-  uint64_t* rs_full = sc_empty + kScaleSlots;  // [2]
-  uint64_t* rs_empty = rs_full + 2;
   float* sc = reinterpret_cast<float*>(sbase + L::kOffSc);
-  float* rs = reinterpret_cast<float*>(sbase + L::kOffRs);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rs_empty + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + kScaleSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* first_entry = reinterpret_cast<int*>(tmem_slot + 2);
 
@@ -117,8 +114,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
         gemm::mbar_init(&drain[t * 2 + i], 1);
       }
       gemm::mbar_init(&o_free[t], 4);
-      gemm::mbar_init(&rs_full[t], 4);
-      gemm::mbar_init(&rs_empty[t], 8);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
       gemm::mbar_init(&sc_full[i], 2);
@@ -149,7 +144,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
   }
   const Ctl ctl{abort_flag, p.status, static_cast<uint64_t>(p.timeout_ns)};
   const Shared b{q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_free, drain, sQ, sK, sV, nullptr,
-                 sc_full, sc_empty, rs_full, rs_empty, sc, rs};
+                 sc_full, sc_empty, sc};
 
   if (warp >= 8 && warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -171,35 +166,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
     Portion po;
     int c = 0;
     bool ok = true;
-    for (int li = 0; ok && walk.next(p, po); ++li) {
-      if (BF16) {
-        // the portion's queries in place, a row of each tile a thread
-        if (!(ok = warp_wait(q_full, li & 1, ctl) && warp_wait(&rs_empty[li & 1], ((li >> 1) & 1) ^ 1, ctl))) break;
-        const int row = (warp - 16) * 32 + lane;
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {
-          if (walk.u.r0 + t * 128 >= walk.u.rows) break;
-          uint8_t* q = sQ + t * L::kTile + row * 128;
-          uint32_t top = 0;
-#pragma unroll
-          for (int k = 0; k < D / 8; ++k) {
-            const uint4 x = *reinterpret_cast<const uint4*>(q + (k >> 3) * kHalfTile + (((k & 7) ^ (row & 7)) << 4));
-#pragma unroll
-            for (uint32_t w : {x.x, x.y, x.z, x.w}) top = max(top, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
-          }
-          const RowScale s = row_scale(top);
-#pragma unroll
-          for (int k = 0; k < D / 8; ++k) {
-            uint4* at = reinterpret_cast<uint4*>(q + (k >> 3) * kHalfTile + (((k & 7) ^ (row & 7)) << 4));
-            const uint4 x = *at;
-            *at = make_uint4(bf16_to_f16(x.x, s.div), bf16_to_f16(x.y, s.div), bf16_to_f16(x.z, s.div), bf16_to_f16(x.w, s.div));
-          }
-          rs[(li & 1) * kUnitRows + t * 128 + row] = s.mul;
-        }
-        gemm::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) gemm::mbar_arrive(&rs_full[li & 1]);
-      }
+    while (ok && walk.next(p, po)) {
       for (int j = po.beg; j < po.end; ++j, ++c) {
         const int rst = c % R, st = c % S, slot = c % kScaleSlots;
         if (!(ok = warp_wait(&r_full[rst], (c / R) & 1, ctl) && warp_wait(&empty[st], ((c / S) & 1) ^ 1, ctl))) break;
@@ -231,12 +198,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
           const int idx = i * 64 + first, row = idx / kChunks, ch = idx % kChunks;
           const uint4 x = src[idx];
           uint32_t y[8] = {codes_lo(x.x), codes_hi(x.x), codes_lo(x.y), codes_hi(x.y), codes_lo(x.z), codes_hi(x.z), codes_lo(x.w), codes_hi(x.w)};
-          if (is_v) {
-            const float f = raw_sc[rst * kBlock + row] * down;
+          if (is_v || BF16) {
+            const float f = is_v ? raw_sc[rst * kBlock + row] * down : 1.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&y[k]));
-              y[k] = pack16<false>(a.x * f, a.y * f);
+              y[k] = is_v ? pack16<false>(a.x * f, a.y * f) : pack16<BF16>(a.x, a.y);
             }
           }
           // two 16-byte chunks; the upper half's lanes write theirs the other way
