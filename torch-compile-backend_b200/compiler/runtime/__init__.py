@@ -149,9 +149,9 @@ def check_status(device: int = 0) -> None:
     load()
     v = gemm_status(device, reset=True)
     if v == 9:
-        raise RuntimeError(f"b200::rope_append(_quant) or paged_attention(_quant) on cuda:{device} reported status {v}: "
-                           "a slot, position, page or length is out of range")
+        raise RuntimeError("b200::rope_append, rope_append_quant, paged_attention or paged_attention_quant "
+                           f"on cuda:{device} reported status {v}: a slot, position, page or length is out of range")
     if v != 0:
-        raise RuntimeError(f"b200::gemm_epilogue, scaled_mm, attention or paged_attention(_quant) on cuda:{device} reported "
-                           f"status {v} "
+        raise RuntimeError("b200::gemm_epilogue, scaled_mm, attention, paged_attention or paged_attention_quant "
+                           f"on cuda:{device} reported status {v} "
                            "(6 = a device-side wait timed out): an earlier call's output is incomplete")

@@ -329,9 +329,9 @@ int64_t status_check(int64_t device, bool arm) {
   }
   if (seen != 0) {
     word.zero_();
-    TORCH_CHECK(seen != B200K_ERR_INDEX, "b200::rope_append(_quant) or paged_attention(_quant) on cuda:", dev, " reported ",
+    TORCH_CHECK(seen != B200K_ERR_INDEX, "b200::rope_append, rope_append_quant, paged_attention or paged_attention_quant on cuda:", dev, " reported ",
                 b200k_status_string(static_cast<int>(seen)), " (code ", seen, ")");
-    TORCH_CHECK(false, "b200::gemm_epilogue, scaled_mm, attention or paged_attention(_quant) on cuda:", dev, " reported ",
+    TORCH_CHECK(false, "b200::gemm_epilogue, scaled_mm, attention, paged_attention or paged_attention_quant on cuda:", dev, " reported ",
                 b200k_status_string(static_cast<int>(seen)), " (code ", seen, "): an earlier call's output is incomplete");
   }
   return 0;
