@@ -704,14 +704,15 @@ int b200k_rope_append_quant(const B200kRopeAppendQuantArgs* args, void* stream);
  * base.dtype is that of q and out, f16 or bf16; cache_strides in elements, multiples of 16.
  * Scales are positive; value scales below 1e-12 / 448 count as it.  Scores,
  * softmax and sums are fp32, keys' codes enter the products as they are and their
- * scales the scores.  Queries are rounded to f16 after each row was divided by a
- * power of two (bf16: exact but for values below 2^-28 of the row's largest),
- * weights to f16.  In sequences of few query rows values' codes enter the products
- * as they are too; in those of many (more than 32, or more than 16 with many keys)
- * code * scale is rounded to f16 relative to the largest scale of 64 keys (values
- * below 2^-23 of that by less than 2^-34 of it), and the values of keys that some
- * query of the sequence sees and another does not must be finite and below 2^70.
- * A NaN scale or code counts as a NaN key or value.  Workspace as for that entry, by
+ * scales the scores; weights are rounded to f16.  In sequences of few query rows
+ * values' codes enter the products as they are too, and bf16 queries are rounded
+ * to f16 after each row was divided by a power of two (exact but for values below
+ * 2^-28 of the row's largest).  In those of many (more than 32, or more than 16
+ * with many keys) code * scale is rounded to f16 relative to the largest value
+ * scale of 64 keys (values below 2^-23 of that by less than 2^-34 of it), and the
+ * values of keys that some query of the sequence sees and another does not must
+ * be finite and below 2^70.  A NaN scale or code counts as a NaN key or value.
+ * Workspace as for that entry, by
  * b200k_paged_attention_quant_workspace.
  */
 typedef struct {

@@ -7,7 +7,9 @@
 // No reference counterpart.  fp32 throughout, one rounding to e4m3; bound by
 // HBM: x is read once, one or two bytes (four with a gate) for each byte
 // written.  16 lanes hold the 128 columns of a scale, 8 each, so its maximum
-// is four shuffles; each takes kUnits groups, whose loads are issued together.
+// is four shuffles; with many rows each takes four groups, whose loads are issued
+// together.  Measured: the SwiGLU of [16384, 2 x 8192] bf16 115 us = 5.9 TB/s, 64
+// rows of 4096 1.7 us.
 #include <algorithm>
 #include <cstring>
 
