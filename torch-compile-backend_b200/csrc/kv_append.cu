@@ -240,12 +240,12 @@ __global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_con
       *reinterpret_cast<uint4*>(dst + c0) = !turns ? a[i] : BF16 ? pack_bf16x8(u) : pack_f16x8(u);
       *reinterpret_cast<uint4*>(dst + c1) = !turns ? b[i] : BF16 ? pack_bf16x8(w) : pack_f16x8(w);
     } else if (pl.cache >= 0) {
-      float inv;
-      const float s = scale_of(top, inv);
+      float inv, rest;
+      const float s = scale_of(top, inv, rest);
       const int kvh = h - p.heads - (is_v ? p.kv_heads : 0);
       uint8_t* dst = (is_v ? p.v8 : p.k8) + pl.cache + kvh * p.c_head;
-      *reinterpret_cast<uint2*>(dst + c0) = e4m3x8(u, inv);
-      *reinterpret_cast<uint2*>(dst + c1) = e4m3x8(w, inv);
+      *reinterpret_cast<uint2*>(dst + c0) = e4m3x8(u, inv, rest);
+      *reinterpret_cast<uint2*>(dst + c1) = e4m3x8(w, inv, rest);
       if (unit == 0) (is_v ? p.vs : p.ks)[pl.scale + kvh * p.s_head] = s;
     }
   }
@@ -285,10 +285,10 @@ __global__ void __launch_bounds__(256) rope_append8_any_kernel(const __grid_cons
     uint32_t top = 0;
     for (int j = lane; j < p.dim; j += 32) top = max(top, mag(value(j)));
     top = __reduce_max_sync(0xffffffffu, top);
-    float inv;
-    const float s = scale_of(top, inv);
+    float inv, rest;
+    const float s = scale_of(top, inv, rest);
     uint8_t* dst = (is_v ? p.v8 : p.k8) + pl.cache + kvh * p.c_head;
-    for (int j = lane; j < p.dim; j += 32) dst[j] = static_cast<uint8_t>(e4m3x2(value(j) * inv, 0.0f) & 0xff);
+    for (int j = lane; j < p.dim; j += 32) dst[j] = e4m3(value(j), inv, rest);
     if (lane == 0) (is_v ? p.vs : p.ks)[pl.scale + kvh * p.s_head] = s;
   }
 }

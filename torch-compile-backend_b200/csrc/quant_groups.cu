@@ -81,10 +81,10 @@ __global__ void __launch_bounds__(kThreads) quant16_kernel(const __grid_constant
     uint32_t top = top8(y);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float inv;
-    const float s = scale_of(top, inv);
+    float inv, rest;
+    const float s = scale_of(top, inv, rest);
     if (col[i] >= p.cols) continue;
-    *reinterpret_cast<uint2*>(p.out + row[i] * p.cols + col[i]) = e4m3x8(y, inv);
+    *reinterpret_cast<uint2*>(p.out + row[i] * p.cols + col[i]) = e4m3x8(y, inv, rest);
     if (c0 == 0) p.scale[row[i] * p.groups + col[i] / 128] = s;
   }
 }
@@ -112,12 +112,12 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const __grid_consta
       top = max(top, mag(y[j]));
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    float inv;
-    const float s = scale_of(top, inv);
+    float inv, rest;
+    const float s = scale_of(top, inv, rest);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = g * 128 + j * 32 + lane;
-      if (c < p.cols) p.out[row * p.cols + c] = static_cast<uint8_t>(e4m3x2(y[j] * inv, 0.0f) & 0xff);
+      if (c < p.cols) p.out[row * p.cols + c] = e4m3(y[j], inv, rest);
     }
     if (lane == 0) p.scale[unit] = s;
   }
