@@ -318,8 +318,7 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
           }
         }
       }
-      // No load is in flight, and no commit of the even CTA's on its way to the
-      // odd one's barriers, when the MMAs have read every stage; after a timeout
+      // No load is in flight when the MMAs have read every stage; after a timeout
       // the loads that no MMA waited for are waited for here.
       for (int x = 0; x < S; ++x)
         if (issued > x) wait_bar_drain(&empty[x], x < s ? ph : (ph ^ 1u), ok ? 100000000ull : 1000000ull);
@@ -327,7 +326,11 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
         for (int64_t k = issued > S ? issued - S : 0; k < issued; ++k)
           wait_bar_drain(&full[k % S], static_cast<uint32_t>((k / S) & 1), 100000000ull);
       }
-    } else if ((warp & 1) && (!WIDE || rank == 0)) {
+    } else if (WIDE && (warp & 1) && rank != 0) {
+      // The even CTA's commits arrive here too: the last of each issuer, behind all
+      // its MMAs, before this CTA's shared memory may become another's.
+      wait_bar_drain(&drain[warp >> 1], 0, 100000000ull);
+    } else if (warp & 1) {
       // ----------------------------------------------------------- MMA issuers
       // fp32 accumulators, both operands e4m3 (format 0) and K-major
       const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) | ((WIDE ? 256u : 128u) >> 4 << 24);
@@ -356,7 +359,8 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
           bph ^= 1u;
         }
       }
-      // every MMA of this warp completes before tensor memory is freed
+      // every MMA of this warp completes before tensor memory is freed (the odd CTA
+      // waits for its arrival as well)
       commit<WIDE>(&drain[which]);
       wait_bar_drain(&drain[which], 0, 100000000ull);
     } else if (warp == 2) {
