@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int box = p.box_rows;                          // 0: no TMA
       const int boxes = box > 0 ? kBlock / box : 0;        // of one 64-element half
       int c = 0;
+      int issued = 0, q_issued = 0;  // blocks and portions' queries whose copies have been issued
       bool ok = true;
       for (int li = 0; ok && walk.next(p, po); ++li) {
         const Unit& u = walk.u;
@@ -215,9 +216,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             cp_arrive(&full[st]);
           }
+          issued = c + 1;
           if (j == po.beg) {
             // the portion's queries, when the products of the one before have read theirs
             if (li > 0 && !(ok = warp_wait(q_empty, (li - 1) & 1, ctl))) break;
+            q_issued = li + 1;
             if (p.q_box > 0) {
               // tiles of 128 / G tokens
               const int t = is_v ? 1 : 0, r0 = u.r0 + t * 128;
@@ -248,11 +251,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      // The last TMA boxes have landed when the issuers are done with them;
-      // after a timeout they are waited for here.
-      if (!ok) {
-        for (int k = max(0, c - S); k < c; ++k) gemm::wait_bar_drain(&full[k % S], (k / S) & 1, 100000000ull);
-      }
+      // No box is on its way when this warp leaves: the last ones have landed when
+      // their readers are done with them, except after a timeout.  (Queries wait for
+      // the other loader's arrivals too, which may not come then.)
+      for (int k = max(0, issued - S); k < issued; ++k) gemm::wait_bar_drain(&full[k % S], (k / S) & 1, 100000000ull);
+      if (q_issued > 0) gemm::wait_bar_drain(q_full, (q_issued - 1) & 1, 10000000ull);
       __syncwarp();
   } else {
     softmax_rows<BF16, D, CAP, false>(p, walk, ctl, b, tmem_base, run, warp, lane);

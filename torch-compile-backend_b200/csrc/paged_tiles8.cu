@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
       const int boxes = box > 0 ? kBlock / box : 0;
       Portion po;
       int c = 0;
+      int issued = 0, q_issued = 0;  // blocks and portions' queries whose copies have been issued
       bool ok = true;
       for (int li = 0; ok && walk.next(p, po); ++li) {
         const Unit& u = walk.u;
@@ -292,9 +293,11 @@ __global__ void __launch_bounds__(kThreads8, 1)
           for (int i = 0; i < 2; ++i)
             cp4(ring_sc + (st * kBlock + i * 32 + lane) * 4, scales + (at[i].scale >= 0 ? at[i].scale : 0), at[i].scale >= 0);
           cp_arrive(&full[st]);
+          issued = c + 1;
           if (j == po.beg) {
             // the portion's queries, when the products of the one before have read theirs
             if (li > 0 && !(ok = warp_wait(q_empty, (li - 1) & 1, ctl))) break;
+            q_issued = li + 1;
             const int t = is_v ? 1 : 0;
             if (p.q_box > 0) {
               // tiles of 128 / G tokens
@@ -327,11 +330,11 @@ __global__ void __launch_bounds__(kThreads8, 1)
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      // The last TMA boxes have landed when the converters are done with them;
-      // after a timeout they are waited for here.
-      if (!ok) {
-        for (int k = max(0, c - R); k < c; ++k) gemm::wait_bar_drain(&full[k % R], (k / R) & 1, 100000000ull);
-      }
+      // No box is on its way when this warp leaves: the last ones have landed when
+      // their readers are done with them, except after a timeout.  (Queries wait for
+      // the other loader's arrivals too, which may not come then.)
+      for (int k = max(0, issued - R); k < issued; ++k) gemm::wait_bar_drain(&full[k % R], (k / R) & 1, 100000000ull);
+      if (q_issued > 0) gemm::wait_bar_drain(q_full, (q_issued - 1) & 1, 10000000ull);
       __syncwarp();
     }
   } else {
