@@ -31,14 +31,25 @@ __device__ __forceinline__ float round_f16(float x) { return __half2float(__floa
 // ---------------------------------------------------------------------------
 // Element loads / stores with conversion to/from fp32.
 // ---------------------------------------------------------------------------
+// Read-only loads are for memory that nobody writes while the kernel runs, and may be
+// moved ahead of any wait.  A kernel that starts under the end of the one before it
+// (launch_early) reads what that one writes: EARLY, by ordinary loads, which stay
+// behind griddepcontrol.wait.
+template <bool EARLY, typename T>
+__device__ __forceinline__ T fetch(const T* p) {
+  if constexpr (EARLY) return *p;
+  else return __ldg(p);
+}
+
+template <bool EARLY = false>
 __device__ __forceinline__ float load_scalar(const void* base, int64_t off, int dt) {
   switch (dt) {
-    case B200K_F32: return __ldg(reinterpret_cast<const float*>(base) + off);
-    case B200K_F16: return __half2float(__ldg(reinterpret_cast<const __half*>(base) + off));
-    case B200K_BF16: return __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(base) + off));
-    case B200K_F64: return static_cast<float>(__ldg(reinterpret_cast<const double*>(base) + off));
-    case B200K_I32: return static_cast<float>(__ldg(reinterpret_cast<const int32_t*>(base) + off));
-    case B200K_I64: return static_cast<float>(__ldg(reinterpret_cast<const long long*>(base) + off));
+    case B200K_F32: return fetch<EARLY>(reinterpret_cast<const float*>(base) + off);
+    case B200K_F16: return __half2float(fetch<EARLY>(reinterpret_cast<const __half*>(base) + off));
+    case B200K_BF16: return __bfloat162float(fetch<EARLY>(reinterpret_cast<const __nv_bfloat16*>(base) + off));
+    case B200K_F64: return static_cast<float>(fetch<EARLY>(reinterpret_cast<const double*>(base) + off));
+    case B200K_I32: return static_cast<float>(fetch<EARLY>(reinterpret_cast<const int32_t*>(base) + off));
+    case B200K_I64: return static_cast<float>(fetch<EARLY>(reinterpret_cast<const long long*>(base) + off));
     case B200K_BOOL:
     case B200K_U8: return static_cast<float>(reinterpret_cast<const uint8_t*>(base)[off]);
     default: return 0.0f;
@@ -47,10 +58,11 @@ __device__ __forceinline__ float load_scalar(const void* base, int64_t off, int 
 
 // Loads 8 consecutive elements starting at element offset `off` (16-byte
 // aligned for 2-byte types, 32-byte for fp32: the host guarantees it).
+template <bool EARLY = false>
 __device__ __forceinline__ void load_vec8(const void* base, int64_t off, int dt, float (&v)[8]) {
   switch (dt) {
     case B200K_BF16: {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + off));
+      const uint4 u = fetch<EARLY>(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + off));
       const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -61,7 +73,7 @@ __device__ __forceinline__ void load_vec8(const void* base, int64_t off, int dt,
       break;
     }
     case B200K_F16: {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(base) + off));
+      const uint4 u = fetch<EARLY>(reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(base) + off));
       const __half2* h = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -73,14 +85,14 @@ __device__ __forceinline__ void load_vec8(const void* base, int64_t off, int dt,
     }
     case B200K_F32: {
       const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + off);
-      const float4 a = __ldg(p), b = __ldg(p + 1);
+      const float4 a = fetch<EARLY>(p), b = fetch<EARLY>(p + 1);
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
       v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
       break;
     }
     default: {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = load_scalar(base, off + j, dt);
+      for (int j = 0; j < 8; ++j) v[j] = load_scalar<EARLY>(base, off + j, dt);
       break;
     }
   }

@@ -49,8 +49,9 @@ struct AppendParams {
   int32_t q8;
 };
 
+template <bool EARLY>
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
-  return is64 ? __ldg(static_cast<const long long*>(p) + i) : __ldg(static_cast<const int*>(p) + i);
+  return is64 ? fetch<EARLY>(static_cast<const long long*>(p) + i) : fetch<EARLY>(static_cast<const int*>(p) + i);
 }
 
 // Where a token goes: its table row (clamped into the table) and its offset
@@ -60,8 +61,9 @@ struct Place {
   int64_t row, cache;
   int64_t scale;  // with cache >= 0: of the e4m3 caches' scales
 };
+template <bool EARLY>
 __device__ __forceinline__ Place place_of(const AppendParams& p, int64_t t) {
-  int64_t pos = load_index(p.positions, t, p.pos64), slot = load_index(p.slots, t, p.slot64);
+  int64_t pos = load_index<EARLY>(p.positions, t, p.pos64), slot = load_index<EARLY>(p.slots, t, p.slot64);
   const bool pos_ok = pos >= 0 && pos < p.table_rows;
   if (slot >= p.total_slots || (!pos_ok && slot >= 0)) {
     if (p.status) atomicCAS(p.status, 0, B200K_ERR_INDEX);
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_cons
     a[i] = __ldg(reinterpret_cast<const uint4*>(src + c0));
     b[i] = __ldg(reinterpret_cast<const uint4*>(src + c1));
   }
-  const Place pl = place_of(p, tok);
+  const Place pl = place_of<false>(p, tok);
   float cs[8], sn[8];
   if (turns) {
     load_vec8(p.cos, pl.row * p.table_stride + c0, TAB_DT, cs);
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(256) rope_append_any_kernel(const __grid_const
     const int64_t tok = e / per_tok;
     const int in_tok = static_cast<int>(e - tok * per_tok);
     const int h = in_tok / p.dim, j = in_tok - h * p.dim;
-    const Place pl = place_of(p, tok);
+    const Place pl = place_of<false>(p, tok);
     const uint16_t* src;
     if (h < p.heads) src = p.q + tok * p.q_t + h * p.q_h;
     else if (h < p.heads + p.kv_heads) src = p.k + tok * p.k_t + (h - p.heads) * p.k_h;
@@ -204,14 +206,14 @@ __global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_con
     if (h < p.heads) src = p.q + tok * p.q_t + h * p.q_h;
     else if (h < p.heads + p.kv_heads) src = p.k + tok * p.k_t + (h - p.heads) * p.k_h;
     else src = p.v + tok * p.v_t + (h - p.heads - p.kv_heads) * p.v_h;
-    a[i] = __ldg(reinterpret_cast<const uint4*>(src + c0));
-    b[i] = __ldg(reinterpret_cast<const uint4*>(src + c1));
+    a[i] = fetch<true>(reinterpret_cast<const uint4*>(src + c0));
+    b[i] = fetch<true>(reinterpret_cast<const uint4*>(src + c1));
   }
-  const Place pl = place_of(p, tok);
+  const Place pl = place_of<true>(p, tok);
   float cs[8], sn[8];
   if (turns) {
-    load_vec8(p.cos, pl.row * p.table_stride + c0, TAB_DT, cs);
-    load_vec8(p.sin, pl.row * p.table_stride + c0, TAB_DT, sn);
+    load_vec8<true>(p.cos, pl.row * p.table_stride + c0, TAB_DT, cs);
+    load_vec8<true>(p.sin, pl.row * p.table_stride + c0, TAB_DT, sn);
   }
 #pragma unroll
   for (int i = 0; i < NH; ++i) {
@@ -262,15 +264,15 @@ __global__ void __launch_bounds__(256) rope_append8_any_kernel(const __grid_cons
   for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
     const int64_t tok = r / all;
     const int h = static_cast<int>(r - tok * all);
-    const Place pl = place_of(p, tok);
+    const Place pl = place_of<true>(p, tok);
     const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
     const int kvh = h - p.heads - (is_v ? p.kv_heads : 0);
     const uint16_t* src = is_q ? p.q + tok * p.q_t + h * p.q_h : is_v ? p.v + tok * p.v_t + kvh * p.v_h : p.k + tok * p.k_t + kvh * p.k_h;
     auto value = [&](int j) {
-      if (j >= p.rot || is_v) return load_scalar(src, j, DT);
+      if (j >= p.rot || is_v) return load_scalar<true>(src, j, DT);
       const int half = p.rot >> 1, i = j < half ? j : j - half;
-      const float c = load_scalar(p.cos, pl.row * p.table_stride + i, TAB_DT), s = load_scalar(p.sin, pl.row * p.table_stride + i, TAB_DT);
-      const float x = load_scalar(src, i, DT), y = load_scalar(src, i + half, DT);
+      const float c = load_scalar<true>(p.cos, pl.row * p.table_stride + i, TAB_DT), s = load_scalar<true>(p.sin, pl.row * p.table_stride + i, TAB_DT);
+      const float x = load_scalar<true>(src, i, DT), y = load_scalar<true>(src, i + half, DT);
       return j < half ? x * c - y * s : y * c + x * s;
     };
     if (is_q) {

@@ -96,7 +96,8 @@ struct Seq {
 
 __device__ __forceinline__ Seq seq_at(const Params& p, int b) {
   Seq s;
-  const int a0 = __ldg(p.q_start + b), a1 = __ldg(p.q_start + b + 1), n = __ldg(p.kv_len + b);
+  // (in the row kernel over e4m3 caches, launched early)
+  const int a0 = fetch<true>(p.q_start + b), a1 = fetch<true>(p.q_start + b + 1), n = fetch<true>(p.kv_len + b);
   s.t0 = min(max(a0, 0), p.T);
   s.m = min(max(a1, s.t0), p.T) - s.t0;
   s.n = min(max(n, 0), p.capacity);

@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas8<D, ROWS>) rows8_kernel(con
   auto page_of = [&](const Cursor<kKeys8, ROWS>& c) {
     const int key = c.w.base + c.tile * kKeys8 + lane;
     if (key < c.w.s.lo || key >= c.w.s.n) return -1;
-    return __ldg(p.table + c.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
+    return fetch<true>(p.table + c.b * p.table_stride + fdiv(static_cast<uint32_t>(key), p.div_page));
   };
   int page = page_of(ld);
   int ld_stage = 0;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas8<D, ROWS>) rows8_kernel(con
         uint4 q[D / 32];
 #pragma unroll
         for (int k = 0; k < D / 32; ++k)  // 16 of every 64 columns
-          q[k] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + (k >> 1) * 64 + (k & 1) * 8)) : make_uint4(0, 0, 0, 0);
+          q[k] = r < rows ? fetch<true>(reinterpret_cast<const uint4*>(src + (k >> 1) * 64 + (k & 1) * 8)) : make_uint4(0, 0, 0, 0);
         float mul = 1.0f;
         if (BF16) {
           uint32_t top = 0;

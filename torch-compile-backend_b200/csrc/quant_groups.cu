@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(kThreads) quant16_kernel(const __grid_constant
     }
     if (col[i] < p.cols) {
       const uint16_t* x = static_cast<const uint16_t*>(p.x) + row[i] * p.x_stride + col[i];
-      a[i] = __ldg(reinterpret_cast<const uint4*>(x));
-      if (SWIGLU) b[i] = __ldg(reinterpret_cast<const uint4*>(x + p.cols));
+      a[i] = fetch<true>(reinterpret_cast<const uint4*>(x));
+      if (SWIGLU) b[i] = fetch<true>(reinterpret_cast<const uint4*>(x + p.cols));
     }
   }
 #pragma unroll
@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const __grid_consta
       const int c = g * 128 + j * 32 + lane;
       y[j] = 0.0f;
       if (c < p.cols) {
-        y[j] = load_scalar(p.x, row * p.x_stride + c, DT);
-        if (p.swiglu) y[j] = gated(y[j], load_scalar(p.x, row * p.x_stride + p.cols + c, DT));
+        y[j] = load_scalar<true>(p.x, row * p.x_stride + c, DT);
+        if (p.swiglu) y[j] = gated(y[j], load_scalar<true>(p.x, row * p.x_stride + p.cols + c, DT));
       }
       top = max(top, mag(y[j]));
     }

@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
           const int n = tn * kTileN + (WIDE ? (lane >> 1 & 1) * 128 : 0);
           float b[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = j < left && n < p.N ? __ldg(p.sb + (k0 + j) * p.sb_k + n / kBlk * p.sb_n) : 0.0f;
+          for (int j = 0; j < 4; ++j) b[j] = j < left && n < p.N ? fetch<true>(p.sb + (k0 + j) * p.sb_k + n / kBlk * p.sb_n) : 0.0f;
           float* to = reinterpret_cast<float*>(sbase + C::kOffSc + (c & 1) * kScaleBytes) + kb4 * (kScaleRow + 4);
           if (WIDE && !(ok = warp_wait(&sc_empty[c & 1], ((c >> 1) & 1) ^ 1, ctl))) break;
 #pragma unroll 1
@@ -391,14 +391,14 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
               const int m = tm * kTileM + rows_at + r0 + (i0 + i) * 16;
               const float* pa = p.sa + m * p.sa_m + k0 * p.sa_k;
               if (vec && left > 0 && k0 + 4 <= p.k_blocks && m < p.M) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(pa));
+                const float4 v = fetch<true>(reinterpret_cast<const float4*>(pa));
                 a[i][0] = v.x;
                 a[i][1] = v.y;
                 a[i][2] = v.z;
                 a[i][3] = v.w;
               } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) a[i][j] = j < left && m < p.M ? __ldg(pa + j * p.sa_k) : 0.0f;
+                for (int j = 0; j < 4; ++j) a[i][j] = j < left && m < p.M ? fetch<true>(pa + j * p.sa_k) : 0.0f;
               }
             }
             if (!WIDE && i0 == 0 && !(ok = warp_wait(&sc_empty[c & 1], ((c >> 1) & 1) ^ 1, ctl))) break;
