@@ -703,15 +703,14 @@ int b200k_rope_append_quant(const B200kRopeAppendQuantArgs* args, void* stream);
  * them: key and value rows are code * scale, with k_scale and v_scale as there.
  * base.dtype is that of q and out, f16 or bf16; cache_strides in elements, multiples of 16.
  * Scales are positive; value scales below 1e-12 / 448 count as it.  Scores,
- * softmax and sums are fp32, keys' codes enter the products as they are and their
- * scales the scores; weights are rounded to f16.  In sequences of few query rows
- * values' codes enter the products as they are too, and bf16 queries are rounded
- * to f16 after each row was divided by a power of two (exact but for values below
- * 2^-28 of the row's largest).  In those of many (more than 32, or more than 16
- * with many keys) code * scale is rounded to f16 relative to the largest value
- * scale of 64 keys (values below 2^-23 of that by less than 2^-34 of it), and the
- * values of keys that some query of the sequence sees and another does not must
- * be finite and below 2^70.  A NaN scale or code counts as a NaN key or value.
+ * softmax and sums are fp32.  Codes enter both products as they are, keys' scales
+ * the scores and values' scales the weights, which are rounded to f16: half a step
+ * each, those below 2^-26 of a row's largest (a probability times its value's
+ * scale) by less than 2^-36 of it.  In sequences of few query rows bf16 queries are
+ * rounded to f16 after each row was divided by a power of two (exact but for values
+ * below 2^-28 of the row's largest).  A NaN scale or code counts as a NaN key or
+ * value; of keys that some query of the sequence sees and another does not, the
+ * values' codes and scales must not be NaN, and may be of any size.
  * Workspace as for that entry, by
  * b200k_paged_attention_quant_workspace.
  */

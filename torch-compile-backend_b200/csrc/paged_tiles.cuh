@@ -105,12 +105,14 @@ __device__ __forceinline__ float max2(float a, float b) {
 // integer (read off the low bits of x + 1.5 * 2^23), 2^f on [-1/2, 1/2] by
 // the polynomial of least relative error (Remez exchange; 7.5e-5 in degree 3
 // for bf16 probabilities, 2.6e-6 in degree 4 for f16: below half a step of
-// the type), n added to the exponent.  x below -125 gives 2^-125; x is not NaN
-// unless the row's maximum is.
-template <bool BF16>
+// the type), n added to the exponent.  x below -125 gives 2^-125, with ZERO 0 (x from
+// -250 on, whose exponents come out as negative integers); x is not NaN unless the
+// row's maximum is.
+template <bool BF16, bool ZERO>
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  x.x = fmaxf(x.x, -125.0f);
-  x.y = fmaxf(x.y, -125.0f);
+  constexpr float kLeast = ZERO ? -250.0f : -125.0f;
+  x.x = fmaxf(x.x, kLeast);
+  x.y = fmaxf(x.y, kLeast);
   const float big = 12582912.0f;
   const float2 t = __fadd2_rn(x, make_float2(big, big));
   const float2 n = __fadd2_rn(t, make_float2(-big, -big));
@@ -127,8 +129,12 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
     r = __ffma2_rn(r, f, both(0.69312181f));
     r = __ffma2_rn(r, f, both(0.99999926f));
   }
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+  int a = __float_as_int(r.x) + (__float_as_int(t.x) << 23), b = __float_as_int(r.y) + (__float_as_int(t.y) << 23);
+  if (ZERO) {
+    a = max(a, 0);
+    b = max(b, 0);
+  }
+  return make_float2(__int_as_float(a), __int_as_float(b));
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Ctl& c) {
   const bool ok = gemm::wait_bar(bar, parity, c);
@@ -219,13 +225,14 @@ struct Shared {
   const volatile int* copied;                     // [2 stages] of K, of V: the stage's block came by cp.async
   // over e4m3 caches (paged_tiles8.cu)
   uint64_t *sc_full, *sc_empty;                   // [kScaleSlots] by block
-  const float* sc;                                // [kScaleSlots][kScaleFloats]: 64 keys' scales, E, 2^-E
+  const float* sc;                                // [kScaleSlots][kScaleFloats]: 64 keys' ks, log2 vs, 1 / vs
 };
-constexpr int kScaleSlots = 8, kScaleFloats = kBlock + 4;
+// ks: times the scores' factor, except under a cap
+constexpr int kScaleSlots = 8, kScaleFloats = 3 * kBlock;
 
 // The MMA issuers: warps 8, 9 of S_t = Q_t K^T of tile t = 0, 1, warps 10, 11 of
-// O_t += P_t V.  S: stages; Q8: blocks made 16-bit
-// by warps that fence their writes themselves, keys in q's type, values in f16.
+// O_t += P_t V.  S: stages; Q8: codes made 16-bit by warps that fence their writes
+// themselves, keys' in q's type, values' in f16.
 template <bool BF16, int D, int S, bool Q8>
 __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
                                                int warp, int lane) {
@@ -302,10 +309,10 @@ __device__ __forceinline__ void issue_products(const Params& p, Walk& walk, cons
   __syncwarp();
 }
 
-// The softmax warps 0-7, one thread a query row.  Q8: scores are of codes, so each
-// is multiplied by its key's scale; values have been divided by a power of two a
-// block, 2^E, so the weights of a block are 2^(score + E - max (score + E)), and
-// their sum's share is multiplied by 2^-E.
+// The softmax warps 0-7, one thread a query row.  Q8: both products are of codes, so
+// a score is multiplied by its key's scale and has the logarithm of its value's added,
+// and a weight enters the sum over its value's scale (paged.cuh).  What a row does
+// not see has weight zero there, exactly: 1 / vs may be anything beside it.
 template <bool BF16, int D, int CAP, bool Q8>
 __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const Ctl& ctl, const Shared& b, uint32_t tmem_base,
                                              int64_t run, int warp, int lane) {
@@ -358,25 +365,24 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
 #pragma unroll
           for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(raw[c][i]);
       }
-      float shift = 0.0f, unshift = 1.0f;  // E, 2^-E
       if (Q8) {
 #pragma unroll
         for (int c = 0; c < kBlock; c += 4) {
-          const float4 k = *reinterpret_cast<const float4*>(scales + c);
-          const float2 x = __fmul2_rn(make_float2(s[c], s[c + 1]), make_float2(k.x, k.y));
-          const float2 y = __fmul2_rn(make_float2(s[c + 2], s[c + 3]), make_float2(k.z, k.w));
+          const float4 k = *reinterpret_cast<const float4*>(scales + c), lv = *reinterpret_cast<const float4*>(scales + kBlock + c);
+          float2 x = make_float2(s[c], s[c + 1]), y = make_float2(s[c + 2], s[c + 3]);
+          if (CAP == kNoCap) {
+            x = __ffma2_rn(x, make_float2(k.x, k.y), make_float2(lv.x, lv.y));
+            y = __ffma2_rn(y, make_float2(k.z, k.w), make_float2(lv.z, lv.w));
+          } else {
+            x = make_float2(score<CAP>(p, x.x * k.x) + lv.x, score<CAP>(p, x.y * k.y) + lv.y);
+            y = make_float2(score<CAP>(p, y.x * k.z) + lv.z, score<CAP>(p, y.y * k.w) + lv.w);
+          }
           s[c] = x.x;
           s[c + 1] = x.y;
           s[c + 2] = y.x;
           s[c + 3] = y.y;
         }
-        const float2 e = *reinterpret_cast<const float2*>(scales + kBlock);
-        shift = e.x;
-        unshift = e.y;
-        __syncwarp();
-        if (lane == 0) gemm::mbar_arrive(&b.sc_empty[slot]);
-      }
-      if (CAP != kNoCap) {
+      } else if (CAP != kNoCap) {
 #pragma unroll
         for (int c = 0; c < kBlock; ++c) s[c] = score<CAP>(p, s[c]);
       }
@@ -395,8 +401,8 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx[i] = max2(mx[i], s[kBlock - 4 + i]);
       float top = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
-      if (CAP == kNoCap) top *= p.mul;
-      if (Q8) top += shift;
+      constexpr bool kRaw = CAP == kNoCap && !Q8;  // scores that p.mul is still to be multiplied with
+      if (kRaw) top *= p.mul;
       const float was = m;
       float alpha = 1.0f;
       bool moved = false;
@@ -411,18 +417,22 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
       // down to 2^-26 of the row's maximum (smaller ones by less than 2^-36 of it)
       const float ref = (m == -INFINITY ? 0.0f : m) - kTileReach<P16>;
       float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-      const float off = Q8 ? shift - ref : -ref;
-      const float2 sc2 = CAP != kNoCap ? make_float2(1.0f, 1.0f) : make_float2(p.mul, p.mul), nm2 = make_float2(off, off);
+      const float2 sc2 = kRaw ? make_float2(p.mul, p.mul) : make_float2(1.0f, 1.0f), nm2 = make_float2(-ref, -ref);
       uint32_t pk[kBlock / 2];
 #pragma unroll
       for (int c = 0; c < kBlock; c += 2) {
         const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
-        const float2 e = c % kFmaEvery == kFmaEvery - 2 ? ex2_fma<P16>(x) : make_float2(ex2(x.x), ex2(x.y));
-        sum2[c / 2 % 2] = __fadd2_rn(sum2[c / 2 % 2], e);
+        const float2 e = c % kFmaEvery == kFmaEvery - 2 ? ex2_fma<P16, Q8>(x) : make_float2(ex2(x.x), ex2(x.y));
+        sum2[c / 2 % 2] = Q8 ? __ffma2_rn(e, *reinterpret_cast<const float2*>(scales + 2 * kBlock + c), sum2[c / 2 % 2])
+                             : __fadd2_rn(sum2[c / 2 % 2], e);
         pk[c / 2] = pack16<P16>(e.x, e.y);
       }
+      if (Q8) {
+        __syncwarp();
+        if (lane == 0) gemm::mbar_arrive(&b.sc_empty[slot]);
+      }
       const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-      l = fmaf(l, alpha, Q8 ? sum * unshift : sum);
+      l = fmaf(l, alpha, sum);
       if (__any_sync(0xffffffffu, moved)) {
         // P V of the block before has written O
         if (!(ok = warp_wait(&b.o_done[t * 2 + (buf ^ 1)], ((g - 1) >> 1) & 1, ctl))) break;
@@ -448,7 +458,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
     const bool had = je > jb;
     if (had && !(ok = warp_wait(&b.o_done[t * 2 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, ctl))) break;
     gemm::tc_fence_after();
-    // a row without keys has m = -inf (and l the sum of its 2^-125)
+    // a row without keys has m = -inf (and l the sum of its 2^-125, or 0)
     const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
     const int64_t part = static_cast<int64_t>(blockIdx.x) * 2 + po.slot;
 #pragma unroll

@@ -2,16 +2,14 @@
 // rows over e4m3 caches.  The plan, the portions, the products, the softmax and
 // the parts are the 16-bit tile kernel's (paged_tiles.cuh); here
 //   warps 12, 13 load codes (TMA boxes or 16-byte cp.async copies) and scales,
-//   warps 16, 17 make a block's key codes 16-bit in shared memory, of q's type and
-//                as they are (both types hold every code);
-//   warps 18, 19 its values f16, code * scale / 2^E rounded once, 2^E a power of
-//                two that no scale of the block is above, so that any magnitude
-//                fits.
-// Q K^T runs in q's type, P V in f16.  The keys' scales stay out of the products:
-// rounded into bf16 keys they would move every score, the output by 0.4 %.  The
-// softmax, which bounds the kernel, multiplies the scores by them; with the
-// values' scales there too, and queries made f16 first, chunks of prompts took
-// 517 us.  The registers are shared out by setmaxnreg: five warpgroups are
+//   warps 16, 17 make a block's key codes 16-bit in shared memory, of q's type,
+//   warps 18, 19 its value codes, f16: as they are (both types hold every code).
+// Q K^T runs in q's type, P V in f16.  All scales stay out of the products: rounded
+// into bf16 keys they would move every score, the output by 0.4 %; values of code *
+// scale have to be divided by something that all rows share for f16 (the block's
+// largest scale), and then a value that a row does not see, or gives no weight,
+// takes bits from those that it does.  The softmax, which bounds the kernel, takes
+// the scales in.  The registers are shared out by setmaxnreg: five warpgroups are
 // launched with 96 a thread.  Measured: 5 chunks of 1024 behind up to 6000 keys, 32 /
 // 8 heads of 128, 490 us = 535 TFLOP/s; 8 prompts of 2048, heads of 64, 490 us.
 #include "paged_tiles.cuh"
@@ -170,41 +168,37 @@ __global__ void __launch_bounds__(kThreads8, 1)
     while (ok && walk.next(p, po)) {
       for (int j = po.beg; j < po.end; ++j, ++c) {
         const int rst = c % R, st = c % S, slot = c % kScaleSlots;
-        if (!(ok = warp_wait(&r_full[rst], (c / R) & 1, ctl) && warp_wait(&empty[st], ((c / S) & 1) ^ 1, ctl))) break;
-        const uint4* src = reinterpret_cast<const uint4*>(raw + rst * L::kCodes);
-        uint8_t* dst = dst0 + st * L::kBlk;
-        const float s0 = raw_sc[rst * kBlock + lane], s1 = raw_sc[rst * kBlock + 32 + lane];
-        // 2^E from the exponent of the largest scale (a NaN or infinite one
-        // makes its own row NaN), and 2^-E
-        float up = 1.0f, down = 1.0f;
-        if (is_v) {
-          auto bits = [](float x) { return x < 3e38f ? __float_as_uint(fmaxf(x, kMinVs)) : __float_as_uint(kMinVs); };
-          const uint32_t e = min((__reduce_max_sync(0xffffffffu, max(bits(s0), bits(s1))) >> 23) + 1, 253u);
-          up = __uint_as_float(e << 23);
-          down = __uint_as_float((254u - e) << 23);
-        }
+        if (!(ok = warp_wait(&r_full[rst], (c / R) & 1, ctl))) break;
         if (signs) {
           if (!(ok = warp_wait(&sc_empty[slot], ((c / kScaleSlots) & 1) ^ 1, ctl))) break;
           float* to = sc + slot * kScaleFloats;
-          if (!is_v) {
-            to[lane] = s0;
-            to[32 + lane] = s1;
-          } else if (lane == 0) {
-            to[kBlock] = static_cast<float>(static_cast<int>(__float_as_uint(up) >> 23) - 127);
-            to[kBlock + 1] = down;
+#pragma unroll
+          for (int i = lane; i < kBlock; i += 32) {
+            const float x = raw_sc[rst * kBlock + i];
+            if (is_v) {
+              const float v = value_scale(x);
+              to[kBlock + i] = lg2(v);
+              to[2 * kBlock + i] = 1.0f / v;
+            } else {
+              to[i] = CAP == kNoCap ? x * p.mul : x;
+            }
           }
+          __syncwarp();
+          if (lane == 0) gemm::mbar_arrive(&sc_full[slot]);
         }
+        if (!(ok = warp_wait(&empty[st], ((c / S) & 1) ^ 1, ctl))) break;
+        const uint4* src = reinterpret_cast<const uint4*>(raw + rst * L::kCodes);
+        uint8_t* dst = dst0 + st * L::kBlk;
 #pragma unroll 2
         for (int i = 0; i < kBlock * kChunks / 64; ++i) {
           const int idx = i * 64 + first, row = idx / kChunks, ch = idx % kChunks;
           const uint4 x = src[idx];
           uint32_t y[8] = {codes_lo(x.x), codes_hi(x.x), codes_lo(x.y), codes_hi(x.y), codes_lo(x.z), codes_hi(x.z), codes_lo(x.w), codes_hi(x.w)};
-          if (is_v || BF16) {
-            const float f = is_v ? raw_sc[rst * kBlock + row] * down : 1.0f;
+          if (BF16 && !is_v) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&y[k]));
-              y[k] = is_v ? pack16<false>(a.x * f, a.y * f) : pack16<BF16>(a.x, a.y);
+              y[k] = pack16<BF16>(a.x, a.y);
             }
           }
           // two 16-byte chunks; the upper half's lanes write theirs the other way
@@ -220,7 +214,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
         if (lane == 0) {
           gemm::mbar_arrive(&full[st]);
           gemm::mbar_arrive(&r_empty[rst]);
-          if (signs) gemm::mbar_arrive(&sc_full[slot]);
         }
       }
     }
