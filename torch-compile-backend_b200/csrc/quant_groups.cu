@@ -32,8 +32,24 @@ struct QuantParams {
   float* scale;
 };
 
-// silu(g) u
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// silu(g) u of two values, with h = e^(-|g| / 2):
+//   g u / (1 + h^2) for g >= 0,  (g / (1 + h^2) h) (h u) below,
+// so nothing overflows and no factor vanishes before the result does, whatever u is
+// (g / (1 + e^-g) divides by more than 2^126 from g = -87.3 on, where fast division
+// gives 0).  Packed but for the exponential, the reciprocal and the choice.
+__device__ __forceinline__ float2 gated2(float2 g, float2 u) {
+  constexpr float kHalfLog2e = 0.5f * 1.4426950408889634f;
+  const float2 one = make_float2(1.0f, 1.0f), a = __fmul2_rn(g, make_float2(kHalfLog2e, kHalfLog2e));
+  float2 h, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h.x) : "f"(-fabsf(a.x)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h.y) : "f"(-fabsf(a.y)));
+  const float2 d = __ffma2_rn(h, h, one);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  const float2 m = make_float2(g.x < 0.0f ? h.x : 1.0f, g.y < 0.0f ? h.y : 1.0f);
+  return __fmul2_rn(__fmul2_rn(__fmul2_rn(g, r), m), __fmul2_rn(m, u));
+}
+__device__ __forceinline__ float gated(float g, float u) { return gated2(make_float2(g, g), make_float2(u, u)).x; }
 
 __device__ __forceinline__ void row_of(const QuantParams& p, int64_t unit, int64_t& row, int& group) {
   row = p.big ? unit / p.groups : fdiv(static_cast<uint32_t>(unit), p.div_groups);
@@ -76,7 +92,11 @@ __global__ void __launch_bounds__(kThreads) quant16_kernel(const __grid_constant
       float u[8];
       unpack16<BF16>(b[i], u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = gated(y[j], u[j]);
+      for (int j = 0; j < 8; j += 2) {
+        const float2 z = gated2(make_float2(y[j], y[j + 1]), make_float2(u[j], u[j + 1]));
+        y[j] = z.x;
+        y[j + 1] = z.y;
+      }
     }
     uint32_t top = top8(y);
 #pragma unroll
