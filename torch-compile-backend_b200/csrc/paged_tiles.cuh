@@ -359,7 +359,8 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
         uint32_t raw[kBlock / 32][32];
 #pragma unroll
         for (int c = 0; c < kBlock / 32; ++c) gemm::tmem_ld32(tS + buf * 64 + c * 32, raw[c]);
-        gemm::tmem_wait_ld();
+        // (the waits name the registers, so that no use of them is scheduled ahead)
+        gemm::tmem_wait_ld_regs2(raw[0], raw[1]);
 #pragma unroll
         for (int c = 0; c < kBlock / 32; ++c)
 #pragma unroll
@@ -441,7 +442,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           gemm::tmem_ld32(tO + c * 32, o);
-          gemm::tmem_wait_ld();
+          gemm::tmem_wait_ld_regs(o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
           tmem_st32(tO + c * 32, o);
@@ -466,7 +467,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, Walk& walk, const 
       uint32_t o[32];
       if (had) {
         gemm::tmem_ld32(tO + c * 32, o);
-        gemm::tmem_wait_ld();
+        gemm::tmem_wait_ld_regs(o);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0u;
