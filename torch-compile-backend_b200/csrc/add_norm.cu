@@ -29,7 +29,6 @@
 namespace b200k {
 namespace {
 
-
 struct AddNormParams {
   int64_t rows;
   int32_t cols;

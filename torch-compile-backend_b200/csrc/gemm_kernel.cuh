@@ -48,6 +48,13 @@
 namespace b200k {
 namespace gemm {
 
+// Host helpers of the kernels with tensor maps (gemm_sm100.cu).
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn();
+CUtensorMapDataType tma_dtype(int dt);
+
 constexpr int BM = 128;
 constexpr int BK = 64;  // one 128-byte swizzle atom of 16-bit elements
 constexpr int UMMA_K = 16;

@@ -30,7 +30,6 @@
 #include <cstring>
 #include <type_traits>
 
-#include "e4m3.cuh"
 #include "host_common.h"
 #include "paged.cuh"
 #include "rowreduce.cuh"
@@ -48,9 +47,6 @@ constexpr uint32_t kRingBytes = 24576;  // of one warp
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

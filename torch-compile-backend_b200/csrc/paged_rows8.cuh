@@ -23,9 +23,6 @@
 template <int ROWS>
 constexpr uint32_t kRing8Bytes = ROWS == 8 ? 18432 : 27648;
 
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 r;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");

@@ -7,15 +7,6 @@
 #include "paged.cuh"
 
 namespace b200k {
-namespace gemm {
-// Host helpers defined with the GEMM's host code (gemm_sm100.cu).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn();
-CUtensorMapDataType tma_dtype(int dt);
-}  // namespace gemm
-
 namespace paged {
 namespace {
 
@@ -28,12 +19,6 @@ constexpr uint32_t kHalfBlk = kBlock * 128;
 // 2048 (32 heads of 64): 277 us, 291 with none, 286 with half of them.
 constexpr int kFmaEvery = 8;
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
-}
 // The barrier's arrival of this thread, when its copies so far have landed.
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");

@@ -41,15 +41,6 @@
 #include "gemm_kernel.cuh"
 
 namespace b200k {
-namespace gemm {
-// Host helpers defined with the GEMM's host code (gemm_sm100.cu).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn();
-CUtensorMapDataType tma_dtype(int dt);
-}  // namespace gemm
-
 namespace mm8 {
 namespace {
 
