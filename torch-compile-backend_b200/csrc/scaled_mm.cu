@@ -254,6 +254,11 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
     prefetch_map(&tmB);
     if (WIDE) prefetch_map(&tmO);
   }
+  // Launched under the end of the kernel before, whose writes are waited for here.
+  // Tensor memory is taken behind the wait and what follows in the stream launched
+  // when all CTAs have theirs: of two kernels that overlap neither holds tensor
+  // memory that the other, for which it waits, has still to take.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == 2) {
     if (WIDE) {
       tmem_alloc_pair(tmem_slot, C::kTmemCols);
@@ -264,13 +269,10 @@ __global__ void __launch_bounds__(Cfg8<BN>::kThreads, Cfg8<BN>::kCtas)
     }
   }
   tc_fence_before();
-  // Launched under the end of the kernel before, whose writes are waited for
-  // here; what follows in the stream may be launched from now on and does so too.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (WIDE) cluster_sync();  // the other CTA's barriers are there too
   else __syncthreads();
   tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
   const Ctl ctl{abort_flag, p.status, static_cast<uint64_t>(p.timeout_ns)};
   const int cid = static_cast<int>(blockIdx.x) / cluster, ncl = static_cast<int>(gridDim.x) / cluster;
