@@ -614,7 +614,8 @@ int b200k_paged_attention_workspace(const B200kPagedAttentionArgs* args, int64_t
  * reference has no 8-bit type):
  *   y = x, or with `swiglu` silu(x[:, c]) * x[:, cols + c],  c < cols, fp32
  *   scale[r, g] = max(max |y[r, 128 g ..]|, 1e-12) / 448
- *   out[r, c]   = e4m3(y[r, c] / scale[r, c / 128]), round to nearest even
+ *   out[r, c]   = e4m3(y[r, c] * 448 / max(max |y|, 1e-12)), round to nearest even
+ *   (of 16-bit x the code of the exact quotient; else the quotient is fp32's)
  * of a [rows, cols] view (with `swiglu` [rows, 2 cols]: the gate in front) of
  * f32, f16 or bf16 with unit column stride; the last group of a row may be
  * shorter.  out [rows, cols] and scale [rows, ceil(cols / 128)] are contiguous
@@ -686,8 +687,9 @@ int b200k_scaled_mm(const B200kScaledMmArgs* args, void* stream);
  * s = max(max |row|, 1e-12) / 448 in k_scale / v_scale, [num_pages, page_size,
  * kv_heads] of fp32 with scale_strides (page, slot, head; the same for both).
  * base.k_cache and base.v_cache are e4m3, cache_strides in elements; q_out is
- * of the inputs' type.  All else is as there; NaN and infinite values as in
- * b200k_quant_groups.
+ * of the inputs' type.  Slots that appear twice leave codes and scale of either
+ * token, in any mixture.  All else is as there; roundings, NaN and infinite values
+ * as in b200k_quant_groups.
  */
 typedef struct {
   B200kRopeAppendArgs base;

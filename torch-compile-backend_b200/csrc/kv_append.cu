@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256) rope_append_any_kernel(const __grid_const
 // is its largest magnitude / 448, found by the units' threads of its head (a
 // power of two of neighbouring lanes) from the fp32 values, which are rounded
 // once.  All lanes stay to the end for the shuffles.  Bound by the chain of index,
-// table and data loads at 24 warps an SM (76 registers): 16384 tokens of 32 / 8
+// table and data loads at 24 warps an SM (77 to 80 registers): 16384 tokens of 32 / 8
 // heads of 64 43 us = 4.3 TB/s; 64 tokens of 32 / 8 heads of 128 2.1 us.
 template <bool BF16, int TAB_DT, int NH>
 __global__ void __launch_bounds__(kThreads) rope_append8_kernel(const __grid_constant__ AppendParams p) {

@@ -937,13 +937,18 @@ int check_shape(const B200kPagedAttentionArgs* a) {
 // Sequences of more query rows than this run the tile kernel.  With 16 and 64
 // in place of 32: 20 rows of 32 sequences to 4000 keys 82 and 75 us (32: 75),
 // 32 rows 85 and 91 (91), 20 rows of 2 sequences to 1000 keys 28 and 12 (12), up
-// to 68 rows of 8 sequences to 1500 keys, heads of 64, 22 and 29 (27).
+// to 68 rows of 8 sequences to 1500 keys, heads of 64, 22 and 29 (27).  Those are
+// figures of 16-bit caches; e4m3 ones take the same limits, which are low for them:
+// row and tile kernel, 36 rows of 16 sequences to 4000 keys, 88 and 121 us, 64 rows
+// 115 and 121, 68 rows of 8 sequences to 1500 keys, heads of 64, 36 and 38.
 constexpr int kLongRows = 32;
 
 // ... and sequences of more rows than one block of the row kernel where all
 // such have this many steps of 128 values together.  Five tokens of 16
 // sequences, 32 / 8 heads of 128, to 1000 (8000 steps), 2000, 4000 and 8000
-// keys: row kernel 30, 52, 90 and 165 us, tile kernel 32, 44, 64 and 108.  Only
+// keys: row kernel 30, 52, 90 and 165 us, tile kernel 32, 44, 64 and 108.  Over e4m3
+// caches, whose steps are twice the keys, to 2000, 4000 and 8000 keys: row kernel 41,
+// 66 and 111, tile kernel 77, 119 and 197, so there the row kernel would do.  Only
 // the device knows the lengths; where the page table could hold as many steps
 // the tile kernel is launched, which costs 2 to 6 us when it has no work.
 constexpr int64_t kMidSteps = 12288;

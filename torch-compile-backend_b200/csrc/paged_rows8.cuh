@@ -13,9 +13,9 @@
 // of four keys, byte permutes pair the keys of a column, and a lane ends with
 // those columns of its rows.  Both rings are swizzled for these loads.  Scales:
 // see paged.cuh.  Measured: one token of 64 sequences to 8192 keys, 32 / 8 heads of
-// 128, 131-135 us = 5.2-5.4 TB/s (121 with the cache laid out head by head: rows of
+// 128, 130-136 us = 5.2-5.4 TB/s (121 with the cache laid out head by head: rows of
 // 128 bytes at 1 KB steps are what bounds it, the loads alone take 94 % of the
-// time); of 3 sequences to 65536 keys 57-59 us.  Codes straight into e4m3 products,
+// time); of 3 sequences to 65536 keys 57-60 us.  Codes straight into e4m3 products,
 // with queries as sums of two or three e4m3 numbers, were no faster (132 us) and in
 // f16 slower (four proposed tokens in a window 17.9 us in place of 13.3).
 

@@ -11,7 +11,9 @@
 // takes bits from those that it does.  The softmax, which bounds the kernel, takes
 // the scales in.  The registers are shared out by setmaxnreg: five warpgroups are
 // launched with 96 a thread.  Measured: 5 chunks of 1024 behind up to 6000 keys, 32 /
-// 8 heads of 128, 490 us = 535 TFLOP/s; 8 prompts of 2048, heads of 64, 490 us.
+// 8 heads of 128, 484-495 us = 535 TFLOP/s, with a cap in f16 680; 8 prompts of 2048, heads
+// of 64, 515 us (values of code * scale / 2^E: 493, 652 and 490).  No unit is full (tensor
+// pipe 25 %, issue 48 %, exponentials 20 %): the warps wait for one another.
 #include "paged_tiles.cuh"
 
 namespace b200k {

@@ -8,8 +8,9 @@
 // HBM: x is read once, one or two bytes (four with a gate) for each byte
 // written.  16 lanes hold the 128 columns of a scale, 8 each, so its maximum
 // is four shuffles; with many rows each takes four groups, whose loads are issued
-// together.  Measured: the SwiGLU of [16384, 2 x 8192] bf16 115 us = 5.9 TB/s, 64
-// rows of 4096 1.7 us.
+// together.  Measured: the SwiGLU of [16384, 2 x 8192] bf16 127-135 us = 5.0-5.3 TB/s
+// (154 with every call's output in memory of its own), issue slots 76 % busy; 64 rows
+// of 4096 2.0 us.
 #include <algorithm>
 #include <cstring>
 

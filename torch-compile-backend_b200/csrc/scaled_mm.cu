@@ -30,12 +30,13 @@
 //               memory in the order of the ranks.  For few rows, where b's
 //               bytes are the bound: every SM fetches some of them, and the
 //               tensor-memory lanes are full whatever the number of rows.
-// Measured: [16384, 4096] x [4096, 14336] 865 us = 2.2 PFLOP/s in a short run (1000 us
-// in a long one, at 1.5 GHz under the power limit); the tensor pipe waits for the
-// sums: a buffer's way from the MMAs' issue over the epilogue back takes 1700
+// Measured: [16384, 4096] x [4096, 14336] 980-1040 us = 1.9 PFLOP/s in long runs, at 1.5
+// GHz under the power limit (870-910 us in four calls after a pause).  No unit is
+// full (8192 rows: tensor pipe 60 %, issue 42 %, L2 37 %): the tensor pipe waits for
+// the sums, a buffer's way from the MMAs' issue over the epilogue back takes 1700
 // clocks, of which two buffers hide half (MMAs of 128 columns, which would give
-// four, cost more than they hide: 1010 us).  64 rows of [4096, 14336] 16.5 us = 3.7
-// TB/s, a row of [8192, 2048] 7.3 us.
+// four, cost more than they hide: 1010 us in place of 940).  64 rows of [4096, 14336]
+// 17.8 us = 3.4 TB/s, a row of [8192, 2048] 7.4 us.
 #include <type_traits>
 
 #include "gemm_kernel.cuh"
@@ -761,7 +762,10 @@ extern "C" int b200k_scaled_mm(const B200kScaledMmArgs* a, void* stream_) {
   // when split, its join cost, in blocks).  64 rows of [4096, 14336] (112 tiles)
   // with 1, 2 and 4: 22, 18 and 25 us; a row of [8192, 2048] (16 tiles) with 4 and
   // 8: 9.7 and 8.0.  Clusters of 8 CTAs that have an SM each do not all find room
-  // at once: 128 rows of [8192, 2048] with 4 and 8: 12.5 and 20.6 us.
+  // at once: 128 rows of [8192, 2048] with 4 and 8: 12.5 and 20.6 us.  Of 16 shapes of 1
+  // to 128 rows the choice is within 5 % of the best split in 15; in the other it
+  // takes 48 clusters of 3, which do not all find room either: 100 rows of [4096,
+  // 6144] 19.5 us, 12.5 with 2.
   const int64_t tiles = (a->M + tile - 1) / tile * ((a->N + 127) / 128), slots = static_cast<int64_t>(sms) * (tile <= 64 ? 2 : 1);
   int64_t best = INT64_MAX;
   for (int split = 1; split <= std::min<int32_t>(tile <= 64 ? mm8::kMaxSplit : 4, p.k_blocks); ++split) {
