@@ -35,8 +35,8 @@
 // full (8192 rows: tensor pipe 60 %, issue 42 %, L2 37 %): the tensor pipe waits for
 // the sums, a buffer's way from the MMAs' issue over the epilogue back takes 1700
 // clocks, of which two buffers hide half (MMAs of 128 columns, which would give
-// four, cost more than they hide: 1010 us in place of 940).  64 rows of [4096, 14336]
-// 17.8 us = 3.4 TB/s, a row of [8192, 2048] 7.4 us.
+// four, cost more than they hide: 1010 us with an earlier version).  64 rows of
+// [4096, 14336] 17.8 us = 3.4 TB/s, a row of [8192, 2048] 7.4 us.
 #include <type_traits>
 
 #include "gemm_kernel.cuh"
